@@ -378,6 +378,112 @@ int mhc_wrapper_static_bwd(const float* grad_out, const void* residual, const vo
                            void* workspace, size_t workspace_bytes, int64_t tokens, int32_t n, int32_t hidden,
                            int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps, void* stream);
 
+/* ---- 8-bit checkpoints of rows ----------------------------------------------
+ * No counterpart in the reference.  Rows that a backward pass will read, held
+ * in 8 bits: a row is cut into blocks of 32 values (the last may be shorter);
+ * with a = max |x| of a block and M = 127 (INT8) or 448 (E4M3), e is the least
+ * integer with a <= M 2^e, at least -100.  The block holds x 2^-e rounded to
+ * nearest even as a signed byte or an OCP e4m3 number, and the byte e + 127.
+ * x^ = q 2^e is exact in fp32 and bf16.  A block with a value that is not
+ * finite has the scale byte 255 and comes back as NaN; a value that rounds to
+ * 2^128 comes back as infinity, as it does in bf16.
+ * `values` [rows, ceil16(hidden)] (padded with zeros; 16-byte aligned) and
+ * `scales` [rows, ceil(hidden / 32)] have the sizes of the two queries. */
+#define MHC_CHECKPOINT_NONE (-1)
+#define MHC_CHECKPOINT_INT8 0
+#define MHC_CHECKPOINT_E4M3 1
+
+size_t mhc_checkpoint_values_size(int64_t rows, int32_t hidden);
+size_t mhc_checkpoint_scales_size(int64_t rows, int32_t hidden);
+int mhc_checkpoint_pack(const void* x, int32_t dtype, int32_t format, void* values, void* scales, int64_t rows,
+                        int32_t hidden, void* stream);
+/* out [rows, hidden] = x^ in dtype (exact in either). */
+int mhc_checkpoint_unpack(const void* values, const void* scales, int32_t format, void* out, int32_t dtype,
+                          int64_t rows, int32_t hidden, void* stream);
+
+/* mhc_rmsnorm_fwd that also writes the checkpoint of inp; the backward is the
+ * gradient of RMSNorm at x^ (its rms recomputed from x^).  hidden <= 16384. */
+int mhc_rmsnorm_checkpoint_fwd(const void* inp, int32_t dtype, const float* weight, void* out, int32_t format,
+                               void* values, void* scales, int64_t batch, int32_t hidden, float eps, void* stream);
+size_t mhc_rmsnorm_checkpoint_bwd_workspace_size(int64_t batch, int32_t hidden, int32_t dtype, int32_t format);
+int mhc_rmsnorm_checkpoint_bwd(const void* grad_out, int32_t dtype, const void* values, const void* scales,
+                               int32_t format, const float* weight, void* grad_inp, float* grad_weight,
+                               void* workspace, size_t workspace_bytes, int64_t batch, int32_t hidden, float eps,
+                               void* stream);
+
+/* mhc_layer_static_fwd that also writes the checkpoint of x's batch * n rows,
+ * and its backward at x^: mhc_layer_static_bwd with x^ in x's place. */
+int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype,
+                                    const float* h_pre, const float* h_post, const float* h_res, float* out,
+                                    float* saved, int32_t format, void* values, void* scales, int64_t batch,
+                                    int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
+                                    float rmsnorm_eps, void* stream);
+size_t mhc_layer_static_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype);
+int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
+                                    int32_t x_dtype, int32_t weight_dtype, const float* h_pre, const float* h_post,
+                                    const float* h_res, const float* saved, void* grad_x, void* grad_weight,
+                                    float* grad_h_pre, float* grad_h_post, float* grad_h_res, void* workspace,
+                                    size_t workspace_bytes, int64_t batch, int32_t n, int32_t hidden,
+                                    int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps, void* stream);
+
+/* mhc_layer_dynamic_fwd that also writes the checkpoint of x's batch * n rows,
+ * and its backward: mhc_layer_dynamic_bwd with x^ in x's place (`saved` holds
+ * the forward's own coefficients, projections and r_h, those of x). */
+int mhc_layer_dynamic_checkpoint_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype,
+                                     const float* phi_pre, const float* phi_post, const float* phi_res,
+                                     const float* alpha_pre, const float* alpha_post, const float* alpha_res,
+                                     const float* b_pre, const float* b_post, const float* b_res, float* out,
+                                     float* saved, int32_t format, void* values, void* scales, void* workspace,
+                                     size_t workspace_bytes, int64_t batch, int32_t n, int32_t hidden,
+                                     int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps, void* stream);
+size_t mhc_layer_dynamic_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype);
+int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
+                                     int32_t x_dtype, int32_t weight_dtype, const float* phi_pre,
+                                     const float* phi_post, const float* phi_res, const float* alpha_pre,
+                                     const float* alpha_post, const float* alpha_res, const float* b_pre,
+                                     const float* b_post, const float* b_res, const float* saved, void* grad_x,
+                                     void* grad_weight, float* grad_phi, float* grad_alpha, float* grad_b,
+                                     void* workspace, size_t workspace_bytes, int64_t batch, int32_t n,
+                                     int32_t hidden, int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps,
+                                     void* stream);
+
+/* ---- per-head norm of queries and keys, with the rotation of positions ---------
+ * No counterpart in the reference.  For every head row x of q [tokens, q_heads,
+ * head_dim] and k [tokens, k_heads, head_dim] (dtype; strides in elements, the
+ * last 1):  y = x / sqrt(mean x^2 + eps) * weight, then the pairs (a, b) of the
+ * first rotary_dim channels become (a c - b s, b c + a s), with c, s = column p
+ * of cos / sin [table_rows, rotary_dim / 2] at the token's position; pair p is
+ * channels (p, p + rotary_dim / 2), or (2p, 2p + 1) with interleaved != 0.
+ * Token t's position is entry t % position_period of positions (position_bytes
+ * 4 or 8: int32 or int64), or t % position_period itself (position_bytes 0,
+ * positions NULL).  Rows of a position outside the table become NaN.
+ * q_out / k_out are contiguous.  weights [head_dim] (weight_dtype); head_dim <=
+ * 1024, 2 <= rotary_dim <= head_dim, even.
+ * With a format other than MHC_CHECKPOINT_NONE the checkpoints of q's and k's
+ * rows are written too, and the backward reads them in place of q and k. */
+int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                         int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
+                         void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales, void* k_values,
+                         void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                         int32_t rotary_dim, int32_t interleaved, float eps, void* stream);
+size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                           int32_t dtype, int32_t format);
+/* grad_q / grad_k contiguous (dtype); grad_weight [2, head_dim] (weight_dtype):
+ * that of q_weight, then that of k_weight, summed over tokens and heads in a
+ * fixed order. */
+int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
+                         const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
+                         const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
+                         void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
+                         int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                         int32_t interleaved, float eps, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,11 @@ from .ops import (  # noqa: E402
     mhc_layer_static,
     mhc_layer_fused_dynamic_training,
     mhc_layer_fused_dynamic_inference,
+    PackedActivation,
+    activation_pack,
+    activation_unpack,
+    rope_table,
+    qk_norm_rope,
 )
 
 __all__ = [
@@ -38,4 +43,9 @@ __all__ = [
     "mhc_layer_static",
     "mhc_layer_fused_dynamic_training",
     "mhc_layer_fused_dynamic_inference",
+    "PackedActivation",
+    "activation_pack",
+    "activation_unpack",
+    "rope_table",
+    "qk_norm_rope",
 ]

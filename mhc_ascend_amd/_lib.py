@@ -30,6 +30,8 @@ TIMED_LIB_PATH = os.path.join(_PKG, "libmhc_hip_timed.so")
 
 F32 = 0
 BF16 = 1
+INT8 = 0
+E4M3 = 1
 WRAPPER_DECAY = 0
 WRAPPER_ZERO = 1
 
@@ -111,6 +113,34 @@ SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "mhc_layer_static_bwd": (ctypes.c_int, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp,
                                             _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                             _i64, _i32, _i32, _i32, _f32, _f32, _vp]),
+    "mhc_checkpoint_values_size": (_sz, [_i64, _i32]),
+    "mhc_checkpoint_scales_size": (_sz, [_i64, _i32]),
+    "mhc_checkpoint_pack": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i64, _i32, _vp]),
+    "mhc_checkpoint_unpack": (ctypes.c_int, [_vp, _vp, _i32, _vp, _i32, _i64, _i32, _vp]),
+    "mhc_rmsnorm_checkpoint_fwd": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _f32, _vp]),
+    "mhc_rmsnorm_checkpoint_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "mhc_rmsnorm_checkpoint_bwd": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _i64, _i32, _f32,
+                                                  _vp]),
+    "mhc_layer_static_checkpoint_fwd": (ctypes.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp,
+                                                       _i64, _i32, _i32, _i32, _f32, _f32, _vp]),
+    "mhc_layer_static_checkpoint_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "mhc_layer_static_checkpoint_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                       _vp, _vp, _vp, _vp, _sz, _i64, _i32, _i32, _i32, _f32, _f32,
+                                                       _vp]),
+    "mhc_layer_dynamic_checkpoint_fwd": (ctypes.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                        _vp, _vp, _vp, _i32, _vp, _vp, _vp, _sz, _i64, _i32, _i32,
+                                                        _i32, _f32, _f32, _vp]),
+    "mhc_layer_dynamic_checkpoint_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "mhc_layer_dynamic_checkpoint_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                        _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64,
+                                                        _i32, _i32, _i32, _f32, _f32, _vp]),
+    "mhc_qk_norm_rope_fwd": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _i64,
+                                            _vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32,
+                                            _i32, _i32, _i32, _f32, _vp]),
+    "mhc_qk_norm_rope_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
+    "mhc_qk_norm_rope_bwd": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
+                                            _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _i32, _i64,
+                                            _vp, _vp, _vp, _vp, _sz, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
 }
 
 # The benchmark build's extra entries (include/mhc_hip_timing.h).

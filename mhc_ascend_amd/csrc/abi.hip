@@ -13,6 +13,7 @@
 #ifdef MHC_KERNEL_TIMING
 #include "mhc_hip_timing.h"
 #endif
+#include "mhc_ckpt.h"
 #include "mhc_internal.h"
 
 namespace mhc {
@@ -224,7 +225,7 @@ using namespace mhc;
 
 extern "C" {
 
-int mhc_abi_version(void) { return 101; }
+int mhc_abi_version(void) { return 102; }
 
 const char* mhc_last_error(void) { return g_last_error.c_str(); }
 
@@ -2072,6 +2073,370 @@ int mhc_wrapper_static_bwd(const float* grad_out, const void* residual, const vo
     if (e == hipSuccess && wrap_res_grad_vanishes(num_iters, sinkhorn_eps))
         e = launch_fill_zero_carry(grad_h_res, (int64_t)n * n, nullptr, 0, grad_h_pre, n, s);
     return hip_status(e);
+}
+
+// ---- 8-bit checkpoints --------------------------------------------------------
+}  // extern "C"
+
+// The entries from here on let no C++ exception out (error texts allocate).
+template <typename F>
+static int guarded(F f) noexcept {
+    try {
+        return f();
+    } catch (...) {
+        return MHC_ERR_INVALID;
+    }
+}
+
+static bool valid_format(int f) { return f == kCkInt8 || f == kCkE4M3; }
+
+static int check_ckpt(const char* fn, int64_t rows, int64_t hidden, int32_t dtype, int32_t format, bool pointers) {
+    if (rows < 0) return fail(MHC_ERR_INVALID, std::string(fn) + ": the number of rows must be >= 0");
+    if (hidden < 1) return fail(MHC_ERR_INVALID, std::string(fn) + ": hidden must be >= 1");
+    if (!valid_dtype(dtype)) return fail(MHC_ERR_INVALID, std::string(fn) + ": dtype must be F32 or BF16");
+    if (!valid_format(format)) return fail(MHC_ERR_INVALID, std::string(fn) + ": format must be INT8 or E4M3");
+    if (rows > 0 && !pointers) return fail(MHC_ERR_INVALID, std::string(fn) + ": null pointer");
+    return MHC_SUCCESS;
+}
+
+static size_t ckpt_rows_bytes(int64_t rows, int32_t hidden, int32_t dtype) {
+    return align256((size_t)rows * (size_t)hidden * (size_t)dtype_size(dtype));
+}
+
+extern "C" {
+
+size_t mhc_checkpoint_values_size(int64_t rows, int32_t hidden) {
+    if (rows < 0 || hidden < 1) return 0;
+    return (size_t)rows * (size_t)ck_stride(hidden);
+}
+
+size_t mhc_checkpoint_scales_size(int64_t rows, int32_t hidden) {
+    if (rows < 0 || hidden < 1) return 0;
+    return (size_t)rows * (size_t)ck_blocks(hidden);
+}
+
+int mhc_checkpoint_pack(const void* x, int32_t dtype, int32_t format, void* values, void* scales, int64_t rows,
+                        int32_t hidden, void* stream) {
+    return guarded([&]() -> int {
+        const int st = check_ckpt("checkpoint_pack", rows, hidden, dtype, format, x && values && scales);
+        if (st) return st;
+        MHC_REQUIRE((uintptr_t)values % 16 == 0, "checkpoint_pack: values must be 16-byte aligned");
+        return hip_status(launch_ckpt_pack(dtype, format, x, values, scales, rows, hidden, (hipStream_t)stream));
+    });
+}
+
+int mhc_checkpoint_unpack(const void* values, const void* scales, int32_t format, void* out, int32_t dtype,
+                          int64_t rows, int32_t hidden, void* stream) {
+    return guarded([&]() -> int {
+        const int st = check_ckpt("checkpoint_unpack", rows, hidden, dtype, format, out && values && scales);
+        if (st) return st;
+        MHC_REQUIRE((uintptr_t)values % 16 == 0, "checkpoint_unpack: values must be 16-byte aligned");
+        return hip_status(launch_ckpt_unpack(dtype, format, values, scales, out, rows, hidden, (hipStream_t)stream));
+    });
+}
+
+// ---- RMSNorm with a checkpoint -------------------------------------------------
+static int check_rmsnorm_ckpt(const char* fn, int64_t batch, int32_t hidden, int32_t dtype, int32_t format,
+                              bool pointers, const void* values) {
+    const int st = check_ckpt(fn, batch, hidden, dtype, format, pointers);
+    if (st) return st;
+    if (batch > 0x7fffffff) return fail(MHC_ERR_UNSUPPORTED, std::string(fn) + ": batch must be < 2^31");
+    if (!rmsnorm_ckpt_supported(hidden))
+        return fail(MHC_ERR_UNSUPPORTED, std::string(fn) + ": hidden=" + std::to_string(hidden) +
+                                             " is too large for the row kernels (at most " +
+                                             std::to_string(kCkMaxRow) + ")");
+    if ((uintptr_t)values % 16 != 0) return fail(MHC_ERR_INVALID, std::string(fn) + ": values must be 16-byte aligned");
+    return MHC_SUCCESS;
+}
+
+int mhc_rmsnorm_checkpoint_fwd(const void* inp, int32_t dtype, const float* weight, void* out, int32_t format,
+                               void* values, void* scales, int64_t batch, int32_t hidden, float eps, void* stream) {
+    return guarded([&]() -> int {
+        const int st = check_rmsnorm_ckpt("rmsnorm_checkpoint_fwd", batch, hidden, dtype, format,
+                                          inp && weight && out && values && scales, values);
+        if (st) return st;
+        return hip_status(launch_rmsnorm_ckpt_fwd(dtype, format, inp, weight, out, values, scales, batch, hidden, eps,
+                                                  (hipStream_t)stream));
+    });
+}
+
+static RowsBwdWs rmsnorm_ckpt_bwd_ws(int64_t batch, int32_t hidden, int32_t dtype, int32_t format) {
+    RowsBwdWs w{};
+    w.grid = batch > 0 ? rmsnorm_ckpt_bwd_grid(dtype, format, batch, hidden) : 1;
+    w.stage_off = align256((size_t)w.grid * hidden * sizeof(float));
+    w.total = w.stage_off + align256(column_sums_stage_floats(hidden) * sizeof(float));
+    return w;
+}
+
+size_t mhc_rmsnorm_checkpoint_bwd_workspace_size(int64_t batch, int32_t hidden, int32_t dtype, int32_t format) {
+    if (batch < 0 || !rmsnorm_ckpt_supported(hidden) || !valid_dtype(dtype) || !valid_format(format)) return 0;
+    return rmsnorm_ckpt_bwd_ws(batch, hidden, dtype, format).total;
+}
+
+int mhc_rmsnorm_checkpoint_bwd(const void* grad_out, int32_t dtype, const void* values, const void* scales,
+                               int32_t format, const float* weight, void* grad_inp, float* grad_weight,
+                               void* workspace, size_t workspace_bytes, int64_t batch, int32_t hidden, float eps,
+                               void* stream) {
+    return guarded([&]() -> int {
+        const int st = check_rmsnorm_ckpt("rmsnorm_checkpoint_bwd", batch, hidden, dtype, format,
+                                          grad_out && values && scales && weight && grad_inp, values);
+        if (st) return st;
+        MHC_REQUIRE(grad_weight, "rmsnorm_checkpoint_bwd: null grad_weight");
+        const RowsBwdWs w = rmsnorm_ckpt_bwd_ws(batch, hidden, dtype, format);
+        if (!workspace || workspace_bytes < w.total)
+            return fail(MHC_ERR_WORKSPACE, "rmsnorm_checkpoint_bwd: workspace smaller than "
+                                           "mhc_rmsnorm_checkpoint_bwd_workspace_size()");
+        hipStream_t s = (hipStream_t)stream;
+        float* part = (float*)workspace;
+        float* stage = (float*)((char*)workspace + w.stage_off);
+        hipError_t e = batch == 0 ? launch_fill_zero(part, hidden, s)
+                                  : launch_rmsnorm_ckpt_bwd(dtype, format, grad_out, values, scales, weight, grad_inp,
+                                                            part, w.grid, batch, hidden, eps, s);
+        if (e == hipSuccess)
+            e = launch_column_finalize(0, kF32, part, w.grid, hidden, stage, grad_weight, nullptr, 0, nullptr, nullptr,
+                                       nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+        return hip_status(e);
+    });
+}
+
+// ---- layers with a checkpoint --------------------------------------------------
+int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype,
+                                    const float* h_pre, const float* h_post, const float* h_res, float* out,
+                                    float* saved, int32_t format, void* values, void* scales, int64_t batch,
+                                    int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
+                                    float rmsnorm_eps, void* stream) {
+    return guarded([&]() -> int {
+        int st = check_ckpt("layer_static_checkpoint_fwd", batch, hidden, x_dtype, format, x && values && scales);
+        if (st) return st;
+        MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_static_checkpoint_fwd: values must be 16-byte aligned");
+        st = mhc_layer_static_fwd(x, x_dtype, weight, weight_dtype, h_pre, h_post, h_res, out, nullptr, saved, batch, n,
+                                  hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
+        if (st) return st;
+        return hip_status(launch_ckpt_pack(x_dtype, format, x, values, scales, batch * n, hidden, (hipStream_t)stream));
+    });
+}
+
+// workspace: [x^ rows | the layer's backward]
+size_t mhc_layer_static_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
+    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype)) return 0;
+    return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
+           mhc_layer_static_bwd_workspace_size(batch, n, hidden, x_dtype);
+}
+
+int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
+                                    int32_t x_dtype, int32_t weight_dtype, const float* h_pre, const float* h_post,
+                                    const float* h_res, const float* saved, void* grad_x, void* grad_weight,
+                                    float* grad_h_pre, float* grad_h_post, float* grad_h_res, void* workspace,
+                                    size_t workspace_bytes, int64_t batch, int32_t n, int32_t hidden,
+                                    int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps, void* stream) {
+    return guarded([&]() -> int {
+        const char* fn = "layer_static_checkpoint_bwd";
+        int st = check_ckpt(fn, batch, hidden, x_dtype, format, grad_out && values && scales && grad_x);
+        if (st) return st;
+        st = check_layer_shape(fn, batch, n, hidden, x_dtype, num_iters);
+        if (st) return st;
+        MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_static_checkpoint_bwd: values must be 16-byte aligned");
+        const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
+        if (!workspace ||
+            workspace_bytes < mhc_layer_static_checkpoint_bwd_workspace_size(batch, n, hidden, x_dtype))
+            return fail(MHC_ERR_WORKSPACE, "layer_static_checkpoint_bwd: workspace smaller than "
+                                           "mhc_layer_static_checkpoint_bwd_workspace_size()");
+        const hipError_t e =
+            launch_ckpt_unpack(x_dtype, format, values, scales, workspace, batch * n, hidden, (hipStream_t)stream);
+        if (e != hipSuccess) return hip_status(e);
+        return mhc_layer_static_bwd(grad_out, workspace, x_dtype, weight_dtype, h_pre, h_post, h_res, saved, grad_x,
+                                    grad_weight, grad_h_pre, grad_h_post, grad_h_res, (char*)workspace + rows,
+                                    workspace_bytes - rows, batch, n, hidden, num_iters, sinkhorn_eps, rmsnorm_eps,
+                                    stream);
+    });
+}
+
+int mhc_layer_dynamic_checkpoint_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype,
+                                     const float* phi_pre, const float* phi_post, const float* phi_res,
+                                     const float* alpha_pre, const float* alpha_post, const float* alpha_res,
+                                     const float* b_pre, const float* b_post, const float* b_res, float* out,
+                                     float* saved, int32_t format, void* values, void* scales, void* workspace,
+                                     size_t workspace_bytes, int64_t batch, int32_t n, int32_t hidden,
+                                     int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps, void* stream) {
+    return guarded([&]() -> int {
+        int st = check_ckpt("layer_dynamic_checkpoint_fwd", batch, hidden, x_dtype, format, x && values && scales);
+        if (st) return st;
+        MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_dynamic_checkpoint_fwd: values must be 16-byte aligned");
+        st = mhc_layer_dynamic_fwd(x, x_dtype, weight, weight_dtype, phi_pre, phi_post, phi_res, alpha_pre, alpha_post,
+                                   alpha_res, b_pre, b_post, b_res, out, saved, workspace, workspace_bytes, batch, n,
+                                   hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
+        if (st) return st;
+        return hip_status(launch_ckpt_pack(x_dtype, format, x, values, scales, batch * n, hidden, (hipStream_t)stream));
+    });
+}
+
+size_t mhc_layer_dynamic_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
+    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype)) return 0;
+    return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
+           mhc_layer_dynamic_bwd_workspace_size(batch, n, hidden, x_dtype);
+}
+
+int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
+                                     int32_t x_dtype, int32_t weight_dtype, const float* phi_pre,
+                                     const float* phi_post, const float* phi_res, const float* alpha_pre,
+                                     const float* alpha_post, const float* alpha_res, const float* b_pre,
+                                     const float* b_post, const float* b_res, const float* saved, void* grad_x,
+                                     void* grad_weight, float* grad_phi, float* grad_alpha, float* grad_b,
+                                     void* workspace, size_t workspace_bytes, int64_t batch, int32_t n,
+                                     int32_t hidden, int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps,
+                                     void* stream) {
+    return guarded([&]() -> int {
+        const char* fn = "layer_dynamic_checkpoint_bwd";
+        int st = check_ckpt(fn, batch, hidden, x_dtype, format, grad_out && values && scales && grad_x);
+        if (st) return st;
+        st = check_dyn(fn, batch, n, hidden, x_dtype, weight_dtype, num_iters);
+        if (st) return st;
+        MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_dynamic_checkpoint_bwd: values must be 16-byte aligned");
+        const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
+        if (!workspace ||
+            workspace_bytes < mhc_layer_dynamic_checkpoint_bwd_workspace_size(batch, n, hidden, x_dtype))
+            return fail(MHC_ERR_WORKSPACE, "layer_dynamic_checkpoint_bwd: workspace smaller than "
+                                           "mhc_layer_dynamic_checkpoint_bwd_workspace_size()");
+        const hipError_t e =
+            launch_ckpt_unpack(x_dtype, format, values, scales, workspace, batch * n, hidden, (hipStream_t)stream);
+        if (e != hipSuccess) return hip_status(e);
+        return mhc_layer_dynamic_bwd(grad_out, workspace, x_dtype, weight_dtype, phi_pre, phi_post, phi_res, alpha_pre,
+                                     alpha_post, alpha_res, b_pre, b_post, b_res, saved, grad_x, grad_weight, grad_phi,
+                                     grad_alpha, grad_b, (char*)workspace + rows, workspace_bytes - rows, batch, n,
+                                     hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
+    });
+}
+
+// ---- queries and keys -----------------------------------------------------------
+static int check_qk(const char* fn, const QkArgs& a, int32_t dtype, int32_t format) {
+    const std::string f(fn);
+    if (a.T < 0 || a.T > 0x7fffffff) return fail(MHC_ERR_INVALID, f + ": tokens must be in 0 .. 2^31 - 1");
+    if (a.heads[0] < 0 || a.heads[1] < 0 || (int64_t)a.heads[0] + a.heads[1] > 65535 * 4)
+        return fail(MHC_ERR_INVALID, f + ": the heads must be >= 0 and at most 262140 together");
+    if (a.D < 2 || a.D > kQkMaxDim)
+        return fail(a.D > kQkMaxDim ? MHC_ERR_UNSUPPORTED : MHC_ERR_INVALID,
+                    f + ": head_dim must be in 2 .. " + std::to_string(kQkMaxDim));
+    if (a.R < 2 || a.R > a.D || a.R % 2 != 0)
+        return fail(MHC_ERR_INVALID, f + ": rotary_dim must be even, in 2 .. head_dim");
+    if (!valid_dtype(dtype)) return fail(MHC_ERR_INVALID, f + ": dtype must be F32 or BF16");
+    if (!valid_dtype(a.w_dtype)) return fail(MHC_ERR_INVALID, f + ": weight_dtype must be F32 or BF16");
+    if (format != -1 && !valid_format(format))
+        return fail(MHC_ERR_INVALID, f + ": format must be NONE, INT8 or E4M3");
+    if (a.pos_bytes != 0 && a.pos_bytes != 4 && a.pos_bytes != 8)
+        return fail(MHC_ERR_INVALID, f + ": position_bytes must be 0, 4 or 8");
+    if (a.T > 0 && (a.pos_bytes == 0) != (a.pos == nullptr))
+        return fail(MHC_ERR_INVALID, f + ": positions and position_bytes do not match");
+    if (a.period < 1 || a.period > 0x7fffffff)
+        return fail(MHC_ERR_INVALID, f + ": position_period must be in 1 .. 2^31 - 1");
+    if (a.table_rows < 1) return fail(MHC_ERR_INVALID, f + ": the table must have rows");
+    if (!a.w[0] || !a.w[1] || !a.cos || !a.sin) return fail(MHC_ERR_INVALID, f + ": null weight or table");
+    for (int s = 0; s < 2; ++s) {
+        if (a.T == 0 || a.heads[s] == 0) continue;
+        if (!a.y[s]) return fail(MHC_ERR_INVALID, f + ": null output");
+        if (format >= 0 && (!a.q[s] || !a.sc[s] || (uintptr_t)a.q[s] % 16 != 0))
+            return fail(MHC_ERR_INVALID, f + ": null checkpoint, or values not 16-byte aligned");
+    }
+    return MHC_SUCCESS;
+}
+
+int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                         int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
+                         void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales, void* k_values,
+                         void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                         int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
+    return guarded([&]() -> int {
+        QkArgs a{};
+        a.x[0] = q; a.x_token[0] = q_token_stride; a.x_head[0] = q_head_stride;
+        a.x[1] = k; a.x_token[1] = k_token_stride; a.x_head[1] = k_head_stride;
+        a.y[0] = q_out; a.y[1] = k_out;
+        a.q[0] = (uint8_t*)q_values; a.sc[0] = (uint8_t*)q_scales;
+        a.q[1] = (uint8_t*)k_values; a.sc[1] = (uint8_t*)k_scales;
+        a.w[0] = q_weight; a.w[1] = k_weight;
+        a.cos = cos; a.sin = sin; a.pos = positions;
+        a.table_rows = table_rows; a.period = position_period; a.T = tokens;
+        a.heads[0] = q_heads; a.heads[1] = k_heads;
+        a.w_dtype = weight_dtype; a.pos_bytes = position_bytes; a.D = head_dim; a.R = rotary_dim;
+        a.interleaved = interleaved != 0; a.eps = eps;
+        const int st = check_qk("qk_norm_rope_fwd", a, dtype, format);
+        if (st) return st;
+        MHC_REQUIRE(tokens == 0 || ((q || q_heads == 0) && (k || k_heads == 0)), "qk_norm_rope_fwd: null q/k");
+        return hip_status(launch_qk_norm_rope_fwd(dtype, format, a, (hipStream_t)stream));
+    });
+}
+
+static RowsBwdWs qk_bwd_ws(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t dtype,
+                           int32_t format) {
+    RowsBwdWs w{};
+    (void)q_heads; (void)k_heads; (void)dtype; (void)format;
+    w.grid = qk_norm_rope_bwd_grid(tokens);
+    w.stage_off = align256((size_t)w.grid * 2 * head_dim * sizeof(float));
+    w.total = w.stage_off + align256(column_sums_stage_floats(2 * (int64_t)head_dim) * sizeof(float));
+    return w;
+}
+
+size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                                           int32_t dtype, int32_t format) {
+    if (tokens < 0 || tokens > 0x7fffffff || q_heads < 0 || k_heads < 0 || head_dim < 2 || head_dim > kQkMaxDim ||
+        !valid_dtype(dtype) || (format != -1 && !valid_format(format)))
+        return 0;
+    return qk_bwd_ws(tokens, q_heads, k_heads, head_dim, dtype, format).total;
+}
+
+int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
+                         const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
+                         const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
+                         void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
+                         int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                         int32_t interleaved, float eps, void* stream) {
+    return guarded([&]() -> int {
+        QkArgs a{};
+        a.x[0] = q; a.x_token[0] = q_token_stride; a.x_head[0] = q_head_stride;
+        a.x[1] = k; a.x_token[1] = k_token_stride; a.x_head[1] = k_head_stride;
+        a.g[0] = grad_q_out; a.g_token[0] = gq_token_stride; a.g_head[0] = gq_head_stride;
+        a.g[1] = grad_k_out; a.g_token[1] = gk_token_stride; a.g_head[1] = gk_head_stride;
+        a.y[0] = grad_q; a.y[1] = grad_k;
+        a.q[0] = (uint8_t*)q_values; a.sc[0] = (uint8_t*)q_scales;
+        a.q[1] = (uint8_t*)k_values; a.sc[1] = (uint8_t*)k_scales;
+        a.w[0] = q_weight; a.w[1] = k_weight;
+        a.cos = cos; a.sin = sin; a.pos = positions;
+        a.table_rows = table_rows; a.period = position_period; a.T = tokens;
+        a.heads[0] = q_heads; a.heads[1] = k_heads;
+        a.w_dtype = weight_dtype; a.pos_bytes = position_bytes; a.D = head_dim; a.R = rotary_dim;
+        a.interleaved = interleaved != 0; a.eps = eps;
+        const int st = check_qk("qk_norm_rope_bwd", a, dtype, format);
+        if (st) return st;
+        MHC_REQUIRE(tokens == 0 || ((grad_q_out || q_heads == 0) && (grad_k_out || k_heads == 0)),
+                    "qk_norm_rope_bwd: null grad_q_out/grad_k_out");
+        MHC_REQUIRE(tokens == 0 || format >= 0 || ((q || q_heads == 0) && (k || k_heads == 0)),
+                    "qk_norm_rope_bwd: null q/k");
+        MHC_REQUIRE(grad_weight, "qk_norm_rope_bwd: null grad_weight");
+        const RowsBwdWs w = qk_bwd_ws(tokens, q_heads, k_heads, head_dim, dtype, format);
+        if (!workspace || workspace_bytes < w.total)
+            return fail(MHC_ERR_WORKSPACE,
+                        "qk_norm_rope_bwd: workspace smaller than mhc_qk_norm_rope_bwd_workspace_size()");
+        hipStream_t s = (hipStream_t)stream;
+        float* part = (float*)workspace;
+        float* stage = (float*)((char*)workspace + w.stage_off);
+        const int64_t cols = 2 * (int64_t)head_dim;
+        int rows = w.grid;
+        hipError_t e;
+        if (tokens == 0 || q_heads + k_heads == 0) {
+            rows = 1;
+            e = launch_fill_zero(part, cols, s);
+        } else {
+            e = launch_qk_norm_rope_bwd(dtype, format, a, part, w.grid, s);
+        }
+        if (e == hipSuccess)
+            e = launch_column_finalize(0, weight_dtype, part, rows, cols, stage, grad_weight, nullptr, 0, nullptr,
+                                       nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+        return hip_status(e);
+    });
 }
 
 }  // extern "C"

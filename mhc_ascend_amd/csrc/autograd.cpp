@@ -63,7 +63,23 @@ using torch::autograd::tensor_list;
     X(mhc_wrapper_dynamic_bwd)                \
     X(mhc_wrapper_static_fwd)                 \
     X(mhc_wrapper_static_bwd_workspace_size)  \
-    X(mhc_wrapper_static_bwd)
+    X(mhc_wrapper_static_bwd)                 \
+    X(mhc_checkpoint_values_size)             \
+    X(mhc_checkpoint_scales_size)             \
+    X(mhc_checkpoint_pack)                    \
+    X(mhc_checkpoint_unpack)                  \
+    X(mhc_rmsnorm_checkpoint_fwd)             \
+    X(mhc_rmsnorm_checkpoint_bwd_workspace_size) \
+    X(mhc_rmsnorm_checkpoint_bwd)             \
+    X(mhc_layer_static_checkpoint_fwd)        \
+    X(mhc_layer_static_checkpoint_bwd_workspace_size) \
+    X(mhc_layer_static_checkpoint_bwd)        \
+    X(mhc_layer_dynamic_checkpoint_fwd)       \
+    X(mhc_layer_dynamic_checkpoint_bwd_workspace_size) \
+    X(mhc_layer_dynamic_checkpoint_bwd)       \
+    X(mhc_qk_norm_rope_fwd)                   \
+    X(mhc_qk_norm_rope_bwd_workspace_size)    \
+    X(mhc_qk_norm_rope_bwd)
 
 struct Entries {
 #define MHC_DECLARE(name) decltype(&::name) name = nullptr;
@@ -185,10 +201,54 @@ void* stream() { return at::hip::getCurrentHIPStream().stream(); }
 
 float* fp(const Tensor& t) { return t.data_ptr<float>(); }
 
+// ---- 8-bit checkpoints of saved rows ---------------------------------------------
+// A node called with a format (MHC_CHECKPOINT_INT8 / _E4M3) saves the rows its
+// backward reads in 8 bits; MHC_CHECKPOINT_NONE saves them as they are.
+struct Held {
+    Tensor values, scales;
+};
+
+Held held_alloc(const Tensor& x) {
+    const int64_t C = x.size(-1), rows = C > 0 ? x.numel() / C : 0;
+    TORCH_CHECK(C >= 1 && C <= INT32_MAX, "checkpoint: rows of ", C, " values");
+    const auto opt = x.options().dtype(at::kByte);
+    return {at::empty({(int64_t)lib.mhc_checkpoint_values_size(rows, (int32_t)C)}, opt),
+            at::empty({(int64_t)lib.mhc_checkpoint_scales_size(rows, (int32_t)C)}, opt)};
+}
+
+// x contiguous, in storage dtype
+Held hold(const Tensor& x, int64_t fmt) {
+    Held h = held_alloc(x);
+    const int64_t C = x.size(-1);
+    check(lib.mhc_checkpoint_pack(x.data_ptr(), dtype_code(x.scalar_type()), (int32_t)fmt, h.values.data_ptr(),
+                                  h.scales.data_ptr(), x.numel() / C, (int32_t)C, stream()),
+          "mhc_checkpoint_pack");
+    return h;
+}
+
+Tensor held_rows(const Tensor& values, const Tensor& scales, int64_t fmt, at::IntArrayRef sizes, at::ScalarType dt) {
+    Tensor x = at::empty(sizes, values.options().dtype(dt));
+    const int64_t C = sizes.back();
+    check(lib.mhc_checkpoint_unpack(values.data_ptr(), scales.data_ptr(), (int32_t)fmt, x.data_ptr(), dtype_code(dt),
+                                    x.numel() / C, (int32_t)C, stream()),
+          "mhc_checkpoint_unpack");
+    return x;
+}
+
+// The format a call runs with: none where no backward will read the rows.
+int64_t format_for(int64_t fmt, std::initializer_list<const Tensor*> inputs) {
+    TORCH_CHECK(fmt >= MHC_CHECKPOINT_NONE && fmt <= MHC_CHECKPOINT_E4M3, "unknown checkpoint format ", fmt);
+    if (fmt == MHC_CHECKPOINT_NONE || !at::GradMode::is_enabled()) return MHC_CHECKPOINT_NONE;
+    for (const Tensor* t : inputs)
+        if (t->requires_grad()) return fmt;
+    return MHC_CHECKPOINT_NONE;
+}
+
 // ---- static H: mhc_ascend_amd.ops.MHCLayerStaticFunction (layer.py:142-170) --
 struct StaticLayer : public torch::autograd::Function<StaticLayer> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, const Tensor& hp_in,
-                          const Tensor& hq_in, const Tensor& hr_in, int64_t iters, double sk_eps, double rms_eps) {
+                          const Tensor& hq_in, const Tensor& hr_in, int64_t iters, double sk_eps, double rms_eps,
+                          int64_t fmt) {
         const char* fn = "mhc_layer_static_fwd";
         check_device(fn, {&x_in, &w_in, &hp_in, &hq_in, &hr_in});
         const at::DeviceGuard guard(x_in.device());
@@ -199,16 +259,30 @@ struct StaticLayer : public torch::autograd::Function<StaticLayer> {
         const Tensor w = weight(w_in), hp = f32c(hp_in), hq = f32c(hq_in), hr = f32c(hr_in);
         const auto f32 = x.options().dtype(at::kFloat);
         Tensor out = at::empty({B, n, C}, f32);
-        Tensor rms = at::empty({B}, f32);
         Tensor saved = at::empty({(int64_t)(lib.mhc_layer_static_saved_size((int32_t)n, (int32_t)C) / 4)}, f32);
+        ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
+        ctx->saved_data["cfg"] = std::vector<double>{(double)iters, sk_eps, rms_eps};
+        ctx->saved_data["fmt"] = fmt;
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            const Held held = held_alloc(x);
+            check(lib.mhc_layer_static_checkpoint_fwd(
+                      x.data_ptr(), dtype_code(x.scalar_type()), w.data_ptr(), dtype_code(w.scalar_type()), fp(hp),
+                      fp(hq), fp(hr), fp(out), fp(saved), (int32_t)fmt, held.values.data_ptr(),
+                      held.scales.data_ptr(), B, (int32_t)n, (int32_t)C, (int32_t)iters, (float)sk_eps,
+                      (float)rms_eps, stream()),
+                  "mhc_layer_static_checkpoint_fwd");
+            ctx->saved_data["sizes"] = x.sizes().vec();
+            ctx->saved_data["store"] = (int64_t)x.scalar_type();
+            ctx->save_for_backward({held.values, w, hp, hq, hr, saved, held.scales});
+            return out;
+        }
+        Tensor rms = at::empty({B}, f32);
         check(lib.mhc_layer_static_fwd(x.data_ptr(), dtype_code(x.scalar_type()), w.data_ptr(),
                                        dtype_code(w.scalar_type()), fp(hp), fp(hq), fp(hr), fp(out), fp(rms),
                                        fp(saved), B, (int32_t)n, (int32_t)C, (int32_t)iters, (float)sk_eps,
                                        (float)rms_eps, stream()),
               fn);
         ctx->save_for_backward({x, w, hp, hq, hr, saved});
-        ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
-        ctx->saved_data["cfg"] = std::vector<double>{(double)iters, sk_eps, rms_eps};
         return out;
     }
 
@@ -219,23 +293,38 @@ struct StaticLayer : public torch::autograd::Function<StaticLayer> {
         check_device(fn, {&grads[0], &x});
         const at::DeviceGuard guard(x.device());
         const auto cfg = ctx->saved_data["cfg"].toDoubleVector();
-        const int64_t B = x.size(0), n = x.size(1), C = x.size(2);
-        TORCH_CHECK(grads[0].sizes() == x.sizes(), "mhc_layer_static_bwd: grad_out must match x [B, n, C]");
+        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const bool is_held = fmt != MHC_CHECKPOINT_NONE;  // x is the checkpoint's values then
+        const auto sizes = is_held ? ctx->saved_data["sizes"].toIntVector() : x.sizes().vec();
+        const auto store = is_held ? (at::ScalarType)ctx->saved_data["store"].toInt() : x.scalar_type();
+        const int64_t B = sizes[0], n = sizes[1], C = sizes[2];
+        TORCH_CHECK(grads[0].sizes() == sizes, "mhc_layer_static_bwd: grad_out must match x [B, n, C]");
         const Tensor g = f32c(grads[0]);
         const auto f32 = x.options().dtype(at::kFloat);
-        Tensor grad_x = at::empty_like(x);
+        Tensor grad_x = at::empty(sizes, x.options().dtype(store));
         Tensor gw = at::empty({C}, w.options());
         Tensor ghp = at::empty(hp.sizes(), f32), ghq = at::empty(hq.sizes(), f32), ghr = at::empty(hr.sizes(), f32);
-        const int xd = dtype_code(x.scalar_type());
-        const size_t wsb = lib.mhc_layer_static_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
-        Tensor ws = workspace(wsb, x);
-        check(lib.mhc_layer_static_bwd(fp(g), x.data_ptr(), xd, dtype_code(w.scalar_type()), fp(hp), fp(hq), fp(hr),
-                                       fp(saved), grad_x.data_ptr(), gw.data_ptr(), fp(ghp), fp(ghq), fp(ghr),
-                                       ws.data_ptr(), wsb, B, (int32_t)n, (int32_t)C, (int32_t)cfg[0],
-                                       (float)cfg[1], (float)cfg[2], stream()),
-              fn);
+        const int xd = dtype_code(store);
+        if (is_held) {
+            const size_t wsb = lib.mhc_layer_static_checkpoint_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
+            Tensor ws = workspace(wsb, x);
+            check(lib.mhc_layer_static_checkpoint_bwd(
+                      fp(g), x.data_ptr(), sv[6].data_ptr(), (int32_t)fmt, xd, dtype_code(w.scalar_type()), fp(hp),
+                      fp(hq), fp(hr), fp(saved), grad_x.data_ptr(), gw.data_ptr(), fp(ghp), fp(ghq), fp(ghr),
+                      ws.data_ptr(), wsb, B, (int32_t)n, (int32_t)C, (int32_t)cfg[0], (float)cfg[1], (float)cfg[2],
+                      stream()),
+                  "mhc_layer_static_checkpoint_bwd");
+        } else {
+            const size_t wsb = lib.mhc_layer_static_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
+            Tensor ws = workspace(wsb, x);
+            check(lib.mhc_layer_static_bwd(fp(g), x.data_ptr(), xd, dtype_code(w.scalar_type()), fp(hp), fp(hq),
+                                           fp(hr), fp(saved), grad_x.data_ptr(), gw.data_ptr(), fp(ghp), fp(ghq),
+                                           fp(ghr), ws.data_ptr(), wsb, B, (int32_t)n, (int32_t)C, (int32_t)cfg[0],
+                                           (float)cfg[1], (float)cfg[2], stream()),
+                  fn);
+        }
         const auto x_dtype = (at::ScalarType)ctx->saved_data["x_dtype"].toInt();
-        return {grad_x.to(x_dtype), gw, ghp, ghq, ghr, Tensor(), Tensor(), Tensor()};
+        return {grad_x.to(x_dtype), gw, ghp, ghq, ghr, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -254,7 +343,7 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, const Tensor& pp_in,
                           const Tensor& pq_in, const Tensor& pr_in, const Tensor& ap_in, const Tensor& aq_in,
                           const Tensor& ar_in, const Tensor& bp_in, const Tensor& bq_in, const Tensor& br_in,
-                          int64_t iters, double sk_eps, double rms_eps) {
+                          int64_t iters, double sk_eps, double rms_eps, int64_t fmt) {
         const char* fn = "mhc_layer_dynamic_fwd";
         check_device(fn, {&x_in, &w_in, &pp_in, &pq_in, &pr_in, &bp_in, &bq_in, &br_in});
         const at::DeviceGuard guard(x_in.device());
@@ -271,6 +360,23 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
         Tensor saved = at::empty({(int64_t)(lib.mhc_layer_dynamic_saved_size(B, (int32_t)n, (int32_t)C) / 4)}, f32);
         const size_t wsb = lib.mhc_layer_dynamic_fwd_workspace_size(B, (int32_t)n, (int32_t)C);
         Tensor ws = workspace(wsb, x);
+        ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
+        ctx->saved_data["cfg"] = std::vector<double>{(double)iters, sk_eps, rms_eps};
+        ctx->saved_data["fmt"] = fmt;
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            const Held held = held_alloc(x);
+            check(lib.mhc_layer_dynamic_checkpoint_fwd(
+                      x.data_ptr(), dtype_code(x.scalar_type()), w.data_ptr(), dtype_code(w.scalar_type()), fp(ph[0]),
+                      fp(ph[1]), fp(ph[2]), fp(ap), fp(aq), fp(ar), fp(bp), fp(bq), fp(br), fp(out), fp(saved),
+                      (int32_t)fmt, held.values.data_ptr(), held.scales.data_ptr(), ws.data_ptr(), wsb, B, (int32_t)n,
+                      (int32_t)C, (int32_t)iters, (float)sk_eps, (float)rms_eps, stream()),
+                  "mhc_layer_dynamic_checkpoint_fwd");
+            ctx->saved_data["sizes"] = x.sizes().vec();
+            ctx->saved_data["store"] = (int64_t)x.scalar_type();
+            ctx->save_for_backward(
+                {held.values, w, saved, ph[0], ph[1], ph[2], ap, aq, ar, bp, bq, br, held.scales});
+            return out;
+        }
         check(lib.mhc_layer_dynamic_fwd(x.data_ptr(), dtype_code(x.scalar_type()), w.data_ptr(),
                                         dtype_code(w.scalar_type()), fp(ph[0]), fp(ph[1]), fp(ph[2]), fp(ap), fp(aq),
                                         fp(ar), fp(bp), fp(bq), fp(br), fp(out), fp(saved), ws.data_ptr(), wsb, B,
@@ -278,8 +384,6 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
                                         stream()),
               fn);
         ctx->save_for_backward({x, w, saved, ph[0], ph[1], ph[2], ap, aq, ar, bp, bq, br});
-        ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
-        ctx->saved_data["cfg"] = std::vector<double>{(double)iters, sk_eps, rms_eps};
         return out;
     }
 
@@ -290,34 +394,49 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
         check_device(fn, {&grads[0], &x});
         const at::DeviceGuard guard(x.device());
         const auto cfg = ctx->saved_data["cfg"].toDoubleVector();
-        const int64_t B = x.size(0), n = x.size(1), C = x.size(2), np = 2 * n + n * n;
-        TORCH_CHECK(grads[0].sizes() == x.sizes(), "mhc_layer_dynamic_bwd: grad_output must match x [B, n, C]");
+        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const bool is_held = fmt != MHC_CHECKPOINT_NONE;  // x is the checkpoint's values then
+        const auto sizes = is_held ? ctx->saved_data["sizes"].toIntVector() : x.sizes().vec();
+        const auto store = is_held ? (at::ScalarType)ctx->saved_data["store"].toInt() : x.scalar_type();
+        const int64_t B = sizes[0], n = sizes[1], C = sizes[2], np = 2 * n + n * n;
+        TORCH_CHECK(grads[0].sizes() == sizes, "mhc_layer_dynamic_bwd: grad_output must match x [B, n, C]");
         const Tensor g = f32c(grads[0]);
         const auto f32 = x.options().dtype(at::kFloat);
-        Tensor grad_x = at::empty_like(x);
+        Tensor grad_x = at::empty(sizes, x.options().dtype(store));
         Tensor gw = at::empty({C}, w.options());
         Tensor gphi = at::empty({np, n * C}, f32);
         Tensor galpha = at::empty({3}, f32);
         Tensor gb = at::empty({np}, f32);
-        const int xd = dtype_code(x.scalar_type());
-        const size_t wsb = lib.mhc_layer_dynamic_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
-        Tensor ws = workspace(wsb, x);
-        check(lib.mhc_layer_dynamic_bwd(fp(g), x.data_ptr(), xd, dtype_code(w.scalar_type()), fp(sv[3]), fp(sv[4]),
-                                        fp(sv[5]), fp(sv[6]), fp(sv[7]), fp(sv[8]), fp(sv[9]), fp(sv[10]),
-                                        fp(sv[11]), fp(saved), grad_x.data_ptr(), gw.data_ptr(), fp(gphi),
-                                        fp(galpha), fp(gb), ws.data_ptr(), wsb, B, (int32_t)n, (int32_t)C,
-                                        (int32_t)cfg[0], (float)cfg[1], (float)cfg[2], stream()),
-              fn);
+        const int xd = dtype_code(store);
+        if (is_held) {
+            const size_t wsb = lib.mhc_layer_dynamic_checkpoint_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
+            Tensor ws = workspace(wsb, x);
+            check(lib.mhc_layer_dynamic_checkpoint_bwd(
+                      fp(g), x.data_ptr(), sv[12].data_ptr(), (int32_t)fmt, xd, dtype_code(w.scalar_type()), fp(sv[3]),
+                      fp(sv[4]), fp(sv[5]), fp(sv[6]), fp(sv[7]), fp(sv[8]), fp(sv[9]), fp(sv[10]), fp(sv[11]),
+                      fp(saved), grad_x.data_ptr(), gw.data_ptr(), fp(gphi), fp(galpha), fp(gb), ws.data_ptr(), wsb, B,
+                      (int32_t)n, (int32_t)C, (int32_t)cfg[0], (float)cfg[1], (float)cfg[2], stream()),
+                  "mhc_layer_dynamic_checkpoint_bwd");
+        } else {
+            const size_t wsb = lib.mhc_layer_dynamic_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
+            Tensor ws = workspace(wsb, x);
+            check(lib.mhc_layer_dynamic_bwd(fp(g), x.data_ptr(), xd, dtype_code(w.scalar_type()), fp(sv[3]),
+                                            fp(sv[4]), fp(sv[5]), fp(sv[6]), fp(sv[7]), fp(sv[8]), fp(sv[9]),
+                                            fp(sv[10]), fp(sv[11]), fp(saved), grad_x.data_ptr(), gw.data_ptr(),
+                                            fp(gphi), fp(galpha), fp(gb), ws.data_ptr(), wsb, B, (int32_t)n,
+                                            (int32_t)C, (int32_t)cfg[0], (float)cfg[1], (float)cfg[2], stream()),
+                  fn);
+        }
         const auto x_dtype = (at::ScalarType)ctx->saved_data["x_dtype"].toInt();
         tensor_list out;
-        out.reserve(14);
+        out.reserve(15);
         out.push_back(grad_x.to(x_dtype));
         out.push_back(gw);
         push_param_grads(out,
                          {sv[3].sizes(), sv[4].sizes(), sv[5].sizes(), sv[6].sizes(), sv[7].sizes(), sv[8].sizes(),
                           sv[9].sizes(), sv[10].sizes(), sv[11].sizes()},
                          n, gphi, galpha, gb);
-        out.resize(14);
+        out.resize(15);
         return out;
     }
 };
@@ -340,10 +459,36 @@ int32_t wrapper_mode(const std::string& mode, int64_t n, const char* fn) {
     return mode == "decay" ? MHC_WRAPPER_DECAY : MHC_WRAPPER_ZERO;
 }
 
+// The wrapper's saved list: its two rows, `rest`, and with a checkpoint the
+// rows' scales behind them.
+void save_wrapper_rows(AutogradContext* ctx, int64_t fmt, const Tensor& r, const Tensor& b, tensor_list rest) {
+    tensor_list sv = {r, b};
+    ctx->saved_data["fmt"] = fmt;
+    if (fmt != MHC_CHECKPOINT_NONE) {
+        const Held hr = hold(r, fmt), hb = hold(b, fmt);
+        sv = {hr.values, hb.values};
+        rest.push_back(hr.scales);
+        rest.push_back(hb.scales);
+        ctx->saved_data["sizes"] = r.sizes().vec();
+        ctx->saved_data["store"] = (int64_t)r.scalar_type();
+    }
+    sv.insert(sv.end(), rest.begin(), rest.end());
+    ctx->save_for_backward(std::move(sv));
+}
+
+std::pair<Tensor, Tensor> wrapper_rows(AutogradContext* ctx, const tensor_list& sv) {
+    const int64_t fmt = ctx->saved_data["fmt"].toInt();
+    if (fmt == MHC_CHECKPOINT_NONE) return {sv[0], sv[1]};
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    const auto store = (at::ScalarType)ctx->saved_data["store"].toInt();
+    return {held_rows(sv[0], sv[sv.size() - 2], fmt, sizes, store),
+            held_rows(sv[1], sv[sv.size() - 1], fmt, sizes, store)};
+}
+
 struct StaticWrapper : public torch::autograd::Function<StaticWrapper> {
     static Tensor forward(AutogradContext* ctx, const Tensor& res_in, const Tensor& br_in, const Tensor& w_in,
                           const Tensor& hp_in, const Tensor& hq_in, const Tensor& hr_in, int64_t mode, int64_t n,
-                          int64_t iters, double sk_eps, double rms_eps) {
+                          int64_t iters, double sk_eps, double rms_eps, int64_t fmt) {
         const char* fn = "wrapper_static_fwd";
         auto [r, b] = wrapper_inputs(fn, res_in, br_in);
         check_device(fn, {&r, &w_in, &hp_in, &hq_in, &hr_in});
@@ -361,7 +506,7 @@ struct StaticWrapper : public torch::autograd::Function<StaticWrapper> {
                                          fp(saved), T, (int32_t)n, (int32_t)C, (int32_t)iters, (float)sk_eps,
                                          (float)rms_eps, stream()),
               "mhc_wrapper_static_fwd");
-        ctx->save_for_backward({r, b, w, hp, hq, hr, saved});
+        save_wrapper_rows(ctx, fmt, r, b, {w, hp, hq, hr, saved});
         ctx->saved_data["dtypes"] = std::vector<int64_t>{(int64_t)res_in.scalar_type(), (int64_t)br_in.scalar_type()};
         ctx->saved_data["cfg"] = std::vector<double>{(double)mode, (double)n, (double)iters, sk_eps, rms_eps};
         return out;
@@ -370,9 +515,10 @@ struct StaticWrapper : public torch::autograd::Function<StaticWrapper> {
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const char* fn = "wrapper_static_bwd";
         const auto sv = ctx->get_saved_variables();
-        const Tensor &r = sv[0], &b = sv[1], &w = sv[2], &saved = sv[6];
-        check_device(fn, {&grads[0], &r});
-        const at::DeviceGuard guard(r.device());
+        check_device(fn, {&grads[0], &sv[0]});
+        const at::DeviceGuard guard(sv[0].device());
+        const auto [r, b] = wrapper_rows(ctx, sv);
+        const Tensor &w = sv[2], &saved = sv[6];
         const auto cfg = ctx->saved_data["cfg"].toDoubleVector();
         const int64_t T = r.size(0), C = r.size(1), n = (int64_t)cfg[1];
         const int32_t mode = (int32_t)cfg[0];
@@ -393,7 +539,7 @@ struct StaticWrapper : public torch::autograd::Function<StaticWrapper> {
               "mhc_wrapper_static_bwd");
         const auto dts = ctx->saved_data["dtypes"].toIntVector();
         return {gr.to((at::ScalarType)dts[0]), gb.to((at::ScalarType)dts[1]), gw, ghp, ghq, ghr, Tensor(), Tensor(),
-                Tensor(), Tensor(), Tensor()};
+                Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -402,7 +548,7 @@ struct DynamicWrapper : public torch::autograd::Function<DynamicWrapper> {
                           const Tensor& pp_in, const Tensor& pq_in, const Tensor& pr_in, const Tensor& ap_in,
                           const Tensor& aq_in, const Tensor& ar_in, const Tensor& bp_in, const Tensor& bq_in,
                           const Tensor& bres_in, int64_t mode, int64_t n, int64_t iters, double sk_eps,
-                          double rms_eps) {
+                          double rms_eps, int64_t fmt) {
         const char* fn = "wrapper_dynamic_fwd";
         auto [r, b] = wrapper_inputs(fn, res_in, br_in);
         check_device(fn, {&r, &w_in, &pp_in, &pq_in, &pr_in, &bp_in, &bq_in, &bres_in});
@@ -427,7 +573,7 @@ struct DynamicWrapper : public torch::autograd::Function<DynamicWrapper> {
                                           ws.data_ptr(), wsb, T, (int32_t)n, (int32_t)C, (int32_t)iters,
                                           (float)sk_eps, (float)rms_eps, stream()),
               "mhc_wrapper_dynamic_fwd");
-        ctx->save_for_backward({r, b, w, saved, ph[0], ph[1], ph[2], ap, aq, ar, bres});
+        save_wrapper_rows(ctx, fmt, r, b, {w, saved, ph[0], ph[1], ph[2], ap, aq, ar, bres});
         // b_pre and b_post are not read by the backward: their shapes only
         ctx->saved_data["b_pre"] = bp.sizes().vec();
         ctx->saved_data["b_post"] = bq.sizes().vec();
@@ -439,9 +585,10 @@ struct DynamicWrapper : public torch::autograd::Function<DynamicWrapper> {
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const char* fn = "wrapper_dynamic_bwd";
         const auto sv = ctx->get_saved_variables();
-        const Tensor &r = sv[0], &b = sv[1], &w = sv[2], &saved = sv[3];
-        check_device(fn, {&grads[0], &r});
-        const at::DeviceGuard guard(r.device());
+        check_device(fn, {&grads[0], &sv[0]});
+        const at::DeviceGuard guard(sv[0].device());
+        const auto [r, b] = wrapper_rows(ctx, sv);
+        const Tensor &w = sv[2], &saved = sv[3];
         const auto cfg = ctx->saved_data["cfg"].toDoubleVector();
         const int64_t T = r.size(0), C = r.size(1), n = (int64_t)cfg[1], np = 2 * n + n * n;
         const int32_t mode = (int32_t)cfg[0];
@@ -466,7 +613,7 @@ struct DynamicWrapper : public torch::autograd::Function<DynamicWrapper> {
               "mhc_wrapper_dynamic_bwd");
         const auto dts = ctx->saved_data["dtypes"].toIntVector();
         tensor_list out;
-        out.reserve(17);
+        out.reserve(18);
         out.push_back(gr.to((at::ScalarType)dts[0]));
         out.push_back(gb.to((at::ScalarType)dts[1]));
         out.push_back(gw);
@@ -475,7 +622,7 @@ struct DynamicWrapper : public torch::autograd::Function<DynamicWrapper> {
                          {sv[4].sizes(), sv[5].sizes(), sv[6].sizes(), sv[7].sizes(), sv[8].sizes(), sv[9].sizes(), bp,
                           bq, sv[10].sizes()},
                          n, gphi, galpha, gbias);
-        out.resize(17);
+        out.resize(18);
         return out;
     }
 };
@@ -604,8 +751,56 @@ struct RmsNorm : public torch::autograd::Function<RmsNorm> {
     }
 };
 
+// RMSNorm whose backward reads an 8-bit checkpoint of its input's rows.
+struct RmsNormHeld : public torch::autograd::Function<RmsNormHeld> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& inp, const Tensor& w_in, double eps, int64_t fmt) {
+        check_device("rmsnorm_fwd", {&inp, &w_in});
+        const at::DeviceGuard guard(inp.device());
+        TORCH_CHECK(inp.dim() == 2, "Input must be 2D tensor [B, C]");
+        const Tensor x = storage(inp);
+        const int64_t B = x.size(0), C = x.size(1);
+        TORCH_CHECK(w_in.numel() == C, "weight must have C elements");
+        const Tensor w = f32c(w_in);
+        Tensor out = at::empty_like(x);
+        const Held held = held_alloc(x);
+        check(lib.mhc_rmsnorm_checkpoint_fwd(x.data_ptr(), dtype_code(x.scalar_type()), fp(w), out.data_ptr(),
+                                             (int32_t)fmt, held.values.data_ptr(), held.scales.data_ptr(), B,
+                                             (int32_t)C, (float)eps, stream()),
+              "mhc_rmsnorm_checkpoint_fwd");
+        ctx->save_for_backward({held.values, held.scales, w_in});
+        ctx->saved_data["x_dtype"] = (int64_t)inp.scalar_type();
+        ctx->saved_data["store"] = (int64_t)x.scalar_type();
+        ctx->saved_data["B"] = B;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["fmt"] = fmt;
+        return out;
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        const auto sv = ctx->get_saved_variables();
+        const Tensor &values = sv[0], &scales = sv[1], &w_in = sv[2];
+        check_device("rmsnorm_bwd", {&grads[0], &values, &w_in});
+        const at::DeviceGuard guard(values.device());
+        const auto store = (at::ScalarType)ctx->saved_data["store"].toInt();
+        const int64_t B = ctx->saved_data["B"].toInt(), C = w_in.numel(), fmt = ctx->saved_data["fmt"].toInt();
+        const Tensor g = grads[0].to(store).contiguous();
+        TORCH_CHECK(g.dim() == 2 && g.size(0) == B && g.size(1) == C, "grad_out shape must match inp");
+        const Tensor w = f32c(w_in);
+        Tensor gx = at::empty({B, C}, g.options());
+        Tensor gw = at::empty({C}, g.options().dtype(at::kFloat));
+        const int dt = dtype_code(store);
+        const size_t wsb = lib.mhc_rmsnorm_checkpoint_bwd_workspace_size(B, (int32_t)C, dt, (int32_t)fmt);
+        Tensor ws = workspace(wsb, g);
+        check(lib.mhc_rmsnorm_checkpoint_bwd(g.data_ptr(), dt, values.data_ptr(), scales.data_ptr(), (int32_t)fmt,
+                                             fp(w), gx.data_ptr(), fp(gw), ws.data_ptr(), wsb, B, (int32_t)C,
+                                             (float)ctx->saved_data["eps"].toDouble(), stream()),
+              "mhc_rmsnorm_checkpoint_bwd");
+        return {gx.to((at::ScalarType)ctx->saved_data["x_dtype"].toInt()), gw, Tensor(), Tensor()};
+    }
+};
+
 struct Aggregate : public torch::autograd::Function<Aggregate> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& inp, const Tensor& h_in) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& inp, const Tensor& h_in, int64_t fmt) {
         const char* fn = "stream_aggregate_fwd";
         check_device(fn, {&inp, &h_in});
         const at::DeviceGuard guard(inp.device());
@@ -618,6 +813,15 @@ struct Aggregate : public torch::autograd::Function<Aggregate> {
         check(lib.mhc_stream_aggregate_fwd(x.data_ptr(), dtype_code(x.scalar_type()), fp(h), hs, out.data_ptr(),
                                            fp(act), B, (int32_t)n, (int32_t)C, stream()),
               "mhc_stream_aggregate_fwd");
+        ctx->saved_data["fmt"] = fmt;
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            const Held held = hold(x, fmt);
+            ctx->saved_data["sizes"] = x.sizes().vec();
+            ctx->saved_data["store"] = (int64_t)x.scalar_type();
+            ctx->saved_data["x_dtype"] = (int64_t)inp.scalar_type();
+            ctx->save_for_backward({held.values, act, held.scales});
+            return out;
+        }
         ctx->save_for_backward({inp, act});
         return out;
     }
@@ -627,7 +831,12 @@ struct Aggregate : public torch::autograd::Function<Aggregate> {
         const Tensor &inp = sv[0], &act = sv[1];
         check_device("stream_aggregate_bwd", {&grads[0], &inp, &act});
         const at::DeviceGuard guard(inp.device());
-        const Tensor x = storage(inp);
+        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const bool is_held = fmt != MHC_CHECKPOINT_NONE;
+        const Tensor x = is_held ? held_rows(inp, sv[2], fmt, ctx->saved_data["sizes"].toIntVector(),
+                                             (at::ScalarType)ctx->saved_data["store"].toInt())
+                                 : storage(inp);
+        const auto x_dtype = is_held ? (at::ScalarType)ctx->saved_data["x_dtype"].toInt() : inp.scalar_type();
         const int64_t B = x.size(0), n = x.size(1), C = x.size(2);
         const Tensor g = grads[0].to(x.scalar_type()).contiguous();
         TORCH_CHECK(g.dim() == 2 && g.size(0) == B && g.size(1) == C, "grad_out must be [B, C]");
@@ -636,13 +845,13 @@ struct Aggregate : public torch::autograd::Function<Aggregate> {
         check(lib.mhc_stream_aggregate_bwd(g.data_ptr(), x.data_ptr(), dtype_code(x.scalar_type()), fp(act), n,
                                            gx.data_ptr(), nullptr, fp(graw), B, (int32_t)n, (int32_t)C, stream()),
               "mhc_stream_aggregate_bwd");
-        return {gx.to(inp.scalar_type()), graw};
+        return {gx.to(x_dtype), graw, Tensor()};
     }
 };
 
 struct Distribute : public torch::autograd::Function<Distribute> {
     static Tensor forward(AutogradContext* ctx, const Tensor& y_in, const Tensor& h_in, const Tensor& m_in,
-                          const Tensor& x_in) {
+                          const Tensor& x_in, int64_t fmt) {
         const char* fn = "stream_distribute_mix_add_fwd";
         check_device(fn, {&y_in, &h_in, &m_in, &x_in});
         const at::DeviceGuard guard(x_in.device());
@@ -660,6 +869,15 @@ struct Distribute : public torch::autograd::Function<Distribute> {
                                                     dtype_code(x.scalar_type()), fp(out), fp(act), B, (int32_t)n,
                                                     (int32_t)C, stream()),
               "mhc_stream_distribute_mix_add_fwd");
+        ctx->saved_data["fmt"] = fmt;
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            const Held hx = hold(x, fmt), hy = hold(y, fmt);
+            ctx->saved_data["sizes"] = x.sizes().vec();
+            ctx->saved_data["store"] = (int64_t)x.scalar_type();
+            ctx->saved_data["dtypes"] = std::vector<int64_t>{(int64_t)x_in.scalar_type(), (int64_t)y_in.scalar_type()};
+            ctx->save_for_backward({hx.values, hy.values, m_in, act, hx.scales, hy.scales});
+            return out;
+        }
         ctx->save_for_backward({x_in, y_in, m_in, act});
         return out;
     }
@@ -670,9 +888,22 @@ struct Distribute : public torch::autograd::Function<Distribute> {
         const Tensor &x_in = sv[0], &y_in = sv[1], &m_in = sv[2], &act = sv[3];
         check_device(fn, {&grads[0], &x_in, &y_in, &m_in, &act});
         const at::DeviceGuard guard(x_in.device());
-        const Tensor x = storage(x_in);
+        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        Tensor x, y;
+        at::ScalarType x_dtype = x_in.scalar_type(), y_dtype = y_in.scalar_type();
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            const auto sizes = ctx->saved_data["sizes"].toIntVector();
+            const auto store = (at::ScalarType)ctx->saved_data["store"].toInt();
+            const auto dts = ctx->saved_data["dtypes"].toIntVector();
+            x = held_rows(x_in, sv[4], fmt, sizes, store);
+            y = held_rows(y_in, sv[5], fmt, {sizes[0], sizes[2]}, store);
+            x_dtype = (at::ScalarType)dts[0];
+            y_dtype = (at::ScalarType)dts[1];
+        } else {
+            x = storage(x_in);
+            y = y_in.to(x.scalar_type()).contiguous();
+        }
         const int64_t B = x.size(0), n = x.size(1), C = x.size(2);
-        const Tensor y = y_in.to(x.scalar_type()).contiguous();
         const Tensor g = f32c(grads[0]);
         TORCH_CHECK(g.sizes() == x.sizes(), "grad_out shape must match x_inp");
         const auto [m, ms] = coef_view(fn, m_in, B, n * n);
@@ -683,7 +914,111 @@ struct Distribute : public torch::autograd::Function<Distribute> {
                                                     fp(m), ms, fp(act), n, gx.data_ptr(), gy.data_ptr(), fp(gm),
                                                     nullptr, fp(graw), B, (int32_t)n, (int32_t)C, stream()),
               "mhc_stream_distribute_mix_add_bwd");
-        return {gy.to(y_in.scalar_type()), graw, gm, gx.to(x_in.scalar_type())};
+        return {gy.to(y_dtype), graw, gm, gx.to(x_dtype), Tensor()};
+    }
+};
+
+// ---- per-head norm of queries and keys, with the rotation of positions ----------
+// What the entries take besides rows: weights in one dtype, fp32 tables.
+struct QkTables {
+    Tensor wq, wk, cos, sin, pos;
+    int64_t period;
+
+    QkTables(const Tensor& wq_in, const Tensor& wk_in, const Tensor& cos_in, const Tensor& sin_in,
+             const Tensor& pos_in, int64_t period_in)
+        : cos(f32c(cos_in)), sin(f32c(sin_in)), pos(pos_in), period(period_in) {
+        const bool one = wq_in.scalar_type() == wk_in.scalar_type() && storage_dtype(wq_in.scalar_type());
+        wq = one ? wq_in.contiguous() : f32c(wq_in);
+        wk = one ? wk_in.contiguous() : f32c(wk_in);
+    }
+    int w_dtype() const { return dtype_code(wq.scalar_type()); }
+    const void* pos_ptr() const { return pos.defined() ? pos.data_ptr() : nullptr; }
+    int32_t pos_bytes() const { return pos.defined() ? (int32_t)pos.element_size() : 0; }
+};
+
+// Rows as the kernels read them: storage dtype, channels next to each other.
+Tensor qk_rows(const Tensor& t, at::ScalarType dt) {
+    const Tensor s = t.to(dt);
+    return s.stride(2) == 1 || s.size(2) == 1 ? s : s.contiguous();
+}
+
+struct QkNormRope : public torch::autograd::Function<QkNormRope> {
+    static tensor_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& wq_in,
+                               const Tensor& wk_in, const Tensor& cos, const Tensor& sin,
+                               const c10::optional<Tensor>& positions, int64_t period, double eps, bool interleaved,
+                               int64_t fmt) {
+        const char* fn = "qk_norm_rope_fwd";
+        const at::DeviceGuard guard(q_in.device());
+        const auto dt = storage_dtype(q_in.scalar_type()) ? q_in.scalar_type() : at::kFloat;
+        const Tensor q = qk_rows(q_in, dt), k = qk_rows(k_in, dt);
+        const QkTables t(wq_in, wk_in, cos, sin, positions.has_value() ? positions->contiguous() : Tensor(), period);
+        const int64_t T = q.size(0), H = q.size(1), K = k.size(1), D = q.size(2);
+        Tensor qo = at::empty({T, H, D}, q.options()), ko = at::empty({T, K, D}, k.options());
+        Held hq, hk;
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            hq = held_alloc(q);
+            hk = held_alloc(k);
+        }
+        const auto held = [&](const Tensor& h) { return h.defined() ? h.data_ptr() : nullptr; };
+        check(lib.mhc_qk_norm_rope_fwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                                       dtype_code(dt), t.wq.data_ptr(), t.wk.data_ptr(), t.w_dtype(), fp(t.cos),
+                                       fp(t.sin), t.cos.size(0), t.pos_ptr(), t.pos_bytes(), t.period, qo.data_ptr(),
+                                       ko.data_ptr(), (int32_t)fmt, held(hq.values), held(hq.scales),
+                                       held(hk.values), held(hk.scales), T, (int32_t)H, (int32_t)K, (int32_t)D,
+                                       (int32_t)(2 * t.cos.size(1)), interleaved, (float)eps, stream()),
+              fn);
+        tensor_list sv = {t.wq, t.wk, t.cos, t.sin};
+        if (fmt != MHC_CHECKPOINT_NONE) {
+            sv.insert(sv.end(), {hq.values, hk.values, hq.scales, hk.scales});
+        } else {
+            sv.insert(sv.end(), {q, k});
+        }
+        if (t.pos.defined()) sv.push_back(t.pos);
+        ctx->save_for_backward(std::move(sv));
+        ctx->saved_data["ints"] = std::vector<int64_t>{T, H, K, D, t.period, interleaved, fmt, t.pos.defined(),
+                                                       (int64_t)dt, (int64_t)q_in.scalar_type(),
+                                                       (int64_t)k_in.scalar_type(), (int64_t)wq_in.scalar_type(),
+                                                       (int64_t)wk_in.scalar_type()};
+        ctx->saved_data["eps"] = eps;
+        return {qo, ko};
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        const char* fn = "qk_norm_rope_bwd";
+        const auto sv = ctx->get_saved_variables();
+        const auto v = ctx->saved_data["ints"].toIntVector();
+        const int64_t T = v[0], H = v[1], K = v[2], D = v[3], fmt = v[6];
+        const bool is_held = fmt != MHC_CHECKPOINT_NONE;
+        const auto dt = (at::ScalarType)v[8];
+        check_device(fn, {&grads[0], &grads[1], &sv[0]});
+        const at::DeviceGuard guard(sv[0].device());
+        const QkTables t(sv[0], sv[1], sv[2], sv[3], v[7] ? sv.back() : Tensor(), v[4]);
+        const Tensor gq = qk_rows(grads[0], dt), gk = qk_rows(grads[1], dt);
+        TORCH_CHECK(gq.sizes() == at::IntArrayRef({T, H, D}) && gk.sizes() == at::IntArrayRef({T, K, D}), fn,
+                    ": the cotangents must match the outputs");
+        Tensor dq = at::empty({T, H, D}, gq.options()), dk = at::empty({T, K, D}, gk.options());
+        Tensor dw = at::empty({2, D}, t.wq.options());
+        const size_t wsb = lib.mhc_qk_norm_rope_bwd_workspace_size(T, (int32_t)H, (int32_t)K, (int32_t)D,
+                                                                   dtype_code(dt), (int32_t)fmt);
+        Tensor ws = workspace(wsb, dq);
+        const Tensor none;
+        const Tensor &q = is_held ? none : sv[4], &k = is_held ? none : sv[5];
+        const auto at_ptr = [](const Tensor& h) { return h.defined() ? h.data_ptr() : nullptr; };
+        const auto st = [](const Tensor& h, int d) { return h.defined() ? h.stride(d) : (int64_t)0; };
+        check(lib.mhc_qk_norm_rope_bwd(
+                  gq.data_ptr(), gq.stride(0), gq.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1), at_ptr(q),
+                  st(q, 0), st(q, 1), at_ptr(k), st(k, 0), st(k, 1), dtype_code(dt), (int32_t)fmt,
+                  is_held ? sv[4].data_ptr() : nullptr, is_held ? sv[6].data_ptr() : nullptr,
+                  is_held ? sv[5].data_ptr() : nullptr, is_held ? sv[7].data_ptr() : nullptr, t.wq.data_ptr(),
+                  t.wk.data_ptr(), t.w_dtype(), fp(t.cos), fp(t.sin), t.cos.size(0), t.pos_ptr(), t.pos_bytes(),
+                  t.period, dq.data_ptr(), dk.data_ptr(), dw.data_ptr(), ws.data_ptr(), wsb, T, (int32_t)H, (int32_t)K,
+                  (int32_t)D, (int32_t)(2 * t.cos.size(1)), (int32_t)v[5],
+                  (float)ctx->saved_data["eps"].toDouble(), stream()),
+              fn);
+        tensor_list out = {dq.to((at::ScalarType)v[9]), dk.to((at::ScalarType)v[10]),
+                           dw.select(0, 0).to((at::ScalarType)v[11]), dw.select(0, 1).to((at::ScalarType)v[12])};
+        out.resize(11);
+        return out;
     }
 };
 
@@ -692,77 +1027,134 @@ Tensor sinkhorn_knopp(const Tensor& inp, int64_t iters, double eps) {
     return Sinkhorn::apply(inp, iters, eps);
 }
 
-Tensor rmsnorm(const Tensor& inp, const Tensor& w, double eps) {
+Tensor rmsnorm(const Tensor& inp, const Tensor& w, double eps, int64_t checkpoint) {
     require_bound();
-    return RmsNorm::apply(inp, w, eps);
+    const int64_t fmt = format_for(checkpoint, {&inp, &w});
+    return fmt == MHC_CHECKPOINT_NONE ? RmsNorm::apply(inp, w, eps) : RmsNormHeld::apply(inp, w, eps, fmt);
 }
 
-Tensor stream_aggregate(const Tensor& inp, const Tensor& h) {
+Tensor stream_aggregate(const Tensor& inp, const Tensor& h, int64_t checkpoint) {
     require_bound();
-    return Aggregate::apply(inp, h);
+    return Aggregate::apply(inp, h, format_for(checkpoint, {&inp, &h}));
 }
 
-Tensor stream_distribute_mix_add(const Tensor& y, const Tensor& h, const Tensor& m, const Tensor& x) {
+Tensor stream_distribute_mix_add(const Tensor& y, const Tensor& h, const Tensor& m, const Tensor& x,
+                                 int64_t checkpoint) {
     require_bound();
-    return Distribute::apply(y, h, m, x);
+    return Distribute::apply(y, h, m, x, format_for(checkpoint, {&y, &h, &m, &x}));
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk,
+                                        const Tensor& cos, const Tensor& sin, const c10::optional<Tensor>& positions,
+                                        int64_t period, double eps, bool interleaved, int64_t checkpoint) {
+    require_bound();
+    const char* fn = "qk_norm_rope";
+    check_device(fn, {&q, &k, &wq, &wk, &cos, &sin});
+    if (positions.has_value()) check_device(fn, {&q, &*positions});
+    TORCH_CHECK(q.dim() == 3 && k.dim() == 3, fn, ": q and k must be [tokens, heads, head_dim]");
+    TORCH_CHECK(q.size(0) == k.size(0) && q.size(2) == k.size(2), fn,
+                ": q and k must have the same tokens and head_dim, got ", q.sizes(), " and ", k.sizes());
+    TORCH_CHECK(q.scalar_type() == k.scalar_type() && at::isFloatingType(q.scalar_type()), fn,
+                ": q and k must have one floating dtype, got ", q.scalar_type(), " and ", k.scalar_type());
+    TORCH_CHECK(wq.numel() == q.size(2) && wk.numel() == q.size(2) && wq.dim() == 1 && wk.dim() == 1, fn,
+                ": the weights must be [head_dim]");
+    TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), fn, ": cos and sin must be [positions, rotary_dim / 2]");
+    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), fn, ": cos and sin get no gradient");
+    if (positions.has_value()) {
+        const auto pt = positions->scalar_type();
+        TORCH_CHECK(pt == at::kLong || pt == at::kInt, fn, ": positions must be int64 or int32, got ", pt);
+        TORCH_CHECK(positions->numel() == period, fn, ": positions must have one entry a token");
+    }
+    // an outer loop over tokens of the same positions is whole
+    TORCH_CHECK(q.size(0) == 0 || (period > 0 && q.size(0) % period == 0), fn, ": ", q.size(0),
+                " tokens do not repeat ", period, " positions");
+    const tensor_list out = QkNormRope::apply(q, k, wq, wk, cos, sin, positions, std::max<int64_t>(period, 1), eps,
+                                              interleaved, format_for(checkpoint, {&q, &k, &wq, &wk}));
+    return {out[0], out[1]};
 }
 
 Tensor static_layer(const Tensor& x, const Tensor& w, const Tensor& hp, const Tensor& hq, const Tensor& hr,
-                    int64_t iters, double sk_eps, double rms_eps) {
+                    int64_t iters, double sk_eps, double rms_eps, int64_t checkpoint) {
     require_bound();
-    return StaticLayer::apply(x, w, hp, hq, hr, iters, sk_eps, rms_eps);
+    return StaticLayer::apply(x, w, hp, hq, hr, iters, sk_eps, rms_eps,
+                              format_for(checkpoint, {&x, &w, &hp, &hq, &hr}));
 }
 
 Tensor dynamic_layer(const Tensor& x, const Tensor& w, const Tensor& pp, const Tensor& pq, const Tensor& pr,
                      const Tensor& ap, const Tensor& aq, const Tensor& ar, const Tensor& bp, const Tensor& bq,
-                     const Tensor& br, int64_t iters, double sk_eps, double rms_eps) {
+                     const Tensor& br, int64_t iters, double sk_eps, double rms_eps, int64_t checkpoint) {
     require_bound();
-    return DynamicLayer::apply(x, w, pp, pq, pr, ap, aq, ar, bp, bq, br, iters, sk_eps, rms_eps);
+    return DynamicLayer::apply(x, w, pp, pq, pr, ap, aq, ar, bp, bq, br, iters, sk_eps, rms_eps,
+                               format_for(checkpoint, {&x, &w, &pp, &pq, &pr, &ap, &aq, &ar, &bp, &bq, &br}));
 }
 
 Tensor static_wrapper(const Tensor& residual, const Tensor& branch, const Tensor& w, const Tensor& hp,
                       const Tensor& hq, const Tensor& hr, const std::string& mode, int64_t n, int64_t iters,
-                      double sk_eps, double rms_eps) {
+                      double sk_eps, double rms_eps, int64_t checkpoint) {
     require_bound();
     const int32_t m = wrapper_mode(mode, n, "wrapper_static_fwd");
-    return StaticWrapper::apply(residual, branch, w, hp, hq, hr, (int64_t)m, n, iters, sk_eps, rms_eps);
+    return StaticWrapper::apply(residual, branch, w, hp, hq, hr, (int64_t)m, n, iters, sk_eps, rms_eps,
+                                format_for(checkpoint, {&residual, &branch, &w, &hp, &hq, &hr}));
 }
 
 Tensor dynamic_wrapper(const Tensor& residual, const Tensor& branch, const Tensor& w, const Tensor& pp,
                        const Tensor& pq, const Tensor& pr, const Tensor& ap, const Tensor& aq, const Tensor& ar,
                        const Tensor& bp, const Tensor& bq, const Tensor& bres, const std::string& mode, int64_t n,
-                       int64_t iters, double sk_eps, double rms_eps) {
+                       int64_t iters, double sk_eps, double rms_eps, int64_t checkpoint) {
     require_bound();
     const int32_t m = wrapper_mode(mode, n, "wrapper_dynamic_fwd");
     return DynamicWrapper::apply(residual, branch, w, pp, pq, pr, ap, aq, ar, bp, bq, bres, (int64_t)m, n, iters,
-                                 sk_eps, rms_eps);
+                                 sk_eps, rms_eps,
+                                 format_for(checkpoint, {&residual, &branch, &w, &pp, &pq, &pr, &ap, &aq, &ar, &bp,
+                                                         &bq, &bres}));
 }
 
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    namespace py = pybind11;
     m.doc() = "C++ autograd nodes of the fused mHC layers and the standalone operators over libmhc_hip's C ABI";
     m.def("entry_names", &entry_names, "C-ABI entry points bind() needs");
     m.def("bind", &bind, "set the C-ABI entry points from {name: address}");
     m.def("static_layer", &static_layer,
           "static-H layer with autograd: (x, weight, H_pre, H_post, H_res, num_iters, sinkhorn_eps, "
-          "rmsnorm_eps) -> fp32 [B, n, C]");
+          "rmsnorm_eps) -> fp32 [B, n, C]",
+          py::arg("x"), py::arg("weight"), py::arg("H_pre"), py::arg("H_post"), py::arg("H_res"), py::arg("num_iters"),
+          py::arg("sinkhorn_eps"), py::arg("rmsnorm_eps"), py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
     m.def("dynamic_layer", &dynamic_layer,
           "dynamic-H layer with autograd: (x, weight, phi_pre, phi_post, phi_res, alpha_pre, alpha_post, "
-          "alpha_res, b_pre, b_post, b_res, num_iters, sinkhorn_eps, rmsnorm_eps) -> fp32 [B, n, C]");
+          "alpha_res, b_pre, b_post, b_res, num_iters, sinkhorn_eps, rmsnorm_eps) -> fp32 [B, n, C]",
+          py::arg("x"), py::arg("weight"), py::arg("phi_pre"), py::arg("phi_post"), py::arg("phi_res"),
+          py::arg("alpha_pre"), py::arg("alpha_post"), py::arg("alpha_res"), py::arg("b_pre"), py::arg("b_post"),
+          py::arg("b_res"), py::arg("num_iters"), py::arg("sinkhorn_eps"), py::arg("rmsnorm_eps"),
+          py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
     m.def("static_wrapper", &static_wrapper,
           "fused static-H MHCResidualWrapper with autograd: (residual, branch, weight, H_pre, H_post, H_res, "
-          "residual_mode, n, num_iters, sinkhorn_eps, rmsnorm_eps) -> fp32 [tokens, C]");
+          "residual_mode, n, num_iters, sinkhorn_eps, rmsnorm_eps) -> fp32 [tokens, C]",
+          py::arg("residual"), py::arg("branch"), py::arg("weight"), py::arg("H_pre"), py::arg("H_post"),
+          py::arg("H_res"), py::arg("residual_mode"), py::arg("n"), py::arg("num_iters"), py::arg("sinkhorn_eps"),
+          py::arg("rmsnorm_eps"), py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
     m.def("dynamic_wrapper", &dynamic_wrapper,
           "fused dynamic-H MHCResidualWrapper with autograd: (residual, branch, weight, phi_pre, phi_post, phi_res, "
           "alpha_pre, alpha_post, alpha_res, b_pre, b_post, b_res, residual_mode, n, num_iters, sinkhorn_eps, "
-          "rmsnorm_eps) -> fp32 [tokens, C]");
+          "rmsnorm_eps) -> fp32 [tokens, C]",
+          py::arg("residual"), py::arg("branch"), py::arg("weight"), py::arg("phi_pre"), py::arg("phi_post"),
+          py::arg("phi_res"), py::arg("alpha_pre"), py::arg("alpha_post"), py::arg("alpha_res"), py::arg("b_pre"),
+          py::arg("b_post"), py::arg("b_res"), py::arg("residual_mode"), py::arg("n"), py::arg("num_iters"),
+          py::arg("sinkhorn_eps"), py::arg("rmsnorm_eps"), py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
     m.def("dynamic_infer", &dynamic_infer,
           "forward-only dynamic-H layer: (x, packed, alpha_pre, alpha_post, alpha_res, b_pre, b_post, b_res, "
           "num_iters, sinkhorn_eps, rmsnorm_eps, out_bf16) -> [B, n, C]");
     m.def("sinkhorn_knopp", &sinkhorn_knopp, "(inp [B, n, n] fp32, num_iters, eps) with autograd");
-    m.def("rmsnorm", &rmsnorm, "(inp [B, C], weight, eps) with autograd");
-    m.def("stream_aggregate", &stream_aggregate, "(inp [B, n, C], H_pre_raw [B, n]) with autograd");
+    m.def("rmsnorm", &rmsnorm, "(inp [B, C], weight, eps) with autograd",
+          py::arg("inp"), py::arg("weight"), py::arg("eps"), py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
+    m.def("stream_aggregate", &stream_aggregate, "(inp [B, n, C], H_pre_raw [B, n]) with autograd",
+          py::arg("inp"), py::arg("H_pre_raw"), py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
     m.def("stream_distribute_mix_add", &stream_distribute_mix_add,
-          "(y_norm [B, C], H_post_raw [B, n], M [B, n, n], x_inp [B, n, C]) -> fp32 [B, n, C] with autograd");
+          "(y_norm [B, C], H_post_raw [B, n], M [B, n, n], x_inp [B, n, C]) -> fp32 [B, n, C] with autograd",
+          py::arg("y_norm"), py::arg("H_post_raw"), py::arg("M"), py::arg("x_inp"),
+          py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
+    m.def("qk_norm_rope", &qk_norm_rope,
+          "(q [T, H, D], k [T, K, D], q_weight, k_weight, cos, sin, positions or None, period, eps, interleaved, "
+          "checkpoint) -> (q, k) with autograd");
 }

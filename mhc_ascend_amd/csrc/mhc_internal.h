@@ -274,6 +274,51 @@ hipError_t launch_distribute_bwd(int dt, int n, const float* g, const void* x, c
                                  int64_t ms, const float* h_act, int64_t hs, void* gx, void* gy, float* gM,
                                  float* gh_act, float* gh_raw, int64_t B, int64_t C, hipStream_t s);
 
+// ---- ckpt.hip --------------------------------------------------------------
+// 8-bit checkpoints of rows (fmt: CkFormat of mhc_ckpt.h) and RMSNorm rows of
+// up to kCkMaxRow channels that write and read them.
+constexpr int kCkMaxRow = 16384;
+hipError_t launch_ckpt_pack(int dt, int fmt, const void* x, void* values, void* scales, int64_t rows, int64_t C,
+                            hipStream_t s);
+hipError_t launch_ckpt_unpack(int dt, int fmt, const void* values, const void* scales, void* out, int64_t rows,
+                              int64_t C, hipStream_t s);
+bool rmsnorm_ckpt_supported(int64_t C);
+hipError_t launch_rmsnorm_ckpt_fwd(int dt, int fmt, const void* x, const float* w, void* y, void* values,
+                                   void* scales, int64_t B, int64_t C, float eps, hipStream_t s);
+// partial rows of dw: dw_part[grid][C]
+int rmsnorm_ckpt_bwd_grid(int dt, int fmt, int64_t B, int64_t C);
+hipError_t launch_rmsnorm_ckpt_bwd(int dt, int fmt, const void* g, const void* values, const void* scales,
+                                   const float* w, void* gx, float* dw_part, int grid, int64_t B, int64_t C,
+                                   float eps, hipStream_t s);
+
+// ---- qk_norm_rope.hip ------------------------------------------------------
+// Head rows of queries ([0]) and keys ([1]); strides in elements.  Token t's
+// table row is entry t % period of pos (pos_bytes 4 or 8), or t % period
+// itself (pos_bytes 0).
+constexpr int kQkMaxDim = 1024;
+struct QkArgs {
+    const void* x[2];
+    int64_t x_token[2], x_head[2];
+    const void* g[2];  // the backward's cotangents
+    int64_t g_token[2], g_head[2];
+    void* y[2];  // [T, heads, D]: the forward's outputs, the backward's gradients
+    uint8_t* q[2];
+    uint8_t* sc[2];
+    const void* w[2];
+    const float* cos;
+    const float* sin;
+    const void* pos;
+    int64_t table_rows, period, T;
+    int heads[2];
+    int w_dtype, pos_bytes, D, R, interleaved;
+    float eps;
+};
+// fmt: a CkFormat, or -1 for the rows themselves
+hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t s);
+// partial rows of both weights' gradients: dw_part[grid][2 D]
+int qk_norm_rope_bwd_grid(int64_t T);
+hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, int grid, hipStream_t s);
+
 // ---- dynamic.hip -----------------------------------------------------------
 typedef uint16_t bf16_raw_t;
 // Projection outputs come in tiles of 32 rows (two 16-wide MFMA tiles).

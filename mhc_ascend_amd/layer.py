@@ -7,6 +7,8 @@ dynamic-H projections are [out, n*C] fp32 ~ N(0, 0.02), biases zero, alphas
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.nn as nn
 
@@ -19,7 +21,12 @@ class MHCLayer(nn.Module):
     Args mirror the reference: hidden_dim (C), expansion_rate (n),
     num_sinkhorn_iters, sinkhorn_eps, rmsnorm_eps, use_dynamic_h, alpha_init.
     The output is fp32 [B, n, C] for fp32 or bf16 input (layer.py:101).
+
+    ``checkpoint`` ("int8" or "e4m3"; None saves the rows as they are) keeps
+    the streams in 8 bits between forward and backward (ops.activation_pack).
     """
+
+    checkpoint: Optional[str] = None  # of modules unpickled from before it existed
 
     def __init__(
         self,
@@ -30,8 +37,11 @@ class MHCLayer(nn.Module):
         rmsnorm_eps: float = 1e-5,
         use_dynamic_h: bool = True,
         alpha_init: float = 0.01,
+        checkpoint: Optional[str] = None,
     ):
         super().__init__()
+        ops._checkpoint_code(checkpoint)
+        self.checkpoint = checkpoint
         self.hidden_dim = hidden_dim
         self.expansion_rate = expansion_rate
         self.num_sinkhorn_iters = num_sinkhorn_iters
@@ -74,9 +84,9 @@ class MHCLayer(nn.Module):
             return ops.mhc_layer_fused_dynamic_training(
                 x, self.rmsnorm_weight, self.phi_pre, self.phi_post, self.phi_res,
                 self.alpha_pre, self.alpha_post, self.alpha_res, self.b_pre, self.b_post, self.b_res,
-                self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps)
+                self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps, self.checkpoint)
         return ops.mhc_layer_static(x, self.rmsnorm_weight, self.H_pre, self.H_post, self.H_res,
-                                    self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps)
+                                    self.num_sinkhorn_iters, self.sinkhorn_eps, self.rmsnorm_eps, self.checkpoint)
 
     # ---- forward-only dynamic H ------------------------------------------
     def _pack_key(self):
@@ -125,11 +135,12 @@ def create_mhc_layer(
     rmsnorm_eps: float = 1e-5,
     use_dynamic_h: bool = True,
     alpha_init: float = 0.01,
+    checkpoint: Optional[str] = None,
 ) -> MHCLayer:
     """Factory for :class:`MHCLayer` (layer.py:186-218)."""
     return MHCLayer(hidden_dim=hidden_dim, expansion_rate=expansion_rate, num_sinkhorn_iters=num_sinkhorn_iters,
                     sinkhorn_eps=sinkhorn_eps, rmsnorm_eps=rmsnorm_eps, use_dynamic_h=use_dynamic_h,
-                    alpha_init=alpha_init)
+                    alpha_init=alpha_init, checkpoint=checkpoint)
 
 
 class MHCResidualWrapper(nn.Module):
@@ -139,7 +150,8 @@ class MHCResidualWrapper(nn.Module):
     ('decay') or zeros ('zero'), run through an :class:`MHCLayer` and
     averaged over streams; [B, T, C] inputs come back as [B, T, C] when
     T > 1 and as [B*T, C] otherwise (layer.py:319-320).  ``use_post_norm``
-    is accepted and ignored, as in the reference (layer.py:261).
+    is accepted and ignored, as in the reference (layer.py:261).  The layer's
+    ``checkpoint`` keeps residual and branch in 8 bits for the backward.
 
     For hidden % 4 == 0 and n = 2..32 it runs fused
     (ops.mhc_residual_wrapper; with dynamic H past n = 10 at Sinkhorn

@@ -17,7 +17,7 @@ PyTorch reference math, which is the contract):
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -38,6 +38,67 @@ class _NodeFunction(torch.autograd.Function):
         if "node" not in vars(cls) or torch.jit.is_tracing():
             return super().apply(*args)
         return cls.node(*args)
+
+
+# =============================================================================
+# 8-bit checkpoints of saved rows (no counterpart in the reference)
+# =============================================================================
+
+_CHECKPOINTS = {None: -1, "int8": _lib.INT8, "e4m3": _lib.E4M3}
+
+
+def _checkpoint_code(checkpoint: Optional[str]) -> int:
+    """The library's code of a ``checkpoint`` argument."""
+    try:
+        return _CHECKPOINTS[checkpoint]
+    except (KeyError, TypeError):
+        raise ValueError(f"Unknown checkpoint format: {checkpoint!r} (None, 'int8' or 'e4m3')") from None
+
+
+def _operator_checkpoint(checkpoint: Optional[str]) -> int:
+    """The same for the operators that torch.jit.trace records: it records
+    their Python functions, which save the rows as they are."""
+    code = _checkpoint_code(checkpoint)
+    if code >= 0 and torch.jit.is_tracing():
+        raise RuntimeError("checkpoint= is not recorded by torch.jit.trace")
+    return code
+
+
+class PackedActivation(NamedTuple):
+    """Rows in 8 bits, from :func:`activation_pack`.
+
+    ``values`` [..., ceil16(hidden)] uint8 are int8 or e4m3 numbers (the bytes
+    past ``hidden`` are zero), ``scales`` [..., ceil(hidden / 32)] uint8 the
+    exponents e + 127 of their blocks of 32: a value stands for q * 2**e, or
+    NaN where the byte is 255 (the block held a value that is not finite)."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+    format: str
+    hidden: int
+    dtype: torch.dtype
+
+
+def activation_pack(x: torch.Tensor, format: str = "int8") -> PackedActivation:
+    """Hold x [..., C] in 8 bits, 33/32 bytes a value (rows padded to 16).
+
+    With a = max |x| of a block of 32 and M = 127 ("int8") or 448 ("e4m3"), e
+    is the least integer with a <= M 2^e (at least -100); the block holds
+    x 2^-e rounded to nearest even.  The error is at most 2^(e-1) ("int8") or
+    max(2^-4 |x|, 2^(e-10)) ("e4m3").  No gradient flows through."""
+    if format is None:
+        raise ValueError("activation_pack: format must be 'int8' or 'e4m3'")
+    return PackedActivation(*native.checkpoint_pack(x, _checkpoint_code(format)), format, x.shape[-1],
+                            x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32)
+
+
+def activation_unpack(packed: PackedActivation, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values a :class:`PackedActivation` stands for, exactly, in ``dtype``
+    (float32 or bfloat16; the packed tensor's storage dtype by default)."""
+    if packed.format is None:
+        raise ValueError("activation_unpack: format must be 'int8' or 'e4m3'")
+    return native.checkpoint_unpack(packed.values, packed.scales, _checkpoint_code(packed.format), packed.hidden,
+                                    packed.dtype if dtype is None else dtype)
 
 
 # =============================================================================
@@ -96,8 +157,16 @@ class RMSNormFunction(_NodeFunction):
         return _lib.autograd().rmsnorm(inp, weight, float(eps))
 
 
-def rmsnorm(inp: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
-    """RMSNorm of inp [B, C]; the output keeps inp's dtype (fp32 or bf16)."""
+def rmsnorm(inp: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
+            checkpoint: Optional[str] = None) -> torch.Tensor:
+    """RMSNorm of inp [B, C]; the output keeps inp's dtype (fp32 or bf16).
+
+    ``checkpoint`` ("int8" or "e4m3", see :func:`activation_pack`) saves inp in
+    8 bits for the backward, which is then RMSNorm's gradient at the values
+    that checkpoint stands for (C <= 16384)."""
+    code = _operator_checkpoint(checkpoint)
+    if code >= 0:
+        return _lib.autograd().rmsnorm(inp, weight, float(eps), code)
     return RMSNormFunction.apply(inp, weight, eps)
 
 
@@ -125,8 +194,12 @@ class StreamAggregateFunction(_NodeFunction):
         return _lib.autograd().stream_aggregate(inp, H_pre_raw)
 
 
-def stream_aggregate(inp: torch.Tensor, H_pre_raw: torch.Tensor) -> torch.Tensor:
-    """Aggregate [B, n, C] streams with sigmoid weights H_pre_raw [B, n]."""
+def stream_aggregate(inp: torch.Tensor, H_pre_raw: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
+    """Aggregate [B, n, C] streams with sigmoid weights H_pre_raw [B, n].
+    ``checkpoint`` saves inp in 8 bits for the backward, as :func:`rmsnorm`'s."""
+    code = _operator_checkpoint(checkpoint)
+    if code >= 0:
+        return _lib.autograd().stream_aggregate(inp, H_pre_raw, code)
     return StreamAggregateFunction.apply(inp, H_pre_raw)
 
 
@@ -155,8 +228,12 @@ class StreamDistributeMixAddFunction(_NodeFunction):
 
 
 def stream_distribute_mix_add(y_norm: torch.Tensor, H_post_raw: torch.Tensor, M: torch.Tensor,
-                              x_inp: torch.Tensor) -> torch.Tensor:
-    """Distribute y_norm [B, C] to n streams, mix x_inp [B, n, C] with M and add (fp32 out)."""
+                              x_inp: torch.Tensor, checkpoint: Optional[str] = None) -> torch.Tensor:
+    """Distribute y_norm [B, C] to n streams, mix x_inp [B, n, C] with M and add (fp32 out).
+    ``checkpoint`` saves y_norm and x_inp in 8 bits for the backward, as :func:`rmsnorm`'s."""
+    code = _operator_checkpoint(checkpoint)
+    if code >= 0:
+        return _lib.autograd().stream_distribute_mix_add(y_norm, H_post_raw, M, x_inp, code)
     return StreamDistributeMixAddFunction.apply(y_norm, H_post_raw, M, x_inp)
 
 
@@ -174,11 +251,15 @@ def compute_rms(x_flat: torch.Tensor, eps: float = 1e-8) -> torch.Tensor:
 
 def mhc_layer_static(x: torch.Tensor, rmsnorm_weight: torch.Tensor, H_pre: torch.Tensor, H_post: torch.Tensor,
                      H_res: torch.Tensor, sinkhorn_iters: int = 20, sinkhorn_eps: float = 1e-8,
-                     rmsnorm_eps: float = 1e-5) -> torch.Tensor:
+                     rmsnorm_eps: float = 1e-5, checkpoint: Optional[str] = None) -> torch.Tensor:
     """Static-H mHC layer on x [B, n, C] -> fp32 [B, n, C]: one fused pass per
-    direction (layer.py:142-170), autograd node in C++ (_mhc_autograd.so)."""
+    direction (layer.py:142-170), autograd node in C++ (_mhc_autograd.so).
+
+    ``checkpoint`` ("int8" or "e4m3", see :func:`activation_pack`) saves x in 8
+    bits for the backward, which is then the layer's gradient at the values
+    that checkpoint stands for."""
     return _lib.autograd().static_layer(x, rmsnorm_weight, H_pre, H_post, H_res, int(sinkhorn_iters),
-                                        float(sinkhorn_eps), float(rmsnorm_eps))
+                                        float(sinkhorn_eps), float(rmsnorm_eps), _checkpoint_code(checkpoint))
 
 
 # =============================================================================
@@ -240,9 +321,14 @@ def mhc_layer_fused_dynamic_inference(x_expanded, rmsnorm_weight, phi_pre, phi_p
 
 def mhc_layer_fused_dynamic_training(x_expanded, rmsnorm_weight, phi_pre, phi_post, phi_res, alpha_pre, alpha_post,
                                      alpha_res, b_pre, b_post, b_res, sinkhorn_iters: int = 20,
-                                     sinkhorn_eps: float = 1e-8, rmsnorm_eps: float = 1e-5) -> torch.Tensor:
+                                     sinkhorn_eps: float = 1e-8, rmsnorm_eps: float = 1e-5,
+                                     checkpoint: Optional[str] = None) -> torch.Tensor:
     """Dynamic-H layer with autograd (ops.py:567-628).  Float alphas become
-    device tensors; alpha tensors stay on the device (no .item() syncs)."""
+    device tensors; alpha tensors stay on the device (no .item() syncs).
+
+    ``checkpoint`` ("int8" or "e4m3", see :func:`activation_pack`) saves x in 8
+    bits: the backward takes the streams from it and keeps the forward's own
+    per-token coefficients, projections and their RMS, which it saves as well."""
     dev = phi_pre.device
     if not torch.is_tensor(alpha_pre):
         alpha_pre = torch.tensor(alpha_pre, device=dev, dtype=torch.float32)
@@ -252,7 +338,7 @@ def mhc_layer_fused_dynamic_training(x_expanded, rmsnorm_weight, phi_pre, phi_po
         alpha_res = torch.tensor(alpha_res, device=dev, dtype=torch.float32)
     return _lib.autograd().dynamic_layer(x_expanded, rmsnorm_weight, phi_pre, phi_post, phi_res, alpha_pre,
                                          alpha_post, alpha_res, b_pre, b_post, b_res, int(sinkhorn_iters),
-                                         float(sinkhorn_eps), float(rmsnorm_eps))
+                                         float(sinkhorn_eps), float(rmsnorm_eps), _checkpoint_code(checkpoint))
 
 
 # =============================================================================
@@ -261,7 +347,10 @@ def mhc_layer_fused_dynamic_training(x_expanded, rmsnorm_weight, phi_pre, phi_po
 
 def mhc_residual_wrapper(residual: torch.Tensor, branch_output: torch.Tensor, layer, residual_mode: str = "decay"):
     """Fused MHCResidualWrapper on residual / branch_output [tokens, C] for the
-    parameters of ``layer`` (an MHCLayer); returns fp32 [tokens, C]."""
+    parameters of ``layer`` (an MHCLayer); returns fp32 [tokens, C].  With the
+    layer's ``checkpoint`` the saved rows, residual and branch_output (or the
+    streams of a shape that is not fused), are kept in 8 bits."""
+    checkpoint = _checkpoint_code(getattr(layer, "checkpoint", None))
     n = layer.expansion_rate
     C = residual.shape[-1]
     # The fused wrapper kernels take 4-channel rows and n = 2..32; with
@@ -294,6 +383,65 @@ def mhc_residual_wrapper(residual: torch.Tensor, branch_output: torch.Tensor, la
     if layer.use_dynamic_h:
         return ag.dynamic_wrapper(residual, branch_output, layer.rmsnorm_weight, layer.phi_pre, layer.phi_post,
                                   layer.phi_res, layer.alpha_pre, layer.alpha_post, layer.alpha_res, layer.b_pre,
-                                  layer.b_post, layer.b_res, residual_mode, n, iters, sk_eps, rms_eps)
+                                  layer.b_post, layer.b_res, residual_mode, n, iters, sk_eps, rms_eps, checkpoint)
     return ag.static_wrapper(residual, branch_output, layer.rmsnorm_weight, layer.H_pre, layer.H_post, layer.H_res,
-                             residual_mode, n, iters, sk_eps, rms_eps)
+                             residual_mode, n, iters, sk_eps, rms_eps, checkpoint)
+
+
+# =============================================================================
+# Per-head norm of queries and keys with the rotation of positions (no
+# counterpart in the reference)
+# =============================================================================
+
+def rope_table(length: int, rotary_dim: int, base: float = 10000.0, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin, fp32 [length, rotary_dim / 2], of the angles
+    position * base**(-2 p / rotary_dim), formed in 64 bits."""
+    if length < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rope_table: length must be >= 1 and rotary_dim even and >= 2")
+    p = torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64)
+    angle = torch.arange(length, device=device, dtype=torch.float64).unsqueeze(1) * base ** (-p / rotary_dim)
+    return angle.cos().float(), angle.sin().float()
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                 interleaved: bool = False, checkpoint: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every head of q and k, then the rotation of its token's
+    position, in one pass (no counterpart in the reference).
+
+    q [..., heads, D] and k [..., kv_heads, D] are [tokens, heads, D] or
+    [batch, seq, heads, D] in one dtype, D <= 1024; they may be strided views
+    (of a joint projection's output, say): rows of D channels next to each
+    other are read in place.  Each head row becomes y = x / sqrt(mean x^2 +
+    eps) * weight, with q_weight and k_weight [D]; then the first R = 2 *
+    cos.shape[1] channels rotate by pairs (p, p + R/2), or (2p, 2p + 1) with
+    ``interleaved``: (a, b) -> (a c - b s, b c + a s) with c, s column p of cos
+    and sin [positions, R/2] (:func:`rope_table`).
+
+    ``positions`` (int64 or int32) is [tokens], or [batch, seq] or [seq];
+    without it they count 0, 1, ... along tokens or seq.  A position outside
+    the table makes its rows NaN.  The outputs are contiguous, in q's dtype
+    (fp32 or bf16; others become fp32); cos and sin get no gradient.
+
+    ``checkpoint`` ("int8" or "e4m3", see :func:`activation_pack`) saves q and
+    k in 8 bits for the backward, which is then the gradient at the values that
+    checkpoint stands for."""
+    code = _checkpoint_code(checkpoint)
+    if q.dim() not in (3, 4) or k.dim() != q.dim():
+        raise RuntimeError("qk_norm_rope: q and k must both be [tokens, heads, D] or [batch, seq, heads, D], got "
+                           f"{tuple(q.shape)} and {tuple(k.shape)}")
+    if q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise RuntimeError("qk_norm_rope: q and k must have the same tokens and head_dim, got "
+                           f"{tuple(q.shape)} and {tuple(k.shape)}")
+    lead = q.shape[:-2]
+    if positions is not None and positions.shape not in (lead, lead[-1:]):
+        raise RuntimeError(f"qk_norm_rope: positions must be {tuple(lead)} or {tuple(lead[-1:])}, got "
+                           f"{tuple(positions.shape)}")
+    period = lead[-1] if positions is None else positions.numel()
+    if q.dim() == 4:
+        q, k = q.flatten(0, 1), k.flatten(0, 1)
+    q, k = _lib.autograd().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, period, float(eps),
+                                        bool(interleaved), code)
+    if len(lead) == 2:
+        q, k = q.unflatten(0, lead), k.unflatten(0, lead)
+    return q, k
