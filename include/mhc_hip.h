@@ -469,7 +469,7 @@ int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_s
                          void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
                          int32_t rotary_dim, int32_t interleaved, float eps, void* stream);
 size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
-                                           int32_t dtype, int32_t format);
+                                           int32_t rotary_dim, int32_t interleaved);
 /* grad_q / grad_k contiguous (dtype); grad_weight [2, head_dim] (weight_dtype):
  * that of q_weight, then that of k_weight, summed over tokens and heads in a
  * fixed order. */

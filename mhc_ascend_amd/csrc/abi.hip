@@ -2366,22 +2366,28 @@ int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_s
     });
 }
 
-static RowsBwdWs qk_bwd_ws(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t dtype,
-                           int32_t format) {
+static RowsBwdWs qk_bwd_ws(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                           int32_t interleaved) {
+    QkArgs a{};
+    a.T = tokens;
+    a.heads[0] = q_heads;
+    a.heads[1] = k_heads;
+    a.D = head_dim;
+    a.R = rotary_dim;
+    a.interleaved = interleaved != 0;
     RowsBwdWs w{};
-    (void)q_heads; (void)k_heads; (void)dtype; (void)format;
-    w.grid = qk_norm_rope_bwd_grid(tokens);
-    w.stage_off = align256((size_t)w.grid * 2 * head_dim * sizeof(float));
-    w.total = w.stage_off + align256(column_sums_stage_floats(2 * (int64_t)head_dim) * sizeof(float));
+    w.grid = qk_norm_rope_bwd_rows(a);
+    w.total = align256((size_t)w.grid * 2 * head_dim * sizeof(float));
     return w;
 }
 
 size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
-                                           int32_t dtype, int32_t format) {
-    if (tokens < 0 || tokens > 0x7fffffff || q_heads < 0 || k_heads < 0 || head_dim < 2 || head_dim > kQkMaxDim ||
-        !valid_dtype(dtype) || (format != -1 && !valid_format(format)))
+                                           int32_t rotary_dim, int32_t interleaved) {
+    if (tokens < 0 || tokens > 0x7fffffff || q_heads < 0 || k_heads < 0 ||
+        (int64_t)q_heads + k_heads > 65535 * 4 || head_dim < 2 || head_dim > kQkMaxDim || rotary_dim < 2 ||
+        rotary_dim > head_dim || rotary_dim % 2 != 0)
         return 0;
-    return qk_bwd_ws(tokens, q_heads, k_heads, head_dim, dtype, format).total;
+    return qk_bwd_ws(tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved).total;
 }
 
 int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
@@ -2416,25 +2422,21 @@ int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_
         MHC_REQUIRE(tokens == 0 || format >= 0 || ((q || q_heads == 0) && (k || k_heads == 0)),
                     "qk_norm_rope_bwd: null q/k");
         MHC_REQUIRE(grad_weight, "qk_norm_rope_bwd: null grad_weight");
-        const RowsBwdWs w = qk_bwd_ws(tokens, q_heads, k_heads, head_dim, dtype, format);
+        const RowsBwdWs w = qk_bwd_ws(tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved);
         if (!workspace || workspace_bytes < w.total)
             return fail(MHC_ERR_WORKSPACE,
                         "qk_norm_rope_bwd: workspace smaller than mhc_qk_norm_rope_bwd_workspace_size()");
         hipStream_t s = (hipStream_t)stream;
         float* part = (float*)workspace;
-        float* stage = (float*)((char*)workspace + w.stage_off);
-        const int64_t cols = 2 * (int64_t)head_dim;
         int rows = w.grid;
         hipError_t e;
         if (tokens == 0 || q_heads + k_heads == 0) {
             rows = 1;
-            e = launch_fill_zero(part, cols, s);
+            e = launch_fill_zero(part, 2 * (int64_t)head_dim, s);
         } else {
-            e = launch_qk_norm_rope_bwd(dtype, format, a, part, w.grid, s);
+            e = launch_qk_norm_rope_bwd(dtype, format, a, part, s);
         }
-        if (e == hipSuccess)
-            e = launch_column_finalize(0, weight_dtype, part, rows, cols, stage, grad_weight, nullptr, 0, nullptr,
-                                       nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+        if (e == hipSuccess) e = launch_qk_norm_rope_dw(weight_dtype, part, rows, head_dim, grad_weight, s);
         return hip_status(e);
     });
 }

@@ -999,7 +999,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
         Tensor dq = at::empty({T, H, D}, gq.options()), dk = at::empty({T, K, D}, gk.options());
         Tensor dw = at::empty({2, D}, t.wq.options());
         const size_t wsb = lib.mhc_qk_norm_rope_bwd_workspace_size(T, (int32_t)H, (int32_t)K, (int32_t)D,
-                                                                   dtype_code(dt), (int32_t)fmt);
+                                                                   (int32_t)(2 * t.cos.size(1)), (int32_t)v[5]);
         Tensor ws = workspace(wsb, dq);
         const Tensor none;
         const Tensor &q = is_held ? none : sv[4], &k = is_held ? none : sv[5];

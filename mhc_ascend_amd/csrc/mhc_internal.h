@@ -315,9 +315,12 @@ struct QkArgs {
 };
 // fmt: a CkFormat, or -1 for the rows themselves
 hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t s);
-// partial rows of both weights' gradients: dw_part[grid][2 D]
-int qk_norm_rope_bwd_grid(int64_t T);
-hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, int grid, hipStream_t s);
+// Partial rows of both weights' gradients, dw_part[rows][2 D]: by T, heads, D,
+// R and interleaved of `a` alone.
+int qk_norm_rope_bwd_rows(const QkArgs& a);
+hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, hipStream_t s);
+// dw[2 D] (w_dtype) = their sums
+hipError_t launch_qk_norm_rope_dw(int w_dtype, const float* dw_part, int rows, int D, void* dw, hipStream_t s);
 
 // ---- dynamic.hip -----------------------------------------------------------
 typedef uint16_t bf16_raw_t;

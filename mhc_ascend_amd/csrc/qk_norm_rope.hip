@@ -161,6 +161,393 @@ __global__ __launch_bounds__(256) void qk_bwd_any_kernel(QkArgs a, float* __rest
 }
 
 // ---------------------------------------------------------------------------
+// Heads of whole pieces: V channels a lane, a group of G lanes (a power of
+// two, D / V or the next) a head row, so a wave takes 64 / G heads of one token
+// at a time and keeps the token's table row in registers for all of them.  A
+// lane of the rotated halves reads its partner's piece itself: the bytes are
+// in the cache line of another lane's load, and no exchange between lanes
+// waits on the sums.  Tasks of U such steps have all their loads in flight.
+// Few tokens: their tasks are spread over Y workgroups each.
+// ---------------------------------------------------------------------------
+typedef uint32_t qk_u2_t __attribute__((ext_vector_type(2)));
+typedef qk_u2_t qk_u2_a2_t __attribute__((aligned(2)));
+
+template <typename T, int V> struct QkPiece;  // V elements as raw words
+template <> struct QkPiece<float, 8> {
+    ck_u4_t w[2];
+    __device__ __forceinline__ void load(const float* p) {
+        w[0] = *reinterpret_cast<const ck_u4_a4_t*>(p);
+        w[1] = *reinterpret_cast<const ck_u4_a4_t*>(p + 4);
+    }
+    __device__ __forceinline__ float get(int e) const { return __uint_as_float(w[e / 4][e % 4]); }
+};
+template <> struct QkPiece<float, 4> {
+    ck_u4_t w;
+    __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const ck_u4_a4_t*>(p); }
+    __device__ __forceinline__ float get(int e) const { return __uint_as_float(w[e]); }
+};
+template <> struct QkPiece<bf16_t, 8> {
+    ck_u4_t w;
+    __device__ __forceinline__ void load(const bf16_t* p) { w = *reinterpret_cast<const ck_u4_a2_t*>(p); }
+    __device__ __forceinline__ float get(int e) const {
+        return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+};
+template <> struct QkPiece<bf16_t, 4> {
+    qk_u2_t w;
+    __device__ __forceinline__ void load(const bf16_t* p) { w = *reinterpret_cast<const qk_u2_a2_t*>(p); }
+    __device__ __forceinline__ float get(int e) const {
+        return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void qk_store(T* p, const float (&v)[V]) {
+    if constexpr (V == 8) {
+        ck_store8(p, v);
+    } else if constexpr (sizeof(T) == 4) {
+        const ck_u4_t a = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        __builtin_nontemporal_store(a, reinterpret_cast<ck_u4_a4_t*>(p));
+    } else {
+        const qk_u2_t a = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        __builtin_nontemporal_store(a, reinterpret_cast<qk_u2_a2_t*>(p));
+    }
+}
+
+// Sum over the aligned group of 2^lg lanes (lg >= 2), in every lane of it.
+__device__ __forceinline__ float qk_group_sum(float v, int lg) {
+    v = group_sum<4>(v);
+    if (lg >= 3) v += dpp::mov<dpp::kRowHalfMirror>(v);
+    if (lg >= 4) v += dpp::mov<dpp::kRowMirror>(v);
+    if (lg >= 5) v = xor16_add(v);
+    if (lg >= 6) v = xor32_add(v);
+    return v;
+}
+
+// One lane's place in its head row.
+template <int V, bool IL>
+struct QkLane {
+    int c0;       // its first channel
+    bool in;      // within the head
+    bool turned;  // some channel of the piece rotates
+    int other;    // first channel of its partners' piece (its own where it has none)
+    float sign;   // of the partner's sine product
+
+    __device__ __forceinline__ QkLane(const QkArgs& a, int lane, int lg) {
+        c0 = (lane & ((1 << lg) - 1)) * V;
+        in = c0 < a.D;
+        turned = c0 < a.R;
+        other = c0;
+        sign = 1.f;
+        if (!IL && turned) {
+            const int half = a.R >> 1;
+            other = c0 < half ? c0 + half : c0 - half;
+            sign = c0 < half ? -1.f : 1.f;
+        }
+    }
+
+    // The lane's table entries of table row `tab`: per channel with halves
+    // (the sine with its sign), per pair interleaved.  1 and 0 elsewhere.
+    static constexpr int kTab = IL ? V / 2 : V;
+    __device__ __forceinline__ void table(const QkArgs& a, int64_t row, float (&c)[kTab], float (&s)[kTab]) const {
+        const int half = a.R >> 1;
+        const int64_t at = (row < 0 ? 0 : row) * half;
+        if constexpr (IL) {
+#pragma unroll
+            for (int p = 0; p < kTab; ++p) {
+                const int col = (c0 >> 1) + p;
+                const bool on = col < half;
+                c[p] = on ? a.cos[at + col] : 1.f;
+                s[p] = on ? a.sin[at + col] : 0.f;
+            }
+        } else {
+            QkPiece<float, V> pc, ps;
+            const int col = c0 < half ? c0 : c0 - half;
+            pc.load(a.cos + at + (turned ? col : 0));
+            ps.load(a.sin + at + (turned ? col : 0));
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                c[e] = turned ? pc.get(e) : 1.f;
+                s[e] = turned ? sign * ps.get(e) : 0.f;
+            }
+        }
+    }
+
+    // Channel e's rotation of v (this piece) and o (the partners' piece) by
+    // `way` = 1 or -1 times the angle.
+    __device__ __forceinline__ float turn(const float (&v)[V], const float (&o)[V], const float (&c)[kTab],
+                                          const float (&s)[kTab], int e, float way, int R) const {
+        if constexpr (IL) {
+            const float x = (e & 1) ? v[e - 1] : -v[e + 1];
+            return c0 + e < R ? v[e] * c[e / 2] + way * x * s[e / 2] : v[e];
+        } else {
+            return turned ? v[e] * c[e] + way * o[e] * s[e] : v[e];
+        }
+    }
+
+    __device__ __forceinline__ void weights(const QkArgs& a, int s, int at, float (&w)[V]) const {
+        if (a.w_dtype == kBF16) {
+            QkPiece<bf16_t, V> p;
+            p.load(static_cast<const bf16_t*>(a.w[s]) + (in ? at : 0));
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e] = in ? p.get(e) : 0.f;
+        } else {
+            QkPiece<float, V> p;
+            p.load(static_cast<const float*>(a.w[s]) + (in ? at : 0));
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e] = in ? p.get(e) : 0.f;
+        }
+    }
+};
+
+constexpr int kQkU = 2;
+// Tasks of a token: its queries' steps, then its keys', U at a time.
+struct QkTasks {
+    int per;    // heads of a task
+    int nq, n;  // tasks of the queries, of both
+    __host__ __device__ QkTasks(int H, int K, int lg) : per(kQkU * (64 >> lg)) {
+        nq = (H + per - 1) / per;
+        n = nq + (K + per - 1) / per;
+    }
+};
+
+// A task's loads.
+template <typename T, int V, bool IL>
+struct QkRows {
+    QkPiece<T, V> own[kQkU], far[IL ? 1 : kQkU];
+    __device__ __forceinline__ void load(const QkLane<V, IL>& ln, const T* base, int64_t head_stride, int h0, int step,
+                                         int heads) {
+#pragma unroll
+        for (int u = 0; u < kQkU; ++u) {
+            const int h = h0 + u * step;
+            const T* row = base + (h < heads ? h : 0) * head_stride;
+            own[u].load(row + (ln.in ? ln.c0 : 0));
+            if constexpr (!IL) far[u].load(row + (ln.in ? ln.other : 0));
+        }
+    }
+};
+
+template <typename T, int FMT, int V, bool IL>
+__global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg) {
+    const int lane = threadIdx.x & 63;
+    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (t >= a.T) return;
+    const QkLane<V, IL> ln(a, lane, lg);
+    const QkTasks tasks(a.heads[0], a.heads[1], lg);
+    const int sub = lane >> lg, step = 64 >> lg;
+    const int stride = (int)ck_stride(a.D), nb = (int)ck_blocks(a.D);
+    const auto side = [&](int j) { return j < tasks.nq ? 0 : 1; };
+    const auto first = [&](int j, int s) { return (s ? j - tasks.nq : j) * tasks.per + sub; };
+    const auto fetch = [&](int j, QkRows<T, V, IL>& r) {
+        const int s = side(j);
+        r.load(ln, static_cast<const T*>(a.x[s]) + t * a.x_token[s], a.x_head[s], first(j, s), step, a.heads[s]);
+    };
+    int j = blockIdx.y;
+    QkRows<T, V, IL> next;
+    fetch(j, next);  // the grid's y is at most the number of tasks
+    const int64_t pos = qk_position(a, t);
+    float c[QkLane<V, IL>::kTab], sn[QkLane<V, IL>::kTab];
+    ln.table(a, pos, c, sn);
+    float w[V], wo[V];
+    int at = -1;  // whose weights w and wo are
+    for (; j < tasks.n; j += gridDim.y) {
+        const int s = side(j), h0 = first(j, s);
+        const QkRows<T, V, IL> rows = next;
+        if (j + (int)gridDim.y < tasks.n) fetch(j + gridDim.y, next);
+        if (s != at) {
+            at = s;
+            ln.weights(a, s, ln.c0, w);
+            if constexpr (!IL) ln.weights(a, s, ln.other, wo);
+        }
+#pragma unroll
+        for (int u = 0; u < kQkU; ++u) {
+            const int h = h0 + u * step;
+            const bool on = h < a.heads[s];
+            const int64_t row = t * a.heads[s] + h;
+            float v[V], o[V], y[V];
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[e] = ln.in ? rows.own[u].get(e) : 0.f;
+                ss += v[e] * v[e];
+            }
+            if constexpr (FMT >= 0) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < V; ++e) m = m > ck_abs_bits(v[e]) ? m : ck_abs_bits(v[e]);
+                const uint32_t sc = Ck<FMT>::scale(ck_group_max<32 / V>(m));
+                const float up = Ck<FMT>::up(sc);
+                const uint32_t keep = sc == 255u ? 0u : ~0u;
+                uint32_t q[V / 4];
+#pragma unroll
+                for (int e = 0; e < V; e += 4)
+                    q[e / 4] = Ck<FMT>::pack4(v[e], v[e + 1], v[e + 2], v[e + 3], up, keep);
+                if (on && ln.c0 < stride) {
+                    uint8_t* qp = a.q[s] + row * stride + ln.c0;
+                    if constexpr (V == 8) st8_nt(qp, make_uint2(q[0], q[1]));
+                    else __builtin_nontemporal_store(q[0], reinterpret_cast<uint32_t*>(qp));
+                }
+                if (on && ln.in && (ln.c0 & 31) == 0) a.sc[s][row * nb + (ln.c0 >> 5)] = (uint8_t)sc;
+            }
+            ss = qk_group_sum(ss, lg);
+            const float inv = pos < 0 ? __uint_as_float(0x7fc00000u) : 1.f / sqrtf(ss / (float)a.D + a.eps);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[e] = v[e] * inv * w[e];
+                o[e] = 0.f;
+                if constexpr (!IL) o[e] = rows.far[u].get(e) * inv * wo[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = ln.turn(v, o, c, sn, e, 1.f, a.R);
+            if (on && ln.in) qk_store<T, V>(static_cast<T*>(a.y[s]) + row * a.D + ln.c0, y);
+        }
+    }
+}
+
+// Persistent waves over tokens; both weights' gradients in registers, added
+// over the wave's groups and the workgroup's waves at the end, in a fixed
+// order: dw_part[workgroup][2 D].
+template <typename T, int FMT, int V, bool IL>
+__global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, float* __restrict__ dw_part) {
+    extern __shared__ float red[];  // [8 waves][2][D]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const QkLane<V, IL> ln(a, lane, lg);
+    const QkTasks tasks(a.heads[0], a.heads[1], lg);
+    const int sub = lane >> lg, step = 64 >> lg;
+    const int stride = (int)ck_stride(a.D), nb = (int)ck_blocks(a.D);
+    float dw[2][V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[0][e] = dw[1][e] = 0.f;
+    for (int64_t t = (int64_t)blockIdx.x * 8 + wave; t < a.T; t += (int64_t)gridDim.x * 8) {
+        const int64_t pos = qk_position(a, t);
+        float c[QkLane<V, IL>::kTab], sn[QkLane<V, IL>::kTab];
+        ln.table(a, pos, c, sn);
+        for (int j = blockIdx.y; j < tasks.n; j += gridDim.y) {
+            const int s = j < tasks.nq ? 0 : 1;
+            const int h0 = (s ? j - tasks.nq : j) * tasks.per + sub;
+            const T* g = static_cast<const T*>(a.g[s]) + t * a.g_token[s];
+            QkPiece<T, V> gown[kQkU], gfar[kQkU], xr[kQkU];
+            uint32_t q[kQkU][V / 4], sc[kQkU];
+#pragma unroll
+            for (int u = 0; u < kQkU; ++u) {
+                const int h = h0 + u * step < a.heads[s] ? h0 + u * step : 0;
+                const T* grow = g + h * a.g_head[s];
+                gown[u].load(grow + (ln.in ? ln.c0 : 0));
+                if constexpr (!IL) gfar[u].load(grow + (ln.in ? ln.other : 0));
+                if constexpr (FMT >= 0) {
+                    const int64_t row = t * a.heads[s] + h;
+                    const uint8_t* qp = a.q[s] + row * stride + (ln.in ? ln.c0 : 0);
+                    if constexpr (V == 8) {
+                        const uint2 p = ld8_nt(qp);
+                        q[u][0] = p.x;
+                        q[u][V / 4 - 1] = p.y;
+                    } else {
+                        q[u][0] = *reinterpret_cast<const uint32_t*>(qp);
+                    }
+                    sc[u] = a.sc[s][row * nb + (ln.in ? ln.c0 >> 5 : 0)];
+                } else {
+                    xr[u].load(static_cast<const T*>(a.x[s]) + t * a.x_token[s] + h * a.x_head[s] +
+                               (ln.in ? ln.c0 : 0));
+                }
+            }
+            float w[V];
+            ln.weights(a, s, ln.c0, w);
+#pragma unroll
+            for (int u = 0; u < kQkU; ++u) {
+                const int h = h0 + u * step;
+                const bool on = h < a.heads[s] && ln.in;
+                float v[V], z[V], o[V], d[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    z[e] = on ? gown[u].get(e) : 0.f;
+                    o[e] = IL || !on ? 0.f : gfar[u].get(e);
+                }
+                if constexpr (FMT >= 0) {
+#pragma unroll
+                    for (int e = 0; e < V; e += 4) {
+                        float f[4];
+                        Ck<FMT>::unpack4(q[u][e / 4], Ck<FMT>::down(sc[u]), f);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[e + k] = on ? f[k] : 0.f;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) v[e] = on ? xr[u].get(e) : 0.f;
+                }
+                float ss = 0.f, dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) d[e] = ln.turn(z, o, c, sn, e, -1.f, a.R);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    ss += v[e] * v[e];
+                    dot += d[e] * w[e] * v[e];
+                }
+                ss = qk_group_sum(ss, lg);
+                dot = qk_group_sum(dot, lg);
+                const float inv = pos < 0 ? __uint_as_float(0x7fc00000u) : 1.f / sqrtf(ss / (float)a.D + a.eps);
+                const float k2 = dot * inv * inv * inv / (float)a.D;
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float p = on ? d[e] * v[e] * inv : 0.f;  // a head past the last adds nothing (inv may be infinite)
+                    dw[0][e] += s == 0 ? p : 0.f;
+                    dw[1][e] += s == 0 ? 0.f : p;
+                    d[e] = w[e] * d[e] * inv - v[e] * k2;
+                }
+                if (on) qk_store<T, V>(static_cast<T*>(a.y[s]) + (t * a.heads[s] + h) * a.D + ln.c0, d);
+            }
+        }
+    }
+    // the wave's groups, then its channels to LDS
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float v = dw[s][e];
+            for (int k = 1 << lg; k < 64; k <<= 1) v += __shfl_xor(v, k);
+            if (sub == 0 && ln.in) red[(wave * 2 + s) * a.D + ln.c0 + e] = v;
+        }
+    }
+    __syncthreads();
+    const int64_t row = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    for (int i = threadIdx.x; i < 2 * a.D; i += 512) {
+        float v = 0.f;
+        for (int w = 0; w < 8; ++w) v += red[w * 2 * a.D + i];
+        dw_part[row * 2 * a.D + i] = v;
+    }
+}
+
+// Sums of part[rows][cols] over rows, 32 columns a workgroup in 32 phases of
+// rows: 512 rows of 256 columns take two rounds of eight loads and one LDS
+// sum, against 16 rounds with 256 lanes on 64 columns.
+template <typename TW>
+__global__ __launch_bounds__(1024) void qk_dw_kernel(const float* __restrict__ part, int rows, int cols,
+                                                     TW* __restrict__ dw) {
+    __shared__ float red[32][33];
+    const int cl = threadIdx.x & 31, ph = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + cl;
+    float s = 0.f;
+    if (c < cols) {
+        int r = ph;
+        for (; r + 7 * 32 < rows; r += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(r + u * 32) * cols + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; r < rows; r += 32) s += part[(int64_t)r * cols + c];
+    }
+    red[ph][cl] = s;
+    __syncthreads();
+    if (ph == 0 && c < cols) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += red[k][cl];
+        VecIO<TW>::put(dw + c, t);
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Host launchers
 // ---------------------------------------------------------------------------
 #define MHC_QK_TYPED(dt, fmt, ...)                                            \
@@ -175,28 +562,99 @@ __global__ __launch_bounds__(256) void qk_bwd_any_kernel(QkArgs a, float* __rest
         else pick(std::integral_constant<int, kCkE4M3>{});                    \
     } while (0)
 
+// V channels a lane (0: the kernels of any size) and log2 of the lanes a head.
+struct QkTiling {
+    int v, lg;
+};
+static QkTiling qk_tiling(int D, int R, bool interleaved) {
+    for (int v = 8; v >= 4; v -= 4) {
+        if (D % v != 0 || (!interleaved && R % (2 * v) != 0)) continue;
+        int lg = v == 8 ? 2 : 3;  // a block of 32 channels lies in one group
+        while ((v << lg) < D) ++lg;
+        if (lg <= 6) return QkTiling{v, lg};
+    }
+    return QkTiling{0, 0};
+}
+
+// Workgroups that share a token's tasks: enough waves for the device.
+static int qk_splits(int64_t T, const QkTasks& tasks) {
+    const int64_t want = 16 * (int64_t)device_cu_count();
+    int64_t y = (want + T - 1) / T;
+    if (y > tasks.n) y = tasks.n;
+    return (int)(y < 1 ? 1 : y);
+}
+
+#define MHC_QK_TILED(dt, fmt, t, il, ...)                                            \
+    MHC_QK_TYPED(dt, fmt, {                                                          \
+        auto tiled = [&](auto v_, auto il_) {                                        \
+            constexpr int V_ = decltype(v_)::value;                                  \
+            constexpr bool I_ = decltype(il_)::value;                                \
+            __VA_ARGS__;                                                             \
+        };                                                                           \
+        using V8 = std::integral_constant<int, 8>;                                   \
+        using V4 = std::integral_constant<int, 4>;                                   \
+        if (t.v == 8) { if (il) tiled(V8{}, std::true_type{}); else tiled(V8{}, std::false_type{}); } \
+        else { if (il) tiled(V4{}, std::true_type{}); else tiled(V4{}, std::false_type{}); }          \
+    })
+
 hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t s) {
     const int H = a.heads[0] + a.heads[1];
     if (a.T == 0 || H == 0) return hipSuccess;
+    const QkTiling t = qk_tiling(a.D, a.R, a.interleaved);
     const int tok = timing_begin("qk_norm_rope_fwd", s);
-    MHC_QK_TYPED(dt, fmt,
-                 MHC_LAUNCH_GGL((qk_fwd_any_kernel<T_, F_>), dim3((unsigned)a.T, (unsigned)((H + 3) / 4)), dim3(256),
-                                0, s, a));
+    if (t.v == 0) {
+        MHC_QK_TYPED(dt, fmt,
+                     MHC_LAUNCH_GGL((qk_fwd_any_kernel<T_, F_>), dim3((unsigned)a.T, (unsigned)((H + 3) / 4)),
+                                    dim3(256), 0, s, a));
+    } else {
+        const int y = qk_splits(a.T, QkTasks(a.heads[0], a.heads[1], t.lg));
+        MHC_QK_TILED(dt, fmt, t, a.interleaved,
+                     MHC_LAUNCH_GGL((qk_fwd_kernel<T_, F_, V_, I_>), dim3((unsigned)((a.T + 3) / 4), (unsigned)y),
+                                    dim3(256), 0, s, a, t.lg));
+    }
     timing_end(tok, s);
     return hipGetLastError();
 }
 
-int qk_norm_rope_bwd_grid(int64_t T) {
-    const int64_t g = 2 * (int64_t)device_cu_count();
-    return (int)(T < g ? (T < 1 ? 1 : T) : g);
+static dim3 qk_bwd_dims(const QkArgs& a) {
+    const QkTiling t = qk_tiling(a.D, a.R, a.interleaved);
+    const int64_t two = 2 * (int64_t)device_cu_count();
+    if (a.T == 0) return dim3(1, 1);
+    if (t.v == 0) return dim3((unsigned)(a.T < two ? a.T : two), 1);
+    const int y = qk_splits(a.T, QkTasks(a.heads[0], a.heads[1], t.lg));
+    const int64_t x = (a.T + 7) / 8, most = two / y > 1 ? two / y : 1;
+    return dim3((unsigned)(x < most ? x : most), (unsigned)y);
 }
 
-hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, int grid, hipStream_t s) {
+int qk_norm_rope_bwd_rows(const QkArgs& a) {
+    const dim3 g = qk_bwd_dims(a);
+    return (int)(g.x * g.y);
+}
+
+hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, hipStream_t s) {
+    const QkTiling t = qk_tiling(a.D, a.R, a.interleaved);
+    const dim3 grid = qk_bwd_dims(a);
     const int tok = timing_begin("qk_norm_rope_bwd", s);
-    MHC_QK_TYPED(dt, fmt,
-                 MHC_LAUNCH_GGL((qk_bwd_any_kernel<T_, F_>), dim3((unsigned)grid), dim3(256),
-                                (size_t)a.D * 8 * sizeof(float), s, a, dw_part));
+    if (t.v == 0) {
+        MHC_QK_TYPED(dt, fmt,
+                     MHC_LAUNCH_GGL((qk_bwd_any_kernel<T_, F_>), grid, dim3(256), (size_t)a.D * 8 * sizeof(float), s,
+                                    a, dw_part));
+    } else {
+        MHC_QK_TILED(dt, fmt, t, a.interleaved,
+                     MHC_LAUNCH_GGL((qk_bwd_kernel<T_, F_, V_, I_>), grid, dim3(512),
+                                    (size_t)a.D * 16 * sizeof(float), s, a, t.lg, dw_part));
+    }
     timing_end(tok, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_qk_norm_rope_dw(int w_dtype, const float* dw_part, int rows, int D, void* dw, hipStream_t s) {
+    const dim3 grid((unsigned)((2 * D + 31) / 32));
+    if (w_dtype == kBF16) {
+        MHC_LAUNCH_GGL((qk_dw_kernel<bf16_t>), grid, dim3(1024), 0, s, dw_part, rows, 2 * D, (bf16_t*)dw);
+    } else {
+        MHC_LAUNCH_GGL((qk_dw_kernel<float>), grid, dim3(1024), 0, s, dw_part, rows, 2 * D, (float*)dw);
+    }
     return hipGetLastError();
 }
 

@@ -104,7 +104,7 @@ def test_sizes_on_host():
     assert lib.mhc_checkpoint_values_size(1 << 33, 4096) == (1 << 33) * 4096
     assert lib.mhc_checkpoint_values_size(-1, 4) == 0 and lib.mhc_checkpoint_scales_size(1, 0) == 0
     assert lib.mhc_rmsnorm_checkpoint_bwd_workspace_size(4, 16385, 0, 0) == 0
-    assert lib.mhc_qk_norm_rope_bwd_workspace_size(4, 1, 1, 1025, 0, -1) == 0
+    assert lib.mhc_qk_norm_rope_bwd_workspace_size(4, 1, 1, 1025, 64, 0) == 0
 
 
 def test_checkpoint_entries_reject_bad_arguments_on_host():
