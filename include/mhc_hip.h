@@ -419,6 +419,12 @@ int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* 
                                     int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
                                     float rmsnorm_eps, void* stream);
 size_t mhc_layer_static_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype);
+/* What a backward on these arrays needs, at most the query above: no share for
+ * x^ rows where the row kernel reads the checkpoint (n = 2..8, hidden a
+ * multiple of 4 that fits its registers, 16-byte aligned arrays). */
+size_t mhc_layer_static_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
+                                                      int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
+                                                      int32_t format);
 int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
                                     int32_t x_dtype, int32_t weight_dtype, const float* h_pre, const float* h_post,
                                     const float* h_res, const float* saved, void* grad_x, void* grad_weight,

@@ -2209,18 +2209,51 @@ int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* 
         int st = check_ckpt("layer_static_checkpoint_fwd", batch, hidden, x_dtype, format, x && values && scales);
         if (st) return st;
         MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_static_checkpoint_fwd: values must be 16-byte aligned");
+        hipStream_t s = (hipStream_t)stream;
+        if (layer_ckpt_fwd_rows(n, batch, hidden, {x, out, saved, values})) {
+            st = check_layer_shape("layer_static_checkpoint_fwd", batch, n, hidden, x_dtype, num_iters);
+            if (st) return st;
+            MHC_REQUIRE(valid_dtype(weight_dtype), "layer_static_checkpoint_fwd: weight_dtype must be F32 or BF16");
+            MHC_REQUIRE(weight && h_pre && h_post && h_res && saved && out,
+                        "layer_static_checkpoint_fwd: null parameter pointer");
+            hipError_t e = launch_static_coef(n, h_pre, h_post, h_res, weight, weight_dtype, hidden, saved, num_iters,
+                                              sinkhorn_eps, s);
+            if (e == hipSuccess)
+                e = launch_layer_ckpt_fwd(x_dtype, format, n, x, saved + saved_w_offset(n), saved, 0, out, values,
+                                          scales, batch, hidden, rmsnorm_eps, s);
+            return hip_status(e);
+        }
         st = mhc_layer_static_fwd(x, x_dtype, weight, weight_dtype, h_pre, h_post, h_res, out, nullptr, saved, batch, n,
                                   hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
         if (st) return st;
-        return hip_status(launch_ckpt_pack(x_dtype, format, x, values, scales, batch * n, hidden, (hipStream_t)stream));
+        return hip_status(launch_ckpt_pack(x_dtype, format, x, values, scales, batch * n, hidden, s));
     });
 }
 
-// workspace: [x^ rows | the layer's backward]
+// Rows read from the checkpoint: the partials of static_bwd_ws.
+static StaticBwdWs static_ckpt_bwd_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype, int32_t format) {
+    StaticBwdWs w{};
+    w.grid = layer_ckpt_bwd_grid(x_dtype, format, n, 0, batch, hidden);
+    w.scal_off = align256((size_t)w.grid * hidden * sizeof(float));
+    w.stage_off = w.scal_off + align256((size_t)w.grid * (n * n + 2 * n) * sizeof(float));
+    w.total = w.stage_off + align256(column_sums_stage_floats(hidden) * sizeof(float));
+    return w;
+}
+
+// workspace: that, or [x^ rows | the layer's backward]
 size_t mhc_layer_static_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
     if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype)) return 0;
     return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
            mhc_layer_static_bwd_workspace_size(batch, n, hidden, x_dtype);
+}
+
+size_t mhc_layer_static_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
+                                                      int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
+                                                      int32_t format) {
+    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype) || !valid_format(format)) return 0;
+    if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}))
+        return static_ckpt_bwd_ws(batch, n, hidden, x_dtype, format).total;
+    return mhc_layer_static_checkpoint_bwd_workspace_size(batch, n, hidden, x_dtype);
 }
 
 int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
@@ -2236,11 +2269,30 @@ int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, c
         st = check_layer_shape(fn, batch, n, hidden, x_dtype, num_iters);
         if (st) return st;
         MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_static_checkpoint_bwd: values must be 16-byte aligned");
-        const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
-        if (!workspace ||
-            workspace_bytes < mhc_layer_static_checkpoint_bwd_workspace_size(batch, n, hidden, x_dtype))
+        if (!workspace || workspace_bytes < mhc_layer_static_checkpoint_bwd_workspace_need(
+                                                grad_out, grad_x, saved, batch, n, hidden, x_dtype, format))
             return fail(MHC_ERR_WORKSPACE, "layer_static_checkpoint_bwd: workspace smaller than "
-                                           "mhc_layer_static_checkpoint_bwd_workspace_size()");
+                                           "mhc_layer_static_checkpoint_bwd_workspace_need()");
+        if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved})) {
+            MHC_REQUIRE(valid_dtype(weight_dtype), "layer_static_checkpoint_bwd: weight_dtype must be F32 or BF16");
+            MHC_REQUIRE(h_pre && h_post && h_res && saved, "layer_static_checkpoint_bwd: null parameter pointer");
+            MHC_REQUIRE(grad_weight && grad_h_pre && grad_h_post && grad_h_res,
+                        "layer_static_checkpoint_bwd: null gradient pointer");
+            const StaticBwdWs w = static_ckpt_bwd_ws(batch, n, hidden, x_dtype, format);
+            hipStream_t s = (hipStream_t)stream;
+            float* dw_part = (float*)workspace;
+            float* scal_part = (float*)((char*)workspace + w.scal_off);
+            hipError_t e = launch_layer_ckpt_bwd(x_dtype, format, n, 0, grad_out, values, scales,
+                                                 saved + saved_w_offset(n), saved, 0, grad_x, dw_part, scal_part,
+                                                 w.grid, batch, hidden, rmsnorm_eps, s);
+            if (e == hipSuccess)
+                e = launch_column_finalize(n, weight_dtype, dw_part, w.grid, hidden,
+                                           (float*)((char*)workspace + w.stage_off), grad_weight, scal_part, w.grid,
+                                           h_pre, h_post, h_res, grad_h_pre, grad_h_post, grad_h_res, num_iters,
+                                           sinkhorn_eps, s, nullptr);
+            return hip_status(e);
+        }
+        const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
         const hipError_t e =
             launch_ckpt_unpack(x_dtype, format, values, scales, workspace, batch * n, hidden, (hipStream_t)stream);
         if (e != hipSuccess) return hip_status(e);

@@ -72,7 +72,7 @@ using torch::autograd::tensor_list;
     X(mhc_rmsnorm_checkpoint_bwd_workspace_size) \
     X(mhc_rmsnorm_checkpoint_bwd)             \
     X(mhc_layer_static_checkpoint_fwd)        \
-    X(mhc_layer_static_checkpoint_bwd_workspace_size) \
+    X(mhc_layer_static_checkpoint_bwd_workspace_need) \
     X(mhc_layer_static_checkpoint_bwd)        \
     X(mhc_layer_dynamic_checkpoint_fwd)       \
     X(mhc_layer_dynamic_checkpoint_bwd_workspace_size) \
@@ -306,7 +306,8 @@ struct StaticLayer : public torch::autograd::Function<StaticLayer> {
         Tensor ghp = at::empty(hp.sizes(), f32), ghq = at::empty(hq.sizes(), f32), ghr = at::empty(hr.sizes(), f32);
         const int xd = dtype_code(store);
         if (is_held) {
-            const size_t wsb = lib.mhc_layer_static_checkpoint_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
+            const size_t wsb = lib.mhc_layer_static_checkpoint_bwd_workspace_need(
+                fp(g), grad_x.data_ptr(), fp(saved), B, (int32_t)n, (int32_t)C, xd, (int32_t)fmt);
             Tensor ws = workspace(wsb, x);
             check(lib.mhc_layer_static_checkpoint_bwd(
                       fp(g), x.data_ptr(), sv[6].data_ptr(), (int32_t)fmt, xd, dtype_code(w.scalar_type()), fp(hp),

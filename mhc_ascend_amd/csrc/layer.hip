@@ -23,11 +23,10 @@
 
 #include "mhc_device.h"
 #include "mhc_internal.h"
+#include "mhc_layer_rows.h"
 #include "mhc_rows.h"
 
 namespace mhc {
-
-template <int N> constexpr int coef_size() { return 2 * N + N * N; }
 
 // The shared N x N matrix (N = 3..8) on lanes 0 .. S^2 - 1 of one wave, one
 // element per lane: `at` = the lane's element r N + c when `on`.  The wave's
@@ -131,70 +130,6 @@ __global__ __launch_bounds__(256) void static_coef_kernel(const float* __restric
 // this pass (C4 bf16 147 -> 136 us; fp32 equal).
 // ---------------------------------------------------------------------------
 template <typename TX, typename TO, int N, int VPT>
-__device__ __forceinline__ void fwd_token(int64_t b, const float* __restrict__ coef, int64_t coef_stride,
-                                          const float (&wv)[VPT][kLayerWC],
-                                          const float (&xv)[N][VPT][kLayerWC], TO* __restrict__ out,
-                                          float* __restrict__ rms_out, int C, float eps, float* red) {
-    constexpr int WC = kLayerWC;
-    constexpr int NC = coef_size<N>();
-    const float* cf = coef + b * coef_stride;
-    float cfv[NC];
-#pragma unroll
-    for (int k = 0; k < NC; ++k) cfv[k] = cf[k];
-    float xa[VPT][WC];
-    float ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-#pragma unroll
-        for (int e = 0; e < WC; ++e) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) s += cfv[i] * xv[i][k][e];
-            xa[k][e] = s;
-            ss += s * s;
-        }
-    }
-    float v[1] = {ss};
-    block_sum<1>(v, red);
-    const float r = sqrtf(v[0] / (float)C + eps);
-    const float inv = 1.f / r;
-    // stores through a resource over the token's output rows, out-of-range
-    // offsets past the row end (no store behind a branch)
-    const buf_rsrc_t ors = make_buf_rsrc(out + b * (int64_t)N * C, (uint32_t)((int64_t)N * C * (int64_t)sizeof(TO)));
-    static_assert(WC == 4, "4-channel chunks: one 16-byte (fp32) or 8-byte (bf16) store");
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int c0 = (k * blockDim.x + threadIdx.x) * WC;
-        const uint32_t o0 = c0 < C ? (uint32_t)c0 * (uint32_t)sizeof(TO) : kBufOff;
-        float y[WC];
-#pragma unroll
-        for (int e = 0; e < WC; ++e) y[e] = xa[k][e] * inv * wv[k][e];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            float o[WC];
-#pragma unroll
-            for (int e = 0; e < WC; ++e) {
-                float s = kTermLast<N> ? 0.f : cfv[N + i] * y[e];
-#pragma unroll
-                for (int j = 0; j < N; ++j) s += cfv[2 * N + i * N + j] * xv[j][k][e];
-                o[e] = kTermLast<N> ? s + cfv[N + i] * y[e] : s;
-            }
-            const uint32_t off = o0 + (uint32_t)(i * C * (int)sizeof(TO));
-            if constexpr (sizeof(TO) == 4) {
-                buf_st16<true>(ors, off, 0u, make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]),
-                                                        __float_as_uint(o[2]), __float_as_uint(o[3])));
-            } else {
-                buf_st8<true>(ors, off, 0u, make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])));
-            }
-        }
-    }
-    if (rms_out) {
-        const buf_rsrc_t rrs = make_buf_rsrc(rms_out + b, 4u);
-        buf_st4(rrs, threadIdx.x == 0 ? 0u : kBufOff, 0u, r);
-    }
-}
-
-template <typename TX, typename TO, int N, int VPT>
 __global__ MHC_ROW_BOUNDS(false) void layer_fwd_kernel(const TX* __restrict__ x, const float* __restrict__ w,
                                                        const float* __restrict__ coef, int64_t coef_stride,
                                                        TO* __restrict__ out, float* __restrict__ rms_out, int64_t B,
@@ -296,198 +231,6 @@ __global__ MHC_ROW_BOUNDS(false) void layer_static_fwd_kernel(const TX* __restri
 // projection and r_h terms).  MODE 2 is MODE 1 with an fp32 dx of bf16 x.  dw
 // accumulates in registers and goes to dw_part[blockIdx.x][C].
 // ---------------------------------------------------------------------------
-// dx of a mode: the storage type, or fp32 with MODE 2
-template <typename TX, int MODE>
-using BwdDx = std::conditional_t<MODE == 2, float, TX>;
-
-template <typename TX, int N, int VPT, int MODE>
-__device__ __forceinline__ void bwd_token(int64_t b, const float* __restrict__ coef, int64_t coef_stride,
-                                          const float (&wv)[VPT][kLayerWC],
-                                          const float (&xv)[N][VPT][kLayerWC],
-                                          const float (&gv)[N][VPT][kLayerWC],
-                                          float (&dwacc)[VPT][kLayerWC], float& sacc,
-                                          BwdDx<TX, MODE>* __restrict__ dx, float* __restrict__ scal_out, int32_t* __restrict__ dx_scale, int C,
-                                          float eps, float* red) {
-    constexpr int WC = kLayerWC;
-    constexpr int NC = coef_size<N>();
-    constexpr int NS = N * N + 2 * N;
-    constexpr int NR = 2 + N * N + 3 * N;  // ss, dot, dM, t_i, u_j, v_j
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = threadIdx.x / kWave;
-    const int nwaves = blockDim.x / kWave;
-    float* tot = red + 8 * NR;
-    const float* cf = coef + b * coef_stride;
-    float cfv[NC];
-#pragma unroll
-    for (int k = 0; k < NC; ++k) cfv[k] = cf[k];
-    {
-        float rv[NR];
-#pragma unroll
-        for (int k = 0; k < NR; ++k) rv[k] = 0.f;
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-#pragma unroll
-            for (int e = 0; e < WC; ++e) {
-                float xa = 0.f, gy = 0.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    xa += cfv[i] * xv[i][k][e];
-                    gy += cfv[N + i] * gv[i][k][e];
-                }
-                const float wgy = wv[k][e] * gy;
-                const float wxa = wv[k][e] * xa;
-                rv[0] += xa * xa;
-                rv[1] += wgy * xa;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) rv[2 + i * N + j] += gv[i][k][e] * xv[j][k][e];
-                    rv[2 + N * N + i] += gv[i][k][e] * wxa;
-                    rv[2 + N * N + N + i] += wgy * xv[i][k][e];
-                    rv[2 + N * N + 2 * N + i] += xa * xv[i][k][e];
-                }
-            }
-        }
-        wave_sum_last<NR>(rv);
-        if (lane == kWave - 1) {
-#pragma unroll
-            for (int k = 0; k < NR; ++k) red[wave * NR + k] = rv[k];
-        }
-    }
-    __syncthreads();
-    if (threadIdx.x < NR) {
-        float s = 0.f;
-        for (int q = 0; q < nwaves; ++q) s += red[q * NR + threadIdx.x];
-        tot[threadIdx.x] = s;
-    }
-    __syncthreads();
-    const float r = sqrtf(tot[0] / (float)C + eps);
-    const float inv = 1.f / r;
-    const float k2 = tot[1] * inv * inv * inv / (float)C;
-
-    // Global stores of this routine go through resources with out-of-range
-    // offsets for lanes that store nothing: no store sits behind a branch
-    // (the caller's prefetch of the next token keeps exact wait counts).
-    float v = 0.f;
-    if (threadIdx.x < NS + 2) {
-        const int t = threadIdx.x;
-        if (t < N * N) {
-            v = tot[2 + t];
-        } else if (t < N * N + N) {
-            v = tot[2 + t] * inv;  // dh_post_act = (sum G_i xa w) / r
-        } else if (t < NS) {
-            const int j = t - N * N - N;
-            v = inv * tot[2 + N * N + N + j] - k2 * tot[2 + N * N + 2 * N + j];  // dh_pre_act
-        } else {
-            v = (t == NS) ? inv : k2;
-        }
-        if (MODE == 0) sacc += v;
-    }
-    if constexpr (MODE != 0) {
-        const buf_rsrc_t srs = make_buf_rsrc(scal_out + b * (NS + 2), (uint32_t)((NS + 2) * 4));
-        buf_st4(srs, threadIdx.x < NS + 2 ? (uint32_t)threadIdx.x * 4u : kBufOff, 0u, v);
-    }
-
-    if constexpr (MODE == 1 && sizeof(TX) == 2) {
-        // The dynamic backward's stream part with bf16 x: the projection
-        // kernel adds its terms and rounds the sum once, so this part travels
-        // as fp16 against a power-of-two scale (part_pack4), one scale
-        // exponent per half wave of this token: dx_scale[b][threadIdx.x / 32].
-        float a[N][VPT][WC];
-        float m = 0.f;  // largest |value|: fmaxf drops NaN, keeps +Inf
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-#pragma unroll
-            for (int e = 0; e < WC; ++e) {
-                float xa = 0.f, gy = 0.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    xa += cfv[i] * xv[i][k][e];
-                    gy += cfv[N + i] * gv[i][k][e];
-                }
-                const float gxa = wv[k][e] * gy * inv - xa * k2;
-                dwacc[k][e] += gy * xa * inv;
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    float s = kTermLast<N> ? 0.f : cfv[j] * gxa;
-#pragma unroll
-                    for (int i = 0; i < N; ++i) s += cfv[2 * N + i * N + j] * gv[i][k][e];
-                    if (kTermLast<N>) s += cfv[j] * gxa;
-                    a[j][k][e] = s;
-                    m = fmaxf(m, fabsf(s));
-                }
-            }
-        }
-        m = half_wave_max_nonneg(m);
-        if (__ballot(!(m < INFINITY))) {
-            // an infinite value in this wave: the scale comes from the finite
-            // values only (the whole wave takes this branch)
-            m = 0.f;
-#pragma unroll
-            for (int k = 0; k < VPT; ++k)
-#pragma unroll
-                for (int e = 0; e < WC; ++e)
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        const float v = fabsf(a[j][k][e]);
-                        m = v < INFINITY ? fmaxf(m, v) : m;
-                    }
-            m = half_wave_max_nonneg(m);
-        }
-        const int ks = part_scale_exp(m);
-        const buf_rsrc_t drs = make_buf_rsrc(dx + b * (int64_t)N * C, (uint32_t)((int64_t)N * C * 2));
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int c0 = (k * blockDim.x + threadIdx.x) * WC;
-            const uint32_t o0 = c0 < C ? (uint32_t)c0 * 2u : kBufOff;
-#pragma unroll
-            for (int j = 0; j < N; ++j) buf_st8<true>(drs, o0 + (uint32_t)(j * C * 2), 0u, part_pack4(a[j][k], ks));
-        }
-        const int ng = blockDim.x / 32;
-        const buf_rsrc_t qrs = make_buf_rsrc(dx_scale + b * ng, (uint32_t)(ng * 4));
-        buf_st4(qrs, (threadIdx.x & 31) == 0 ? (uint32_t)(threadIdx.x / 32) * 4u : kBufOff, 0u, __int_as_float(ks));
-    } else {
-        using TD = BwdDx<TX, MODE>;
-        const buf_rsrc_t drs = make_buf_rsrc(dx + b * (int64_t)N * C, (uint32_t)((int64_t)N * C * (int64_t)sizeof(TD)));
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int c0 = (k * blockDim.x + threadIdx.x) * WC;
-            float gxa[WC];
-#pragma unroll
-            for (int e = 0; e < WC; ++e) {
-                float xa = 0.f, gy = 0.f;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    xa += cfv[i] * xv[i][k][e];
-                    gy += cfv[N + i] * gv[i][k][e];
-                }
-                gxa[e] = wv[k][e] * gy * inv - xa * k2;
-                dwacc[k][e] += gy * xa * inv;
-            }
-            const uint32_t o0 = c0 < C ? (uint32_t)c0 * (uint32_t)sizeof(TD) : kBufOff;
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                float d[WC];
-#pragma unroll
-                for (int e = 0; e < WC; ++e) {
-                    float s = kTermLast<N> ? 0.f : cfv[j] * gxa[e];
-#pragma unroll
-                    for (int i = 0; i < N; ++i) s += cfv[2 * N + i * N + j] * gv[i][k][e];
-                    d[e] = kTermLast<N> ? s + cfv[j] * gxa[e] : s;
-                }
-                const uint32_t o = o0 + (uint32_t)(j * C * (int)sizeof(TD));
-                static_assert(WC == 4, "4-channel chunks: one 16-byte (fp32) or 8-byte (bf16) store");
-                if constexpr (sizeof(TD) == 4) {
-                    buf_st16<true>(drs, o, 0u, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]),
-                                                          __float_as_uint(d[2]), __float_as_uint(d[3])));
-                } else {
-                    buf_st8<true>(drs, o, 0u, make_uint2(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3])));
-                }
-            }
-        }
-    }
-}
-
 template <typename TX, int N, int VPT, int MODE, bool PF>
 __global__ MHC_ROW_BOUNDS(PF) void layer_bwd_kernel(const float* __restrict__ g, const TX* __restrict__ x,
                                                     const float* __restrict__ w, const float* __restrict__ coef,
@@ -1033,7 +776,7 @@ static bool use_prefetch(const RowTiling& t) { return t.threads <= 256; }
 // The register-row kernels take n <= 8 and a multiple of the 4-channel
 // chunk that fits their row state; everything else runs the channel-loop
 // kernels of wide.hip.
-static RowTiling fwd_tiling(int64_t C, int n) {
+RowTiling layer_fwd_tiling(int64_t C, int n) {
     if (n > 8 || (generic_layer_n(n) && !odd_row_n(n))) return RowTiling{0, 0};
     return choose_row_tiling(C, kLayerWC, n, 512);
 }
@@ -1050,13 +793,13 @@ static RowPath row_path(const RowTiling& t, int n, int64_t C, bool aligned) {
     return generic_layer_n(n) ? RowPath::kGen : RowPath::kWide;
 }
 
-bool layer_fwd_is_wide(int n, int64_t C) { return fwd_tiling(C, n).vpt <= 0; }
+bool layer_fwd_is_wide(int n, int64_t C) { return layer_fwd_tiling(C, n).vpt <= 0; }
 
 hipError_t launch_layer_fwd(int x_dtype, int n, const void* x, const float* w, const float* coef,
                             int64_t coef_stride, void* out, int out_dtype, float* rms_out, int64_t B, int64_t C,
                             float eps, hipStream_t s, int64_t rms_scratch) {
     if (B == 0) return hipSuccess;
-    const RowTiling t = fwd_tiling(C, n);
+    const RowTiling t = layer_fwd_tiling(C, n);
     const RowPath path = row_path(t, n, C, rows_aligned(n, {x, w, out}));
     if (path == RowPath::kGen)
         return launch_gen_layer_fwd(x_dtype, out_dtype, n, x, w, coef, coef_stride, out, rms_out, B, C, eps, s);
@@ -1082,13 +825,13 @@ static const void* static_fwd_fn() {
     return nullptr;
 }
 
-bool layer_static_fwd_fused(int n, int64_t C) { return n <= 8 && fwd_tiling(C, n).vpt > 0; }
+bool layer_static_fwd_fused(int n, int64_t C) { return n <= 8 && layer_fwd_tiling(C, n).vpt > 0; }
 
 hipError_t launch_layer_static_fwd(int x_dtype, int n, const void* x, const void* weight, int w_dtype,
                                    const float* h_pre, const float* h_post, const float* h_res, float* saved,
                                    int iters, float sk_eps, float* out, float* rms_out, int64_t B, int64_t C,
                                    float eps, hipStream_t s) {
-    const RowTiling t = fwd_tiling(C, n);
+    const RowTiling t = layer_fwd_tiling(C, n);
     if (t.vpt <= 0 || n > 8 || !rows_aligned(n, {x, weight, saved, out})) return hipErrorInvalidValue;
     if (B == 0) {
         // no tokens: the saved state alone (the backward still needs it)
@@ -1143,7 +886,7 @@ hipError_t launch_layer_static_fwd(int x_dtype, int n, const void* x, const void
 // once the CUs walk several tokens (B) and not before.  Backward row pass, dynamic n = 6, 2047 x 1040 bf16:
 // 43 us for 49; n = 5, 4096 x 1600 bf16: 72 for 85; n = 8, 4096 x 1280 fp32: 138
 // for 142; static n = 7, 4096 x 1184 fp32: 98 for 118.
-static RowTiling bwd_tiling(int64_t C, int n, int64_t B = 0) {
+RowTiling layer_bwd_tiling(int64_t C, int n, int64_t B) {
     if (n > 8 || (generic_layer_n(n) && !odd_row_n(n))) return RowTiling{0, 0};
     RowTiling t = choose_row_tiling(C, kLayerWC, 2 * n, 256);
     if (n >= 5 && t.vpt == 1 && t.threads > 256 && B >= 4 * (int64_t)device_cu_count() && layer_row_fits(2 * n, 2)) {
@@ -1153,20 +896,20 @@ static RowTiling bwd_tiling(int64_t C, int n, int64_t B = 0) {
     return with_min_threads(t, 2 + n * n + 3 * n);
 }
 
-bool layer_bwd_is_wide(int n, int64_t C) { return bwd_tiling(C, n).vpt <= 0; }
+bool layer_bwd_is_wide(int n, int64_t C) { return layer_bwd_tiling(C, n).vpt <= 0; }
 
 bool layer_bwd_f32_dx_ok(int n, int64_t C, bool aligned) {
-    return (n == 3 || (n >= 5 && n <= 8)) && row_path(bwd_tiling(C, n), n, C, aligned) == RowPath::kRegs;
+    return (n == 3 || (n >= 5 && n <= 8)) && row_path(layer_bwd_tiling(C, n), n, C, aligned) == RowPath::kRegs;
 }
 
 int layer_bwd_part_groups(int x_dtype, int n, int64_t C) {
     (void)x_dtype;  // the fp16 stream part is that of bf16 x at n = 2 and 4
-    const RowTiling t = bwd_tiling(C, n);
+    const RowTiling t = layer_bwd_tiling(C, n);
     return t.vpt > 0 ? t.threads / 32 : 0;
 }
 
 int layer_bwd_grid(int x_dtype, int n, int64_t B, int64_t C, bool aligned) {
-    const RowTiling t = bwd_tiling(C, n, B);
+    const RowTiling t = layer_bwd_tiling(C, n, B);
     const RowPath path = row_path(t, n, C, aligned);
     if (path == RowPath::kGen) return gen_layer_bwd_grid(B);
     if (path == RowPath::kWide) return wide_bwd_grid(x_dtype, n, B, C);
@@ -1174,7 +917,7 @@ int layer_bwd_grid(int x_dtype, int n, int64_t B, int64_t C, bool aligned) {
 }
 
 size_t layer_bwd_scratch_bytes(int x_dtype, int n, int64_t B, int64_t C, bool aligned) {
-    const RowPath path = row_path(bwd_tiling(C, n, B), n, C, aligned);
+    const RowPath path = row_path(layer_bwd_tiling(C, n, B), n, C, aligned);
     if (path == RowPath::kGen) return gen_layer_bwd_scratch_bytes(B, C);
     return path == RowPath::kWide ? wide_bwd_scratch_bytes(n, B, C) : 0;
 }
@@ -1183,7 +926,7 @@ hipError_t launch_layer_bwd(int x_dtype, int n, int mode, const float* g, const 
                             const float* coef, int64_t coef_stride, void* dx, float* dw_part, float* scal_out,
                             int grid, int64_t B, int64_t C, float eps, float* scratch, hipStream_t s,
                             int32_t* dx_scale, bool aligned) {
-    const RowTiling t = bwd_tiling(C, n, B);
+    const RowTiling t = layer_bwd_tiling(C, n, B);
     const RowPath path = row_path(t, n, C, aligned);
     if (mode == 2 && path != RowPath::kRegs) return hipErrorInvalidValue;
     if (path == RowPath::kGen) {

@@ -1,0 +1,292 @@
+// The fused layer's register-row passes with the token rows in 8 bits
+// (mhc_ckpt.h): the forward writes the checkpoint of the row it holds, the
+// backward reads the row x^ from it.  Arithmetic per token as the kernels of
+// layer.hip (mhc_layer_rows.h), n = 2..8 on rows those take, 16-byte aligned
+// arrays; other shapes run layer.hip / wide.hip / generic.hip with a pack or
+// unpack pass.
+//
+// A lane holds 4 channels of a chunk, so 8 lanes a block of 32: the block's
+// maximum is three DPP steps.  Both passes are bound by their bytes; the
+// pack pass (a second read of x) and the unpack pass (x^ written and read)
+// are what they save.
+#include "mhc_ckpt.h"
+#include "mhc_device.h"
+#include "mhc_internal.h"
+#include "mhc_layer_rows.h"
+#include "mhc_rows.h"
+
+namespace mhc {
+
+// ---------------------------------------------------------------------------
+// Rows to and from the checkpoint, through buffer resources over one token's
+// values [N][stride] and scales [N][nb] (no access behind a branch).
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t held_ld4(buf_rsrc_t r, uint32_t off) {
+    return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 2);
+}
+__device__ __forceinline__ uint32_t held_ld1(buf_rsrc_t r, uint32_t off) {
+    return (uint32_t)(uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
+}
+
+template <int N, int VPT>
+struct HeldRows {
+    uint32_t q[N][VPT];  // 4 values
+    uint32_t s[N][VPT];  // their block's scale byte
+};
+
+// Lanes past the row read zeros, and a token past the end (no bytes) too:
+// zeros stand for 0.
+template <int N, int VPT>
+__device__ __forceinline__ void held_load(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc, int64_t b,
+                                          int64_t B, int C, HeldRows<N, VPT>& r) {
+    const int stride = (int)ck_stride(C), nb = (int)ck_blocks(C);
+    const int64_t bb = b < B ? b : 0;
+    const buf_rsrc_t rq = make_buf_rsrc(q + bb * N * stride, b < B ? (uint32_t)(N * stride) : 0u);
+    const buf_rsrc_t rs = make_buf_rsrc(sc + bb * N * nb, b < B ? (uint32_t)(N * nb) : 0u);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * kLayerWC;
+        const uint32_t oq = c0 < C ? (uint32_t)c0 : kBufOff, os = c0 < C ? (uint32_t)(c0 >> 5) : kBufOff;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            r.q[i][k] = held_ld4(rq, oq + (uint32_t)(i * stride));
+            r.s[i][k] = held_ld1(rs, os + (uint32_t)(i * nb));
+        }
+    }
+}
+
+template <int FMT, int N, int VPT>
+__device__ __forceinline__ void held_get(const HeldRows<N, VPT>& r, float (&v)[N][VPT][kLayerWC]) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) Ck<FMT>::unpack4(r.q[i][k], Ck<FMT>::down(r.s[i][k]), v[i][k]);
+    }
+}
+
+template <int FMT, int N, int VPT>
+__device__ __forceinline__ void held_put(const float (&v)[N][VPT][kLayerWC], uint8_t* __restrict__ q,
+                                         uint8_t* __restrict__ sc, int64_t b, int C) {
+    const int stride = (int)ck_stride(C), nb = (int)ck_blocks(C);
+    const buf_rsrc_t rq = make_buf_rsrc(q + b * N * stride, (uint32_t)(N * stride));
+    const buf_rsrc_t rs = make_buf_rsrc(sc + b * N * nb, (uint32_t)(N * nb));
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * kLayerWC;
+        const uint32_t oq = c0 < stride ? (uint32_t)c0 : kBufOff;  // the padding too
+        const uint32_t os = c0 < C && (threadIdx.x & 7) == 0 ? (uint32_t)(c0 >> 5) : kBufOff;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float(&f)[kLayerWC] = v[i][k];
+            uint32_t a = ck_abs_bits(f[0]);
+#pragma unroll
+            for (int e = 1; e < kLayerWC; ++e) a = a > ck_abs_bits(f[e]) ? a : ck_abs_bits(f[e]);
+            const uint32_t s = Ck<FMT>::scale(ck_group_max<8>(a));
+            const uint32_t w = Ck<FMT>::pack4(f[0], f[1], f[2], f[3], Ck<FMT>::up(s), s == 255u ? 0u : ~0u);
+            __builtin_amdgcn_raw_buffer_store_b32(w, rq, (int)(oq + (uint32_t)(i * stride)), 0, 2);
+            __builtin_amdgcn_raw_buffer_store_b8((uint8_t)s, rs, (int)(os + (uint32_t)(i * nb)), 0, 0);
+        }
+    }
+}
+
+template <typename TX, int N, int VPT, int FMT>
+__global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(const TX* __restrict__ x, const float* __restrict__ w,
+                                                            const float* __restrict__ coef, int64_t coef_stride,
+                                                            float* __restrict__ out, uint8_t* __restrict__ q,
+                                                            uint8_t* __restrict__ sc, int C, float eps) {
+    constexpr int WC = kLayerWC;
+    __shared__ float red[8];
+    const int64_t b = blockIdx.x;  // one token per workgroup
+    RawRows<TX, N, VPT, WC> xr;
+    load_rows_raw<TX, N, VPT, WC, true>(x + b * (int64_t)N * C, C, xr);
+    float wv[VPT][WC];
+    load_weight<VPT, WC>(w, C, wv);
+    float xv[N][VPT][WC];
+    unpack_rows<TX, N, VPT, WC>(xr, C, xv);
+    held_put<FMT, N, VPT>(xv, q, sc, b, C);
+    fwd_token<TX, float, N, VPT>(b, coef, coef_stride, wv, xv, out, nullptr, C, eps, red);
+}
+
+// As layer_bwd_kernel: persistent workgroups over tokens, with PF the next
+// token's rows in flight.  TX is dx's storage type.
+template <typename TX, int N, int VPT, int MODE, int FMT, bool PF>
+__global__ MHC_ROW_BOUNDS(PF) void layer_ckpt_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict__ q,
+                                                         const uint8_t* __restrict__ sc, const float* __restrict__ w,
+                                                         const float* __restrict__ coef, int64_t coef_stride,
+                                                         BwdDx<TX, MODE>* __restrict__ dx,
+                                                         float* __restrict__ dw_part, float* __restrict__ scal_out,
+                                                         int32_t* __restrict__ dx_scale, int64_t B, int C, float eps) {
+    constexpr int WC = kLayerWC;
+    constexpr int NS = N * N + 2 * N;
+    constexpr int NR = 2 + N * N + 3 * N;
+    __shared__ float red[9 * NR];  // 8 wave partials + totals
+    float wv[VPT][WC];
+    load_weight<VPT, WC>(w, C, wv);
+    float dwacc[VPT][WC];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+        for (int e = 0; e < WC; ++e) dwacc[k][e] = 0.f;
+    }
+    float sacc = 0.f;
+    const int64_t G = gridDim.x;
+    int64_t b = blockIdx.x;
+    float xv[N][VPT][WC], gv[N][VPT][WC];
+    const auto token = [&](int64_t t, const HeldRows<N, VPT>& xr, const RawRows<float, N, VPT, WC>& gr) {
+        held_get<FMT, N, VPT>(xr, xv);
+        unpack_rows<float, N, VPT, WC>(gr, C, gv);
+        bwd_token<TX, N, VPT, MODE>(t, coef, coef_stride, wv, xv, gv, dwacc, sacc, dx, scal_out, dx_scale, C, eps, red);
+    };
+    if constexpr (PF) {
+        HeldRows<N, VPT> xA, xB;
+        RawRows<float, N, VPT, WC> gA, gB;
+        held_load<N, VPT>(q, sc, b, B, C, xA);
+        load_rows_raw_rs<float, N, VPT, WC, true>(token_rows_rsrc(g, b, B, N, C), C, gA);
+        while (b < B) {
+            const int64_t b1 = b + G;
+            held_load<N, VPT>(q, sc, b1, B, C, xB);
+            load_rows_raw_rs<float, N, VPT, WC, true>(token_rows_rsrc(g, b1, B, N, C), C, gB);
+            token(b, xA, gA);
+            if (b1 >= B) break;
+            const int64_t b2 = b1 + G;
+            held_load<N, VPT>(q, sc, b2, B, C, xA);
+            load_rows_raw_rs<float, N, VPT, WC, true>(token_rows_rsrc(g, b2, B, N, C), C, gA);
+            token(b1, xB, gB);
+            b = b2;
+        }
+    } else {
+        for (; b < B; b += G) {
+            HeldRows<N, VPT> xr;
+            RawRows<float, N, VPT, WC> gr;
+            held_load<N, VPT>(q, sc, b, B, C, xr);
+            load_rows_raw<float, N, VPT, WC, true>(g + b * (int64_t)N * C, C, gr);
+            token(b, xr, gr);
+        }
+    }
+    float* dwp = dw_part + (int64_t)blockIdx.x * C;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * WC;
+        if (c0 < C) store_run<float, WC>(dwp + c0, dwacc[k]);
+    }
+    if (MODE == 0 && threadIdx.x < NS) scal_out[(int64_t)blockIdx.x * NS + threadIdx.x] = sacc;
+}
+
+// ---------------------------------------------------------------------------
+// Host launchers
+// ---------------------------------------------------------------------------
+#define MHC_CL_VPT(v, ...)                                       \
+    switch (v) {                                                 \
+        case 1: { constexpr int V_ = 1; __VA_ARGS__; break; }    \
+        case 2: { constexpr int V_ = 2; __VA_ARGS__; break; }    \
+        case 4: { constexpr int V_ = 4; __VA_ARGS__; break; }    \
+        case 8: { constexpr int V_ = 8; __VA_ARGS__; break; }    \
+        default: break;                                          \
+    }
+#define MHC_CL_N(n, ...)                                         \
+    switch (n) {                                                 \
+        case 2: { constexpr int N_ = 2; __VA_ARGS__; break; }    \
+        case 3: { constexpr int N_ = 3; __VA_ARGS__; break; }    \
+        case 4: { constexpr int N_ = 4; __VA_ARGS__; break; }    \
+        case 5: { constexpr int N_ = 5; __VA_ARGS__; break; }    \
+        case 6: { constexpr int N_ = 6; __VA_ARGS__; break; }    \
+        case 7: { constexpr int N_ = 7; __VA_ARGS__; break; }    \
+        case 8: { constexpr int N_ = 8; __VA_ARGS__; break; }    \
+        default: break;                                          \
+    }
+
+template <typename TX, int N, int V, int FMT>
+static const void* ck_fwd_fn() {
+    if constexpr (layer_row_fits(N, V)) return reinterpret_cast<const void*>(&layer_ckpt_fwd_kernel<TX, N, V, FMT>);
+    return nullptr;
+}
+
+template <typename TX, int N, int V, int MODE, int FMT>
+static const void* ck_bwd_fn(bool pf) {
+    if constexpr (layer_row_fits(2 * N, V))
+        return pf ? reinterpret_cast<const void*>(&layer_ckpt_bwd_kernel<TX, N, V, MODE, FMT, true>)
+                  : reinterpret_cast<const void*>(&layer_ckpt_bwd_kernel<TX, N, V, MODE, FMT, false>);
+    return nullptr;
+}
+
+static const void* pick_ck_fwd(int x_dtype, int fmt, int n, int vpt) {
+    const void* fn = nullptr;
+    MHC_CL_N(n, MHC_CL_VPT(vpt, {
+                 if (x_dtype == kBF16)
+                     fn = fmt == kCkInt8 ? ck_fwd_fn<bf16_t, N_, V_, kCkInt8>() : ck_fwd_fn<bf16_t, N_, V_, kCkE4M3>();
+                 else
+                     fn = fmt == kCkInt8 ? ck_fwd_fn<float, N_, V_, kCkInt8>() : ck_fwd_fn<float, N_, V_, kCkE4M3>();
+             }));
+    return fn;
+}
+
+template <int FMT, int N, int V>
+static const void* pick_ck_bwd_mode(int x_dtype, int mode, bool pf) {
+    const bool bf = x_dtype == kBF16;
+    if (mode == 0) return bf ? ck_bwd_fn<bf16_t, N, V, 0, FMT>(pf) : ck_bwd_fn<float, N, V, 0, FMT>(pf);
+    return nullptr;
+}
+
+static const void* pick_ck_bwd(int x_dtype, int fmt, int n, int vpt, int mode, bool pf) {
+    const void* fn = nullptr;
+    MHC_CL_N(n, MHC_CL_VPT(vpt, fn = fmt == kCkInt8 ? pick_ck_bwd_mode<kCkInt8, N_, V_>(x_dtype, mode, pf)
+                                                    : pick_ck_bwd_mode<kCkE4M3, N_, V_>(x_dtype, mode, pf)));
+    return fn;
+}
+
+static bool ck_aligned(std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return false;
+    return true;
+}
+
+bool layer_ckpt_fwd_rows(int n, int64_t B, int64_t C, std::initializer_list<const void*> ps) {
+    return n >= 2 && n <= 8 && B > 0 && B <= 0x7fffffff && layer_fwd_tiling(C, n).vpt > 0 && ck_aligned(ps);
+}
+
+bool layer_ckpt_bwd_rows(int n, int64_t B, int64_t C, std::initializer_list<const void*> ps) {
+    return n >= 2 && n <= 8 && B > 0 && layer_bwd_tiling(C, n, B).vpt > 0 && ck_aligned(ps);
+}
+
+hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, const float* w, const float* coef,
+                                 int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
+                                 float eps, hipStream_t s) {
+    const RowTiling t = layer_fwd_tiling(C, n);
+    const void* fn = pick_ck_fwd(x_dtype, fmt, n, t.vpt);
+    if (!fn) return hipErrorInvalidValue;
+    int Ci = (int)C;
+    void* args[] = {(void*)&x,   (void*)&w,      (void*)&coef,   (void*)&coef_stride, (void*)&out,
+                    (void*)&values, (void*)&scales, (void*)&Ci, (void*)&eps};
+    const int tok = timing_begin("layer_ckpt_fwd", s);
+    hipError_t e = mhc_launch_kernel(fn, dim3((unsigned)B), dim3(t.threads), args, 0, s);
+    timing_end(tok, s);
+    return e != hipSuccess ? e : hipGetLastError();
+}
+
+// workgroups of at most 256 lanes prefetch (layer.hip)
+static bool ck_prefetch(const RowTiling& t) { return t.threads <= 256; }
+
+int layer_ckpt_bwd_grid(int x_dtype, int fmt, int n, int mode, int64_t B, int64_t C) {
+    const RowTiling t = layer_bwd_tiling(C, n, B);
+    const int64_t g = (int64_t)device_cu_count() *
+                      occupancy_per_cu(pick_ck_bwd(x_dtype, fmt, n, t.vpt, mode, ck_prefetch(t)), t.threads, 0);
+    return (int)(g < B ? g : (B < 1 ? 1 : B));
+}
+
+hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const float* g, const void* values,
+                                 const void* scales, const float* w, const float* coef, int64_t coef_stride, void* dx,
+                                 float* dw_part, float* scal_out, int grid, int64_t B, int64_t C, float eps,
+                                 hipStream_t s, int32_t* dx_scale) {
+    const RowTiling t = layer_bwd_tiling(C, n, B);
+    const void* fn = pick_ck_bwd(x_dtype, fmt, n, t.vpt, mode, ck_prefetch(t));
+    if (!fn) return hipErrorInvalidValue;
+    int Ci = (int)C;
+    void* args[] = {(void*)&g,       (void*)&values,   (void*)&scales,   (void*)&w, (void*)&coef, (void*)&coef_stride, (void*)&dx,
+                    (void*)&dw_part, (void*)&scal_out, (void*)&dx_scale, (void*)&B, (void*)&Ci,   (void*)&eps};
+    const int tok = timing_begin("layer_ckpt_bwd", s);
+    hipError_t e = mhc_launch_kernel(fn, dim3(grid), dim3(t.threads), args, 0, s);
+    timing_end(tok, s);
+    return e != hipSuccess ? e : hipGetLastError();
+}
+
+}  // namespace mhc

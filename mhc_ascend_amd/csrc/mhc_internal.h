@@ -177,6 +177,9 @@ size_t layer_bwd_scratch_bytes(int x_dtype, int n, int64_t B, int64_t C, bool al
 // Whether the layer forward / backward of (n, C) runs the channel-loop
 // kernels of wide.hip rather than the register rows.
 bool layer_fwd_is_wide(int n, int64_t C);
+// register tilings (vpt 0: none fits)
+RowTiling layer_fwd_tiling(int64_t C, int n);
+RowTiling layer_bwd_tiling(int64_t C, int n, int64_t B = 0);
 bool layer_bwd_is_wide(int n, int64_t C);
 // launch_layer_bwd takes mode 2: register rows of n = 3, 5..8
 bool layer_bwd_f32_dx_ok(int n, int64_t C, bool aligned);
@@ -290,6 +293,21 @@ int rmsnorm_ckpt_bwd_grid(int dt, int fmt, int64_t B, int64_t C);
 hipError_t launch_rmsnorm_ckpt_bwd(int dt, int fmt, const void* g, const void* values, const void* scales,
                                    const float* w, void* gx, float* dw_part, int grid, int64_t B, int64_t C,
                                    float eps, hipStream_t s);
+
+// ---- layer_ckpt.hip --------------------------------------------------------
+// launch_layer_fwd / launch_layer_bwd (modes as there) on rows in a
+// checkpoint: n = 2..8 with register tilings, every array of `ps` 16-byte
+// aligned.
+bool layer_ckpt_fwd_rows(int n, int64_t B, int64_t C, std::initializer_list<const void*> ps);
+bool layer_ckpt_bwd_rows(int n, int64_t B, int64_t C, std::initializer_list<const void*> ps);
+hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, const float* w, const float* coef,
+                                 int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
+                                 float eps, hipStream_t s);
+int layer_ckpt_bwd_grid(int x_dtype, int fmt, int n, int mode, int64_t B, int64_t C);
+hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const float* g, const void* values,
+                                 const void* scales, const float* w, const float* coef, int64_t coef_stride, void* dx,
+                                 float* dw_part, float* scal_out, int grid, int64_t B, int64_t C, float eps,
+                                 hipStream_t s, int32_t* dx_scale = nullptr);
 
 // ---- qk_norm_rope.hip ------------------------------------------------------
 // Head rows of queries ([0]) and keys ([1]); strides in elements.  Token t's

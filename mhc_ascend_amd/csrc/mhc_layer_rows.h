@@ -1,0 +1,272 @@
+// The per-token arithmetic of the fused layer's register-row kernels (layer.hip,
+// and layer_ckpt.hip, whose rows come from or go to an 8-bit checkpoint): one
+// workgroup holds a token's row, as the formulas at the head of layer.hip.
+#pragma once
+
+#include <type_traits>
+
+#include "mhc_device.h"
+#include "mhc_internal.h"
+#include "mhc_rows.h"
+
+namespace mhc {
+
+template <int N> constexpr int coef_size() { return 2 * N + N * N; }
+
+template <typename TX, typename TO, int N, int VPT>
+__device__ __forceinline__ void fwd_token(int64_t b, const float* __restrict__ coef, int64_t coef_stride,
+                                          const float (&wv)[VPT][kLayerWC],
+                                          const float (&xv)[N][VPT][kLayerWC], TO* __restrict__ out,
+                                          float* __restrict__ rms_out, int C, float eps, float* red) {
+    constexpr int WC = kLayerWC;
+    constexpr int NC = coef_size<N>();
+    const float* cf = coef + b * coef_stride;
+    float cfv[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) cfv[k] = cf[k];
+    float xa[VPT][WC];
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+        for (int e = 0; e < WC; ++e) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += cfv[i] * xv[i][k][e];
+            xa[k][e] = s;
+            ss += s * s;
+        }
+    }
+    float v[1] = {ss};
+    block_sum<1>(v, red);
+    const float r = sqrtf(v[0] / (float)C + eps);
+    const float inv = 1.f / r;
+    // stores through a resource over the token's output rows, out-of-range
+    // offsets past the row end (no store behind a branch)
+    const buf_rsrc_t ors = make_buf_rsrc(out + b * (int64_t)N * C, (uint32_t)((int64_t)N * C * (int64_t)sizeof(TO)));
+    static_assert(WC == 4, "4-channel chunks: one 16-byte (fp32) or 8-byte (bf16) store");
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * WC;
+        const uint32_t o0 = c0 < C ? (uint32_t)c0 * (uint32_t)sizeof(TO) : kBufOff;
+        float y[WC];
+#pragma unroll
+        for (int e = 0; e < WC; ++e) y[e] = xa[k][e] * inv * wv[k][e];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float o[WC];
+#pragma unroll
+            for (int e = 0; e < WC; ++e) {
+                float s = kTermLast<N> ? 0.f : cfv[N + i] * y[e];
+#pragma unroll
+                for (int j = 0; j < N; ++j) s += cfv[2 * N + i * N + j] * xv[j][k][e];
+                o[e] = kTermLast<N> ? s + cfv[N + i] * y[e] : s;
+            }
+            const uint32_t off = o0 + (uint32_t)(i * C * (int)sizeof(TO));
+            if constexpr (sizeof(TO) == 4) {
+                buf_st16<true>(ors, off, 0u, make_uint4(__float_as_uint(o[0]), __float_as_uint(o[1]),
+                                                        __float_as_uint(o[2]), __float_as_uint(o[3])));
+            } else {
+                buf_st8<true>(ors, off, 0u, make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])));
+            }
+        }
+    }
+    if (rms_out) {
+        const buf_rsrc_t rrs = make_buf_rsrc(rms_out + b, 4u);
+        buf_st4(rrs, threadIdx.x == 0 ? 0u : kBufOff, 0u, r);
+    }
+}
+
+// dx of a mode: the storage type, or fp32 with MODE 2
+template <typename TX, int MODE>
+using BwdDx = std::conditional_t<MODE == 2, float, TX>;
+
+template <typename TX, int N, int VPT, int MODE>
+__device__ __forceinline__ void bwd_token(int64_t b, const float* __restrict__ coef, int64_t coef_stride,
+                                          const float (&wv)[VPT][kLayerWC],
+                                          const float (&xv)[N][VPT][kLayerWC],
+                                          const float (&gv)[N][VPT][kLayerWC],
+                                          float (&dwacc)[VPT][kLayerWC], float& sacc,
+                                          BwdDx<TX, MODE>* __restrict__ dx, float* __restrict__ scal_out, int32_t* __restrict__ dx_scale, int C,
+                                          float eps, float* red) {
+    constexpr int WC = kLayerWC;
+    constexpr int NC = coef_size<N>();
+    constexpr int NS = N * N + 2 * N;
+    constexpr int NR = 2 + N * N + 3 * N;  // ss, dot, dM, t_i, u_j, v_j
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = threadIdx.x / kWave;
+    const int nwaves = blockDim.x / kWave;
+    float* tot = red + 8 * NR;
+    const float* cf = coef + b * coef_stride;
+    float cfv[NC];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) cfv[k] = cf[k];
+    {
+        float rv[NR];
+#pragma unroll
+        for (int k = 0; k < NR; ++k) rv[k] = 0.f;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < WC; ++e) {
+                float xa = 0.f, gy = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    xa += cfv[i] * xv[i][k][e];
+                    gy += cfv[N + i] * gv[i][k][e];
+                }
+                const float wgy = wv[k][e] * gy;
+                const float wxa = wv[k][e] * xa;
+                rv[0] += xa * xa;
+                rv[1] += wgy * xa;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) rv[2 + i * N + j] += gv[i][k][e] * xv[j][k][e];
+                    rv[2 + N * N + i] += gv[i][k][e] * wxa;
+                    rv[2 + N * N + N + i] += wgy * xv[i][k][e];
+                    rv[2 + N * N + 2 * N + i] += xa * xv[i][k][e];
+                }
+            }
+        }
+        wave_sum_last<NR>(rv);
+        if (lane == kWave - 1) {
+#pragma unroll
+            for (int k = 0; k < NR; ++k) red[wave * NR + k] = rv[k];
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < NR) {
+        float s = 0.f;
+        for (int q = 0; q < nwaves; ++q) s += red[q * NR + threadIdx.x];
+        tot[threadIdx.x] = s;
+    }
+    __syncthreads();
+    const float r = sqrtf(tot[0] / (float)C + eps);
+    const float inv = 1.f / r;
+    const float k2 = tot[1] * inv * inv * inv / (float)C;
+
+    // Global stores of this routine go through resources with out-of-range
+    // offsets for lanes that store nothing: no store sits behind a branch
+    // (the caller's prefetch of the next token keeps exact wait counts).
+    float v = 0.f;
+    if (threadIdx.x < NS + 2) {
+        const int t = threadIdx.x;
+        if (t < N * N) {
+            v = tot[2 + t];
+        } else if (t < N * N + N) {
+            v = tot[2 + t] * inv;  // dh_post_act = (sum G_i xa w) / r
+        } else if (t < NS) {
+            const int j = t - N * N - N;
+            v = inv * tot[2 + N * N + N + j] - k2 * tot[2 + N * N + 2 * N + j];  // dh_pre_act
+        } else {
+            v = (t == NS) ? inv : k2;
+        }
+        if (MODE == 0) sacc += v;
+    }
+    if constexpr (MODE != 0) {
+        const buf_rsrc_t srs = make_buf_rsrc(scal_out + b * (NS + 2), (uint32_t)((NS + 2) * 4));
+        buf_st4(srs, threadIdx.x < NS + 2 ? (uint32_t)threadIdx.x * 4u : kBufOff, 0u, v);
+    }
+
+    if constexpr (MODE == 1 && sizeof(TX) == 2) {
+        // The dynamic backward's stream part with bf16 x: the projection
+        // kernel adds its terms and rounds the sum once, so this part travels
+        // as fp16 against a power-of-two scale (part_pack4), one scale
+        // exponent per half wave of this token: dx_scale[b][threadIdx.x / 32].
+        float a[N][VPT][WC];
+        float m = 0.f;  // largest |value|: fmaxf drops NaN, keeps +Inf
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < WC; ++e) {
+                float xa = 0.f, gy = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    xa += cfv[i] * xv[i][k][e];
+                    gy += cfv[N + i] * gv[i][k][e];
+                }
+                const float gxa = wv[k][e] * gy * inv - xa * k2;
+                dwacc[k][e] += gy * xa * inv;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    float s = kTermLast<N> ? 0.f : cfv[j] * gxa;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) s += cfv[2 * N + i * N + j] * gv[i][k][e];
+                    if (kTermLast<N>) s += cfv[j] * gxa;
+                    a[j][k][e] = s;
+                    m = fmaxf(m, fabsf(s));
+                }
+            }
+        }
+        m = half_wave_max_nonneg(m);
+        if (__ballot(!(m < INFINITY))) {
+            // an infinite value in this wave: the scale comes from the finite
+            // values only (the whole wave takes this branch)
+            m = 0.f;
+#pragma unroll
+            for (int k = 0; k < VPT; ++k)
+#pragma unroll
+                for (int e = 0; e < WC; ++e)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const float v = fabsf(a[j][k][e]);
+                        m = v < INFINITY ? fmaxf(m, v) : m;
+                    }
+            m = half_wave_max_nonneg(m);
+        }
+        const int ks = part_scale_exp(m);
+        const buf_rsrc_t drs = make_buf_rsrc(dx + b * (int64_t)N * C, (uint32_t)((int64_t)N * C * 2));
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c0 = (k * blockDim.x + threadIdx.x) * WC;
+            const uint32_t o0 = c0 < C ? (uint32_t)c0 * 2u : kBufOff;
+#pragma unroll
+            for (int j = 0; j < N; ++j) buf_st8<true>(drs, o0 + (uint32_t)(j * C * 2), 0u, part_pack4(a[j][k], ks));
+        }
+        const int ng = blockDim.x / 32;
+        const buf_rsrc_t qrs = make_buf_rsrc(dx_scale + b * ng, (uint32_t)(ng * 4));
+        buf_st4(qrs, (threadIdx.x & 31) == 0 ? (uint32_t)(threadIdx.x / 32) * 4u : kBufOff, 0u, __int_as_float(ks));
+    } else {
+        using TD = BwdDx<TX, MODE>;
+        const buf_rsrc_t drs = make_buf_rsrc(dx + b * (int64_t)N * C, (uint32_t)((int64_t)N * C * (int64_t)sizeof(TD)));
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c0 = (k * blockDim.x + threadIdx.x) * WC;
+            float gxa[WC];
+#pragma unroll
+            for (int e = 0; e < WC; ++e) {
+                float xa = 0.f, gy = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    xa += cfv[i] * xv[i][k][e];
+                    gy += cfv[N + i] * gv[i][k][e];
+                }
+                gxa[e] = wv[k][e] * gy * inv - xa * k2;
+                dwacc[k][e] += gy * xa * inv;
+            }
+            const uint32_t o0 = c0 < C ? (uint32_t)c0 * (uint32_t)sizeof(TD) : kBufOff;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                float d[WC];
+#pragma unroll
+                for (int e = 0; e < WC; ++e) {
+                    float s = kTermLast<N> ? 0.f : cfv[j] * gxa[e];
+#pragma unroll
+                    for (int i = 0; i < N; ++i) s += cfv[2 * N + i * N + j] * gv[i][k][e];
+                    d[e] = kTermLast<N> ? s + cfv[j] * gxa[e] : s;
+                }
+                const uint32_t o = o0 + (uint32_t)(j * C * (int)sizeof(TD));
+                static_assert(WC == 4, "4-channel chunks: one 16-byte (fp32) or 8-byte (bf16) store");
+                if constexpr (sizeof(TD) == 4) {
+                    buf_st16<true>(drs, o, 0u, make_uint4(__float_as_uint(d[0]), __float_as_uint(d[1]),
+                                                          __float_as_uint(d[2]), __float_as_uint(d[3])));
+                } else {
+                    buf_st8<true>(drs, o, 0u, make_uint2(pack_bf16x2(d[0], d[1]), pack_bf16x2(d[2], d[3])));
+                }
+            }
+        }
+    }
+}
+
+}  // namespace mhc
