@@ -418,13 +418,11 @@ int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* 
                                     float* saved, int32_t format, void* values, void* scales, int64_t batch,
                                     int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
                                     float rmsnorm_eps, void* stream);
-size_t mhc_layer_static_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype);
-/* What a backward on these arrays needs, at most the query above: no share for
- * x^ rows where the row kernel reads the checkpoint (n = 2..8, hidden a
- * multiple of 4 that fits its registers, 16-byte aligned arrays). */
+/* The workspace of a backward on these arrays: the row kernels read the
+ * checkpoint for n = 2..8, hidden a multiple of 4 (8 with dynamic H) that fits
+ * their registers and 16-byte aligned arrays; other calls keep x^ rows there. */
 size_t mhc_layer_static_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
-                                                      int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
-                                                      int32_t format);
+                                                      int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype);
 int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
                                     int32_t x_dtype, int32_t weight_dtype, const float* h_pre, const float* h_post,
                                     const float* h_res, const float* saved, void* grad_x, void* grad_weight,
@@ -442,7 +440,9 @@ int mhc_layer_dynamic_checkpoint_fwd(const void* x, int32_t x_dtype, const void*
                                      float* saved, int32_t format, void* values, void* scales, void* workspace,
                                      size_t workspace_bytes, int64_t batch, int32_t n, int32_t hidden,
                                      int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps, void* stream);
-size_t mhc_layer_dynamic_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype);
+size_t mhc_layer_dynamic_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
+                                                       int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
+                                                       int32_t num_iters);
 int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
                                      int32_t x_dtype, int32_t weight_dtype, const float* phi_pre,
                                      const float* phi_post, const float* phi_res, const float* alpha_pre,

@@ -123,15 +123,14 @@ SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
                                                   _vp]),
     "mhc_layer_static_checkpoint_fwd": (ctypes.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp,
                                                        _i64, _i32, _i32, _i32, _f32, _f32, _vp]),
-    "mhc_layer_static_checkpoint_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
-    "mhc_layer_static_checkpoint_bwd_workspace_need": (_sz, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32]),
+    "mhc_layer_static_checkpoint_bwd_workspace_need": (_sz, [_vp, _vp, _vp, _i64, _i32, _i32, _i32]),
     "mhc_layer_static_checkpoint_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                                        _vp, _vp, _vp, _vp, _sz, _i64, _i32, _i32, _i32, _f32, _f32,
                                                        _vp]),
     "mhc_layer_dynamic_checkpoint_fwd": (ctypes.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                                         _vp, _vp, _vp, _i32, _vp, _vp, _vp, _sz, _i64, _i32, _i32,
                                                         _i32, _f32, _f32, _vp]),
-    "mhc_layer_dynamic_checkpoint_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "mhc_layer_dynamic_checkpoint_bwd_workspace_need": (_sz, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32]),
     "mhc_layer_dynamic_checkpoint_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                                         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64,
                                                         _i32, _i32, _i32, _f32, _f32, _vp]),

@@ -838,12 +838,14 @@ static int check_dyn(const char* fn, int64_t batch, int32_t n, int32_t hidden, i
     return MHC_SUCCESS;
 }
 
-int mhc_layer_dynamic_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype,
-                          const float* phi_pre, const float* phi_post, const float* phi_res, const float* alpha_pre,
-                          const float* alpha_post, const float* alpha_res, const float* b_pre, const float* b_post,
-                          const float* b_res, float* out, float* saved, void* workspace, size_t workspace_bytes,
-                          int64_t batch, int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
-                          float rmsnorm_eps, void* stream) {
+// format >= 0: the checkpoint of x's rows too, by the row pass itself where it
+// can write it
+static int dynamic_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype, const float* phi_pre,
+                       const float* phi_post, const float* phi_res, const float* alpha_pre, const float* alpha_post,
+                       const float* alpha_res, const float* b_pre, const float* b_post, const float* b_res, float* out,
+                       float* saved, int32_t format, void* values, void* scales, void* workspace,
+                       size_t workspace_bytes, int64_t batch, int32_t n, int32_t hidden, int32_t num_iters,
+                       float sinkhorn_eps, float rmsnorm_eps, void* stream) {
     int st = check_dyn("layer_dynamic_fwd", batch, n, hidden, x_dtype, weight_dtype, num_iters);
     if (st) return st;
     MHC_REQUIRE(weight && phi_pre && phi_post && phi_res && alpha_pre && alpha_post && alpha_res && b_pre &&
@@ -882,13 +884,32 @@ int mhc_layer_dynamic_fwd(const void* x, int32_t x_dtype, const void* weight, in
         e = launch_dyn_coef_fwd(n, pp, ss, w.ks, batch, K, alpha_pre, alpha_post, alpha_res, b_pre, b_post, b_res,
                                 saved + d.coef_off, saved + d.p_off, saved + d.rh_off, num_iters, sinkhorn_eps,
                                 rmsnorm_eps, s);
+    if (format >= 0 && layer_ckpt_fwd_rows(n, batch, hidden, {x, out, saved, values})) {
+        if (e == hipSuccess)
+            e = launch_layer_ckpt_fwd(x_dtype, format, n, x, w32, saved + d.coef_off, np, out, values, scales, batch,
+                                      hidden, rmsnorm_eps, s);
+        return hip_status(e);
+    }
     // the channel-loop forward uses the sum x^2 partials (ks * batch floats,
     // free once the coefficients are formed) as scratch for its row sums
     float* rs = layer_fwd_is_wide(n, hidden) ? ss : nullptr;
     if (e == hipSuccess)
         e = launch_layer_fwd(x_dtype, n, x, w32, saved + d.coef_off, np, out, kF32, rs, batch, hidden, rmsnorm_eps, s,
                              rs ? (int64_t)w.ks * batch : 0);
+    if (e == hipSuccess && format >= 0)
+        e = launch_ckpt_pack(x_dtype, format, x, values, scales, batch * n, hidden, s);
     return hip_status(e);
+}
+
+int mhc_layer_dynamic_fwd(const void* x, int32_t x_dtype, const void* weight, int32_t weight_dtype,
+                          const float* phi_pre, const float* phi_post, const float* phi_res, const float* alpha_pre,
+                          const float* alpha_post, const float* alpha_res, const float* b_pre, const float* b_post,
+                          const float* b_res, float* out, float* saved, void* workspace, size_t workspace_bytes,
+                          int64_t batch, int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
+                          float rmsnorm_eps, void* stream) {
+    return dynamic_fwd(x, x_dtype, weight, weight_dtype, phi_pre, phi_post, phi_res, alpha_pre, alpha_post, alpha_res,
+                       b_pre, b_post, b_res, out, saved, -1, nullptr, nullptr, workspace, workspace_bytes, batch, n,
+                       hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
 }
 
 // ---- forward-only dynamic-H layer ---------------------------------------------
@@ -2231,9 +2252,9 @@ int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* 
 }
 
 // Rows read from the checkpoint: the partials of static_bwd_ws.
-static StaticBwdWs static_ckpt_bwd_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype, int32_t format) {
+static StaticBwdWs static_ckpt_bwd_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
     StaticBwdWs w{};
-    w.grid = layer_ckpt_bwd_grid(x_dtype, format, n, 0, batch, hidden);
+    w.grid = layer_ckpt_bwd_grid(x_dtype, n, 0, batch, hidden);
     w.scal_off = align256((size_t)w.grid * hidden * sizeof(float));
     w.stage_off = w.scal_off + align256((size_t)w.grid * (n * n + 2 * n) * sizeof(float));
     w.total = w.stage_off + align256(column_sums_stage_floats(hidden) * sizeof(float));
@@ -2241,19 +2262,13 @@ static StaticBwdWs static_ckpt_bwd_ws(int64_t batch, int32_t n, int32_t hidden, 
 }
 
 // workspace: that, or [x^ rows | the layer's backward]
-size_t mhc_layer_static_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
+size_t mhc_layer_static_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
+                                                      int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
     if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype)) return 0;
+    if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}))
+        return static_ckpt_bwd_ws(batch, n, hidden, x_dtype).total;
     return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
            mhc_layer_static_bwd_workspace_size(batch, n, hidden, x_dtype);
-}
-
-size_t mhc_layer_static_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
-                                                      int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
-                                                      int32_t format) {
-    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype) || !valid_format(format)) return 0;
-    if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}))
-        return static_ckpt_bwd_ws(batch, n, hidden, x_dtype, format).total;
-    return mhc_layer_static_checkpoint_bwd_workspace_size(batch, n, hidden, x_dtype);
 }
 
 int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
@@ -2270,7 +2285,7 @@ int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, c
         if (st) return st;
         MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_static_checkpoint_bwd: values must be 16-byte aligned");
         if (!workspace || workspace_bytes < mhc_layer_static_checkpoint_bwd_workspace_need(
-                                                grad_out, grad_x, saved, batch, n, hidden, x_dtype, format))
+                                                grad_out, grad_x, saved, batch, n, hidden, x_dtype))
             return fail(MHC_ERR_WORKSPACE, "layer_static_checkpoint_bwd: workspace smaller than "
                                            "mhc_layer_static_checkpoint_bwd_workspace_need()");
         if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved})) {
@@ -2278,7 +2293,7 @@ int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, c
             MHC_REQUIRE(h_pre && h_post && h_res && saved, "layer_static_checkpoint_bwd: null parameter pointer");
             MHC_REQUIRE(grad_weight && grad_h_pre && grad_h_post && grad_h_res,
                         "layer_static_checkpoint_bwd: null gradient pointer");
-            const StaticBwdWs w = static_ckpt_bwd_ws(batch, n, hidden, x_dtype, format);
+            const StaticBwdWs w = static_ckpt_bwd_ws(batch, n, hidden, x_dtype);
             hipStream_t s = (hipStream_t)stream;
             float* dw_part = (float*)workspace;
             float* scal_part = (float*)((char*)workspace + w.scal_off);
@@ -2314,18 +2329,107 @@ int mhc_layer_dynamic_checkpoint_fwd(const void* x, int32_t x_dtype, const void*
         int st = check_ckpt("layer_dynamic_checkpoint_fwd", batch, hidden, x_dtype, format, x && values && scales);
         if (st) return st;
         MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_dynamic_checkpoint_fwd: values must be 16-byte aligned");
-        st = mhc_layer_dynamic_fwd(x, x_dtype, weight, weight_dtype, phi_pre, phi_post, phi_res, alpha_pre, alpha_post,
-                                   alpha_res, b_pre, b_post, b_res, out, saved, workspace, workspace_bytes, batch, n,
-                                   hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
-        if (st) return st;
-        return hip_status(launch_ckpt_pack(x_dtype, format, x, values, scales, batch * n, hidden, (hipStream_t)stream));
+        return dynamic_fwd(x, x_dtype, weight, weight_dtype, phi_pre, phi_post, phi_res, alpha_pre, alpha_post,
+                           alpha_res, b_pre, b_post, b_res, out, saved, format, values, scales, workspace,
+                           workspace_bytes, batch, n, hidden, num_iters, sinkhorn_eps, rmsnorm_eps, stream);
     });
 }
 
-size_t mhc_layer_dynamic_checkpoint_bwd_workspace_size(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
-    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype)) return 0;
+// The backward whose row and projection passes read the checkpoint: n = 2..8
+// on register rows, hidden % 8 == 0, 16-byte aligned arrays.
+static bool dyn_ckpt_rows(const float* grad_out, const void* grad_x, const float* saved, int64_t batch, int32_t n,
+                          int32_t hidden) {
+    return layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}) &&
+           proj_ckpt_supported(2 * n + n * n, (int64_t)n * hidden, hidden);
+}
+
+struct DynCkptWs {
+    bool qin;  // dx_in is the fp16 stream part in grad_x; else fp32 in dxw (bf16 x) or grad_x
+    int mode, grid, tiles, groups, rows_c;
+    size_t scal_off, dp_off, s_off, pscale_off, cpart_off, phip_off, stw_off, stp_off, dxw_off, hist_off, total;
+};
+
+static DynCkptWs dyn_ckpt_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype, int32_t num_iters) {
+    DynCkptWs w{};
+    const int np = 2 * n + n * n;
+    const int64_t K = (int64_t)n * hidden;
+    w.qin = x_dtype == kBF16 && (n == 2 || n == 4) && hidden % 128 == 0;
+    w.mode = w.qin || x_dtype == kF32 ? 1 : 2;
+    w.grid = layer_ckpt_bwd_grid(x_dtype, n, w.mode, batch, hidden);
+    w.tiles = proj_ckpt_bwd_tiles(x_dtype, w.qin, np, batch, K);
+    w.groups = w.qin ? layer_bwd_part_groups(kBF16, n, hidden) : 0;
+    w.rows_c = dyn_coef_bwd_rows(n, batch, num_iters, true);
+    size_t o = align256((size_t)w.grid * hidden * 4);
+    w.scal_off = o; o += align256((size_t)batch * (n * n + 2 * n + 2) * 4);
+    w.dp_off = o; o += align256((size_t)batch * dp_stride(np) * 4);
+    w.s_off = o; o += align256((size_t)batch * 4);
+    w.pscale_off = o; o += align256((size_t)batch * w.groups * 4);
+    w.cpart_off = o; o += align256((size_t)dyn_coef_bwd_blocks(n, batch) * (np + 3) * 4);
+    w.phip_off = o; o += align256((size_t)w.tiles * np * K * 4);
+    w.stw_off = o; o += align256(column_sums_stage_floats(hidden) * 4);
+    w.stp_off = o; o += column_sums_direct(w.tiles) ? 0 : align256(column_sums_stage_floats((int64_t)np * K) * 4);
+    w.dxw_off = o; o += w.mode == 2 ? align256((size_t)batch * K * 4) : 0;
+    w.hist_off = o; o += generic_layer_n(n) ? align256(dyn_coef_gen_hist_bytes(n, batch)) : 0;
+    w.total = o;
+    return w;
+}
+
+size_t mhc_layer_dynamic_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
+                                                       int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
+                                                       int32_t num_iters) {
+    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype) || num_iters < 0) return 0;
+    if (dyn_ckpt_rows(grad_out, grad_x, saved, batch, n, hidden))
+        return dyn_ckpt_ws(batch, n, hidden, x_dtype, num_iters).total;
     return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
            mhc_layer_dynamic_bwd_workspace_size(batch, n, hidden, x_dtype);
+}
+
+// The launches of mhc_layer_dynamic_bwd, with x^ read from the checkpoint.
+static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
+                               int32_t x_dtype, int32_t weight_dtype, const float* phi_pre, const float* phi_post,
+                               const float* phi_res, const float* alpha_pre, const float* alpha_post,
+                               const float* alpha_res, const float* b_res, const float* saved, void* grad_x,
+                               void* grad_weight, float* grad_phi, float* grad_alpha, float* grad_b, char* ws,
+                               int64_t batch, int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
+                               float rmsnorm_eps, hipStream_t s) {
+    const DynCkptWs w = dyn_ckpt_ws(batch, n, hidden, x_dtype, num_iters);
+    const DynSaved d = dyn_saved(batch, n, hidden);
+    const int np = 2 * n + n * n;
+    const int64_t K = (int64_t)n * hidden;
+    float* dw_part = (float*)ws;
+    float* scal = (float*)(ws + w.scal_off);
+    float* dp = (float*)(ws + w.dp_off);
+    float* stok = (float*)(ws + w.s_off);
+    int32_t* pscale = w.qin ? (int32_t*)(ws + w.pscale_off) : nullptr;
+    float* cpart = (float*)(ws + w.cpart_off);
+    float* phip = (float*)(ws + w.phip_off);
+    void* part = w.mode == 2 ? (void*)(ws + w.dxw_off) : grad_x;
+    hipError_t e = launch_layer_ckpt_bwd(x_dtype, format, n, w.mode, grad_out, values, scales, saved + d.w_off,
+                                         saved + d.coef_off, np, part, dw_part, scal, w.grid, batch, hidden,
+                                         rmsnorm_eps, s, pscale);
+    if (e == hipSuccess)
+        e = launch_dyn_coef_bwd(n, scal, saved + d.coef_off, saved + d.p_off, saved + d.rh_off, batch, K, alpha_pre,
+                                alpha_post, alpha_res, b_res, dp, stok, cpart, num_iters, sinkhorn_eps,
+                                generic_layer_n(n) ? (float*)(ws + w.hist_off) : nullptr, s);
+    if (e == hipSuccess)
+        e = launch_proj_ckpt_bwd(x_dtype, w.qin, format, values, scales, dp, dp_stride(np), stok, phi_pre, phi_post,
+                                 phi_res, n, np, part, grad_x, pscale, w.groups, phip, w.tiles, batch, K, s);
+    if (e != hipSuccess) return e;
+    if (column_sums_direct(w.tiles) && column_sums_direct(w.grid) && column_sums_direct(w.rows_c)) {
+        ColSumJobs jobs{};
+        jobs.j[0] = ColSumJob{phip, grad_phi, nullptr, (int64_t)np * K, w.tiles, (int)(np * K), 0, 0, 0};
+        jobs.j[1] = ColSumJob{dw_part, grad_weight, nullptr, hidden, w.grid, hidden, weight_dtype == kBF16, 0, 0};
+        jobs.j[2] = ColSumJob{cpart, grad_b, grad_alpha, np + 3, w.rows_c, np, 0, 0, 0};
+        jobs.count = 3;
+        return launch_multi_column_sum(jobs, s);
+    }
+    e = launch_column_finalize(0, kF32, phip, w.tiles, (int64_t)np * K, (float*)(ws + w.stp_off), grad_phi, nullptr, 0,
+                               nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+    if (e == hipSuccess)
+        e = launch_column_finalize(0, weight_dtype, dw_part, w.grid, hidden, (float*)(ws + w.stw_off), grad_weight,
+                                   nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+    if (e == hipSuccess) e = launch_small_column_sum(cpart, w.rows_c, np + 3, grad_b, grad_alpha, np, s);
+    return e;
 }
 
 int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
@@ -2344,11 +2448,21 @@ int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, 
         st = check_dyn(fn, batch, n, hidden, x_dtype, weight_dtype, num_iters);
         if (st) return st;
         MHC_REQUIRE((uintptr_t)values % 16 == 0, "layer_dynamic_checkpoint_bwd: values must be 16-byte aligned");
-        const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
-        if (!workspace ||
-            workspace_bytes < mhc_layer_dynamic_checkpoint_bwd_workspace_size(batch, n, hidden, x_dtype))
+        if (!workspace || workspace_bytes < mhc_layer_dynamic_checkpoint_bwd_workspace_need(
+                                                grad_out, grad_x, saved, batch, n, hidden, x_dtype, num_iters))
             return fail(MHC_ERR_WORKSPACE, "layer_dynamic_checkpoint_bwd: workspace smaller than "
-                                           "mhc_layer_dynamic_checkpoint_bwd_workspace_size()");
+                                           "mhc_layer_dynamic_checkpoint_bwd_workspace_need()");
+        if (dyn_ckpt_rows(grad_out, grad_x, saved, batch, n, hidden)) {
+            MHC_REQUIRE(phi_pre && phi_post && phi_res && alpha_pre && alpha_post && alpha_res && b_res && saved,
+                        "layer_dynamic_checkpoint_bwd: null parameter pointer");
+            MHC_REQUIRE(grad_weight && grad_phi && grad_alpha && grad_b,
+                        "layer_dynamic_checkpoint_bwd: null gradient pointer");
+            return hip_status(dyn_ckpt_bwd(grad_out, values, scales, format, x_dtype, weight_dtype, phi_pre, phi_post,
+                                           phi_res, alpha_pre, alpha_post, alpha_res, b_res, saved, grad_x,
+                                           grad_weight, grad_phi, grad_alpha, grad_b, (char*)workspace, batch, n,
+                                           hidden, num_iters, sinkhorn_eps, rmsnorm_eps, (hipStream_t)stream));
+        }
+        const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
         const hipError_t e =
             launch_ckpt_unpack(x_dtype, format, values, scales, workspace, batch * n, hidden, (hipStream_t)stream);
         if (e != hipSuccess) return hip_status(e);

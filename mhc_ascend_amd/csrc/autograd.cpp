@@ -75,7 +75,7 @@ using torch::autograd::tensor_list;
     X(mhc_layer_static_checkpoint_bwd_workspace_need) \
     X(mhc_layer_static_checkpoint_bwd)        \
     X(mhc_layer_dynamic_checkpoint_fwd)       \
-    X(mhc_layer_dynamic_checkpoint_bwd_workspace_size) \
+    X(mhc_layer_dynamic_checkpoint_bwd_workspace_need) \
     X(mhc_layer_dynamic_checkpoint_bwd)       \
     X(mhc_qk_norm_rope_fwd)                   \
     X(mhc_qk_norm_rope_bwd_workspace_size)    \
@@ -307,7 +307,7 @@ struct StaticLayer : public torch::autograd::Function<StaticLayer> {
         const int xd = dtype_code(store);
         if (is_held) {
             const size_t wsb = lib.mhc_layer_static_checkpoint_bwd_workspace_need(
-                fp(g), grad_x.data_ptr(), fp(saved), B, (int32_t)n, (int32_t)C, xd, (int32_t)fmt);
+                fp(g), grad_x.data_ptr(), fp(saved), B, (int32_t)n, (int32_t)C, xd);
             Tensor ws = workspace(wsb, x);
             check(lib.mhc_layer_static_checkpoint_bwd(
                       fp(g), x.data_ptr(), sv[6].data_ptr(), (int32_t)fmt, xd, dtype_code(w.scalar_type()), fp(hp),
@@ -410,7 +410,8 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
         Tensor gb = at::empty({np}, f32);
         const int xd = dtype_code(store);
         if (is_held) {
-            const size_t wsb = lib.mhc_layer_dynamic_checkpoint_bwd_workspace_size(B, (int32_t)n, (int32_t)C, xd);
+            const size_t wsb = lib.mhc_layer_dynamic_checkpoint_bwd_workspace_need(
+                fp(g), grad_x.data_ptr(), fp(saved), B, (int32_t)n, (int32_t)C, xd, (int32_t)cfg[0]);
             Tensor ws = workspace(wsb, x);
             check(lib.mhc_layer_dynamic_checkpoint_bwd(
                       fp(g), x.data_ptr(), sv[12].data_ptr(), (int32_t)fmt, xd, dtype_code(w.scalar_type()), fp(sv[3]),

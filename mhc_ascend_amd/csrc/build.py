@@ -33,7 +33,7 @@ AUTOGRAD_NAME = "_mhc_autograd"
 AUTOGRAD_PATH = os.path.join(PKG, AUTOGRAD_NAME + ".so")
 
 SOURCES = ["abi.hip", "ckpt.hip", "compat.hip", "dynamic.hip", "generic.hip", "layer.hip",
-           "layer_ckpt.hip", "ops.hip",
+           "layer_ckpt.hip", "ops.hip", "proj_ckpt.hip",
            "qk_norm_rope.hip", "sinkhorn.hip", "wide.hip",
            "wrapper.hip", "wrapper_gen.hip", "wrapper_proj.hip",
            "wrapper_bwd.hip", "wrapper_row.hip"]

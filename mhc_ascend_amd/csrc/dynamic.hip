@@ -18,25 +18,13 @@
 //   proj_bwd_mfma_kernel dx += dP.Phi + s x_flat, dPhi partials (bf16 MFMA, split operands)
 #include "mhc_device.h"
 #include "mhc_internal.h"
+#include "mhc_mfma.h"
 #include "proj_plan.h"
 #include "mhc_rows.h"
 
 namespace mhc {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
-
 constexpr int kNPad = 32;  // projection outputs padded to two 16-wide MFMA tiles
-
-__device__ __forceinline__ f32x4_t mfma16x16x32(u32x4_t a, u32x4_t b, f32x4_t c) {
-    // A rows = lane % 16, B cols = lane % 16, k = 8 * (lane / 16) + 0..7;
-    // D[4 * (lane / 16) + i][lane % 16] in element i.
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
-                                                   c, 0, 0, 0);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) { return pack_bf16x2(lo, hi); }
 
 
 // ---------------------------------------------------------------------------
@@ -1651,15 +1639,6 @@ __global__ __launch_bounds__(1024) void small_column_sum_kernel(const float* __r
 // tiles arrive with coalesced 16-byte loads (two stages in flight), results
 // return to the dx tile in LDS and leave with coalesced 16-byte stores.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ void split_pack8(const float (&v)[8], u32x4_t& hi, u32x4_t& lo) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t h = pack_bf16(v[2 * e], v[2 * e + 1]);
-        hi[e] = h;
-        lo[e] = pack_bf16(v[2 * e] - __uint_as_float(h << 16), v[2 * e + 1] - __uint_as_float(h & 0xffff0000u));
-    }
-}
-
 // Four consecutive elements at an 8-byte aligned LDS address (8-byte accesses only).
 template <typename TX>
 __device__ __forceinline__ void lds_get4(const char* p, float (&v)[4]) {
@@ -1688,7 +1667,6 @@ __device__ __forceinline__ void lds_put4(char* p, const float (&v)[4]) {
 // LDS row pitch of a 128-column stage tile (8-byte aligned rows; 8 extra
 // bytes spread the token rows read by the four lane groups over the banks).
 template <typename TX, int CB> constexpr int pb_pitch() { return CB * (int)sizeof(TX) + 8; }
-constexpr int kDpPitch = 40;  // bf16 per row of the split dP copies (32 + 8 pad)
 
 // Waves per SIMD the register allocation targets: four for bf16 x (128
 // registers, no spills; four 35.6 KB workgroups share a CU's LDS), two for

@@ -56,16 +56,22 @@ __device__ __forceinline__ void held_load(const uint8_t* __restrict__ q, const u
 }
 
 template <int FMT, int N, int VPT>
-__device__ __forceinline__ void held_get(const HeldRows<N, VPT>& r, float (&v)[N][VPT][kLayerWC]) {
+__device__ __forceinline__ void held_get_as(const HeldRows<N, VPT>& r, float (&v)[N][VPT][kLayerWC]) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
 #pragma unroll
         for (int i = 0; i < N; ++i) Ck<FMT>::unpack4(r.q[i][k], Ck<FMT>::down(r.s[i][k]), v[i][k]);
     }
 }
+// The format is an argument (a scalar branch once a token): half the kernels.
+template <int N, int VPT>
+__device__ __forceinline__ void held_get(int fmt, const HeldRows<N, VPT>& r, float (&v)[N][VPT][kLayerWC]) {
+    if (fmt == kCkInt8) held_get_as<kCkInt8, N, VPT>(r, v);
+    else held_get_as<kCkE4M3, N, VPT>(r, v);
+}
 
 template <int FMT, int N, int VPT>
-__device__ __forceinline__ void held_put(const float (&v)[N][VPT][kLayerWC], uint8_t* __restrict__ q,
+__device__ __forceinline__ void held_put_as(const float (&v)[N][VPT][kLayerWC], uint8_t* __restrict__ q,
                                          uint8_t* __restrict__ sc, int64_t b, int C) {
     const int stride = (int)ck_stride(C), nb = (int)ck_blocks(C);
     const buf_rsrc_t rq = make_buf_rsrc(q + b * N * stride, (uint32_t)(N * stride));
@@ -89,8 +95,15 @@ __device__ __forceinline__ void held_put(const float (&v)[N][VPT][kLayerWC], uin
     }
 }
 
-template <typename TX, int N, int VPT, int FMT>
-__global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(const TX* __restrict__ x, const float* __restrict__ w,
+template <int N, int VPT>
+__device__ __forceinline__ void held_put(int fmt, const float (&v)[N][VPT][kLayerWC], uint8_t* __restrict__ q,
+                                         uint8_t* __restrict__ sc, int64_t b, int C) {
+    if (fmt == kCkInt8) held_put_as<kCkInt8, N, VPT>(v, q, sc, b, C);
+    else held_put_as<kCkE4M3, N, VPT>(v, q, sc, b, C);
+}
+
+template <typename TX, int N, int VPT>
+__global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(int fmt, const TX* __restrict__ x, const float* __restrict__ w,
                                                             const float* __restrict__ coef, int64_t coef_stride,
                                                             float* __restrict__ out, uint8_t* __restrict__ q,
                                                             uint8_t* __restrict__ sc, int C, float eps) {
@@ -103,14 +116,14 @@ __global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(const TX* __restrict
     load_weight<VPT, WC>(w, C, wv);
     float xv[N][VPT][WC];
     unpack_rows<TX, N, VPT, WC>(xr, C, xv);
-    held_put<FMT, N, VPT>(xv, q, sc, b, C);
+    held_put<N, VPT>(fmt, xv, q, sc, b, C);
     fwd_token<TX, float, N, VPT>(b, coef, coef_stride, wv, xv, out, nullptr, C, eps, red);
 }
 
 // As layer_bwd_kernel: persistent workgroups over tokens, with PF the next
 // token's rows in flight.  TX is dx's storage type.
-template <typename TX, int N, int VPT, int MODE, int FMT, bool PF>
-__global__ MHC_ROW_BOUNDS(PF) void layer_ckpt_bwd_kernel(const float* __restrict__ g, const uint8_t* __restrict__ q,
+template <typename TX, int N, int VPT, int MODE, bool PF>
+__global__ MHC_ROW_BOUNDS(PF) void layer_ckpt_bwd_kernel(int fmt, const float* __restrict__ g, const uint8_t* __restrict__ q,
                                                          const uint8_t* __restrict__ sc, const float* __restrict__ w,
                                                          const float* __restrict__ coef, int64_t coef_stride,
                                                          BwdDx<TX, MODE>* __restrict__ dx,
@@ -133,7 +146,7 @@ __global__ MHC_ROW_BOUNDS(PF) void layer_ckpt_bwd_kernel(const float* __restrict
     int64_t b = blockIdx.x;
     float xv[N][VPT][WC], gv[N][VPT][WC];
     const auto token = [&](int64_t t, const HeldRows<N, VPT>& xr, const RawRows<float, N, VPT, WC>& gr) {
-        held_get<FMT, N, VPT>(xr, xv);
+        held_get<N, VPT>(fmt, xr, xv);
         unpack_rows<float, N, VPT, WC>(gr, C, gv);
         bwd_token<TX, N, VPT, MODE>(t, coef, coef_stride, wv, xv, gv, dwacc, sacc, dx, scal_out, dx_scale, C, eps, red);
     };
@@ -195,42 +208,40 @@ __global__ MHC_ROW_BOUNDS(PF) void layer_ckpt_bwd_kernel(const float* __restrict
         default: break;                                          \
     }
 
-template <typename TX, int N, int V, int FMT>
+template <typename TX, int N, int V>
 static const void* ck_fwd_fn() {
-    if constexpr (layer_row_fits(N, V)) return reinterpret_cast<const void*>(&layer_ckpt_fwd_kernel<TX, N, V, FMT>);
+    if constexpr (layer_row_fits(N, V)) return reinterpret_cast<const void*>(&layer_ckpt_fwd_kernel<TX, N, V>);
     return nullptr;
 }
 
-template <typename TX, int N, int V, int MODE, int FMT>
+template <typename TX, int N, int V, int MODE>
 static const void* ck_bwd_fn(bool pf) {
     if constexpr (layer_row_fits(2 * N, V))
-        return pf ? reinterpret_cast<const void*>(&layer_ckpt_bwd_kernel<TX, N, V, MODE, FMT, true>)
-                  : reinterpret_cast<const void*>(&layer_ckpt_bwd_kernel<TX, N, V, MODE, FMT, false>);
+        return pf ? reinterpret_cast<const void*>(&layer_ckpt_bwd_kernel<TX, N, V, MODE, true>)
+                  : reinterpret_cast<const void*>(&layer_ckpt_bwd_kernel<TX, N, V, MODE, false>);
     return nullptr;
 }
 
-static const void* pick_ck_fwd(int x_dtype, int fmt, int n, int vpt) {
+static const void* pick_ck_fwd(int x_dtype, int n, int vpt) {
     const void* fn = nullptr;
-    MHC_CL_N(n, MHC_CL_VPT(vpt, {
-                 if (x_dtype == kBF16)
-                     fn = fmt == kCkInt8 ? ck_fwd_fn<bf16_t, N_, V_, kCkInt8>() : ck_fwd_fn<bf16_t, N_, V_, kCkE4M3>();
-                 else
-                     fn = fmt == kCkInt8 ? ck_fwd_fn<float, N_, V_, kCkInt8>() : ck_fwd_fn<float, N_, V_, kCkE4M3>();
-             }));
+    MHC_CL_N(n, MHC_CL_VPT(vpt, fn = x_dtype == kBF16 ? ck_fwd_fn<bf16_t, N_, V_>() : ck_fwd_fn<float, N_, V_>()));
     return fn;
 }
 
-template <int FMT, int N, int V>
+// modes of bwd_token: bf16 rows take 0, 2 and, n = 2 and 4, 1; fp32 rows 0 and 1
+template <int N, int V>
 static const void* pick_ck_bwd_mode(int x_dtype, int mode, bool pf) {
     const bool bf = x_dtype == kBF16;
-    if (mode == 0) return bf ? ck_bwd_fn<bf16_t, N, V, 0, FMT>(pf) : ck_bwd_fn<float, N, V, 0, FMT>(pf);
+    if (mode == 0) return bf ? ck_bwd_fn<bf16_t, N, V, 0>(pf) : ck_bwd_fn<float, N, V, 0>(pf);
+    if (mode == 2) return bf ? ck_bwd_fn<bf16_t, N, V, 2>(pf) : nullptr;
+    if (!bf) return ck_bwd_fn<float, N, V, 1>(pf);
+    if constexpr (N == 2 || N == 4) return ck_bwd_fn<bf16_t, N, V, 1>(pf);
     return nullptr;
 }
 
-static const void* pick_ck_bwd(int x_dtype, int fmt, int n, int vpt, int mode, bool pf) {
+static const void* pick_ck_bwd(int x_dtype, int n, int vpt, int mode, bool pf) {
     const void* fn = nullptr;
-    MHC_CL_N(n, MHC_CL_VPT(vpt, fn = fmt == kCkInt8 ? pick_ck_bwd_mode<kCkInt8, N_, V_>(x_dtype, mode, pf)
-                                                    : pick_ck_bwd_mode<kCkE4M3, N_, V_>(x_dtype, mode, pf)));
+    MHC_CL_N(n, MHC_CL_VPT(vpt, fn = pick_ck_bwd_mode<N_, V_>(x_dtype, mode, pf)));
     return fn;
 }
 
@@ -252,10 +263,10 @@ hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, con
                                  int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
                                  float eps, hipStream_t s) {
     const RowTiling t = layer_fwd_tiling(C, n);
-    const void* fn = pick_ck_fwd(x_dtype, fmt, n, t.vpt);
+    const void* fn = pick_ck_fwd(x_dtype, n, t.vpt);
     if (!fn) return hipErrorInvalidValue;
     int Ci = (int)C;
-    void* args[] = {(void*)&x,   (void*)&w,      (void*)&coef,   (void*)&coef_stride, (void*)&out,
+    void* args[] = {(void*)&fmt, (void*)&x,   (void*)&w,      (void*)&coef,   (void*)&coef_stride, (void*)&out,
                     (void*)&values, (void*)&scales, (void*)&Ci, (void*)&eps};
     const int tok = timing_begin("layer_ckpt_fwd", s);
     hipError_t e = mhc_launch_kernel(fn, dim3((unsigned)B), dim3(t.threads), args, 0, s);
@@ -266,10 +277,10 @@ hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, con
 // workgroups of at most 256 lanes prefetch (layer.hip)
 static bool ck_prefetch(const RowTiling& t) { return t.threads <= 256; }
 
-int layer_ckpt_bwd_grid(int x_dtype, int fmt, int n, int mode, int64_t B, int64_t C) {
+int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C) {
     const RowTiling t = layer_bwd_tiling(C, n, B);
     const int64_t g = (int64_t)device_cu_count() *
-                      occupancy_per_cu(pick_ck_bwd(x_dtype, fmt, n, t.vpt, mode, ck_prefetch(t)), t.threads, 0);
+                      occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t)), t.threads, 0);
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
 
@@ -278,10 +289,10 @@ hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const fl
                                  float* dw_part, float* scal_out, int grid, int64_t B, int64_t C, float eps,
                                  hipStream_t s, int32_t* dx_scale) {
     const RowTiling t = layer_bwd_tiling(C, n, B);
-    const void* fn = pick_ck_bwd(x_dtype, fmt, n, t.vpt, mode, ck_prefetch(t));
+    const void* fn = pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t));
     if (!fn) return hipErrorInvalidValue;
     int Ci = (int)C;
-    void* args[] = {(void*)&g,       (void*)&values,   (void*)&scales,   (void*)&w, (void*)&coef, (void*)&coef_stride, (void*)&dx,
+    void* args[] = {(void*)&fmt, (void*)&g,       (void*)&values,   (void*)&scales,   (void*)&w, (void*)&coef, (void*)&coef_stride, (void*)&dx,
                     (void*)&dw_part, (void*)&scal_out, (void*)&dx_scale, (void*)&B, (void*)&Ci,   (void*)&eps};
     const int tok = timing_begin("layer_ckpt_bwd", s);
     hipError_t e = mhc_launch_kernel(fn, dim3(grid), dim3(t.threads), args, 0, s);

@@ -303,11 +303,24 @@ bool layer_ckpt_bwd_rows(int n, int64_t B, int64_t C, std::initializer_list<cons
 hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, const float* w, const float* coef,
                                  int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
                                  float eps, hipStream_t s);
-int layer_ckpt_bwd_grid(int x_dtype, int fmt, int n, int mode, int64_t B, int64_t C);
+int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C);
 hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const float* g, const void* values,
                                  const void* scales, const float* w, const float* coef, int64_t coef_stride, void* dx,
                                  float* dw_part, float* scal_out, int grid, int64_t B, int64_t C, float eps,
                                  hipStream_t s, int32_t* dx_scale = nullptr);
+
+// ---- proj_ckpt.hip ---------------------------------------------------------
+// The projection backward on rows in a checkpoint, all np <= 96 output rows at
+// once; C a multiple of 8.  dx_in: fp32 [B, K] (dx itself for fp32 dx), or,
+// with qin (bf16 dx, n = 2 or 4, C a multiple of 128), the fp16 stream part
+// of launch_layer_ckpt_bwd's mode 1 in dx.  dphi_part[tiles][np][K].
+bool proj_ckpt_supported(int np, int64_t K, int64_t C);
+int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K);
+hipError_t launch_proj_ckpt_bwd(int dx_dtype, bool qin, int fmt, const void* values, const void* scales,
+                                const float* dP, int dp_stride, const float* s_tok, const float* phi_pre,
+                                const float* phi_post, const float* phi_res, int n, int np, const void* dx_in,
+                                void* dx, const int32_t* dx_scale, int groups, float* dphi_part, int tiles, int64_t B,
+                                int64_t K, hipStream_t s);
 
 // ---- qk_norm_rope.hip ------------------------------------------------------
 // Head rows of queries ([0]) and keys ([1]); strides in elements.  Token t's
