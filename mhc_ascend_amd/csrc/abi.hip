@@ -2184,8 +2184,7 @@ int mhc_rmsnorm_checkpoint_fwd(const void* inp, int32_t dtype, const float* weig
 static RowsBwdWs rmsnorm_ckpt_bwd_ws(int64_t batch, int32_t hidden, int32_t dtype, int32_t format) {
     RowsBwdWs w{};
     w.grid = batch > 0 ? rmsnorm_ckpt_bwd_grid(dtype, format, batch, hidden) : 1;
-    w.stage_off = align256((size_t)w.grid * hidden * sizeof(float));
-    w.total = w.stage_off + align256(column_sums_stage_floats(hidden) * sizeof(float));
+    w.total = align256((size_t)w.grid * hidden * sizeof(float));
     return w;
 }
 
@@ -2209,13 +2208,10 @@ int mhc_rmsnorm_checkpoint_bwd(const void* grad_out, int32_t dtype, const void* 
                                            "mhc_rmsnorm_checkpoint_bwd_workspace_size()");
         hipStream_t s = (hipStream_t)stream;
         float* part = (float*)workspace;
-        float* stage = (float*)((char*)workspace + w.stage_off);
         hipError_t e = batch == 0 ? launch_fill_zero(part, hidden, s)
                                   : launch_rmsnorm_ckpt_bwd(dtype, format, grad_out, values, scales, weight, grad_inp,
                                                             part, w.grid, batch, hidden, eps, s);
-        if (e == hipSuccess)
-            e = launch_column_finalize(0, kF32, part, w.grid, hidden, stage, grad_weight, nullptr, 0, nullptr, nullptr,
-                                       nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+        if (e == hipSuccess) e = launch_weight_grad_sum(kF32, part, w.grid, hidden, grad_weight, s);
         return hip_status(e);
     });
 }
@@ -2357,7 +2353,7 @@ static DynCkptWs dyn_ckpt_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x
     w.mode = w.qin || x_dtype == kF32 ? 1 : 2;
     w.grid = layer_ckpt_bwd_grid(x_dtype, n, w.mode, batch, hidden);
     w.tiles = proj_ckpt_bwd_tiles(x_dtype, w.qin, np, batch, K);
-    w.groups = w.qin ? layer_bwd_part_groups(kBF16, n, hidden) : 0;
+    w.groups = w.qin ? layer_ckpt_bwd_part_groups(n, batch, hidden) : 0;
     w.rows_c = dyn_coef_bwd_rows(n, batch, num_iters, true);
     size_t o = align256((size_t)w.grid * hidden * 4);
     w.scal_off = o; o += align256((size_t)batch * (n * n + 2 * n + 2) * 4);
@@ -2602,7 +2598,7 @@ int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_
         } else {
             e = launch_qk_norm_rope_bwd(dtype, format, a, part, s);
         }
-        if (e == hipSuccess) e = launch_qk_norm_rope_dw(weight_dtype, part, rows, head_dim, grad_weight, s);
+        if (e == hipSuccess) e = launch_weight_grad_sum(weight_dtype, part, rows, 2 * (int64_t)head_dim, grad_weight, s);
         return hip_status(e);
     });
 }

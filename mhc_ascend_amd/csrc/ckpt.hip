@@ -244,43 +244,51 @@ __device__ __forceinline__ void ck_row_put(T* __restrict__ row, int C, const flo
     }
 }
 
+// Persistent workgroups over rows, the weight in registers and the next row's
+// loads in flight.
 template <typename T, int FMT, int VPT, bool RAG>
 __global__ __launch_bounds__(512) void rmsnorm_ckpt_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                T* __restrict__ y, uint8_t* __restrict__ q,
-                                                               uint8_t* __restrict__ sc, int C, float eps) {
+                                                               uint8_t* __restrict__ sc, int64_t B, int C, float eps) {
     __shared__ float red[8];
-    const int64_t b = blockIdx.x;
-    const T* row = x + b * C;
-    CkPiece<T> in[VPT];
-    ck_row_load<T, VPT, RAG>(row, C, in);
-    CkPiece<float> wr[VPT];
-    ck_row_load<float, VPT, RAG>(w, C, wr);
-    float v[VPT][8], wv[VPT][8];
-    ck_row_get<T, VPT, RAG>(row, C, in, v);
-    float t[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) t[0] += v[k][e] * v[k][e];
-    }
     const int nb = (int)ck_blocks(C), stride = (int)ck_stride(C);
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        uint2 p;
-        const uint32_t s = ck_pack8<FMT>(v[k], p);
-        if (c0 < stride) st8_nt(q + b * stride + c0, p);
-        if ((threadIdx.x & 3) == 0 && c0 < C) sc[b * nb + (c0 >> 5)] = (uint8_t)s;
+    float wv[VPT][8];
+    CkPiece<T> in[VPT];
+    int64_t b = blockIdx.x;
+    ck_row_load<T, VPT, RAG>(x + b * C, C, in);
+    {
+        CkPiece<float> wr[VPT];
+        ck_row_load<float, VPT, RAG>(w, C, wr);
+        ck_row_get<float, VPT, RAG>(w, C, wr, wv);
     }
-    block_sum<1>(t, red);
-    const float inv = 1.f / sqrtf(t[0] / (float)C + eps);
-    ck_row_get<float, VPT, RAG>(w, C, wr, wv);
+    for (; b < B; b += gridDim.x) {
+        float v[VPT][8];
+        ck_row_get<T, VPT, RAG>(x + b * C, C, in, v);
+        const int64_t b1 = b + gridDim.x;
+        ck_row_load<T, VPT, RAG>(x + (b1 < B ? b1 : b) * C, C, in);
+        float t[1] = {0.f};
 #pragma unroll
-    for (int k = 0; k < VPT; ++k) {
+        for (int k = 0; k < VPT; ++k) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * inv * wv[k][e];
+            for (int e = 0; e < 8; ++e) t[0] += v[k][e] * v[k][e];
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c0 = (k * blockDim.x + threadIdx.x) * 8;
+            uint2 p;
+            const uint32_t s = ck_pack8<FMT>(v[k], p);
+            if (c0 < stride) st8_nt(q + b * stride + c0, p);
+            if ((threadIdx.x & 3) == 0 && c0 < C) sc[b * nb + (c0 >> 5)] = (uint8_t)s;
+        }
+        block_sum<1>(t, red);
+        const float inv = 1.f / sqrtf(t[0] / (float)C + eps);
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * inv * wv[k][e];
+        }
+        ck_row_put<T, VPT, RAG>(y + b * C, C, v);
     }
-    ck_row_put<T, VPT, RAG>(y + b * C, C, v);
 }
 
 // Persistent workgroups over rows, the next row's loads in flight; dw in
@@ -366,14 +374,58 @@ __global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_kernel(const T* __restri
     }
 }
 
+// ---------------------------------------------------------------------------
+// Sums of a weight gradient's partials part[rows][cols] over rows, 32 columns a
+// workgroup in 32 phases of rows (each in order, then the phases in order):
+// 512 rows take two rounds of eight loads a lane and one LDS sum.  Bound by the
+// latency of those: 256 columns 4 us, with 256 lanes on 64 columns 9.6.
+// ---------------------------------------------------------------------------
+template <typename TW>
+__global__ __launch_bounds__(1024) void weight_grad_sum_kernel(const float* __restrict__ part, int rows, int cols,
+                                                     TW* __restrict__ dw) {
+    __shared__ float red[32][33];
+    const int cl = threadIdx.x & 31, ph = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + cl;
+    float s = 0.f;
+    if (c < cols) {
+        int r = ph;
+        for (; r + 7 * 32 < rows; r += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(r + u * 32) * cols + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        for (; r < rows; r += 32) s += part[(int64_t)r * cols + c];
+    }
+    red[ph][cl] = s;
+    __syncthreads();
+    if (ph == 0 && c < cols) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += red[k][cl];
+        VecIO<TW>::put(dw + c, t);
+    }
+}
+
+hipError_t launch_weight_grad_sum(int w_dtype, const float* part, int rows, int64_t cols, void* dw, hipStream_t s) {
+    if (cols < 1 || cols > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)((cols + 31) / 32));
+    if (w_dtype == kBF16) {
+        MHC_LAUNCH_GGL((weight_grad_sum_kernel<bf16_t>), grid, dim3(1024), 0, s, part, rows, (int)cols, (bf16_t*)dw);
+    } else {
+        MHC_LAUNCH_GGL((weight_grad_sum_kernel<float>), grid, dim3(1024), 0, s, part, rows, (int)cols, (float*)dw);
+    }
+    return hipGetLastError();
+}
+
 struct CkRowTiling {
     int vpt, threads;
 };
-// The fewest pieces a lane that a 512-lane workgroup covers the row with
-// (about 256 lanes where two pieces do).
+// The fewest pieces a lane that a 512-lane workgroup covers the row with.
 static CkRowTiling ck_row_tiling(int64_t C) {
     const int64_t pieces = (C + 7) / 8;
-    const int vpt = pieces <= 256 ? 1 : (pieces <= 1024 ? 2 : 4);
+    const int vpt = pieces <= 512 ? 1 : (pieces <= 1024 ? 2 : 4);
     return CkRowTiling{vpt, (int)(((pieces + vpt - 1) / vpt + 63) / 64 * 64)};
 }
 
@@ -398,9 +450,12 @@ hipError_t launch_rmsnorm_ckpt_fwd(int dt, int fmt, const void* x, const float* 
     const CkRowTiling t = ck_row_tiling(C);
     const bool rag = C % 8 != 0;
     const int tok = timing_begin("rmsnorm_ckpt_fwd", s);
-    MHC_CK_ROWS(dt, fmt, t.vpt, rag,
-                MHC_LAUNCH_GGL((rmsnorm_ckpt_fwd_kernel<T_, F_, V_, R_>), dim3((unsigned)B), dim3(t.threads), 0, s,
-                               (const T_*)x, w, (T_*)y, (uint8_t*)values, (uint8_t*)scales, (int)C, eps));
+    MHC_CK_ROWS(dt, fmt, t.vpt, rag, {
+        const void* fn = reinterpret_cast<const void*>(&rmsnorm_ckpt_fwd_kernel<T_, F_, V_, R_>);
+        const int64_t g = (int64_t)device_cu_count() * occupancy_per_cu(fn, t.threads, 0);
+        MHC_LAUNCH_GGL((rmsnorm_ckpt_fwd_kernel<T_, F_, V_, R_>), dim3((unsigned)(g < B ? g : B)), dim3(t.threads), 0,
+                       s, (const T_*)x, w, (T_*)y, (uint8_t*)values, (uint8_t*)scales, B, (int)C, eps);
+    });
     timing_end(tok, s);
     return hipGetLastError();
 }
@@ -410,7 +465,13 @@ int rmsnorm_ckpt_bwd_grid(int dt, int fmt, int64_t B, int64_t C) {
     const bool rag = C % 8 != 0;
     const void* fn = nullptr;
     MHC_CK_ROWS(dt, fmt, t.vpt, rag, fn = reinterpret_cast<const void*>(&rmsnorm_ckpt_bwd_kernel<T_, F_, V_, R_>));
-    const int64_t g = (int64_t)device_cu_count() * occupancy_per_cu(fn, t.threads, 0);
+    // two workgroups a CU at most: their partial rows of dw cost as many bytes
+    // as rows of x, and a few more of them in flight gain less (2999 x 1001
+    // fp32: 2560 workgroups 20.7 us and two passes over their partials, 512 of
+    // them 10.9 and one)
+    int64_t per_cu = occupancy_per_cu(fn, t.threads, 0);
+    if (per_cu > 2) per_cu = 2;
+    const int64_t g = (int64_t)device_cu_count() * per_cu;
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
 

@@ -123,7 +123,7 @@ __global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(int fmt, const TX* _
 // As layer_bwd_kernel: persistent workgroups over tokens, with PF the next
 // token's rows in flight.  TX is dx's storage type.
 template <typename TX, int N, int VPT, int MODE, bool PF>
-__global__ MHC_ROW_BOUNDS(PF) void layer_ckpt_bwd_kernel(int fmt, const float* __restrict__ g, const uint8_t* __restrict__ q,
+__global__ MHC_ROW_BOUNDS((PF && N * VPT > 8)) void layer_ckpt_bwd_kernel(int fmt, const float* __restrict__ g, const uint8_t* __restrict__ q,
                                                          const uint8_t* __restrict__ sc, const float* __restrict__ w,
                                                          const float* __restrict__ coef, int64_t coef_stride,
                                                          BwdDx<TX, MODE>* __restrict__ dx,
@@ -274,13 +274,28 @@ hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, con
     return e != hipSuccess ? e : hipGetLastError();
 }
 
-// workgroups of at most 256 lanes prefetch (layer.hip)
-static bool ck_prefetch(const RowTiling& t) { return t.threads <= 256; }
+// Workgroups of at most 256 lanes prefetch (layer.hip), and of 512 where two
+// tokens' raw rows and the current one's values fit 256 registers.
+static bool ck_prefetch(const RowTiling& t, int n) { return t.threads <= 256 || n * t.vpt <= 8; }
+// Modes 1 and 2 on half the chunks and twice the lanes where a lane would hold
+// 16 chunks: two waves a SIMD, one's sums under the other's loads (n = 4, 8192
+// x 4096, bf16 dx: 174 us for 198).  Mode 0 keeps one more sum a lane and spills
+// there (fp32: 310 us for 206).
+static RowTiling ck_bwd_tiling(int64_t C, int n, int64_t B, int mode) {
+    RowTiling t = layer_bwd_tiling(C, n, B);
+    if (mode != 0 && t.threads == 256 && t.vpt >= 2 && n * t.vpt == 16) {
+        t.vpt /= 2;
+        t.threads = 512;
+    }
+    return t;
+}
+
+int layer_ckpt_bwd_part_groups(int n, int64_t B, int64_t C) { return ck_bwd_tiling(C, n, B, 1).threads / 32; }
 
 int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C) {
-    const RowTiling t = layer_bwd_tiling(C, n, B);
+    const RowTiling t = ck_bwd_tiling(C, n, B, mode);
     const int64_t g = (int64_t)device_cu_count() *
-                      occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t)), t.threads, 0);
+                      occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n)), t.threads, 0);
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
 
@@ -288,8 +303,8 @@ hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const fl
                                  const void* scales, const float* w, const float* coef, int64_t coef_stride, void* dx,
                                  float* dw_part, float* scal_out, int grid, int64_t B, int64_t C, float eps,
                                  hipStream_t s, int32_t* dx_scale) {
-    const RowTiling t = layer_bwd_tiling(C, n, B);
-    const void* fn = pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t));
+    const RowTiling t = ck_bwd_tiling(C, n, B, mode);
+    const void* fn = pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n));
     if (!fn) return hipErrorInvalidValue;
     int Ci = (int)C;
     void* args[] = {(void*)&fmt, (void*)&g,       (void*)&values,   (void*)&scales,   (void*)&w, (void*)&coef, (void*)&coef_stride, (void*)&dx,

@@ -294,6 +294,9 @@ hipError_t launch_rmsnorm_ckpt_bwd(int dt, int fmt, const void* g, const void* v
                                    const float* w, void* gx, float* dw_part, int grid, int64_t B, int64_t C,
                                    float eps, hipStream_t s);
 
+// dw[cols] (w_dtype) = the sums of part[rows][cols]
+hipError_t launch_weight_grad_sum(int w_dtype, const float* part, int rows, int64_t cols, void* dw, hipStream_t s);
+
 // ---- layer_ckpt.hip --------------------------------------------------------
 // launch_layer_fwd / launch_layer_bwd (modes as there) on rows in a
 // checkpoint: n = 2..8 with register tilings, every array of `ps` 16-byte
@@ -303,6 +306,8 @@ bool layer_ckpt_bwd_rows(int n, int64_t B, int64_t C, std::initializer_list<cons
 hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, const float* w, const float* coef,
                                  int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
                                  float eps, hipStream_t s);
+// scale groups of mode 1's fp16 stream part (layer_bwd_part_groups)
+int layer_ckpt_bwd_part_groups(int n, int64_t B, int64_t C);
 int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C);
 hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const float* g, const void* values,
                                  const void* scales, const float* w, const float* coef, int64_t coef_stride, void* dx,
@@ -350,8 +355,6 @@ hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t
 // R and interleaved of `a` alone.
 int qk_norm_rope_bwd_rows(const QkArgs& a);
 hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, hipStream_t s);
-// dw[2 D] (w_dtype) = their sums
-hipError_t launch_qk_norm_rope_dw(int w_dtype, const float* dw_part, int rows, int D, void* dw, hipStream_t s);
 
 // ---- dynamic.hip -----------------------------------------------------------
 typedef uint16_t bf16_raw_t;

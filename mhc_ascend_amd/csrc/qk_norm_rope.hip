@@ -516,37 +516,6 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, float* __
     }
 }
 
-// Sums of part[rows][cols] over rows, 32 columns a workgroup in 32 phases of
-// rows: 512 rows of 256 columns take two rounds of eight loads and one LDS
-// sum, against 16 rounds with 256 lanes on 64 columns.
-template <typename TW>
-__global__ __launch_bounds__(1024) void qk_dw_kernel(const float* __restrict__ part, int rows, int cols,
-                                                     TW* __restrict__ dw) {
-    __shared__ float red[32][33];
-    const int cl = threadIdx.x & 31, ph = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + cl;
-    float s = 0.f;
-    if (c < cols) {
-        int r = ph;
-        for (; r + 7 * 32 < rows; r += 8 * 32) {
-            float v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = part[(int64_t)(r + u * 32) * cols + c];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s += v[u];
-        }
-        for (; r < rows; r += 32) s += part[(int64_t)r * cols + c];
-    }
-    red[ph][cl] = s;
-    __syncthreads();
-    if (ph == 0 && c < cols) {
-        float t = 0.f;
-#pragma unroll
-        for (int k = 0; k < 32; ++k) t += red[k][cl];
-        VecIO<TW>::put(dw + c, t);
-    }
-}
-
 // ---------------------------------------------------------------------------
 // Host launchers
 // ---------------------------------------------------------------------------
@@ -645,16 +614,6 @@ hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_p
                                     (size_t)a.D * 16 * sizeof(float), s, a, t.lg, dw_part));
     }
     timing_end(tok, s);
-    return hipGetLastError();
-}
-
-hipError_t launch_qk_norm_rope_dw(int w_dtype, const float* dw_part, int rows, int D, void* dw, hipStream_t s) {
-    const dim3 grid((unsigned)((2 * D + 31) / 32));
-    if (w_dtype == kBF16) {
-        MHC_LAUNCH_GGL((qk_dw_kernel<bf16_t>), grid, dim3(1024), 0, s, dw_part, rows, 2 * D, (bf16_t*)dw);
-    } else {
-        MHC_LAUNCH_GGL((qk_dw_kernel<float>), grid, dim3(1024), 0, s, dw_part, rows, 2 * D, (float*)dw);
-    }
     return hipGetLastError();
 }
 
