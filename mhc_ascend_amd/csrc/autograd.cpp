@@ -1024,6 +1024,47 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
     }
 };
 
+// (values, scales) of x [..., C]: uint8 [..., ceil16(C)] and [..., ceil(C / 32)]
+std::tuple<Tensor, Tensor> checkpoint_pack(const Tensor& x_in, int64_t fmt) {
+    require_bound();
+    const char* fn = "checkpoint_pack";
+    const at::NoGradGuard no_grad;
+    check_device(fn, {&x_in});
+    TORCH_CHECK(x_in.dim() >= 1 && at::isFloatingType(x_in.scalar_type()), fn,
+                ": x must be a floating-point tensor [..., C]");
+    TORCH_CHECK(x_in.size(-1) >= 1, fn, ": x must have at least one channel");
+    const at::DeviceGuard guard(x_in.device());
+    const Tensor x = storage(x_in);
+    const int64_t C = x.size(-1);
+    Held h = hold(x, fmt);
+    auto shape = x.sizes().vec();
+    shape.back() = (C + 15) / 16 * 16;
+    const Tensor values = h.values.view(shape);
+    shape.back() = (C + 31) / 32;
+    return {values, h.scales.view(shape)};
+}
+
+// The values [..., hidden] that a checkpoint stands for, in dtype.
+Tensor checkpoint_unpack(const Tensor& values_in, const Tensor& scales_in, int64_t fmt, int64_t hidden,
+                         at::ScalarType dtype) {
+    require_bound();
+    const char* fn = "checkpoint_unpack";
+    const at::NoGradGuard no_grad;
+    check_device(fn, {&values_in, &scales_in});
+    TORCH_CHECK(values_in.scalar_type() == at::kByte && scales_in.scalar_type() == at::kByte, fn,
+                ": values and scales must be uint8");
+    const auto &vs = values_in.sizes(), &ss = scales_in.sizes();
+    TORCH_CHECK(hidden >= 1 && vs.size() >= 1 && vs.size() == ss.size() && vs.back() == (hidden + 15) / 16 * 16 &&
+                    ss.back() == (hidden + 31) / 32 && vs.slice(0, vs.size() - 1) == ss.slice(0, ss.size() - 1),
+                fn, ": values ", vs, " and scales ", ss, " do not match hidden=", hidden);
+    const at::DeviceGuard guard(values_in.device());
+    Tensor values = values_in.contiguous();
+    if (reinterpret_cast<uintptr_t>(values.data_ptr()) % 16 != 0) values = values.clone();
+    auto shape = vs.vec();
+    shape.back() = hidden;
+    return held_rows(values, scales_in.contiguous(), fmt, shape, dtype);
+}
+
 Tensor sinkhorn_knopp(const Tensor& inp, int64_t iters, double eps) {
     require_bound();
     return Sinkhorn::apply(inp, iters, eps);
@@ -1156,6 +1197,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "(y_norm [B, C], H_post_raw [B, n], M [B, n, n], x_inp [B, n, C]) -> fp32 [B, n, C] with autograd",
           py::arg("y_norm"), py::arg("H_post_raw"), py::arg("M"), py::arg("x_inp"),
           py::arg("checkpoint") = MHC_CHECKPOINT_NONE);
+    m.def("checkpoint_pack", &checkpoint_pack, "(x [..., C], format) -> (values, scales), without autograd");
+    m.def("checkpoint_unpack",
+          [](const Tensor& values, const Tensor& scales, int64_t fmt, int64_t hidden, bool bf16) {
+              return checkpoint_unpack(values, scales, fmt, hidden, bf16 ? at::kBFloat16 : at::kFloat);
+          },
+          "(values, scales, format, hidden, bf16) -> [..., hidden]");
     m.def("qk_norm_rope", &qk_norm_rope,
           "(q [T, H, D], k [T, K, D], q_weight, k_weight, cos, sin, positions or None, period, eps, interleaved, "
           "checkpoint) -> (q, k) with autograd");

@@ -350,7 +350,7 @@ int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K) {
     const int nw = proj_ckpt_waves(qin);
     const int64_t gx = (K + 32 * nw - 1) / (32 * nw);
     const int per_cu = occupancy_per_cu(pick_proj_ckpt(dx_dtype, qin, np), 64 * nw, 0);
-    int64_t tiles = 2 * (int64_t)device_cu_count() * per_cu / gx;
+    int64_t tiles = (int64_t)device_cu_count() * per_cu / gx;
     const int64_t blocks = (B + 63) / 64;
     if (tiles > blocks) tiles = blocks;
     if (tiles < 1) tiles = 1;

@@ -590,9 +590,22 @@ static dim3 qk_bwd_dims(const QkArgs& a) {
     const int64_t two = 2 * (int64_t)device_cu_count();
     if (a.T == 0) return dim3(1, 1);
     if (t.v == 0) return dim3((unsigned)(a.T < two ? a.T : two), 1);
-    const int y = qk_splits(a.T, QkTasks(a.heads[0], a.heads[1], t.lg));
-    const int64_t x = (a.T + 7) / 8, most = two / y > 1 ? two / y : 1;
-    return dim3((unsigned)(x < most ? x : most), (unsigned)y);
+    // the split with the fewest rounds: sweeps over the tokens times a wave's
+    // tasks a token and half a task for its table row
+    const int n = QkTasks(a.heads[0], a.heads[1], t.lg).n;
+    const int64_t x = (a.T + 7) / 8;
+    int64_t best = INT64_MAX, bx = 1;
+    int by = 1;
+    for (int y = 1; y <= n && y <= two; ++y) {
+        const int64_t most = two / y, gx = x < most ? x : most;
+        const int64_t cost = (x + gx - 1) / gx * (2 * ((n + y - 1) / y) + 1);
+        if (cost <= best) {
+            best = cost;
+            bx = gx;
+            by = y;
+        }
+    }
+    return dim3((unsigned)bx, (unsigned)by);
 }
 
 int qk_norm_rope_bwd_rows(const QkArgs& a) {

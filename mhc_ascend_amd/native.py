@@ -81,50 +81,6 @@ def sinkhorn_knopp_bwd(grad_out: torch.Tensor, inp: torch.Tensor, out: torch.Ten
 
 
 # =============================================================================
-# 8-bit checkpoints of rows (no counterpart in the reference)
-# =============================================================================
-
-def checkpoint_pack(x: torch.Tensor, format: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(values, scales) of x [..., C], uint8 [..., ceil16(C)] and [..., ceil(C / 32)]."""
-    _check_device("checkpoint_pack", x)
-    if x.dim() < 1 or not x.is_floating_point():
-        raise RuntimeError("checkpoint_pack: x must be a floating-point tensor [..., C]")
-    x = _storage(x)
-    C = x.size(-1)
-    if C < 1:
-        raise RuntimeError("checkpoint_pack: x must have at least one channel")
-    rows = x.numel() // C
-    values = torch.empty((*x.shape[:-1], (C + 15) // 16 * 16), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((*x.shape[:-1], (C + 31) // 32), dtype=torch.uint8, device=x.device)
-    with _lib.on_device(x.device):
-        call("mhc_checkpoint_pack", ptr(x), dtype_code(x.dtype), int(format), ptr(values), ptr(scales), rows, C,
-             stream_of(x))
-    return values, scales
-
-
-def checkpoint_unpack(values: torch.Tensor, scales: torch.Tensor, format: int, hidden: int,
-                      dtype: torch.dtype) -> torch.Tensor:
-    """The values [..., hidden] that a checkpoint stands for, in dtype."""
-    _check_device("checkpoint_unpack", values, scales)
-    C = int(hidden)
-    if values.dtype != torch.uint8 or scales.dtype != torch.uint8:
-        raise RuntimeError("checkpoint_unpack: values and scales must be uint8")
-    if (C < 1 or values.dim() < 1 or scales.dim() < 1 or values.size(-1) != (C + 15) // 16 * 16
-            or scales.size(-1) != (C + 31) // 32 or values.shape[:-1] != scales.shape[:-1]):
-        raise RuntimeError(f"checkpoint_unpack: values {tuple(values.shape)} and scales {tuple(scales.shape)} do not "
-                           f"match hidden={C}")
-    code = dtype_code(dtype)
-    values, scales = values.contiguous(), scales.contiguous()
-    if values.data_ptr() % 16:
-        values = values.clone()
-    out = torch.empty((*values.shape[:-1], C), dtype=dtype, device=values.device)
-    with _lib.on_device(values.device):
-        call("mhc_checkpoint_unpack", ptr(values), ptr(scales), int(format), ptr(out), code, out.numel() // C, C,
-             stream_of(values))
-    return out
-
-
-# =============================================================================
 # RMSNorm (bindings.cpp:237-301) and compute_rms (bindings.cpp:543-566)
 # =============================================================================
 

@@ -88,7 +88,8 @@ def activation_pack(x: torch.Tensor, format: str = "int8") -> PackedActivation:
     max(2^-4 |x|, 2^(e-10)) ("e4m3").  No gradient flows through."""
     if format is None:
         raise ValueError("activation_pack: format must be 'int8' or 'e4m3'")
-    return PackedActivation(*native.checkpoint_pack(x, _checkpoint_code(format)), format, x.shape[-1],
+    code = _checkpoint_code(format)
+    return PackedActivation(*_lib.autograd().checkpoint_pack(x, code), format, x.shape[-1],
                             x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32)
 
 
@@ -97,8 +98,9 @@ def activation_unpack(packed: PackedActivation, dtype: Optional[torch.dtype] = N
     (float32 or bfloat16; the packed tensor's storage dtype by default)."""
     if packed.format is None:
         raise ValueError("activation_unpack: format must be 'int8' or 'e4m3'")
-    return native.checkpoint_unpack(packed.values, packed.scales, _checkpoint_code(packed.format), packed.hidden,
-                                    packed.dtype if dtype is None else dtype)
+    dtype = _lib.dtype_code(packed.dtype if dtype is None else dtype)
+    return _lib.autograd().checkpoint_unpack(packed.values, packed.scales, _checkpoint_code(packed.format),
+                                             int(packed.hidden), dtype == _lib.BF16)
 
 
 # =============================================================================
