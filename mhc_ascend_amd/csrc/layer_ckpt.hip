@@ -148,7 +148,7 @@ __global__ MHC_ROW_BOUNDS((PF && N * VPT > 8)) void layer_ckpt_bwd_kernel(int fm
     const auto token = [&](int64_t t, const HeldRows<N, VPT>& xr, const RawRows<float, N, VPT, WC>& gr) {
         held_get<N, VPT>(fmt, xr, xv);
         unpack_rows<float, N, VPT, WC>(gr, C, gv);
-        bwd_token<TX, N, VPT, MODE>(t, coef, coef_stride, wv, xv, gv, dwacc, sacc, dx, scal_out, dx_scale, C, eps, red);
+        bwd_token<TX, N, VPT, MODE, true>(t, coef, coef_stride, wv, xv, gv, dwacc, sacc, dx, scal_out, dx_scale, C, eps, red);
     };
     if constexpr (PF) {
         HeldRows<N, VPT> xA, xB;

@@ -77,11 +77,77 @@ __device__ __forceinline__ void fwd_token(int64_t b, const float* __restrict__ c
     }
 }
 
+// Wave totals of NV values with each total in one lane: a step folds the
+// values of two lanes in pairs, so one lane goes on with the first half of the
+// values and its partner with the second.  About 2.3 instructions a value in
+// place of wave_sum_last's 6 (n = 4: 70 of 180), which the backward's row sums
+// are a sixth of.  Returns the number of values a lane is left with; lane l's
+// slot i holds the total of value fold_index(l, i) where that is below NV.
+template <int NV>
+constexpr int fold_left() { return (NV + 63) / 64; }
+
+template <int NV>
+__device__ __forceinline__ int fold_index(int lane, int slot) {
+    constexpr int H1 = (NV + 1) / 2, H2 = (H1 + 1) / 2, H3 = (H2 + 1) / 2, H4 = (H3 + 1) / 2, H5 = (H4 + 1) / 2,
+                  H6 = (H5 + 1) / 2;
+    // from the last step to the first: the value among those the step began
+    // with, NV where its second half had none left
+    int i = slot;
+    bool ok = true;
+    const auto up = [&](int bit, int h, int cnt) {
+        i += (lane & bit) ? h : 0;
+        ok = ok && i < cnt;
+    };
+    up(1, H6, H5);
+    up(2, H5, H4);
+    up(4, H4, H3);
+    up(8, H3, H2);
+    up(16, H2, H1);
+    up(32, H1, NV);
+    return ok ? i : NV;
+}
+
+// One step on CNT values: slot i becomes the pair's sum of value i in the lower
+// lanes and of value i + H in the upper (of nothing where there is none).
+template <int CNT, typename F>
+__device__ __forceinline__ void fold_step(float* v, F pair) {
+    constexpr int H = (CNT + 1) / 2;
+#pragma unroll
+    for (int i = 0; i < H; ++i) v[i] = pair(v[i], i + H < CNT ? v[i + H] : 0.f);
+}
+
+template <int NV>
+__device__ __forceinline__ void wave_fold(float (&v)[NV]) {
+    constexpr int H1 = (NV + 1) / 2, H2 = (H1 + 1) / 2, H3 = (H2 + 1) / 2, H4 = (H3 + 1) / 2, H5 = (H4 + 1) / 2;
+    const int lane = threadIdx.x & (kWave - 1);
+    fold_step<NV>(v, [](float a, float b) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    });
+    fold_step<H1>(v, [](float a, float b) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        return __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    });
+    fold_step<H2>(v, [&](float a, float b) {
+        return ((lane & 8) ? b : a) + dpp::mov<dpp::kRowRor8>((lane & 8) ? a : b);
+    });
+    fold_step<H3>(v, [&](float a, float b) {
+        return ((lane & 4) ? b : a) + dpp::mov<dpp::kRowHalfMirror>((lane & 4) ? a : b);
+    });
+    fold_step<H4>(v, [&](float a, float b) {
+        return ((lane & 2) ? b : a) + dpp::mov<dpp::kQuadXor2>((lane & 2) ? a : b);
+    });
+    fold_step<H5>(v, [&](float a, float b) {
+        return ((lane & 1) ? b : a) + dpp::mov<dpp::kQuadXor1>((lane & 1) ? a : b);
+    });
+}
+
 // dx of a mode: the storage type, or fp32 with MODE 2
 template <typename TX, int MODE>
 using BwdDx = std::conditional_t<MODE == 2, float, TX>;
 
-template <typename TX, int N, int VPT, int MODE>
+// FOLD: the wave's row sums by wave_fold (in another order).
+template <typename TX, int N, int VPT, int MODE, bool FOLD = false>
 __device__ __forceinline__ void bwd_token(int64_t b, const float* __restrict__ coef, int64_t coef_stride,
                                           const float (&wv)[VPT][kLayerWC],
                                           const float (&xv)[N][VPT][kLayerWC],
@@ -129,10 +195,19 @@ __device__ __forceinline__ void bwd_token(int64_t b, const float* __restrict__ c
                 }
             }
         }
-        wave_sum_last<NR>(rv);
-        if (lane == kWave - 1) {
+        if constexpr (FOLD) {
+            wave_fold<NR>(rv);
 #pragma unroll
-            for (int k = 0; k < NR; ++k) red[wave * NR + k] = rv[k];
+            for (int k = 0; k < fold_left<NR>(); ++k) {
+                const int i = fold_index<NR>(lane, k);
+                if (i < NR) red[wave * NR + i] = rv[k];
+            }
+        } else {
+            wave_sum_last<NR>(rv);
+            if (lane == kWave - 1) {
+#pragma unroll
+                for (int k = 0; k < NR; ++k) red[wave * NR + k] = rv[k];
+            }
         }
     }
     __syncthreads();
