@@ -466,9 +466,8 @@ int rmsnorm_ckpt_bwd_grid(int dt, int fmt, int64_t B, int64_t C) {
     const void* fn = nullptr;
     MHC_CK_ROWS(dt, fmt, t.vpt, rag, fn = reinterpret_cast<const void*>(&rmsnorm_ckpt_bwd_kernel<T_, F_, V_, R_>));
     // two workgroups a CU at most: their partial rows of dw cost as many bytes
-    // as rows of x, and a few more of them in flight gain less (2999 x 1001
-    // fp32: 2560 workgroups 20.7 us and two passes over their partials, 512 of
-    // them 10.9 and one)
+    // as rows of x (2999 x 1001 fp32: 2560 workgroups 20.7 us and 8.8 for their
+    // partials, 512 of them 14.4 and 3.6)
     int64_t per_cu = occupancy_per_cu(fn, t.threads, 0);
     if (per_cu > 2) per_cu = 2;
     const int64_t g = (int64_t)device_cu_count() * per_cu;

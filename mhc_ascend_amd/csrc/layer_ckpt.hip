@@ -275,14 +275,20 @@ hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, con
 }
 
 // Workgroups of at most 256 lanes prefetch (layer.hip), and of 512 where two
-// tokens' raw rows and the current one's values fit 256 registers.
-static bool ck_prefetch(const RowTiling& t, int n) { return t.threads <= 256 || n * t.vpt <= 8; }
+// tokens' raw rows and the current one's values fit 256 registers and the CUs
+// walk several tokens (n = 4, 320 x 1280 fp32: 8.9 us with, 7.0 without).
+static bool ck_prefetch(const RowTiling& t, int n, int64_t B) {
+    return t.threads <= 256 || (n * t.vpt <= 8 && B >= 4 * (int64_t)device_cu_count());
+}
+// One chunk a lane from n = 5 on too, where bwd_tiling takes two: half the raw
+// words leave room for the prefetch (4096 tokens: n = 8, 1280 fp32 102 -> 93 us, n
+// = 7, 1184 fp32 82 -> 76; n = 5, 1600 bf16 56 -> 61).
 // Modes 1 and 2 on half the chunks and twice the lanes where a lane would hold
 // 16 chunks: two waves a SIMD, one's sums under the other's loads (n = 4, 8192
 // x 4096, bf16 dx: 174 us for 198).  Mode 0 keeps one more sum a lane and spills
 // there (fp32: 310 us for 206).
 static RowTiling ck_bwd_tiling(int64_t C, int n, int64_t B, int mode) {
-    RowTiling t = layer_bwd_tiling(C, n, B);
+    RowTiling t = with_min_threads(choose_row_tiling(C, kLayerWC, 2 * n, 256), 2 + n * n + 3 * n);
     if (mode != 0 && t.threads == 256 && t.vpt >= 2 && n * t.vpt == 16) {
         t.vpt /= 2;
         t.threads = 512;
@@ -295,7 +301,7 @@ int layer_ckpt_bwd_part_groups(int n, int64_t B, int64_t C) { return ck_bwd_tili
 int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C) {
     const RowTiling t = ck_bwd_tiling(C, n, B, mode);
     const int64_t g = (int64_t)device_cu_count() *
-                      occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n)), t.threads, 0);
+                      occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n, B)), t.threads, 0);
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
 
@@ -304,7 +310,7 @@ hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const fl
                                  float* dw_part, float* scal_out, int grid, int64_t B, int64_t C, float eps,
                                  hipStream_t s, int32_t* dx_scale) {
     const RowTiling t = ck_bwd_tiling(C, n, B, mode);
-    const void* fn = pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n));
+    const void* fn = pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n, B));
     if (!fn) return hipErrorInvalidValue;
     int Ci = (int)C;
     void* args[] = {(void*)&fmt, (void*)&g,       (void*)&values,   (void*)&scales,   (void*)&w, (void*)&coef, (void*)&coef_stride, (void*)&dx,
