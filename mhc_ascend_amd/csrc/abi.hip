@@ -2331,30 +2331,34 @@ int mhc_layer_dynamic_checkpoint_fwd(const void* x, int32_t x_dtype, const void*
     });
 }
 
-// The backward whose row and projection passes read the checkpoint: n = 2..8
-// on register rows, hidden % 8 == 0, 16-byte aligned arrays.
-static bool dyn_ckpt_rows(const float* grad_out, const void* grad_x, const float* saved, int64_t batch, int32_t n,
-                          int32_t hidden) {
-    return layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}) &&
-           proj_ckpt_supported(2 * n + n * n, (int64_t)n * hidden, hidden);
-}
-
+// The backward whose projection pass reads the checkpoint, hidden % 8 == 0 and
+// n up to 16.  `rows`: so does the row pass (n = 2..8 on register rows, 16-byte
+// aligned arrays); otherwise it runs on x^ rows unpacked in fp32.
 struct DynCkptWs {
+    bool ok, rows, aligned;
     bool qin;  // dx_in is the fp16 stream part in grad_x; else fp32 in dxw (bf16 x) or grad_x
     int mode, grid, tiles, groups, rows_c;
-    size_t scal_off, dp_off, s_off, pscale_off, cpart_off, phip_off, stw_off, stp_off, dxw_off, hist_off, total;
+    size_t scal_off, dp_off, s_off, pscale_off, cpart_off, phip_off, stw_off, stp_off, dxw_off, hist_off, xw_off,
+        scratch_off, total;
 };
 
-static DynCkptWs dyn_ckpt_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype, int32_t num_iters) {
+static DynCkptWs dyn_ckpt_ws(const float* grad_out, const void* grad_x, const float* saved, int64_t batch, int32_t n,
+                             int32_t hidden, int32_t x_dtype, int32_t num_iters) {
     DynCkptWs w{};
     const int np = 2 * n + n * n;
     const int64_t K = (int64_t)n * hidden;
-    w.qin = x_dtype == kBF16 && (n == 2 || n == 4) && hidden % 128 == 0;
-    w.mode = w.qin || x_dtype == kF32 ? 1 : 2;
-    w.grid = layer_ckpt_bwd_grid(x_dtype, n, w.mode, batch, hidden);
-    w.tiles = proj_ckpt_bwd_tiles(x_dtype, w.qin, np, batch, K);
+    w.ok = batch > 0 && proj_ckpt_supported(np, K, hidden);
+    if (!w.ok) return w;
+    w.rows = layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved});
+    w.aligned = rows_aligned(n, {grad_out, grad_x, saved});
+    w.qin = w.rows && x_dtype == kBF16 && (n == 2 || n == 4) && hidden % 128 == 0;
+    w.mode = !w.rows || w.qin || x_dtype == kF32 ? 1 : 2;
+    w.grid = w.rows ? layer_ckpt_bwd_grid(x_dtype, n, w.mode, batch, hidden)
+                    : layer_bwd_grid(kF32, n, batch, hidden, w.aligned);
+    w.tiles = proj_ckpt_bwd_tiles(x_dtype, w.qin, np < kProjCkptRows ? np : kProjCkptRows, batch, K);
     w.groups = w.qin ? layer_ckpt_bwd_part_groups(n, batch, hidden) : 0;
     w.rows_c = dyn_coef_bwd_rows(n, batch, num_iters, true);
+    const bool fixed16 = n >= 16 && !generic_layer_n(n);
     size_t o = align256((size_t)w.grid * hidden * 4);
     w.scal_off = o; o += align256((size_t)batch * (n * n + 2 * n + 2) * 4);
     w.dp_off = o; o += align256((size_t)batch * dp_stride(np) * 4);
@@ -2364,8 +2368,11 @@ static DynCkptWs dyn_ckpt_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x
     w.phip_off = o; o += align256((size_t)w.tiles * np * K * 4);
     w.stw_off = o; o += align256(column_sums_stage_floats(hidden) * 4);
     w.stp_off = o; o += column_sums_direct(w.tiles) ? 0 : align256(column_sums_stage_floats((int64_t)np * K) * 4);
-    w.dxw_off = o; o += w.mode == 2 ? align256((size_t)batch * K * 4) : 0;
-    w.hist_off = o; o += generic_layer_n(n) ? align256(dyn_coef_gen_hist_bytes(n, batch)) : 0;
+    w.dxw_off = o; o += !w.qin && x_dtype == kBF16 ? align256((size_t)batch * K * 4) : 0;
+    w.hist_off = o;
+    o += fixed16 ? kSkHistBytes : (generic_layer_n(n) ? align256(dyn_coef_gen_hist_bytes(n, batch)) : 0);
+    w.xw_off = o; o += w.rows ? 0 : align256((size_t)batch * K * 4);
+    w.scratch_off = o; o += w.rows ? 0 : align256(layer_bwd_scratch_bytes(kF32, n, batch, hidden, w.aligned));
     w.total = o;
     return w;
 }
@@ -2373,9 +2380,9 @@ static DynCkptWs dyn_ckpt_ws(int64_t batch, int32_t n, int32_t hidden, int32_t x
 size_t mhc_layer_dynamic_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
                                                        int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
                                                        int32_t num_iters) {
-    if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype) || num_iters < 0) return 0;
-    if (dyn_ckpt_rows(grad_out, grad_x, saved, batch, n, hidden))
-        return dyn_ckpt_ws(batch, n, hidden, x_dtype, num_iters).total;
+    if (batch < 0 || n < 1 || n > kGenMaxN || hidden < 1 || !valid_dtype(x_dtype) || num_iters < 0) return 0;
+    const DynCkptWs w = dyn_ckpt_ws(grad_out, grad_x, saved, batch, n, hidden, x_dtype, num_iters);
+    if (w.ok) return w.total;
     return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
            mhc_layer_dynamic_bwd_workspace_size(batch, n, hidden, x_dtype);
 }
@@ -2387,8 +2394,7 @@ static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const 
                                const float* alpha_res, const float* b_res, const float* saved, void* grad_x,
                                void* grad_weight, float* grad_phi, float* grad_alpha, float* grad_b, char* ws,
                                int64_t batch, int32_t n, int32_t hidden, int32_t num_iters, float sinkhorn_eps,
-                               float rmsnorm_eps, hipStream_t s) {
-    const DynCkptWs w = dyn_ckpt_ws(batch, n, hidden, x_dtype, num_iters);
+                               float rmsnorm_eps, const DynCkptWs& w, hipStream_t s) {
     const DynSaved d = dyn_saved(batch, n, hidden);
     const int np = 2 * n + n * n;
     const int64_t K = (int64_t)n * hidden;
@@ -2399,19 +2405,35 @@ static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const 
     int32_t* pscale = w.qin ? (int32_t*)(ws + w.pscale_off) : nullptr;
     float* cpart = (float*)(ws + w.cpart_off);
     float* phip = (float*)(ws + w.phip_off);
-    void* part = w.mode == 2 ? (void*)(ws + w.dxw_off) : grad_x;
-    hipError_t e = launch_layer_ckpt_bwd(x_dtype, format, n, w.mode, grad_out, values, scales, saved + d.w_off,
-                                         saved + d.coef_off, np, part, dw_part, scal, w.grid, batch, hidden,
-                                         rmsnorm_eps, s, pscale);
+    void* part = !w.qin && x_dtype == kBF16 ? (void*)(ws + w.dxw_off) : grad_x;
+    hipError_t e;
+    if (w.rows) {
+        e = launch_layer_ckpt_bwd(x_dtype, format, n, w.mode, grad_out, values, scales, saved + d.w_off,
+                                  saved + d.coef_off, np, part, dw_part, scal, w.grid, batch, hidden, rmsnorm_eps, s,
+                                  pscale);
+    } else {
+        float* xw = (float*)(ws + w.xw_off);
+        e = launch_ckpt_unpack(kF32, format, values, scales, xw, batch * n, hidden, s);
+        if (e == hipSuccess)
+            e = launch_layer_bwd(kF32, n, 1, grad_out, xw, saved + d.w_off, saved + d.coef_off, np, part, dw_part, scal,
+                                 w.grid, batch, hidden, rmsnorm_eps, (float*)(ws + w.scratch_off), s, nullptr,
+                                 w.aligned);
+    }
     if (e == hipSuccess)
         e = launch_dyn_coef_bwd(n, scal, saved + d.coef_off, saved + d.p_off, saved + d.rh_off, batch, K, alpha_pre,
                                 alpha_post, alpha_res, b_res, dp, stok, cpart, num_iters, sinkhorn_eps,
-                                generic_layer_n(n) ? (float*)(ws + w.hist_off) : nullptr, s);
-    if (e == hipSuccess)
-        e = launch_proj_ckpt_bwd(x_dtype, w.qin, format, values, scales, dp, dp_stride(np), stok, phi_pre, phi_post,
-                                 phi_res, n, np, part, grad_x, pscale, w.groups, phip, w.tiles, batch, K, s);
+                                n >= 16 || generic_layer_n(n) ? (float*)(ws + w.hist_off) : nullptr, s);
+    // the partials of a launch's output rows are [tiles][its rows][K]
+    for (int o0 = 0; o0 < np && e == hipSuccess; o0 += kProjCkptRows) {
+        const int cnt = np - o0 < kProjCkptRows ? np - o0 : kProjCkptRows;
+        const bool last = o0 + cnt == np;
+        e = launch_proj_ckpt_bwd(last ? x_dtype : kF32, w.qin, format, values, scales, dp, dp_stride(np),
+                                 o0 == 0 ? stok : nullptr, phi_pre, phi_post, phi_res, n, o0, cnt, part,
+                                 last ? grad_x : part, pscale, w.groups, phip + (size_t)w.tiles * o0 * K, w.tiles,
+                                 batch, K, s);
+    }
     if (e != hipSuccess) return e;
-    if (column_sums_direct(w.tiles) && column_sums_direct(w.grid) && column_sums_direct(w.rows_c)) {
+    if (np <= kProjCkptRows && column_sums_direct(w.tiles) && column_sums_direct(w.grid) && column_sums_direct(w.rows_c)) {
         ColSumJobs jobs{};
         jobs.j[0] = ColSumJob{phip, grad_phi, nullptr, (int64_t)np * K, w.tiles, (int)(np * K), 0, 0, 0};
         jobs.j[1] = ColSumJob{dw_part, grad_weight, nullptr, hidden, w.grid, hidden, weight_dtype == kBF16, 0, 0};
@@ -2419,8 +2441,12 @@ static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const 
         jobs.count = 3;
         return launch_multi_column_sum(jobs, s);
     }
-    e = launch_column_finalize(0, kF32, phip, w.tiles, (int64_t)np * K, (float*)(ws + w.stp_off), grad_phi, nullptr, 0,
-                               nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+    for (int o0 = 0; o0 < np && e == hipSuccess; o0 += kProjCkptRows) {
+        const int cnt = np - o0 < kProjCkptRows ? np - o0 : kProjCkptRows;
+        e = launch_column_finalize(0, kF32, phip + (size_t)w.tiles * o0 * K, w.tiles, (int64_t)cnt * K,
+                                   (float*)(ws + w.stp_off), grad_phi + (size_t)o0 * K, nullptr, 0, nullptr, nullptr,
+                                   nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
+    }
     if (e == hipSuccess)
         e = launch_column_finalize(0, weight_dtype, dw_part, w.grid, hidden, (float*)(ws + w.stw_off), grad_weight,
                                    nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
@@ -2448,7 +2474,11 @@ int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, 
                                                 grad_out, grad_x, saved, batch, n, hidden, x_dtype, num_iters))
             return fail(MHC_ERR_WORKSPACE, "layer_dynamic_checkpoint_bwd: workspace smaller than "
                                            "mhc_layer_dynamic_checkpoint_bwd_workspace_need()");
-        if (dyn_ckpt_rows(grad_out, grad_x, saved, batch, n, hidden)) {
+        const DynCkptWs w = dyn_ckpt_ws(grad_out, grad_x, saved, batch, n, hidden, x_dtype, num_iters);
+        if (w.ok) {
+            if (n >= 16 && !generic_layer_n(n) && dyn_coef_bwd_hist_slots(n, batch, num_iters) < 1)
+                return fail(MHC_ERR_UNSUPPORTED, "layer_dynamic_checkpoint_bwd: num_iters too large for the Sinkhorn "
+                                                 "history at n=" + std::to_string(n));
             MHC_REQUIRE(phi_pre && phi_post && phi_res && alpha_pre && alpha_post && alpha_res && b_res && saved,
                         "layer_dynamic_checkpoint_bwd: null parameter pointer");
             MHC_REQUIRE(grad_weight && grad_phi && grad_alpha && grad_b,
@@ -2456,7 +2486,7 @@ int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, 
             return hip_status(dyn_ckpt_bwd(grad_out, values, scales, format, x_dtype, weight_dtype, phi_pre, phi_post,
                                            phi_res, alpha_pre, alpha_post, alpha_res, b_res, saved, grad_x,
                                            grad_weight, grad_phi, grad_alpha, grad_b, (char*)workspace, batch, n,
-                                           hidden, num_iters, sinkhorn_eps, rmsnorm_eps, (hipStream_t)stream));
+                                           hidden, num_iters, sinkhorn_eps, rmsnorm_eps, w, (hipStream_t)stream));
         }
         const size_t rows = ckpt_rows_bytes(batch * n, hidden, x_dtype);
         const hipError_t e =

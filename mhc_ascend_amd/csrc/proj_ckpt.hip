@@ -3,7 +3,9 @@
 //   dx[b][k] = dx_in[b][k] + s[b] x^[b][k] + sum_o dP[b][o] Phi[o][k]
 //   dPhi_part[tile][o][k] = sum_{b in tile} dP[b][o] x^[b][k]
 // on the bf16 matrix cores: stages of 32 tokens as proj_bwd_mfma_kernel and
-// proj_bwd_tiles_kernel (dynamic.hip), all output rows at once.
+// proj_bwd_tiles_kernel (dynamic.hip), up to 96 output rows at once; more (n >
+// 8) take a launch for each 96, the sum carried in fp32 and the s term on the
+// first.
 //
 // x^ is exact in bf16, so dP alone is split: three bf16 planes for dPhi (to
 // 2^-24 of a term; the kernels that read x use two, 2^-16), two planes of dP
@@ -23,7 +25,7 @@ template <typename TD, bool QIN, int OT, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4 : 2))) void proj_ckpt_bwd_kernel(
     int fmt, const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc, const float* __restrict__ dP,
     int dp_stride, const float* __restrict__ s_tok, const float* __restrict__ phi_pre,
-    const float* __restrict__ phi_post, const float* __restrict__ phi_res, int n, int np, const void* dx_in, TD* dx,
+    const float* __restrict__ phi_post, const float* __restrict__ phi_res, int n, int o0, int np, const void* dx_in, TD* dx,
     const int32_t* __restrict__ dx_scale, int groups, int C, float* __restrict__ dphi_part, int64_t B, int64_t K,
     int64_t tile) {
     constexpr int NT = 64 * NW;
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int o = 32 * ot + 8 * lg + e;
-                v[e] = (wave_on && o < np) ? phi_row(phi_pre, phi_post, phi_res, n, o, K)[k] : 0.f;
+                v[e] = (wave_on && o < np) ? phi_row(phi_pre, phi_post, phi_res, n, o0 + o, K)[k] : 0.f;
             }
             split_pack8(v, phh[ot][ct], phl[ot][ct]);
         }
@@ -99,7 +101,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
     const buf_rsrc_t rs_d = make_buf_rsrc(static_cast<const char*>(dx_in) + tb0 * (int64_t)irow, (uint32_t)nrows * irow);
     const buf_rsrc_t rs_o = make_buf_rsrc(dx + tb0 * K, (uint32_t)nrows * orow);
     const buf_rsrc_t rs_p = make_buf_rsrc(dP + tb0 * dp_stride, (uint32_t)(nrows * dp_stride * 4));
-    const buf_rsrc_t rs_s = make_buf_rsrc(s_tok + tb0, (uint32_t)(nrows * 4));
+    const buf_rsrc_t rs_s = make_buf_rsrc(s_tok ? s_tok + tb0 : nullptr, s_tok ? (uint32_t)(nrows * 4) : 0u);
     const buf_rsrc_t rs_q = make_buf_rsrc(QIN ? dx_scale + tb0 * groups : nullptr, QIN ? (uint32_t)(nrows * groups * 4) : 0u);
     // a piece lies in one stream (C % 8 == 0): its place in the checkpoint's row
     const int64_t si = lcol < K ? lcol / C : 0;
@@ -341,11 +343,12 @@ static int proj_ckpt_waves(bool qin) { return qin ? 8 : 4; }
 static int64_t proj_ckpt_max_tile(int64_t K) { return ((int64_t(1) << 31) - 1) / (K * 4) - 4 * 32; }
 
 bool proj_ckpt_supported(int np, int64_t K, int64_t C) {
-    return np >= 1 && np <= 3 * kProjTile && K % 32 == 0 && C % 8 == 0 && proj_ckpt_max_tile(K) >= 64;
+    return np >= 1 && np <= kProjCkptMaxRows && K % 32 == 0 && C % 8 == 0 && proj_ckpt_max_tile(K) >= 64;
 }
 
-// Column blocks x token tiles fill two rounds of resident workgroups
-// (proj_bwd_tiles).
+// Column blocks x token tiles fill one round of resident workgroups: the
+// partials of dPhi are half of two rounds' (n = 6, 2047 x 1040 bf16: 34.6 us and
+// 9.5 for their sums, against 40.7 and 12).
 int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K) {
     const int nw = proj_ckpt_waves(qin);
     const int64_t gx = (K + 32 * nw - 1) / (32 * nw);
@@ -361,12 +364,13 @@ int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K) {
 
 hipError_t launch_proj_ckpt_bwd(int dx_dtype, bool qin, int fmt, const void* values, const void* scales,
                                 const float* dP, int dp_stride, const float* s_tok, const float* phi_pre,
-                                const float* phi_post, const float* phi_res, int n, int np, const void* dx_in,
-                                void* dx, const int32_t* dx_scale, int groups, float* dphi_part, int tiles, int64_t B,
+                                const float* phi_post, const float* phi_res, int n, int o0, int np,
+                                const void* dx_in, void* dx, const int32_t* dx_scale, int groups, float* dphi_part, int tiles, int64_t B,
                                 int64_t K, hipStream_t s) {
     int C = (int)(K / n);
     if (B == 0) return hipSuccess;
-    if (!proj_ckpt_supported(np, K, C) || tiles < 1) return hipErrorInvalidValue;
+    if (!proj_ckpt_supported(np, K, C) || np > kProjCkptRows || tiles < 1) return hipErrorInvalidValue;
+    dP += o0;
     if (qin && (dx_dtype != kBF16 || !dx_scale || groups < 1 || C % kPartGroup != 0 || np > kProjTile || dx_in != dx))
         return hipErrorInvalidValue;
     int64_t tile = (B + tiles - 1) / tiles;
@@ -375,7 +379,7 @@ hipError_t launch_proj_ckpt_bwd(int dx_dtype, bool qin, int fmt, const void* val
     const int nw = proj_ckpt_waves(qin);
     const dim3 grid((unsigned)((K + 32 * nw - 1) / (32 * nw)), (unsigned)tiles);
     void* args[] = {(void*)&fmt,      (void*)&values,  (void*)&scales, (void*)&dP,     (void*)&dp_stride, (void*)&s_tok,
-                    (void*)&phi_pre,  (void*)&phi_post, (void*)&phi_res, (void*)&n,    (void*)&np,        (void*)&dx_in,
+                    (void*)&phi_pre,  (void*)&phi_post, (void*)&phi_res, (void*)&n,    (void*)&o0, (void*)&np,        (void*)&dx_in,
                     (void*)&dx,       (void*)&dx_scale, (void*)&groups, (void*)&C,     (void*)&dphi_part, (void*)&B,
                     (void*)&K,        (void*)&tile};
     const int tok = timing_begin("proj_ckpt_bwd", s);

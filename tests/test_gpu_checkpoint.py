@@ -263,7 +263,8 @@ def _oracle_dyn_held(d, fmt, iters=20, eps=1e-5):
 
 
 DYN_SHAPES = [(4, 9, 64), (4, 33, 256), (4, 600, 128), (4, 5, 4096), (4, 40, 1024), (2, 37, 256), (8, 12, 1280),
-              (3, 9, 160), (6, 17, 1040), (1, 7, 96), (12, 5, 128), (16, 5, 64)]
+              (3, 9, 160), (6, 17, 1040), (1, 7, 96), (12, 5, 128), (16, 5, 64), (10, 70, 80), (8, 4, 7168), (6, 3, 100 * 16),
+              (8, 300, 100), (20, 3, 32), (4, 1090, 136)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
