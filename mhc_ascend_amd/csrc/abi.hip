@@ -2109,6 +2109,16 @@ static int guarded(F f) noexcept {
     }
 }
 
+// A size query's: 0 where one is thrown.
+template <typename F>
+static size_t guarded_size(F f) noexcept {
+    try {
+        return f();
+    } catch (...) {
+        return 0;
+    }
+}
+
 static bool valid_format(int f) { return f == kCkInt8 || f == kCkE4M3; }
 
 static int check_ckpt(const char* fn, int64_t rows, int64_t hidden, int32_t dtype, int32_t format, bool pointers) {
@@ -2190,7 +2200,7 @@ static RowsBwdWs rmsnorm_ckpt_bwd_ws(int64_t batch, int32_t hidden, int32_t dtyp
 
 size_t mhc_rmsnorm_checkpoint_bwd_workspace_size(int64_t batch, int32_t hidden, int32_t dtype, int32_t format) {
     if (batch < 0 || !rmsnorm_ckpt_supported(hidden) || !valid_dtype(dtype) || !valid_format(format)) return 0;
-    return rmsnorm_ckpt_bwd_ws(batch, hidden, dtype, format).total;
+    return guarded_size([&]() -> size_t { return rmsnorm_ckpt_bwd_ws(batch, hidden, dtype, format).total; });
 }
 
 int mhc_rmsnorm_checkpoint_bwd(const void* grad_out, int32_t dtype, const void* values, const void* scales,
@@ -2261,10 +2271,12 @@ static StaticBwdWs static_ckpt_bwd_ws(int64_t batch, int32_t n, int32_t hidden, 
 size_t mhc_layer_static_checkpoint_bwd_workspace_need(const float* grad_out, const void* grad_x, const float* saved,
                                                       int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype) {
     if (batch < 0 || n < 1 || hidden < 1 || !valid_dtype(x_dtype)) return 0;
-    if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}))
-        return static_ckpt_bwd_ws(batch, n, hidden, x_dtype).total;
-    return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
-           mhc_layer_static_bwd_workspace_size(batch, n, hidden, x_dtype);
+    return guarded_size([&]() -> size_t {
+        if (layer_ckpt_bwd_rows(n, batch, hidden, {grad_out, grad_x, saved}))
+            return static_ckpt_bwd_ws(batch, n, hidden, x_dtype).total;
+        return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
+               mhc_layer_static_bwd_workspace_size(batch, n, hidden, x_dtype);
+    });
 }
 
 int mhc_layer_static_checkpoint_bwd(const float* grad_out, const void* values, const void* scales, int32_t format,
@@ -2381,10 +2393,12 @@ size_t mhc_layer_dynamic_checkpoint_bwd_workspace_need(const float* grad_out, co
                                                        int64_t batch, int32_t n, int32_t hidden, int32_t x_dtype,
                                                        int32_t num_iters) {
     if (batch < 0 || n < 1 || n > kGenMaxN || hidden < 1 || !valid_dtype(x_dtype) || num_iters < 0) return 0;
-    const DynCkptWs w = dyn_ckpt_ws(grad_out, grad_x, saved, batch, n, hidden, x_dtype, num_iters);
-    if (w.ok) return w.total;
-    return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
-           mhc_layer_dynamic_bwd_workspace_size(batch, n, hidden, x_dtype);
+    return guarded_size([&]() -> size_t {
+        const DynCkptWs w = dyn_ckpt_ws(grad_out, grad_x, saved, batch, n, hidden, x_dtype, num_iters);
+        if (w.ok) return w.total;
+        return ckpt_rows_bytes(batch * n, hidden, x_dtype) +
+               mhc_layer_dynamic_bwd_workspace_size(batch, n, hidden, x_dtype);
+    });
 }
 
 // The launches of mhc_layer_dynamic_bwd, with x^ read from the checkpoint.
@@ -2579,7 +2593,9 @@ size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int3
         (int64_t)q_heads + k_heads > 65535 * 4 || head_dim < 2 || head_dim > kQkMaxDim || rotary_dim < 2 ||
         rotary_dim > head_dim || rotary_dim % 2 != 0)
         return 0;
-    return qk_bwd_ws(tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved).total;
+    return guarded_size([&]() -> size_t {
+        return qk_bwd_ws(tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved).total;
+    });
 }
 
 int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,

@@ -124,6 +124,7 @@ class MHCLayer(nn.Module):
             f"expansion_rate={self.expansion_rate}, "
             f"num_sinkhorn_iters={self.num_sinkhorn_iters}, "
             f"use_dynamic_h={self.use_dynamic_h}"
+            + (f", checkpoint={self.checkpoint!r}" if self.checkpoint is not None else "")
         )
 
 

@@ -55,12 +55,19 @@ def _checkpoint_code(checkpoint: Optional[str]) -> int:
         raise ValueError(f"Unknown checkpoint format: {checkpoint!r} (None, 'int8' or 'e4m3')") from None
 
 
+def _not_traced(what: str) -> None:
+    """torch.jit.trace records Python functions only: a C++ node's result would
+    become a constant of the trace."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{what} is not recorded by torch.jit.trace")
+
+
 def _operator_checkpoint(checkpoint: Optional[str]) -> int:
     """The same for the operators that torch.jit.trace records: it records
     their Python functions, which save the rows as they are."""
     code = _checkpoint_code(checkpoint)
-    if code >= 0 and torch.jit.is_tracing():
-        raise RuntimeError("checkpoint= is not recorded by torch.jit.trace")
+    if code >= 0:
+        _not_traced("checkpoint=")
     return code
 
 
@@ -89,6 +96,7 @@ def activation_pack(x: torch.Tensor, format: str = "int8") -> PackedActivation:
     if format is None:
         raise ValueError("activation_pack: format must be 'int8' or 'e4m3'")
     code = _checkpoint_code(format)
+    _not_traced("activation_pack")
     return PackedActivation(*_lib.autograd().checkpoint_pack(x, code), format, x.shape[-1],
                             x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32)
 
@@ -98,6 +106,7 @@ def activation_unpack(packed: PackedActivation, dtype: Optional[torch.dtype] = N
     (float32 or bfloat16; the packed tensor's storage dtype by default)."""
     if packed.format is None:
         raise ValueError("activation_unpack: format must be 'int8' or 'e4m3'")
+    _not_traced("activation_unpack")
     dtype = _lib.dtype_code(packed.dtype if dtype is None else dtype)
     return _lib.autograd().checkpoint_unpack(packed.values, packed.scales, _checkpoint_code(packed.format),
                                              int(packed.hidden), dtype == _lib.BF16)
@@ -429,6 +438,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     k in 8 bits for the backward, which is then the gradient at the values that
     checkpoint stands for."""
     code = _checkpoint_code(checkpoint)
+    _not_traced("qk_norm_rope")
     if q.dim() not in (3, 4) or k.dim() != q.dim():
         raise RuntimeError("qk_norm_rope: q and k must both be [tokens, heads, D] or [batch, seq, heads, D], got "
                            f"{tuple(q.shape)} and {tuple(k.shape)}")

@@ -169,6 +169,23 @@ def test_views_of_a_joint_projection(device, D, fmt, dtype):
         _check([g.cpu() for g in got], inputs, cos.cpu()[:T], sin.cpu()[:T], False, fmt)
 
 
+def test_expanded_keys(device):
+    """Keys repeated to the query heads by expand (head stride 0): their
+    gradient is the sum over the repeats."""
+    q, k, ws, cots = _inputs(9, 4, 1, 64, torch.float32, 11)
+    cos, sin = (t.to(device) for t in mhc.rope_table(9, 64))
+    kd = k.to(device).requires_grad_(True)
+    leaves = [q.to(device).requires_grad_(True), kd, *[w.to(device).requires_grad_(True) for w in ws]]
+    out = mhc.qk_norm_rope(leaves[0], kd.expand(9, 4, 64), *leaves[2:], cos, sin)
+    g = [cots[0].to(device), torch.randn(9, 4, 64, generator=_gen(12)).to(device)]
+    got = [*[o.detach() for o in out], *torch.autograd.grad(out, leaves, g)]
+    # the sum of four rounded rows instead of one row's: four roundings, held by
+    # the row bound's 48
+    want = (q, k, ws, [cots[0], g[1].cpu().sum(1, keepdim=True)])
+    _check([got[0].cpu(), got[1][:, :1].contiguous().cpu(), *[t.cpu() for t in got[2:]]], want, cos.cpu(), sin.cpu(),
+           False, None)
+
+
 def test_expanded_cotangents(device):
     inputs = _inputs(6, 3, 2, 64, torch.float32, 5)
     q, k, ws, _ = inputs
@@ -264,6 +281,29 @@ def test_refusals(device):
     wide = torch.zeros(1, 1, 1026, device=device)
     with pytest.raises(RuntimeError, match="head_dim"):
         mhc.qk_norm_rope(wide, wide, torch.ones(1026, device=device), torch.ones(1026, device=device), cos.detach(), sin)
+
+
+@pytest.mark.parametrize("D", [128, 66])
+@pytest.mark.parametrize("fmt", [None, "int8"])
+def test_offsets_past_32_bits(device, D, fmt):
+    """More than 2^32 values of q: the last tokens against a call on them."""
+    H, K = 64, 1
+    T = (1 << 32) // (H * D) + 70
+    q = torch.empty(T, H, D, dtype=torch.bfloat16, device=device).fill_(0.5)
+    k = torch.empty(T, K, D, dtype=torch.bfloat16, device=device).fill_(0.5)
+    q[-64:] = torch.randn(64, H, D, device=device).bfloat16()
+    k[-64:] = torch.randn(64, K, D, device=device).bfloat16()
+    w = (torch.rand(D, device=device) + 0.5).bfloat16()
+    cos, sin = (t.to(device) for t in mhc.rope_table(1024, 64))
+    pos = torch.arange(T, device=device) % 1024
+    outs = []
+    for a, b, p in ((q, k, pos), (q[-64:].clone(), k[-64:].clone(), pos[-64:])):
+        leaves = [t.detach().requires_grad_(True) for t in (a, b)]
+        out = mhc.qk_norm_rope(*leaves, w, w, cos, sin, p, checkpoint=fmt)
+        grads = torch.autograd.grad(out, leaves, [a, b])
+        outs.append([t.detach()[-64:].clone() for t in (*out, *grads)])
+        del out, grads, leaves
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
 
 
 @pytest.mark.parametrize("fmt", [None, "int8"])
