@@ -2447,12 +2447,14 @@ static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const 
                                  batch, K, s);
     }
     if (e != hipSuccess) return e;
-    if (np <= kProjCkptRows && column_sums_direct(w.tiles) && column_sums_direct(w.grid) && column_sums_direct(w.rows_c)) {
+    // db and dalpha in double always: sums over all tokens that cancel
+    e = launch_small_column_sum(cpart, w.rows_c, np + 3, grad_b, grad_alpha, np, s);
+    if (e != hipSuccess) return e;
+    if (np <= kProjCkptRows && column_sums_direct(w.tiles) && column_sums_direct(w.grid)) {
         ColSumJobs jobs{};
         jobs.j[0] = ColSumJob{phip, grad_phi, nullptr, (int64_t)np * K, w.tiles, (int)(np * K), 0, 0, 0};
         jobs.j[1] = ColSumJob{dw_part, grad_weight, nullptr, hidden, w.grid, hidden, weight_dtype == kBF16, 0, 0};
-        jobs.j[2] = ColSumJob{cpart, grad_b, grad_alpha, np + 3, w.rows_c, np, 0, 0, 0};
-        jobs.count = 3;
+        jobs.count = 2;
         return launch_multi_column_sum(jobs, s);
     }
     for (int o0 = 0; o0 < np && e == hipSuccess; o0 += kProjCkptRows) {
@@ -2464,7 +2466,6 @@ static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const 
     if (e == hipSuccess)
         e = launch_column_finalize(0, weight_dtype, dw_part, w.grid, hidden, (float*)(ws + w.stw_off), grad_weight,
                                    nullptr, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0.f, s);
-    if (e == hipSuccess) e = launch_small_column_sum(cpart, w.rows_c, np + 3, grad_b, grad_alpha, np, s);
     return e;
 }
 
