@@ -1054,7 +1054,7 @@ Tensor checkpoint_unpack(const Tensor& values_in, const Tensor& scales_in, int64
     TORCH_CHECK(values_in.scalar_type() == at::kByte && scales_in.scalar_type() == at::kByte, fn,
                 ": values and scales must be uint8");
     const auto &vs = values_in.sizes(), &ss = scales_in.sizes();
-    TORCH_CHECK(hidden >= 1 && vs.size() >= 1 && vs.size() == ss.size() && vs.back() == (hidden + 15) / 16 * 16 &&
+    TORCH_CHECK(hidden >= 1 && hidden <= INT32_MAX && vs.size() >= 1 && vs.size() == ss.size() && vs.back() == (hidden + 15) / 16 * 16 &&
                     ss.back() == (hidden + 31) / 32 && vs.slice(0, vs.size() - 1) == ss.slice(0, ss.size() - 1),
                 fn, ": values ", vs, " and scales ", ss, " do not match hidden=", hidden);
     const at::DeviceGuard guard(values_in.device());
@@ -1103,6 +1103,8 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
                 ": the weights must be [head_dim]");
     TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), fn, ": cos and sin must be [positions, rotary_dim / 2]");
     TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), fn, ": cos and sin get no gradient");
+    TORCH_CHECK(q.size(1) <= INT32_MAX && k.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX &&
+                    2 * cos.size(1) <= q.size(2), fn, ": rotary_dim must be at most head_dim, and the sizes 32-bit");
     if (positions.has_value()) {
         const auto pt = positions->scalar_type();
         TORCH_CHECK(pt == at::kLong || pt == at::kInt, fn, ": positions must be int64 or int32, got ", pt);

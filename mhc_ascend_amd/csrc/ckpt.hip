@@ -74,7 +74,7 @@ template <typename T, int FMT>
 __global__ __launch_bounds__(256) void ckpt_pack_rows_kernel(const T* __restrict__ x, uint8_t* __restrict__ q,
                                                              uint8_t* __restrict__ sc, uint32_t pieces, int C) {
     const uint32_t per = (uint32_t)ck_blocks(C) * 4u;
-    const int stride = (int)ck_stride(C);
+    const int64_t stride = ck_stride(C);
     const uint32_t p = blockIdx.x * 256u + threadIdx.x;
     const bool on = p < pieces;
     const uint32_t row = on ? p / per : 0u;
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void ckpt_pack_rows_kernel(const T* __restrict
     uint2 w;
     const uint32_t s = ck_pack8<FMT>(v, w);
     if (on) {
-        if (c0 < stride) st8_nt(q + (int64_t)row * stride + c0, w);
+        if (c0 < stride) st8_nt(q + row * stride + c0, w);
         if ((c0 & 31) == 0) sc[(int64_t)row * (per >> 2) + (c0 >> 5)] = (uint8_t)s;
     }
 }
@@ -102,7 +102,7 @@ __global__ __launch_bounds__(256) void ckpt_unpack_rows_kernel(const uint8_t* __
                                                                const uint8_t* __restrict__ sc, T* __restrict__ out,
                                                                uint32_t pieces, int C) {
     const uint32_t per = (uint32_t)ck_blocks(C) * 4u;
-    const int stride = (int)ck_stride(C);
+    const int64_t stride = ck_stride(C);
     const uint32_t p = blockIdx.x * 256u + threadIdx.x;
     if (p >= pieces) return;
     const uint32_t row = p / per;
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256) void ckpt_unpack_rows_kernel(const uint8_t* __
     const int m = C - c0;
     if (m <= 0) return;
     float v[8];
-    ck_unpack8<FMT>(ld8_nt(q + (int64_t)row * stride + c0), sc[(int64_t)row * (per >> 2) + (c0 >> 5)], v);
+    ck_unpack8<FMT>(ld8_nt(q + row * stride + c0), sc[(int64_t)row * (per >> 2) + (c0 >> 5)], v);
     T* op = out + (int64_t)row * C + c0;
     if (m >= 8) {
         ck_store8(op, v);
@@ -137,8 +137,8 @@ template <typename Flat, typename Rows>
 static hipError_t ckpt_run(int64_t rows, int64_t C, Flat flat, Rows ragged) {
     if (rows == 0) return hipSuccess;
     if (C % kCkBlock == 0) {
-        // whole blocks: at most 2^30 workgroups a launch
-        const int64_t pieces = rows * (C / 8), most = ((int64_t)1 << 30) * (256 * kCkU);
+        // whole blocks: at most 2^23 workgroups (2^31 lanes) a launch
+        const int64_t pieces = rows * (C / 8), most = ((int64_t)1 << 23) * (256 * kCkU);
         for (int64_t p = 0; p < pieces; p += most) {
             const int64_t n = pieces - p < most ? pieces - p : most;
             flat(p, n, (unsigned)((n + 256 * kCkU - 1) / (256 * kCkU)));

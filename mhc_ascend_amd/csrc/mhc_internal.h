@@ -348,6 +348,7 @@ struct QkArgs {
     const float* sin;
     const void* pos;
     int64_t table_rows, period, T;
+    int64_t t0;  // the first token of a launch of the forward
     int heads[2];
     int w_dtype, pos_bytes, D, R, interleaved;
     float eps;

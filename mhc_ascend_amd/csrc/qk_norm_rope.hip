@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void qk_fwd_any_kernel(QkArgs a) {
     const int lane = threadIdx.x & 63;
     const int hh = blockIdx.y * 4 + (threadIdx.x >> 6);
     if (hh >= a.heads[0] + a.heads[1]) return;  // whole waves, no barrier below
-    const int64_t t = blockIdx.x;
+    const int64_t t = a.t0 + blockIdx.x;
     const int s = hh < a.heads[0] ? 0 : 1;
     const int h = s ? hh - a.heads[0] : hh;
     const T* x = static_cast<const T*>(a.x[s]) + t * a.x_token[s] + h * a.x_head[s];
@@ -330,7 +330,7 @@ struct QkRows {
 template <typename T, int FMT, int V, bool IL>
 __global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg) {
     const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t t = a.t0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= a.T) return;
     const QkLane<V, IL> ln(a, lane, lg);
     const QkTasks tasks(a.heads[0], a.heads[1], lg);
@@ -570,19 +570,25 @@ hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t
     const int H = a.heads[0] + a.heads[1];
     if (a.T == 0 || H == 0) return hipSuccess;
     const QkTiling t = qk_tiling(a.D, a.R, a.interleaved);
+    const int y = t.v == 0 ? (H + 3) / 4 : qk_splits(a.T, QkTasks(a.heads[0], a.heads[1], t.lg));
+    const int each = t.v == 0 ? 1 : 4;  // tokens a workgroup
+    const int64_t most = (int64_t)1 << 23;  // workgroups along tokens a launch: 2^31 lanes
     const int tok = timing_begin("qk_norm_rope_fwd", s);
-    if (t.v == 0) {
-        MHC_QK_TYPED(dt, fmt,
-                     MHC_LAUNCH_GGL((qk_fwd_any_kernel<T_, F_>), dim3((unsigned)a.T, (unsigned)((H + 3) / 4)),
-                                    dim3(256), 0, s, a));
-    } else {
-        const int y = qk_splits(a.T, QkTasks(a.heads[0], a.heads[1], t.lg));
-        MHC_QK_TILED(dt, fmt, t, a.interleaved,
-                     MHC_LAUNCH_GGL((qk_fwd_kernel<T_, F_, V_, I_>), dim3((unsigned)((a.T + 3) / 4), (unsigned)y),
-                                    dim3(256), 0, s, a, t.lg));
+    hipError_t e = hipSuccess;
+    QkArgs b = a;
+    for (b.t0 = 0; b.t0 < a.T && e == hipSuccess; b.t0 += most * each) {
+        const int64_t x = (a.T - b.t0 + each - 1) / each;
+        const dim3 grid((unsigned)(x < most ? x : most), (unsigned)y);
+        if (t.v == 0) {
+            MHC_QK_TYPED(dt, fmt, MHC_LAUNCH_GGL((qk_fwd_any_kernel<T_, F_>), grid, dim3(256), 0, s, b));
+        } else {
+            MHC_QK_TILED(dt, fmt, t, a.interleaved,
+                         MHC_LAUNCH_GGL((qk_fwd_kernel<T_, F_, V_, I_>), grid, dim3(256), 0, s, b, t.lg));
+        }
+        e = hipGetLastError();
     }
     timing_end(tok, s);
-    return hipGetLastError();
+    return e;
 }
 
 static dim3 qk_bwd_dims(const QkArgs& a) {

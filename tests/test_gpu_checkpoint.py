@@ -501,6 +501,21 @@ def test_offsets_past_32_bits(device):
     assert all(torch.equal(a, b) for a, b in zip(*outs))
 
 
+def test_one_row_of_nearly_two_to_the_31(device):
+    """The padded row is 2^31 bytes: its last blocks against a short row's."""
+    C, tail = (1 << 31) - 1, 32 * 64 - 1
+    x = torch.zeros(1, C, dtype=torch.bfloat16, device=device)
+    x[:, -tail:] = torch.randn(1, tail, device=device).bfloat16()
+    p = mhc.activation_pack(x, "int8")
+    want = mhc.activation_pack(x[:, -tail:], "int8")
+    assert torch.equal(p.values[:, -want.values.shape[1]:], want.values)
+    assert torch.equal(p.scales[:, -want.scales.shape[1]:], want.scales)
+    assert not p.values[:, :1024].any() and not p.values[:, C // 2: C // 2 + 1024].any()
+    del x
+    back = mhc.activation_unpack(p)
+    assert torch.equal(back[:, -tail:], mhc.activation_unpack(want)) and not back[:, :1024].any()
+
+
 @pytest.mark.parametrize("dynamic", [False, True])
 def test_layer_offsets_past_32_bits(device, dynamic):
     n, C = 4, 4096

@@ -406,3 +406,22 @@ def test_a_block_as_a_model_runs_it(device):
         assert float((a.cpu().double() - e).norm() / e.norm()) <= 2e-2
     ref = ref.detach()
     assert float((out.detach().cpu().double() - ref).norm() / ref.norm()) <= 1e-5
+
+
+@pytest.mark.parametrize("T,D", [((1 << 24) + 64, 6), ((1 << 26) + 64, 8)])
+def test_more_tokens_than_a_launch_takes(device, T, D):
+    """2^32 lanes and more: the first and last tokens against calls on them alone."""
+    P = 64
+    q = torch.randn(P, 1, D, device=device).bfloat16().repeat(T // P, 1, 1).view(T // P, P, 1, D)
+    q[-1] = q[-1] * 3 + 1
+    k = q.new_empty(T // P, P, 0, D)
+    w = torch.rand(D, device=device) + 0.5
+    cos, sin = mhc.rope_table(P, D, device=device)
+    with torch.no_grad():
+        out = mhc.qk_norm_rope(q, k, w, w, cos, sin)[0]
+        for at in (0, (1 << 23) // P, 4 * (1 << 23) // P, T // P - 1):
+            if at >= T // P:
+                continue
+            want = mhc.qk_norm_rope(q[at:at + 1], k[at:at + 1], w, w, cos, sin)[0]
+            assert torch.equal(out[at:at + 1], want)
+        assert torch.equal(out[:-1], out[:1].expand_as(out[:-1]))
