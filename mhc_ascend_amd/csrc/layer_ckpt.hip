@@ -300,8 +300,13 @@ int layer_ckpt_bwd_part_groups(int n, int64_t B, int64_t C) { return ck_bwd_tili
 
 int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C) {
     const RowTiling t = ck_bwd_tiling(C, n, B, mode);
-    const int64_t g = (int64_t)device_cu_count() *
-                      occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, ck_prefetch(t, n, B)), t.threads, 0);
+    const bool pf = ck_prefetch(t, n, B);
+    int64_t per_cu = occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, pf), t.threads, 0);
+    // A workgroup that prefetches wants eight tokens: it starts on none and ends
+    // with a row of dw (n = 6, 2047 x 1040: one a CU 35.4 us, two 37.7).
+    const int64_t most = B / (8 * (int64_t)device_cu_count());
+    if (pf && per_cu > most) per_cu = most > 1 ? most : 1;
+    const int64_t g = (int64_t)device_cu_count() * per_cu;
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
 

@@ -167,7 +167,58 @@ __device__ __forceinline__ void bwd_token(int64_t b, const float* __restrict__ c
     float cfv[NC];
 #pragma unroll
     for (int k = 0; k < NC; ++k) cfv[k] = cf[k];
-    {
+    if constexpr (FOLD && N >= 5) {
+        // in groups of at most 32: the sums are what the kernel keeps most of (n =
+        // 6: 124 registers for 183 without the prefetch, three workgroups of 320
+        // lanes a CU for one, 300 tokens x 1040 12.4 -> 9.3 us; n = 7, 8: no spills)
+        float xa[VPT][WC], wgy[VPT][WC];
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < WC; ++e) {
+                float a = 0.f, gy = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    a += cfv[i] * xv[i][k][e];
+                    gy += cfv[N + i] * gv[i][k][e];
+                }
+                xa[k][e] = a;
+                wgy[k][e] = wv[k][e] * gy;
+            }
+        }
+        constexpr int NG = (NR + 31) / 32, PER = (NR + NG - 1) / NG;
+        const auto group = [&](auto g_) {
+            constexpr int F = decltype(g_)::value * PER, L = NR - F < PER ? NR - F : PER;
+            float rv[L];
+#pragma unroll
+            for (int q = 0; q < L; ++q) {
+                rv[q] = 0.f;
+                const int id = F + q, m = id - 2 - N * N, i = m >= 0 ? m % N : (id >= 2 ? (id - 2) / N : 0),
+                          j = id >= 2 && m < 0 ? (id - 2) % N : 0;
+#pragma unroll
+                for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+                    for (int e = 0; e < WC; ++e) {
+                        if (id == 0) rv[q] += xa[k][e] * xa[k][e];
+                        else if (id == 1) rv[q] += wgy[k][e] * xa[k][e];
+                        else if (m < 0) rv[q] += gv[i][k][e] * xv[j][k][e];
+                        else if (m < N) rv[q] += gv[i][k][e] * (wv[k][e] * xa[k][e]);
+                        else if (m < 2 * N) rv[q] += wgy[k][e] * xv[i][k][e];
+                        else rv[q] += xa[k][e] * xv[i][k][e];
+                    }
+                }
+            }
+            wave_fold<L>(rv);
+            static_assert(fold_left<L>() == 1, "a group is a wave's at most");
+            const int i = fold_index<L>(lane, 0);
+            if (i < L) red[wave * NR + F + i] = rv[0];
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        group(std::integral_constant<int, 0>{});
+        if constexpr (NG > 1) group(std::integral_constant<int, 1>{});
+        if constexpr (NG > 2) group(std::integral_constant<int, 2>{});
+        static_assert(NG <= 3, "n up to 8");
+    } else {
         float rv[NR];
 #pragma unroll
         for (int k = 0; k < NR; ++k) rv[k] = 0.f;
