@@ -969,6 +969,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
                                        held(hk.values), held(hk.scales), T, (int32_t)H, (int32_t)K, (int32_t)D,
                                        (int32_t)(2 * t.cos.size(1)), interleaved, (float)eps, stream()),
               fn);
+        if (!ctx) return {qo, ko};  // no backward will run
         tensor_list sv = {t.wq, t.wk, t.cos, t.sin};
         if (fmt != MHC_CHECKPOINT_NONE) {
             sv.insert(sv.end(), {hq.values, hk.values, hq.scales, hk.scales});
@@ -1087,35 +1088,47 @@ Tensor stream_distribute_mix_add(const Tensor& y, const Tensor& h, const Tensor&
     return Distribute::apply(y, h, m, x, format_for(checkpoint, {&y, &h, &m, &x}));
 }
 
-std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk,
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, const Tensor& wq, const Tensor& wk,
                                         const Tensor& cos, const Tensor& sin, const c10::optional<Tensor>& positions,
-                                        int64_t period, double eps, bool interleaved, int64_t checkpoint) {
+                                        double eps, bool interleaved, int64_t checkpoint) {
     require_bound();
     const char* fn = "qk_norm_rope";
-    check_device(fn, {&q, &k, &wq, &wk, &cos, &sin});
-    if (positions.has_value()) check_device(fn, {&q, &*positions});
-    TORCH_CHECK(q.dim() == 3 && k.dim() == 3, fn, ": q and k must be [tokens, heads, head_dim]");
-    TORCH_CHECK(q.size(0) == k.size(0) && q.size(2) == k.size(2), fn,
-                ": q and k must have the same tokens and head_dim, got ", q.sizes(), " and ", k.sizes());
-    TORCH_CHECK(q.scalar_type() == k.scalar_type() && at::isFloatingType(q.scalar_type()), fn,
-                ": q and k must have one floating dtype, got ", q.scalar_type(), " and ", k.scalar_type());
-    TORCH_CHECK(wq.numel() == q.size(2) && wk.numel() == q.size(2) && wq.dim() == 1 && wk.dim() == 1, fn,
+    check_device(fn, {&q_in, &k_in, &wq, &wk, &cos, &sin});
+    if (positions.has_value()) check_device(fn, {&q_in, &*positions});
+    const int64_t dims = q_in.dim();
+    TORCH_CHECK((dims == 3 || dims == 4) && k_in.dim() == dims, fn,
+                ": q and k must both be [tokens, heads, D] or [batch, seq, heads, D], got ", q_in.sizes(), " and ",
+                k_in.sizes());
+    const auto lead = q_in.sizes().slice(0, dims - 2);
+    TORCH_CHECK(lead == k_in.sizes().slice(0, dims - 2) && q_in.size(-1) == k_in.size(-1), fn,
+                ": q and k must have the same tokens and head_dim, got ", q_in.sizes(), " and ", k_in.sizes());
+    TORCH_CHECK(q_in.scalar_type() == k_in.scalar_type() && at::isFloatingType(q_in.scalar_type()), fn,
+                ": q and k must have one floating dtype, got ", q_in.scalar_type(), " and ", k_in.scalar_type());
+    const int64_t D = q_in.size(-1);
+    TORCH_CHECK(wq.numel() == D && wk.numel() == D && wq.dim() == 1 && wk.dim() == 1, fn,
                 ": the weights must be [head_dim]");
     TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), fn, ": cos and sin must be [positions, rotary_dim / 2]");
     TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), fn, ": cos and sin get no gradient");
-    TORCH_CHECK(q.size(1) <= INT32_MAX && k.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX &&
-                    2 * cos.size(1) <= q.size(2), fn, ": rotary_dim must be at most head_dim, and the sizes 32-bit");
+    TORCH_CHECK(q_in.size(-2) <= INT32_MAX && k_in.size(-2) <= INT32_MAX && D <= INT32_MAX && 2 * cos.size(1) <= D, fn,
+                ": rotary_dim must be at most head_dim, and the sizes 32-bit");
+    int64_t period = lead.back();
     if (positions.has_value()) {
         const auto pt = positions->scalar_type();
+        TORCH_CHECK(positions->sizes() == lead || positions->sizes() == lead.slice(lead.size() - 1), fn,
+                    ": positions must be ", lead, " or ", lead.slice(lead.size() - 1), ", got ", positions->sizes());
         TORCH_CHECK(pt == at::kLong || pt == at::kInt, fn, ": positions must be int64 or int32, got ", pt);
-        TORCH_CHECK(positions->numel() == period, fn, ": positions must have one entry a token");
+        period = positions->numel();
     }
-    // an outer loop over tokens of the same positions is whole
-    TORCH_CHECK(q.size(0) == 0 || (period > 0 && q.size(0) % period == 0), fn, ": ", q.size(0),
-                " tokens do not repeat ", period, " positions");
-    const tensor_list out = QkNormRope::apply(q, k, wq, wk, cos, sin, positions, std::max<int64_t>(period, 1), eps,
-                                              interleaved, format_for(checkpoint, {&q, &k, &wq, &wk}));
-    return {out[0], out[1]};
+    const Tensor q = dims == 4 ? q_in.flatten(0, 1) : q_in, k = dims == 4 ? k_in.flatten(0, 1) : k_in;
+    const int64_t fmt = format_for(checkpoint, {&q, &k, &wq, &wk});
+    const bool backward = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
+                                                         wq.requires_grad() || wk.requires_grad());
+    period = std::max<int64_t>(period, 1);
+    const tensor_list out =
+        backward ? QkNormRope::apply(q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt)
+                 : QkNormRope::forward(nullptr, q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt);
+    if (dims == 3) return {out[0], out[1]};
+    return {out[0].unflatten(0, lead), out[1].unflatten(0, lead)};
 }
 
 Tensor static_layer(const Tensor& x, const Tensor& w, const Tensor& hp, const Tensor& hq, const Tensor& hr,
@@ -1206,6 +1219,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           },
           "(values, scales, format, hidden, bf16) -> [..., hidden]");
     m.def("qk_norm_rope", &qk_norm_rope,
-          "(q [T, H, D], k [T, K, D], q_weight, k_weight, cos, sin, positions or None, period, eps, interleaved, "
+          "(q [..., H, D], k [..., K, D], q_weight, k_weight, cos, sin, positions or None, eps, interleaved, "
           "checkpoint) -> (q, k) with autograd");
 }

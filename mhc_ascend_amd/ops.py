@@ -439,21 +439,5 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     checkpoint stands for."""
     code = _checkpoint_code(checkpoint)
     _not_traced("qk_norm_rope")
-    if q.dim() not in (3, 4) or k.dim() != q.dim():
-        raise RuntimeError("qk_norm_rope: q and k must both be [tokens, heads, D] or [batch, seq, heads, D], got "
-                           f"{tuple(q.shape)} and {tuple(k.shape)}")
-    if q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
-        raise RuntimeError("qk_norm_rope: q and k must have the same tokens and head_dim, got "
-                           f"{tuple(q.shape)} and {tuple(k.shape)}")
-    lead = q.shape[:-2]
-    if positions is not None and positions.shape not in (lead, lead[-1:]):
-        raise RuntimeError(f"qk_norm_rope: positions must be {tuple(lead)} or {tuple(lead[-1:])}, got "
-                           f"{tuple(positions.shape)}")
-    period = lead[-1] if positions is None else positions.numel()
-    if q.dim() == 4:
-        q, k = q.flatten(0, 1), k.flatten(0, 1)
-    q, k = _lib.autograd().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, period, float(eps),
-                                        bool(interleaved), code)
-    if len(lead) == 2:
-        q, k = q.unflatten(0, lead), k.unflatten(0, lead)
-    return q, k
+    return _lib.autograd().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved),
+                                        code)
