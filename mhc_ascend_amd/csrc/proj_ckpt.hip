@@ -9,8 +9,9 @@
 //
 // x^ is exact in bf16, so dP alone is split: three bf16 planes for dPhi (to
 // 2^-24 of a term; the kernels that read x use two, 2^-16), two planes of dP
-// and Phi for dx.  Bound by its bytes: 33/32 of x^, dx_in and dx a value (C4,
-// n = 4, bf16: 674 MB).
+// and Phi for dx.  Bound by its bytes: 33/32 of a byte of x^, dx_in and dx a
+// value (8192 x 4 x 4096 bf16: 674 MB in 131-148 us, 4.6-5.1 TB/s; the one that
+// reads x, 806 MB, 143).
 #include "mhc_ckpt.h"
 #include "mhc_device.h"
 #include "mhc_internal.h"
