@@ -204,6 +204,18 @@ hipError_t launch_ckpt_unpack(int dt, int fmt, const void* values, const void* s
     return e;
 }
 
+// A piece that a row of C >= 8 ends in is read as the row's last 8 elements;
+// this moves its own, 8 - m of them on (m = 1 .. 7), to the front, zeros behind.
+__device__ __forceinline__ void ck_shift_part(int m, float (&v)[8]) {
+    const int by = 8 - m;
+#pragma unroll
+    for (int s = 4; s >= 1; s >>= 1) {
+        const bool on = (by & s) != 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = on ? (e + s < 8 ? v[e + s] : 0.f) : v[e];
+    }
+}
+
 // ---------------------------------------------------------------------------
 // RMSNorm rows in registers: VPT pieces of 8 channels a lane (piece q = k *
 // blockDim.x + tid), so any row of up to 512 * 8 * 4 channels fits.  RAG: the
@@ -216,21 +228,24 @@ __device__ __forceinline__ void ck_row_get(const T* __restrict__ row, int C, con
     for (int k = 0; k < VPT; ++k) {
         const int c0 = (k * blockDim.x + threadIdx.x) * 8;
         in[k].get(v[k]);
-        if (RAG && c0 < C && c0 + 8 > C) ck_load_part(row + c0, C - c0, v[k]);
+        if (RAG && c0 < C && c0 + 8 > C) {
+            if (C >= 8) ck_shift_part(C - c0, v[k]);
+            else ck_load_part(row, C, v[k]);
+        }
         if (c0 >= C) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
         }
     }
 }
-// Pieces that lie in the row whole; the others read its first elements (a
-// row under 8 channels: nothing) and are replaced by ck_row_get.
+// Pieces that lie in the row whole, the row's last 8 elements where it ends
+// inside one, and its first for lanes past it (a row under 8: nothing).
 template <typename T, int VPT, bool RAG>
 __device__ __forceinline__ void ck_row_load(const T* __restrict__ row, int C, CkPiece<T> (&in)[VPT]) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        if (!RAG || C >= 8) in[k].load(row + (c0 + 8 <= C ? c0 : 0));
+        if (!RAG || C >= 8) in[k].load(row + (c0 + 8 <= C ? c0 : (RAG && c0 < C ? C - 8 : 0)));
         else in[k] = CkPiece<T>{};
     }
 }
@@ -377,6 +392,155 @@ __global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_kernel(const T* __restri
 }
 
 // ---------------------------------------------------------------------------
+// Narrow rows, C <= 512: a group of 2^lg lanes a row, 8 channels a lane, so a
+// wave takes 64 >> lg rows at once and sums without LDS (forward and backward,
+// against a workgroup a row: 35334 x 104 bf16 23 us for 44, 65536 x 256 bf16 45
+// for 63, 65536 x 512 bf16 75 for 86, 30000 x 500 fp32 78 for 88; 1000 x 400 bf16
+// 17 for 17).  Bound by bytes from 256 channels on.
+// ---------------------------------------------------------------------------
+constexpr int kCkNarrow = 512;
+
+template <typename T, bool RAG>
+struct CkNarrow {
+    int c0, C;
+    __device__ __forceinline__ CkNarrow(int C_, int lg) : C(C_) { c0 = (threadIdx.x & ((1 << lg) - 1)) * 8; }
+    __device__ __forceinline__ bool in() const { return c0 < C; }
+    template <typename U>
+    __device__ __forceinline__ void load(const U* __restrict__ row, CkPiece<U>& p) const {
+        if (!RAG || C >= 8) p.load(row + (c0 + 8 <= C ? c0 : (RAG && c0 < C ? C - 8 : 0)));
+        else p = CkPiece<U>{};
+    }
+    template <typename U>
+    __device__ __forceinline__ void get(const U* __restrict__ row, const CkPiece<U>& p, float (&v)[8]) const {
+        p.get(v);
+        if (RAG && c0 < C && c0 + 8 > C) {
+            if (C >= 8) ck_shift_part(C - c0, v);
+            else ck_load_part(row, C, v);
+        }
+        if (c0 >= C) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void put(T* __restrict__ row, const float (&v)[8]) const {
+        if (c0 + 8 <= C) ck_store8(row + c0, v);
+        else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v);
+    }
+};
+
+template <typename T, int FMT, bool RAG>
+__global__ __launch_bounds__(256) void rmsnorm_ckpt_fwd_narrow_kernel(const T* __restrict__ x,
+                                                                      const float* __restrict__ w, T* __restrict__ y,
+                                                                      uint8_t* __restrict__ q, uint8_t* __restrict__ sc,
+                                                                      int64_t B, int C, int lg, float eps) {
+    const CkNarrow<T, RAG> ln(C, lg);
+    const int nb = (int)ck_blocks(C), stride = (int)ck_stride(C);
+    const int lane = threadIdx.x & 63, rows = 64 >> lg, sub = lane >> lg;
+    float wv[8];
+    {
+        CkPiece<float> p;
+        ln.load(w, p);
+        ln.get(w, p, wv);
+    }
+    const int64_t step = (int64_t)gridDim.x * 4 * rows;
+    int64_t b0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows;  // the wave's first row
+    const auto at = [&](int64_t b) { return b + sub < B ? b + sub : B - 1; };
+    CkPiece<T> in;
+    ln.load(x + at(b0) * C, in);
+    for (; b0 < B; b0 += step) {
+        const int64_t b = b0 + sub;
+        float v[8];
+        ln.get(x + at(b0) * C, in, v);
+        ln.load(x + at(b0 + step) * C, in);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+        uint2 p;
+        const uint32_t s = ck_pack8<FMT>(v, p);
+        if (b < B && ln.c0 < stride) st8_nt(q + b * stride + ln.c0, p);
+        if (b < B && ln.in() && (lane & 3) == 0) sc[b * nb + (ln.c0 >> 5)] = (uint8_t)s;
+        ss = lane_group_sum(ss, lg);
+        const float inv = 1.f / sqrtf(ss / (float)C + eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * wv[e];
+        if (b < B) ln.put(y + b * C, v);
+    }
+}
+
+template <typename T, int FMT, bool RAG>
+__global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_narrow_kernel(const T* __restrict__ g,
+                                                                      const uint8_t* __restrict__ q,
+                                                                      const uint8_t* __restrict__ sc,
+                                                                      const float* __restrict__ w, T* __restrict__ gx,
+                                                                      float* __restrict__ dw_part, int64_t B, int C,
+                                                                      int lg, float eps) {
+    __shared__ float red[8 * kCkNarrow];
+    const CkNarrow<T, RAG> ln(C, lg);
+    const int nb = (int)ck_blocks(C), stride = (int)ck_stride(C);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = 64 >> lg, sub = lane >> lg;
+    float wv[8], dw[8];
+    {
+        CkPiece<float> p;
+        ln.load(w, p);
+        ln.get(w, p, wv);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[e] = 0.f;
+    const int64_t step = (int64_t)gridDim.x * 8 * rows;
+    int64_t b0 = ((int64_t)blockIdx.x * 8 + wave) * rows;
+    const auto at = [&](int64_t b) { return b + sub < B ? b + sub : B - 1; };
+    CkPiece<T> gn;
+    uint2 qn;
+    uint32_t sn;
+    const auto load = [&](int64_t row) {
+        ln.load(g + row * C, gn);
+        const int c0 = ln.in() ? ln.c0 : 0;
+        qn = ld8_nt(q + row * stride + c0);
+        sn = sc[row * nb + (c0 >> 5)];
+    };
+    load(at(b0));
+    for (; b0 < B; b0 += step) {
+        const bool on = b0 + sub < B;
+        const int64_t b = at(b0);
+        float xv[8], gv[8];
+        ln.get(g + b * C, gn, gv);
+        ck_unpack8<FMT>(qn, sn, xv);
+        load(at(b0 + step));
+        float ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            xv[e] = ln.in() ? xv[e] : 0.f;
+            ss += xv[e] * xv[e];
+            dot += gv[e] * wv[e] * xv[e];
+        }
+        ss = lane_group_sum(ss, lg);
+        dot = lane_group_sum(dot, lg);
+        const float inv = 1.f / sqrtf(ss / (float)C + eps);
+        const float k2 = dot * inv * inv * inv / (float)C;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            dw[e] += on ? gv[e] * xv[e] * inv : 0.f;
+            gv[e] = wv[e] * gv[e] * inv - xv[e] * k2;
+        }
+        if (on) ln.put(gx + b * C, gv);
+    }
+    // the wave's groups, the workgroup's waves
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v = dw[e];
+        for (int k = 1 << lg; k < 64; k <<= 1) v += __shfl_xor(v, k);
+        if (sub == 0 && ln.c0 + e < C) red[wave * C + ln.c0 + e] = v;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < C; i += 512) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += red[k * C + i];
+        dw_part[(int64_t)blockIdx.x * C + i] = v;
+    }
+}
+
+// ---------------------------------------------------------------------------
 // Sums of a weight gradient's partials part[rows][cols] over rows, 32 columns a
 // workgroup in 32 phases of rows (each in order, then the phases in order):
 // 512 rows take two rounds of eight loads a lane and one LDS sum.  Bound by the
@@ -431,7 +595,20 @@ static CkRowTiling ck_row_tiling(int64_t C) {
     return CkRowTiling{vpt, (int)(((pieces + vpt - 1) / vpt + 63) / 64 * 64)};
 }
 
+// log2 of the lanes a narrow row takes: 4 (a block of 32) to 64
+static int ck_narrow_lg(int64_t C) {
+    int lg = 2;
+    while ((8 << lg) < C) ++lg;
+    return lg;
+}
+
 bool rmsnorm_ckpt_supported(int64_t C) { return C >= 1 && C <= kCkMaxRow; }
+
+#define MHC_CK_NARROW(dt, fmt, rag, ...)                                                 \
+    MHC_CK_TYPED(dt, fmt, {                                                              \
+        if (rag) { constexpr bool R_ = true; __VA_ARGS__; }                              \
+        else { constexpr bool R_ = false; __VA_ARGS__; }                                 \
+    })
 
 #define MHC_CK_ROWS(dt, fmt, vpt, rag, ...)                                              \
     MHC_CK_TYPED(dt, fmt, {                                                              \
@@ -452,6 +629,19 @@ hipError_t launch_rmsnorm_ckpt_fwd(int dt, int fmt, const void* x, const float* 
     const CkRowTiling t = ck_row_tiling(C);
     const bool rag = C % 8 != 0;
     const int tok = timing_begin("rmsnorm_ckpt_fwd", s);
+    if (C <= kCkNarrow) {
+        const int lg = ck_narrow_lg(C);
+        const int64_t each = 4 * (64 >> lg), most = (B + each - 1) / each;
+        MHC_CK_NARROW(dt, fmt, rag, {
+            const void* fn = reinterpret_cast<const void*>(&rmsnorm_ckpt_fwd_narrow_kernel<T_, F_, R_>);
+            const int64_t g = (int64_t)device_cu_count() * occupancy_per_cu(fn, 256, 0);
+            MHC_LAUNCH_GGL((rmsnorm_ckpt_fwd_narrow_kernel<T_, F_, R_>), dim3((unsigned)(g < most ? g : most)),
+                           dim3(256), 0, s, (const T_*)x, w, (T_*)y, (uint8_t*)values, (uint8_t*)scales, B, (int)C, lg,
+                           eps);
+        });
+        timing_end(tok, s);
+        return hipGetLastError();
+    }
     MHC_CK_ROWS(dt, fmt, t.vpt, rag, {
         const void* fn = reinterpret_cast<const void*>(&rmsnorm_ckpt_fwd_kernel<T_, F_, V_, R_>);
         const int64_t g = (int64_t)device_cu_count() * occupancy_per_cu(fn, t.threads, 0);
@@ -463,15 +653,23 @@ hipError_t launch_rmsnorm_ckpt_fwd(int dt, int fmt, const void* x, const float* 
 }
 
 int rmsnorm_ckpt_bwd_grid(int dt, int fmt, int64_t B, int64_t C) {
+    if (C <= kCkNarrow) {
+        const int64_t each = 8 * (64 >> ck_narrow_lg(C)), most = (B + each - 1) / each;
+        const int64_t g = 2 * (int64_t)device_cu_count();
+        return (int)(g < most ? g : (most < 1 ? 1 : most));
+    }
     const CkRowTiling t = ck_row_tiling(C);
     const bool rag = C % 8 != 0;
     const void* fn = nullptr;
     MHC_CK_ROWS(dt, fmt, t.vpt, rag, fn = reinterpret_cast<const void*>(&rmsnorm_ckpt_bwd_kernel<T_, F_, V_, R_>));
-    // two workgroups a CU at most: their partial rows of dw cost as many bytes
-    // as rows of x (2999 x 1001 fp32: 2560 workgroups 20.7 us and 8.8 for their
-    // partials, 512 of them 14.4 and 3.6)
-    int64_t per_cu = occupancy_per_cu(fn, t.threads, 0);
-    if (per_cu > 2) per_cu = 2;
+    // at most two workgroups a CU, or as many of 1024 lanes together where each
+    // still has 16 rows: their partial rows of dw cost as many bytes as rows of x
+    // (2999 x 1001 fp32: 2560 workgroups 20.7 us and 8.8 for their partials, 512
+    // of them 14.4 and 3.6)
+    int64_t per_cu = occupancy_per_cu(fn, t.threads, 0), most = B / (16 * (int64_t)device_cu_count());
+    if (most > 1024 / t.threads) most = 1024 / t.threads;
+    if (most < 2) most = 2;
+    if (per_cu > most) per_cu = most;
     const int64_t g = (int64_t)device_cu_count() * per_cu;
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
@@ -484,6 +682,14 @@ hipError_t launch_rmsnorm_ckpt_bwd(int dt, int fmt, const void* g, const void* v
     const CkRowTiling t = ck_row_tiling(C);
     const bool rag = C % 8 != 0;
     const int tok = timing_begin("rmsnorm_ckpt_bwd", s);
+    if (C <= kCkNarrow) {
+        MHC_CK_NARROW(dt, fmt, rag,
+                      MHC_LAUNCH_GGL((rmsnorm_ckpt_bwd_narrow_kernel<T_, F_, R_>), dim3(grid), dim3(512), 0, s,
+                                     (const T_*)g, (const uint8_t*)values, (const uint8_t*)scales, w, (T_*)gx, dw_part,
+                                     B, (int)C, ck_narrow_lg(C), eps));
+        timing_end(tok, s);
+        return hipGetLastError();
+    }
     MHC_CK_ROWS(dt, fmt, t.vpt, rag,
                 MHC_LAUNCH_GGL((rmsnorm_ckpt_bwd_kernel<T_, F_, V_, R_>), dim3(grid), dim3(t.threads), 0, s,
                                (const T_*)g, (const uint8_t*)values, (const uint8_t*)scales, w, (T_*)gx, dw_part, B,

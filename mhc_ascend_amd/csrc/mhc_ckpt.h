@@ -43,6 +43,16 @@ __device__ __forceinline__ uint32_t ck_group_max(uint32_t a) {
     return a;
 }
 
+// Sum over the aligned group of 2^lg lanes (lg >= 2), in every lane of it.
+__device__ __forceinline__ float lane_group_sum(float v, int lg) {
+    v = group_sum<4>(v);
+    if (lg >= 3) v += dpp::mov<dpp::kRowHalfMirror>(v);
+    if (lg >= 4) v += dpp::mov<dpp::kRowMirror>(v);
+    if (lg >= 5) v = xor16_add(v);
+    if (lg >= 6) v = xor32_add(v);
+    return v;
+}
+
 // The bits of |x| order as the values do, with infinity and NaN on top.
 __device__ __forceinline__ uint32_t ck_abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 

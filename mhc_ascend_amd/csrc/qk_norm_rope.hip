@@ -219,16 +219,6 @@ __device__ __forceinline__ void qk_store(T* p, const float (&v)[V]) {
     }
 }
 
-// Sum over the aligned group of 2^lg lanes (lg >= 2), in every lane of it.
-__device__ __forceinline__ float qk_group_sum(float v, int lg) {
-    v = group_sum<4>(v);
-    if (lg >= 3) v += dpp::mov<dpp::kRowHalfMirror>(v);
-    if (lg >= 4) v += dpp::mov<dpp::kRowMirror>(v);
-    if (lg >= 5) v = xor16_add(v);
-    if (lg >= 6) v = xor32_add(v);
-    return v;
-}
-
 // One lane's place in its head row.
 template <int V, bool IL>
 struct QkLane {
@@ -394,7 +384,7 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg) {
                 }
                 if (on && ln.in && (ln.c0 & 31) == 0) a.sc[s][row * nb + (ln.c0 >> 5)] = (uint8_t)sc;
             }
-            ss = qk_group_sum(ss, lg);
+            ss = lane_group_sum(ss, lg);
             const float inv = pos < 0 ? __uint_as_float(0x7fc00000u) : 1.f / sqrtf(ss / (float)a.D + a.eps);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -487,8 +477,8 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, float* __
                     ss += v[e] * v[e];
                     dot += d[e] * w[e] * v[e];
                 }
-                ss = qk_group_sum(ss, lg);
-                dot = qk_group_sum(dot, lg);
+                ss = lane_group_sum(ss, lg);
+                dot = lane_group_sum(dot, lg);
                 const float inv = pos < 0 ? __uint_as_float(0x7fc00000u) : 1.f / sqrtf(ss / (float)a.D + a.eps);
                 const float k2 = dot * inv * inv * inv / (float)a.D;
 #pragma unroll

@@ -181,6 +181,16 @@ def test_rmsnorm(device, fmt, dtype, B, C, shift):
     _within(gw, dw, K_DW * 2.0 ** -24 * dwmag + 1e-30, "dw")
 
 
+# Several rows a wave up to 512 values: a lane adds at most 70001 / (4 * 8 * 512)
+# + 1 rows of a weight's gradient, then 6 groups, 8 waves and the partials as above.
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,C,shift", [(70001, 104, 0), (35003, 100, 1), (35000, 33, 0), (20001, 7, 0), (4097, 256, 0),
+                                       (1030, 505, 1), (5, 512, 0), (9, 520, 0), (33, 517, 1), (17, 9, 3)])
+def test_rmsnorm_narrow_rows(device, fmt, dtype, B, C, shift):
+    test_rmsnorm(device, fmt, dtype, B, C, shift)
+
+
 def test_rmsnorm_empty_and_refused_rows(device):
     x = torch.empty(0, 64, device=device, requires_grad=True)
     w = torch.ones(64, device=device, requires_grad=True)
