@@ -381,14 +381,7 @@ __global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_kernel(const T* __restri
         }
         ck_row_put<T, VPT, RAG>(gx + b * C, C, gv);
     }
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        float* p = dw_part + (int64_t)blockIdx.x * C + c0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (c0 + e < C) p[e] = dw[k][e];
-    }
+    ck_row_put<float, VPT, RAG>(dw_part + (int64_t)blockIdx.x * C, C, dw);
 }
 
 // ---------------------------------------------------------------------------

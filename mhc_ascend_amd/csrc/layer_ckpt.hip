@@ -306,9 +306,12 @@ int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C) {
     const bool pf = ck_prefetch(t, n, B);
     int64_t per_cu = occupancy_per_cu(pick_ck_bwd(x_dtype, n, t.vpt, mode, pf), t.threads, 0);
     // A workgroup that prefetches wants eight tokens: it starts on none and ends
-    // with a row of dw (n = 6, 2047 x 1040: one a CU 35.4 us, two 37.7).
-    const int64_t most = B / (8 * (int64_t)device_cu_count());
-    if (pf && per_cu > most) per_cu = most > 1 ? most : 1;
+    // with a row of dw (n = 6, 2047 x 1040: one a CU 35.4 us, two 37.7); narrow
+    // ones fill 512 lanes a CU all the same (n = 6, 3238 x 256 fp32, the dynamic
+    // step: 110 us, 124 with one wave a CU).
+    int64_t most = B / (8 * (int64_t)device_cu_count());
+    if (most < 512 / t.threads) most = 512 / t.threads;
+    if (pf && per_cu > most) per_cu = most;
     const int64_t g = (int64_t)device_cu_count() * per_cu;
     return (int)(g < B ? g : (B < 1 ? 1 : B));
 }
