@@ -169,7 +169,11 @@ __global__ __launch_bounds__(256) void qk_bwd_any_kernel(QkArgs a, float* __rest
 // lane of the rotated halves reads its partner's piece itself: the bytes are
 // in the cache line of another lane's load, and no exchange between lanes
 // waits on the sums.  Tasks of U such steps have all their loads in flight.
-// Few tokens: their tasks are spread over Y workgroups each.  Bound by bytes:
+// Few tokens: their tasks are spread over Y workgroups each.  Few heads and many
+// tokens (MT): the groups of a wave share 2^tw tokens, each with its own table
+// row, so that a step's groups all have a head (forward and backward, against one
+// token a wave: 16384 x 1 + 1 heads of 64 fp32 30 us for 67, 16384 x 4 + 4 of 64
+// bf16 int8 36 for 72, 16384 x 8 + 1 of 128 bf16 55 for 73).  Bound by bytes:
 // 8192 tokens x 40 heads of 128 bf16, forward 32 us (5.2 TB/s), backward 52 (4.8);
 // 16384 x 64 heads with an int8 checkpoint, 135-143 (4.7-5.0) and 164-184
 // (3.7-4.1).  16 tokens x 40 heads: 4.7 us, the latency of its loads.
@@ -296,11 +300,12 @@ struct QkLane {
 };
 
 constexpr int kQkU = 2;
-// Tasks of a token: its queries' steps, then its keys', U at a time.
+// Tasks of a token: its queries' steps, then its keys', U at a time.  lt: log2
+// of the lanes a head times the tokens of a wave.
 struct QkTasks {
     int per;    // heads of a task
     int nq, n;  // tasks of the queries, of both
-    __host__ __device__ QkTasks(int H, int K, int lg) : per(kQkU * (64 >> lg)) {
+    __host__ __device__ QkTasks(int H, int K, int lt) : per(kQkU * (64 >> lt)) {
         nq = (H + per - 1) / per;
         n = nq + (K + per - 1) / per;
     }
@@ -322,14 +327,21 @@ struct QkRows {
     }
 };
 
-template <typename T, int FMT, int V, bool IL>
-__global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg) {
+template <typename T, int FMT, int V, bool IL, bool MT>
+__global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg, int tw) {
     const int lane = threadIdx.x & 63;
-    const int64_t t = a.t0 + (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (!MT) tw = 0;
+    int64_t t = a.t0 + (((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) << tw);
     if (t >= a.T) return;
     const QkLane<V, IL> ln(a, lane, lg);
-    const QkTasks tasks(a.heads[0], a.heads[1], lg);
-    const int sub = lane >> lg, step = 64 >> lg;
+    const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
+    const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
+    bool here = true;
+    if (MT) {
+        t += lane >> (6 - tw);
+        here = t < a.T;
+        t = here ? t : a.T - 1;
+    }
     const int stride = (int)ck_stride(a.D), nb = (int)ck_blocks(a.D);
     const auto side = [&](int j) { return j < tasks.nq ? 0 : 1; };
     const auto first = [&](int j, int s) { return (s ? j - tasks.nq : j) * tasks.per + sub; };
@@ -357,7 +369,7 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg) {
 #pragma unroll
         for (int u = 0; u < kQkU; ++u) {
             const int h = h0 + u * step;
-            const bool on = h < a.heads[s];
+            const bool on = here && h < a.heads[s];
             const int64_t row = t * a.heads[s] + h;
             float v[V], o[V], y[V];
             float ss = 0.f;
@@ -402,18 +414,26 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg) {
 // Persistent waves over tokens; both weights' gradients in registers, added
 // over the wave's groups and the workgroup's waves at the end, in a fixed
 // order: dw_part[workgroup][2 D].
-template <typename T, int FMT, int V, bool IL>
-__global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, float* __restrict__ dw_part) {
+template <typename T, int FMT, int V, bool IL, bool MT>
+__global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, float* __restrict__ dw_part) {
     extern __shared__ float red[];  // [8 waves][2][D]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (!MT) tw = 0;
     const QkLane<V, IL> ln(a, lane, lg);
-    const QkTasks tasks(a.heads[0], a.heads[1], lg);
-    const int sub = lane >> lg, step = 64 >> lg;
+    const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
+    const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
     const int stride = (int)ck_stride(a.D), nb = (int)ck_blocks(a.D);
     float dw[2][V];
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[0][e] = dw[1][e] = 0.f;
-    for (int64_t t = (int64_t)blockIdx.x * 8 + wave; t < a.T; t += (int64_t)gridDim.x * 8) {
+    for (int64_t tb = ((int64_t)blockIdx.x * 8 + wave) << tw; tb < a.T; tb += ((int64_t)gridDim.x * 8) << tw) {
+        int64_t t = tb;
+        bool here = true;
+        if (MT) {
+            t += lane >> (6 - tw);
+            here = t < a.T;
+            t = here ? t : a.T - 1;
+        }
         const int64_t pos = qk_position(a, t);
         float c[QkLane<V, IL>::kTab], sn[QkLane<V, IL>::kTab];
         ln.table(a, pos, c, sn);
@@ -450,7 +470,7 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, float* __
 #pragma unroll
             for (int u = 0; u < kQkU; ++u) {
                 const int h = h0 + u * step;
-                const bool on = h < a.heads[s] && ln.in;
+                const bool on = here && h < a.heads[s] && ln.in;
                 float v[V], z[V], o[V], d[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
@@ -499,7 +519,7 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, float* __
         for (int s = 0; s < 2; ++s) {
             float v = dw[s][e];
             for (int k = 1 << lg; k < 64; k <<= 1) v += __shfl_xor(v, k);
-            if (sub == 0 && ln.in) red[(wave * 2 + s) * a.D + ln.c0 + e] = v;
+            if ((lane >> lg) == 0 && ln.in) red[(wave * 2 + s) * a.D + ln.c0 + e] = v;
         }
     }
     __syncthreads();
@@ -540,20 +560,33 @@ static QkTiling qk_tiling(int D, int R, bool interleaved) {
     return QkTiling{0, 0};
 }
 
-// Workgroups that share a token's tasks: enough waves for the device.
-static int qk_splits(int64_t T, const QkTasks& tasks) {
+// log2 of the tokens a wave takes at once: the fewest rounds a token (its tasks,
+// and half a task for its table row) that leave eight waves a CU; one token
+// where that saves less than a quarter.
+static int qk_tokens(const QkArgs& a, const QkTiling& t) {
+    if (t.v == 0) return 0;
+    const auto cost = [&](int tw) { return 2 * QkTasks(a.heads[0], a.heads[1], t.lg + tw).n + 1; };
+    int best = 0;
+    for (int tw = 1; t.lg + tw <= 6 && (a.T >> tw) >= 8 * (int64_t)device_cu_count(); ++tw)
+        if (cost(tw) << best < cost(best) << tw) best = tw;
+    return cost(best) * 4 <= (cost(0) << best) * 3 ? best : 0;
+}
+
+// Workgroups that share a wave's tasks: enough waves for the device.
+static int qk_splits(int64_t waves, const QkTasks& tasks) {
     const int64_t want = 16 * (int64_t)device_cu_count();
-    int64_t y = (want + T - 1) / T;
+    int64_t y = (want + waves - 1) / waves;
     if (y > tasks.n) y = tasks.n;
     return (int)(y < 1 ? 1 : y);
 }
 
-#define MHC_QK_TILED(dt, fmt, t, il, ...)                                            \
+#define MHC_QK_TILED(dt, fmt, t, il, tw, ...)                                        \
     MHC_QK_TYPED(dt, fmt, {                                                          \
         auto tiled = [&](auto v_, auto il_) {                                        \
             constexpr int V_ = decltype(v_)::value;                                  \
             constexpr bool I_ = decltype(il_)::value;                                \
-            __VA_ARGS__;                                                             \
+            if ((tw) > 0) { constexpr bool M_ = true; __VA_ARGS__; }                 \
+            else { constexpr bool M_ = false; __VA_ARGS__; }                         \
         };                                                                           \
         using V8 = std::integral_constant<int, 8>;                                   \
         using V4 = std::integral_constant<int, 4>;                                   \
@@ -565,8 +598,9 @@ hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t
     const int H = a.heads[0] + a.heads[1];
     if (a.T == 0 || H == 0) return hipSuccess;
     const QkTiling t = qk_tiling(a.D, a.R, a.interleaved);
-    const int y = t.v == 0 ? (H + 3) / 4 : qk_splits(a.T, QkTasks(a.heads[0], a.heads[1], t.lg));
-    const int each = t.v == 0 ? 1 : 4;  // tokens a workgroup
+    const int tw = qk_tokens(a, t);
+    const int y = t.v == 0 ? (H + 3) / 4 : qk_splits(a.T >> tw, QkTasks(a.heads[0], a.heads[1], t.lg + tw));
+    const int each = t.v == 0 ? 1 : 4 << tw;  // tokens a workgroup
     const int64_t most = (int64_t)1 << 23;  // workgroups along tokens a launch: 2^31 lanes
     const int tok = timing_begin("qk_norm_rope_fwd", s);
     hipError_t e = hipSuccess;
@@ -577,8 +611,8 @@ hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t
         if (t.v == 0) {
             MHC_QK_TYPED(dt, fmt, MHC_LAUNCH_GGL((qk_fwd_any_kernel<T_, F_>), grid, dim3(256), 0, s, b));
         } else {
-            MHC_QK_TILED(dt, fmt, t, a.interleaved,
-                         MHC_LAUNCH_GGL((qk_fwd_kernel<T_, F_, V_, I_>), grid, dim3(256), 0, s, b, t.lg));
+            MHC_QK_TILED(dt, fmt, t, a.interleaved, tw,
+                         MHC_LAUNCH_GGL((qk_fwd_kernel<T_, F_, V_, I_, M_>), grid, dim3(256), 0, s, b, t.lg, tw));
         }
         e = hipGetLastError();
     }
@@ -593,8 +627,9 @@ static dim3 qk_bwd_dims(const QkArgs& a) {
     if (t.v == 0) return dim3((unsigned)(a.T < two ? a.T : two), 1);
     // the split with the fewest rounds: sweeps over the tokens times a wave's
     // tasks a token and half a task for its table row
-    const int n = QkTasks(a.heads[0], a.heads[1], t.lg).n;
-    const int64_t x = (a.T + 7) / 8;
+    const int tw = qk_tokens(a, t);
+    const int n = QkTasks(a.heads[0], a.heads[1], t.lg + tw).n;
+    const int64_t x = (a.T + (8 << tw) - 1) / (8 << tw);
     int64_t best = INT64_MAX, bx = 1;
     int by = 1;
     for (int y = 1; y <= n && y <= two; ++y) {
@@ -623,9 +658,10 @@ hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_p
                      MHC_LAUNCH_GGL((qk_bwd_any_kernel<T_, F_>), grid, dim3(256), (size_t)a.D * 8 * sizeof(float), s,
                                     a, dw_part));
     } else {
-        MHC_QK_TILED(dt, fmt, t, a.interleaved,
-                     MHC_LAUNCH_GGL((qk_bwd_kernel<T_, F_, V_, I_>), grid, dim3(512),
-                                    (size_t)a.D * 16 * sizeof(float), s, a, t.lg, dw_part));
+        const int tw = qk_tokens(a, t);
+        MHC_QK_TILED(dt, fmt, t, a.interleaved, tw,
+                     MHC_LAUNCH_GGL((qk_bwd_kernel<T_, F_, V_, I_, M_>), grid, dim3(512),
+                                    (size_t)a.D * 16 * sizeof(float), s, a, t.lg, tw, dw_part));
     }
     timing_end(tok, s);
     return hipGetLastError();

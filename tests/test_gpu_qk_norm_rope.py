@@ -102,6 +102,17 @@ def test_matches_oracle(device, T, H, K, D, Rd, interleaved, dtype, fmt):
     _check([g.cpu() for g in got], inputs, cos[pos], sin[pos], interleaved, fmt)
 
 
+# Few heads and many tokens: several tokens a wave, the last wave's not all there.
+@pytest.mark.parametrize("T,H,K,D,Rd", [(4099, 1, 1, 64, 64), (9001, 4, 1, 72, 36), (9003, 2, 2, 80, 80),
+                                        (16391, 2, 1, 128, 128), (5003, 5, 0, 64, 32), (4501, 0, 1, 256, 256),
+                                        (33001, 1, 1, 32, 32), (20001, 3, 3, 64, 64)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", [None, "int8", "e4m3"])
+def test_several_tokens_a_wave(device, T, H, K, D, Rd, interleaved, dtype, fmt):
+    test_matches_oracle(device, T, H, K, D, Rd, interleaved, dtype, fmt)
+
+
 @pytest.mark.parametrize("w_dtype", DTYPES)
 def test_weights_of_another_dtype(device, w_dtype):
     dtype = torch.bfloat16 if w_dtype == torch.float32 else torch.float32
