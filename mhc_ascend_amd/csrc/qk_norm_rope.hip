@@ -561,13 +561,14 @@ static QkTiling qk_tiling(int D, int R, bool interleaved) {
 }
 
 // log2 of the tokens a wave takes at once: the fewest rounds a token (its tasks,
-// and half a task for its table row) that leave eight waves a CU; one token
-// where that saves less than a quarter.
+// and half a task for its table row) that leave two waves a CU (eight: 4188 x 1 +
+// 1 heads of 64 fp32 int8, forward and backward 36 us, two 23); one token where
+// that saves less than a quarter.
 static int qk_tokens(const QkArgs& a, const QkTiling& t) {
     if (t.v == 0) return 0;
     const auto cost = [&](int tw) { return 2 * QkTasks(a.heads[0], a.heads[1], t.lg + tw).n + 1; };
     int best = 0;
-    for (int tw = 1; t.lg + tw <= 6 && (a.T >> tw) >= 8 * (int64_t)device_cu_count(); ++tw)
+    for (int tw = 1; t.lg + tw <= 6 && (a.T >> tw) >= 2 * (int64_t)device_cu_count(); ++tw)
         if (cost(tw) << best < cost(best) << tw) best = tw;
     return cost(best) * 4 <= (cost(0) << best) * 3 ? best : 0;
 }
