@@ -2243,6 +2243,13 @@ int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* 
             MHC_REQUIRE(valid_dtype(weight_dtype), "layer_static_checkpoint_fwd: weight_dtype must be F32 or BF16");
             MHC_REQUIRE(weight && h_pre && h_post && h_res && saved && out,
                         "layer_static_checkpoint_fwd: null parameter pointer");
+            // few tokens: one launch, the coefficients formed by every workgroup
+            // (2000 x 3 x 1024 fp32, forward and backward: 36 us for 42; 4096 x 8 x
+            // 1280: 188 for 172)
+            if (batch <= 8 * (int64_t)device_cu_count())
+                return hip_status(launch_layer_ckpt_static_fwd(x_dtype, format, n, x, weight, weight_dtype, h_pre,
+                                                               h_post, h_res, saved, num_iters, sinkhorn_eps, out,
+                                                               values, scales, batch, hidden, rmsnorm_eps, s));
             hipError_t e = launch_static_coef(n, h_pre, h_post, h_res, weight, weight_dtype, hidden, saved, num_iters,
                                               sinkhorn_eps, s);
             if (e == hipSuccess)

@@ -123,6 +123,41 @@ __global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(int fmt, const TX* _
     fwd_token<TX, float, N, VPT>(b, coef, coef_stride, wv, xv, out, nullptr, C, eps, red);
 }
 
+// Static H in one launch, as layer_static_fwd_kernel: every workgroup forms the
+// shared coefficients while its row loads are in flight, workgroup 0 writes the
+// saved state.  For few tokens.
+template <typename TX, int N, int VPT>
+__global__ MHC_ROW_BOUNDS(false) void layer_ckpt_static_fwd_kernel(
+    int fmt, const TX* __restrict__ x, const void* __restrict__ weight, int w_bf16, const float* __restrict__ h_pre,
+    const float* __restrict__ h_post, const float* __restrict__ h_res, float* __restrict__ saved, int w_off, int iters,
+    float sk_eps, float* __restrict__ out, uint8_t* __restrict__ q, uint8_t* __restrict__ sc, int C, float eps) {
+    constexpr int WC = kLayerWC;
+    __shared__ float red[8];
+    __shared__ float cf[coef_size<N>()];
+    const int64_t b = blockIdx.x;
+    RawRows<TX, N, VPT, WC> xr;
+    load_rows_raw<TX, N, VPT, WC, true>(x + b * (int64_t)N * C, C, xr);
+    if (threadIdx.x < kWave) static_coefs_wave<N>(h_pre, h_post, h_res, iters, sk_eps, cf, b == 0 ? saved : nullptr);
+    float wv[VPT][WC];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * WC;
+#pragma unroll
+        for (int e = 0; e < WC; ++e) {
+            wv[k][e] = 0.f;
+            if (c0 < C)
+                wv[k][e] = w_bf16 ? VecIO<bf16_t>::scalar(static_cast<const bf16_t*>(weight) + c0 + e)
+                                  : static_cast<const float*>(weight)[c0 + e];
+        }
+        if (b == 0 && c0 < C) store_run<float, WC>(saved + w_off + c0, wv[k]);
+    }
+    __syncthreads();
+    float xv[N][VPT][WC];
+    unpack_rows<TX, N, VPT, WC>(xr, C, xv);
+    held_put<N, VPT>(fmt, xv, q, sc, b, C);
+    fwd_token<TX, float, N, VPT>(b, cf, 0, wv, xv, out, nullptr, C, eps, red);
+}
+
 // As layer_bwd_kernel: persistent workgroups over tokens, with PF the next
 // token's rows in flight.  TX is dx's storage type.
 template <typename TX, int N, int VPT, int MODE, bool PF>
@@ -217,6 +252,12 @@ static const void* ck_fwd_fn() {
     return nullptr;
 }
 
+template <typename TX, int N, int V>
+static const void* ck_static_fwd_fn() {
+    if constexpr (layer_row_fits(N, V)) return reinterpret_cast<const void*>(&layer_ckpt_static_fwd_kernel<TX, N, V>);
+    return nullptr;
+}
+
 template <typename TX, int N, int V, int MODE>
 static const void* ck_bwd_fn(bool pf) {
     if constexpr (layer_row_fits(2 * N, V))
@@ -271,6 +312,26 @@ hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, con
     int Ci = (int)C;
     void* args[] = {(void*)&fmt, (void*)&x,   (void*)&w,      (void*)&coef,   (void*)&coef_stride, (void*)&out,
                     (void*)&values, (void*)&scales, (void*)&Ci, (void*)&eps};
+    const int tok = timing_begin("layer_ckpt_fwd", s);
+    hipError_t e = mhc_launch_kernel(fn, dim3((unsigned)B), dim3(t.threads), args, 0, s);
+    timing_end(tok, s);
+    return e != hipSuccess ? e : hipGetLastError();
+}
+
+hipError_t launch_layer_ckpt_static_fwd(int x_dtype, int fmt, int n, const void* x, const void* weight, int w_dtype,
+                                        const float* h_pre, const float* h_post, const float* h_res, float* saved,
+                                        int iters, float sk_eps, float* out, void* values, void* scales, int64_t B,
+                                        int64_t C, float eps, hipStream_t s) {
+    const RowTiling t = layer_fwd_tiling(C, n);
+    const void* fn = nullptr;
+    MHC_CL_N(n, MHC_CL_VPT(t.vpt, fn = x_dtype == kBF16 ? ck_static_fwd_fn<bf16_t, N_, V_>()
+                                                        : ck_static_fwd_fn<float, N_, V_>()));
+    if (!fn) return hipErrorInvalidValue;
+    int Ci = (int)C, w_bf16 = w_dtype == kBF16, w_off = saved_w_offset(n);
+    void* args[] = {(void*)&fmt,   (void*)&x,     (void*)&weight, (void*)&w_bf16, (void*)&h_pre,
+                    (void*)&h_post, (void*)&h_res, (void*)&saved,  (void*)&w_off,  (void*)&iters,
+                    (void*)&sk_eps, (void*)&out,   (void*)&values, (void*)&scales, (void*)&Ci,
+                    (void*)&eps};
     const int tok = timing_begin("layer_ckpt_fwd", s);
     hipError_t e = mhc_launch_kernel(fn, dim3((unsigned)B), dim3(t.threads), args, 0, s);
     timing_end(tok, s);

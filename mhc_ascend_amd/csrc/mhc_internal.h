@@ -306,6 +306,11 @@ bool layer_ckpt_bwd_rows(int n, int64_t B, int64_t C, std::initializer_list<cons
 hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, const float* w, const float* coef,
                                  int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
                                  float eps, hipStream_t s);
+// with the coefficients and the saved state of static H in the same launch
+hipError_t launch_layer_ckpt_static_fwd(int x_dtype, int fmt, int n, const void* x, const void* weight, int w_dtype,
+                                        const float* h_pre, const float* h_post, const float* h_res, float* saved,
+                                        int iters, float sk_eps, float* out, void* values, void* scales, int64_t B,
+                                        int64_t C, float eps, hipStream_t s);
 // scale groups of mode 1's fp16 stream part (layer_bwd_part_groups)
 int layer_ckpt_bwd_part_groups(int n, int64_t B, int64_t C);
 int layer_ckpt_bwd_grid(int x_dtype, int n, int mode, int64_t B, int64_t C);

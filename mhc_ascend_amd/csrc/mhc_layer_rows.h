@@ -13,6 +13,60 @@ namespace mhc {
 
 template <int N> constexpr int coef_size() { return 2 * N + N * N; }
 
+// The shared N x N matrix (N = 3..8) on lanes 0 .. S^2 - 1 of one wave, one
+// element per lane: `at` = the lane's element r N + c when `on`.  The wave's
+// other lanes compute on zeros.
+template <int N>
+struct SkShared {
+    static constexpr int S = sk_el_size(N);
+    int at;
+    bool on;
+    float er, ec;
+    __device__ __forceinline__ SkShared(int lane, float eps) {
+        const int r = (lane / S) % S, c = lane % S;
+        at = r * N + c;
+        on = lane < S * S && r < N && c < N;
+        er = SkEl<S>::pad_eps(r, N, eps);
+        ec = SkEl<S>::pad_eps(c, N, eps);
+    }
+    __device__ __forceinline__ void forward(float& a, int iters) const { SkEl<S>::forward(a, iters, er, ec); }
+    __device__ __forceinline__ void backward(float& g, float x0, int iters) const {
+        SkEl<S>::backward(g, x0, iters, er, ec, on);
+    }
+};
+
+// The shared coefficients of static H, by the first wave; each value goes to cf (LDS) and, when `save` is
+// not null, to the saved state.
+template <int N>
+__device__ __forceinline__ void static_coefs_wave(const float* __restrict__ h_pre, const float* __restrict__ h_post,
+                                                  const float* __restrict__ h_res, int iters, float eps,
+                                                  float* __restrict__ cf, float* __restrict__ save) {
+    const int r = threadIdx.x;
+    auto put = [&](int i, float v) {
+        cf[i] = v;
+        if (save) save[i] = v;
+    };
+    if (r < N) {
+        put(r, sigmoidf(h_pre[r]));
+        put(N + r, 2.f * sigmoidf(h_post[r]));
+    }
+    if constexpr (N >= 3) {
+        const SkShared<N> k(r, eps);
+        float a = k.on ? expf(h_res[k.at]) : 0.f;
+        k.forward(a, iters);
+        if (k.on) put(2 * N + k.at, a);
+    } else {
+        float a[N];
+#pragma unroll
+        for (int c = 0; c < N; ++c) a[c] = (r < N) ? expf(h_res[r * N + c]) : 0.f;
+        sk_forward<N>(a, iters, eps, r < N);
+        if (r < N) {
+#pragma unroll
+            for (int c = 0; c < N; ++c) put(2 * N + r * N + c, a[c]);
+        }
+    }
+}
+
 template <typename TX, typename TO, int N, int VPT>
 __device__ __forceinline__ void fwd_token(int64_t b, const float* __restrict__ coef, int64_t coef_stride,
                                           const float (&wv)[VPT][kLayerWC],
