@@ -2250,8 +2250,8 @@ int mhc_layer_static_checkpoint_fwd(const void* x, int32_t x_dtype, const void* 
                 return hip_status(launch_layer_ckpt_static_fwd(x_dtype, format, n, x, weight, weight_dtype, h_pre,
                                                                h_post, h_res, saved, num_iters, sinkhorn_eps, out,
                                                                values, scales, batch, hidden, rmsnorm_eps, s));
-            hipError_t e = launch_static_coef(n, h_pre, h_post, h_res, weight, weight_dtype, hidden, saved, num_iters,
-                                              sinkhorn_eps, s);
+            hipError_t e = launch_layer_ckpt_coef(n, h_pre, h_post, h_res, weight, weight_dtype, hidden, saved,
+                                                  num_iters, sinkhorn_eps, s);
             if (e == hipSuccess)
                 e = launch_layer_ckpt_fwd(x_dtype, format, n, x, saved + saved_w_offset(n), saved, 0, out, values,
                                           scales, batch, hidden, rmsnorm_eps, s);

@@ -123,6 +123,29 @@ __global__ MHC_ROW_BOUNDS(false) void layer_ckpt_fwd_kernel(int fmt, const TX* _
     fwd_token<TX, float, N, VPT>(b, coef, coef_stride, wv, xv, out, nullptr, C, eps, red);
 }
 
+// Static H's saved state in a launch of its own: workgroup 0 the coefficients,
+// by the code of the kernel below (so the same bits at any number of tokens),
+// the others the weight in fp32, 4 a lane.
+template <int N>
+__global__ __launch_bounds__(256) void layer_ckpt_coef_kernel(const void* __restrict__ weight, int w_bf16,
+                                                              const float* __restrict__ h_pre,
+                                                              const float* __restrict__ h_post,
+                                                              const float* __restrict__ h_res,
+                                                              float* __restrict__ saved, int w_off, int iters,
+                                                              float sk_eps, int C) {
+    __shared__ float cf[coef_size<N>()];
+    if (blockIdx.x == 0) {
+        if (threadIdx.x < kWave) static_coefs_wave<N>(h_pre, h_post, h_res, iters, sk_eps, cf, saved);
+        return;
+    }
+    const int c0 = ((blockIdx.x - 1) * 256 + threadIdx.x) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (c0 + e < C)
+            saved[w_off + c0 + e] = w_bf16 ? VecIO<bf16_t>::scalar(static_cast<const bf16_t*>(weight) + c0 + e)
+                                           : static_cast<const float*>(weight)[c0 + e];
+}
+
 // Static H in one launch, as layer_static_fwd_kernel: every workgroup forms the
 // shared coefficients while its row loads are in flight, workgroup 0 writes the
 // saved state.  For few tokens.
@@ -316,6 +339,15 @@ hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, con
     hipError_t e = mhc_launch_kernel(fn, dim3((unsigned)B), dim3(t.threads), args, 0, s);
     timing_end(tok, s);
     return e != hipSuccess ? e : hipGetLastError();
+}
+
+hipError_t launch_layer_ckpt_coef(int n, const float* h_pre, const float* h_post, const float* h_res,
+                                  const void* weight, int w_dtype, int64_t C, float* saved, int iters, float sk_eps,
+                                  hipStream_t s) {
+    const dim3 grid((unsigned)(1 + (C + 1023) / 1024));
+    MHC_CL_N(n, MHC_LAUNCH_GGL((layer_ckpt_coef_kernel<N_>), grid, dim3(256), 0, s, weight, w_dtype == kBF16, h_pre,
+                               h_post, h_res, saved, saved_w_offset(n), iters, sk_eps, (int)C));
+    return hipGetLastError();
 }
 
 hipError_t launch_layer_ckpt_static_fwd(int x_dtype, int fmt, int n, const void* x, const void* weight, int w_dtype,

@@ -306,6 +306,10 @@ bool layer_ckpt_bwd_rows(int n, int64_t B, int64_t C, std::initializer_list<cons
 hipError_t launch_layer_ckpt_fwd(int x_dtype, int fmt, int n, const void* x, const float* w, const float* coef,
                                  int64_t coef_stride, float* out, void* values, void* scales, int64_t B, int64_t C,
                                  float eps, hipStream_t s);
+// the saved state of static H (launch_static_coef, n = 2..8)
+hipError_t launch_layer_ckpt_coef(int n, const float* h_pre, const float* h_post, const float* h_res,
+                                  const void* weight, int w_dtype, int64_t C, float* saved, int iters, float sk_eps,
+                                  hipStream_t s);
 // with the coefficients and the saved state of static H in the same launch
 hipError_t launch_layer_ckpt_static_fwd(int x_dtype, int fmt, int n, const void* x, const void* weight, int w_dtype,
                                         const float* h_pre, const float* h_post, const float* h_res, float* saved,

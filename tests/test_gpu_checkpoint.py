@@ -511,6 +511,29 @@ def test_offsets_past_32_bits(device):
     assert all(torch.equal(a, b) for a, b in zip(*outs))
 
 
+@pytest.mark.parametrize("n,C,w_dtype", [(2, 64, torch.float32), (4, 128, torch.bfloat16), (7, 96, torch.float32),
+                                         (8, 1280, torch.bfloat16)])
+def test_static_layer_in_one_launch_or_two(device, n, C, w_dtype):
+    """Few tokens take the coefficients and the rows in one forward launch, many
+    in two: the same bits for the same tokens."""
+    few, many = 33, 9 * torch.cuda.get_device_properties(device).multi_processor_count
+    g = _gen(n)
+    x = torch.randn(many, n, C, generator=g).to(device)
+    cot = torch.randn(many, n, C, generator=g).to(device)
+    params = [torch.randn(C, generator=g).to(device, w_dtype), torch.randn(n, generator=g).to(device),
+              torch.randn(n, generator=g).to(device), torch.randn(n, n, generator=g).to(device)]
+    outs = []
+    for t in (few, many):
+        r = x[:t].clone().requires_grad_(True)
+        out = mhc.mhc_layer_static(r, *params, checkpoint="int8")
+        outs.append((out.detach()[:few], torch.autograd.grad(out, r, cot[:t])[0][:few]))
+    # dx sums a row over other lanes where the two batches tile it differently: a
+    # value has n products and a term of two row sums, 64 of 2^-24 on each
+    assert torch.equal(outs[0][0], outs[1][0])
+    scale = float(outs[0][1].abs().max())
+    assert float((outs[0][1] - outs[1][1]).abs().max()) <= 64 * 2.0 ** -24 * n * scale
+
+
 def test_one_row_of_nearly_two_to_the_31(device):
     """The padded row is 2^31 bytes: its last blocks against a short row's."""
     C, tail = (1 << 31) - 1, 32 * 64 - 1
