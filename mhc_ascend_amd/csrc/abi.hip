@@ -2448,7 +2448,7 @@ static hipError_t dyn_ckpt_bwd(const float* grad_out, const void* values, const 
     for (int o0 = 0; o0 < np && e == hipSuccess; o0 += kProjCkptRows) {
         const int cnt = np - o0 < kProjCkptRows ? np - o0 : kProjCkptRows;
         const bool last = o0 + cnt == np;
-        e = launch_proj_ckpt_bwd(last ? x_dtype : kF32, w.qin, format, values, scales, dp, dp_stride(np),
+        e = launch_proj_ckpt_bwd(last ? x_dtype : kF32, x_dtype, w.qin, format, values, scales, dp, dp_stride(np),
                                  o0 == 0 ? stok : nullptr, phi_pre, phi_post, phi_res, n, o0, cnt, part,
                                  last ? grad_x : part, pscale, w.groups, phip + (size_t)w.tiles * o0 * K, w.tiles,
                                  batch, K, s);

@@ -326,14 +326,15 @@ hipError_t launch_layer_ckpt_bwd(int x_dtype, int fmt, int n, int mode, const fl
 // ---- proj_ckpt.hip ---------------------------------------------------------
 // The projection backward on rows in a checkpoint, output rows o0 .. o0 + np - 1,
 // np <= kProjCkptRows at once (dP and dp_stride of all of them; s_tok may be
-// null); C a multiple of 8, at most kProjCkptMaxRows rows in all (n = 16).  dx_in: fp32 [B, K] (dx itself for fp32 dx), or,
+// null); C a multiple of 8, at most kProjCkptMaxRows rows in all (n = 16).  dx_dtype: what this launch leaves in dx,
+// x_dtype: the rows'.  dx_in: fp32 [B, K] (dx itself for fp32 dx), or,
 // with qin (bf16 dx, n = 2 or 4, C a multiple of 128), the fp16 stream part
 // of launch_layer_ckpt_bwd's mode 1 in dx.  dphi_part[tiles][np][K].
 constexpr int kProjCkptRows = 96;
 constexpr int kProjCkptMaxRows = 288;
 bool proj_ckpt_supported(int np, int64_t K, int64_t C);
-int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K);
-hipError_t launch_proj_ckpt_bwd(int dx_dtype, bool qin, int fmt, const void* values, const void* scales,
+int proj_ckpt_bwd_tiles(int x_dtype, bool qin, int np, int64_t B, int64_t K);
+hipError_t launch_proj_ckpt_bwd(int dx_dtype, int x_dtype, bool qin, int fmt, const void* values, const void* scales,
                                 const float* dP, int dp_stride, const float* s_tok, const float* phi_pre,
                                 const float* phi_post, const float* phi_res, int n, int o0, int np,
                                 const void* dx_in, void* dx, const int32_t* dx_scale, int groups, float* dphi_part, int tiles, int64_t B,

@@ -8,8 +8,11 @@
 // first.
 //
 // x^ is exact in bf16, so dP alone is split: three bf16 planes for dPhi (to
-// 2^-24 of a term; the kernels that read x use two, 2^-16), two planes of dP
-// and Phi for dx.  Bound by its bytes: 33/32 of a byte of x^, dx_in and dx a
+// 2^-24 of a term; the kernels that read x use two, 2^-16).  For dx both dP and
+// Phi are: three planes and the six products of 2^-16 and more for fp32 rows
+// (2-4e-7 of dx in the 2-norm where all of it is dP Phi; two planes, 4.3e-6, and
+// 4096 x 8 x 1280 in 104 us for 114, up to n = 6 1 us less), two planes and three
+// products for bf16 rows, whose dx is rounded to 2^-9.  Bound by its bytes: 33/32 of a byte of x^, dx_in and dx a
 // value (8192 x 4 x 4096 bf16: 674 MB in 131-148 us, 4.6-5.1 TB/s; the one that
 // reads x, 806 MB, 143).
 #include "mhc_ckpt.h"
@@ -19,10 +22,31 @@
 
 namespace mhc {
 
-// TD: dx's type.  QIN: dx_in is the row pass's fp16 stream part against
+// v as the sum of PL bf16 planes, each the rest of the ones before it.
+template <int PL>
+__device__ __forceinline__ void split_planes8(const float (&v)[8], u32x4_t (&p)[PL]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float a = v[2 * e], b = v[2 * e + 1];
+#pragma unroll
+        for (int k = 0; k < PL; ++k) {
+            const uint32_t h = pack_bf16(a, b);
+            p[k][e] = h;
+            a -= __uint_as_float(h << 16);
+            b -= __uint_as_float(h & 0xffff0000u);
+        }
+    }
+}
+
+// Element (row, c) of a plane of dP in LDS: rows of 32 bf16 without padding (two
+// workgroups of three tiles fit a CU), their 16-byte pieces turned by the row's
+// bits 2 and 3, so that 16 rows' reads of one piece meet 64 banks.
+__device__ __forceinline__ int dps_at(int row, int c) { return row * 32 + ((((c >> 3) ^ (row >> 2)) & 3) << 3) + (c & 7); }
+
+// TD: dx's type.  PL: planes of dP and Phi for dx.  QIN: dx_in is the row pass's fp16 stream part against
 // power-of-two scales (part_pack4) in dx itself; otherwise fp32 (dx itself for
 // TD = float).  OT: tiles of 32 output rows.  NW waves of 32 columns each.
-template <typename TD, bool QIN, int OT, int NW>
+template <typename TD, int PL, bool QIN, int OT, int NW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4 : 2))) void proj_ckpt_bwd_kernel(
     int fmt, const uint8_t* __restrict__ q, const uint8_t* __restrict__ sc, const float* __restrict__ dP,
     int dp_stride, const float* __restrict__ s_tok, const float* __restrict__ phi_pre,
@@ -45,8 +69,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
     static_assert(PASSES * RPP == TB && DPASSES * DRPP == TB && NG * TB <= NT && NT >= 256, "stage shape");
     __shared__ __align__(16) char x_lds[TB * XPITCH];
     __shared__ __align__(16) char dx_lds[2][TB * DPITCH];
-    // hi_row, lo_row, then by columns hi, mid, lo
-    __shared__ __align__(16) bf16_t dps_lds[OT][5][32 * kDpPitch];
+    // dP's planes by rows (tokens), PL of them, then by columns, three
+    __shared__ __align__(16) bf16_t dps_lds[OT][PL + 3][32 * 32];
     __shared__ float s_lds[TB];
     __shared__ int q_lds[NG][TB];
 
@@ -67,7 +91,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
     const int dpo = (tid & 7) * 4;     // outputs 32 ot + 4 (tid % 8) .. + 3
 
     // Phi^T: Phi[32 ot + 8 lg + e][column 16 ct + lr]
-    u32x4_t phh[OT][2], phl[OT][2];
+    u32x4_t ph[OT][2][PL];
 #pragma unroll
     for (int ot = 0; ot < OT; ++ot) {
 #pragma unroll
@@ -79,7 +103,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
                 const int o = 32 * ot + 8 * lg + e;
                 v[e] = (wave_on && o < np) ? phi_row(phi_pre, phi_post, phi_res, n, o0 + o, K)[k] : 0.f;
             }
-            split_pack8(v, phh[ot][ct], phl[ot][ct]);
+            split_planes8<PL>(v, ph[ot][ct]);
         }
     }
     f32x4_t accP[2 * OT][2];
@@ -174,13 +198,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
 #pragma unroll
                 for (int k = 0; k < 3; ++k) {
                     const uint32_t p0 = pack_bf16(v[0], v[1]), p1 = pack_bf16(v[2], v[3]);
-                    if (k < 2)
-                        *reinterpret_cast<uint2*>(&dps_lds[ot][k][dtk * kDpPitch + dpo]) = make_uint2(p0, p1);
-                    bf16_t* col = dps_lds[ot][2 + k];
-                    col[(dpo + 0) * kDpPitch + dtk] = (bf16_t)(p0 & 0xffffu);
-                    col[(dpo + 1) * kDpPitch + dtk] = (bf16_t)(p0 >> 16);
-                    col[(dpo + 2) * kDpPitch + dtk] = (bf16_t)(p1 & 0xffffu);
-                    col[(dpo + 3) * kDpPitch + dtk] = (bf16_t)(p1 >> 16);
+                    if (k < PL)
+                        *reinterpret_cast<uint2*>(&dps_lds[ot][k][dps_at(dtk, dpo)]) = make_uint2(p0, p1);
+                    bf16_t* col = dps_lds[ot][PL + k];
+                    col[dps_at(dpo + 0, dtk)] = (bf16_t)(p0 & 0xffffu);
+                    col[dps_at(dpo + 1, dtk)] = (bf16_t)(p0 >> 16);
+                    col[dps_at(dpo + 2, dtk)] = (bf16_t)(p1 & 0xffffu);
+                    col[dps_at(dpo + 3, dtk)] = (bf16_t)(p1 >> 16);
                     v[0] -= __uint_as_float(p0 << 16);
                     v[1] -= __uint_as_float(p0 & 0xffff0000u);
                     v[2] -= __uint_as_float(p1 << 16);
@@ -217,7 +241,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
         for (int ot = 0; ot < 2 * OT; ++ot) {
 #pragma unroll
             for (int k = 0; k < 3; ++k) {
-                const u32x4_t a = read16(&dps_lds[ot / 2][2 + k][(16 * (ot & 1) + lr) * kDpPitch + 8 * lg]);
+                const u32x4_t a = read16(&dps_lds[ot / 2][PL + k][dps_at(16 * (ot & 1) + lr, 8 * lg)]);
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) accP[ot][ct] = mfma16x16x32(a, xh[ct], accP[ot][ct]);
             }
@@ -229,13 +253,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
             f32x4_t d[2] = {f32x4_t{0.f, 0.f, 0.f, 0.f}, f32x4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int ot = 0; ot < OT; ++ot) {
-                const u32x4_t bh = read16(&dps_lds[ot][0][t * kDpPitch + 8 * lg]);
-                const u32x4_t bl = read16(&dps_lds[ot][1][t * kDpPitch + 8 * lg]);
+                u32x4_t b[PL];
+#pragma unroll
+                for (int k = 0; k < PL; ++k) b[k] = read16(&dps_lds[ot][k][dps_at(t, 8 * lg)]);
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {
-                    d[ct] = mfma16x16x32(phh[ot][ct], bh, d[ct]);
-                    d[ct] = mfma16x16x32(phl[ot][ct], bh, d[ct]);
-                    d[ct] = mfma16x16x32(phh[ot][ct], bl, d[ct]);
+#pragma unroll
+                    for (int o = 0; o < PL; ++o) {  // products of 2^(-8 o)
+#pragma unroll
+                        for (int i = o; i >= 0; --i) d[ct] = mfma16x16x32(ph[ot][ct][i], b[o - i], d[ct]);
+                    }
                 }
             }
             const float st = s_lds[t];
@@ -327,12 +354,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(QIN ? 4
 // ---------------------------------------------------------------------------
 // Host launchers
 // ---------------------------------------------------------------------------
-static const void* pick_proj_ckpt(int dx_dtype, bool qin, int np) {
-    if (qin) return reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<bf16_t, true, 1, 8>);
+// x_dtype: the rows'.  Of several launches all but the last leave dx in fp32.
+static const void* pick_proj_ckpt(int dx_dtype, int x_dtype, bool qin, int np) {
+    if (qin) return reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<bf16_t, 2, true, 1, 8>);
     const int ot = proj_tiles(np);
-#define MHC_PC(OT_)                                                                                     \
-    (dx_dtype == kBF16 ? reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<bf16_t, false, OT_, 4>)     \
-                       : reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<float, false, OT_, 4>))
+#define MHC_PC(OT_)                                                                                       \
+    (dx_dtype == kBF16  ? reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<bf16_t, 2, false, OT_, 4>)  \
+     : x_dtype == kBF16 ? reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<float, 2, false, OT_, 4>)   \
+                        : reinterpret_cast<const void*>(&proj_ckpt_bwd_kernel<float, 3, false, OT_, 4>))
     return ot == 1 ? MHC_PC(1) : (ot == 2 ? MHC_PC(2) : MHC_PC(3));
 #undef MHC_PC
 }
@@ -350,10 +379,10 @@ bool proj_ckpt_supported(int np, int64_t K, int64_t C) {
 // Column blocks x token tiles fill one round of resident workgroups: the
 // partials of dPhi are half of two rounds' (n = 6, 2047 x 1040 bf16: 34.6 us and
 // 9.5 for their sums, against 40.7 and 12).
-int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K) {
+int proj_ckpt_bwd_tiles(int x_dtype, bool qin, int np, int64_t B, int64_t K) {
     const int nw = proj_ckpt_waves(qin);
     const int64_t gx = (K + 32 * nw - 1) / (32 * nw);
-    const int per_cu = occupancy_per_cu(pick_proj_ckpt(dx_dtype, qin, np), 64 * nw, 0);
+    const int per_cu = occupancy_per_cu(pick_proj_ckpt(x_dtype, x_dtype, qin, np), 64 * nw, 0);
     int64_t tiles = (int64_t)device_cu_count() * per_cu / gx;
     const int64_t blocks = (B + 63) / 64;
     if (tiles > blocks) tiles = blocks;
@@ -363,7 +392,7 @@ int proj_ckpt_bwd_tiles(int dx_dtype, bool qin, int np, int64_t B, int64_t K) {
     return (int)tiles;
 }
 
-hipError_t launch_proj_ckpt_bwd(int dx_dtype, bool qin, int fmt, const void* values, const void* scales,
+hipError_t launch_proj_ckpt_bwd(int dx_dtype, int x_dtype, bool qin, int fmt, const void* values, const void* scales,
                                 const float* dP, int dp_stride, const float* s_tok, const float* phi_pre,
                                 const float* phi_post, const float* phi_res, int n, int o0, int np,
                                 const void* dx_in, void* dx, const int32_t* dx_scale, int groups, float* dphi_part, int tiles, int64_t B,
@@ -384,7 +413,7 @@ hipError_t launch_proj_ckpt_bwd(int dx_dtype, bool qin, int fmt, const void* val
                     (void*)&dx,       (void*)&dx_scale, (void*)&groups, (void*)&C,     (void*)&dphi_part, (void*)&B,
                     (void*)&K,        (void*)&tile};
     const int tok = timing_begin("proj_ckpt_bwd", s);
-    hipError_t e = mhc_launch_kernel(pick_proj_ckpt(dx_dtype, qin, np), grid, dim3(64 * nw), args, 0, s);
+    hipError_t e = mhc_launch_kernel(pick_proj_ckpt(dx_dtype, x_dtype, qin, np), grid, dim3(64 * nw), args, 0, s);
     timing_end(tok, s);
     return e != hipSuccess ? e : hipGetLastError();
 }

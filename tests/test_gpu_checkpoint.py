@@ -620,3 +620,23 @@ def test_step_replays_in_a_graph(device, dynamic):
     feeds = [lambda: x.copy_(torch.randn(x.shape, generator=g)), lambda: cot.copy_(torch.randn(x.shape, generator=g)),
              lambda: rows.copy_(torch.randn(rows.shape, generator=g))]
     _replays(graph, outs, step, feeds)
+
+
+# x^ is exact in bf16 and dP and Phi are not: with 16 bits of each left in their
+# products, the part of dx that comes through the projections is 4.3e-6 off in
+# the 2-norm.  Roundings of fp32 that are independent add in the 2-norm: 16 *
+# 2^-24 allows a chain of 256 of them (fp32 autograd of these inputs, 2-4e-7).
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n,B,C", [(4, 40, 1024), (4, 300, 96), (2, 64, 2048), (3, 50, 160), (6, 30, 1040), (8, 24, 512),
+                                   (12, 20, 256), (16, 40, 64)])
+def test_dx_of_fp32_rows_is_in_fp32(device, fmt, n, B, C):
+    """Nearly all of dx is sum_o dP_o Phi_o here: the cotangent is x itself."""
+    d = R.dynamic_layer_inputs(B, n, C, seed=n + B, x_dtype=torch.float32, alpha=1.0, phi_std=(n * C) ** -0.5,
+                               b_std=0.5)
+    d["grad"] = d["x"].clone()
+    x = d["x"].to(device).requires_grad_(True)
+    ps = [d[k].to(device).requires_grad_(True) for k in PARAMS]
+    out = mhc.mhc_layer_fused_dynamic_training(x, *ps, checkpoint=fmt)
+    gx, = torch.autograd.grad(out, [x], d["grad"].to(device))
+    want = _oracle_dyn_held(d, fmt)[1]
+    assert float((gx.cpu().double() - want).norm() / want.norm()) <= 16 * 2.0 ** -24
