@@ -1108,7 +1108,14 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, 
     TORCH_CHECK(wq.numel() == D && wk.numel() == D && wq.dim() == 1 && wk.dim() == 1, fn,
                 ": the weights must be [head_dim]");
     TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), fn, ": cos and sin must be [positions, rotary_dim / 2]");
-    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad(), fn, ": cos and sin get no gradient");
+    // forward mode runs without grad mode too, and a tangent of a C++ node's input is an error
+    const auto dual = [](std::initializer_list<const Tensor*> ts) {
+        for (const Tensor* t : ts)
+            if (t->_fw_grad(0).defined()) return true;
+        return false;
+    };
+    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad() && !dual({&cos, &sin}), fn,
+                ": cos and sin get no gradient");
     TORCH_CHECK(q_in.size(-2) <= INT32_MAX && k_in.size(-2) <= INT32_MAX && D <= INT32_MAX && 2 * cos.size(1) <= D, fn,
                 ": rotary_dim must be at most head_dim, and the sizes 32-bit");
     int64_t period = lead.back();
@@ -1121,12 +1128,13 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, 
     }
     const Tensor q = dims == 4 ? q_in.flatten(0, 1) : q_in, k = dims == 4 ? k_in.flatten(0, 1) : k_in;
     const int64_t fmt = format_for(checkpoint, {&q, &k, &wq, &wk});
-    const bool backward = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() ||
-                                                         wq.requires_grad() || wk.requires_grad());
+    const bool node = dual({&q, &k, &wq, &wk}) ||
+                      (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wq.requires_grad() ||
+                                                      wk.requires_grad()));
     period = std::max<int64_t>(period, 1);
     const tensor_list out =
-        backward ? QkNormRope::apply(q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt)
-                 : QkNormRope::forward(nullptr, q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt);
+        node ? QkNormRope::apply(q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt)
+             : QkNormRope::forward(nullptr, q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt);
     if (dims == 3) return {out[0], out[1]};
     return {out[0].unflatten(0, lead), out[1].unflatten(0, lead)};
 }

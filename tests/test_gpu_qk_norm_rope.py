@@ -436,3 +436,20 @@ def test_more_tokens_than_a_launch_takes(device, T, D):
             want = mhc.qk_norm_rope(q[at:at + 1], k[at:at + 1], w, w, cos, sin)[0]
             assert torch.equal(out[at:at + 1], want)
         assert torch.equal(out[:-1], out[:1].expand_as(out[:-1]))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_an_error(device, grad):
+    """A tangent on any input is refused, with and without grad mode: a result
+    that came back without one would be taken for a constant."""
+    q, k, ws, _ = _inputs(5, 2, 1, 64, torch.float32, 3)
+    cos, sin = mhc.rope_table(5, 64)
+    args = [t.to(device) for t in (q, k, *ws, cos, sin)]
+    want = mhc.qk_norm_rope(*args)
+    for i in range(len(args)):
+        with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+            call = [torch.autograd.forward_ad.make_dual(a, torch.ones_like(a)) if j == i else a
+                    for j, a in enumerate(args)]
+            with pytest.raises(RuntimeError, match="jvp is not implemented" if i < 4 else "no gradient"):
+                mhc.qk_norm_rope(*call)
+    assert all(torch.equal(a, b) for a, b in zip(mhc.qk_norm_rope(*args), want))
