@@ -63,8 +63,9 @@ def _not_traced(what: str) -> None:
 
 
 def _operator_checkpoint(checkpoint: Optional[str]) -> int:
-    """The same for the operators that torch.jit.trace records: it records
-    their Python functions, which save the rows as they are."""
+    """The same for an operator's call: with a checkpoint torch.jit.trace does
+    not record it (the Python functions that it does record save the rows as
+    they are)."""
     code = _checkpoint_code(checkpoint)
     if code >= 0:
         _not_traced("checkpoint=")
@@ -270,7 +271,7 @@ def mhc_layer_static(x: torch.Tensor, rmsnorm_weight: torch.Tensor, H_pre: torch
     bits for the backward, which is then the layer's gradient at the values
     that checkpoint stands for."""
     return _lib.autograd().static_layer(x, rmsnorm_weight, H_pre, H_post, H_res, int(sinkhorn_iters),
-                                        float(sinkhorn_eps), float(rmsnorm_eps), _checkpoint_code(checkpoint))
+                                        float(sinkhorn_eps), float(rmsnorm_eps), _operator_checkpoint(checkpoint))
 
 
 # =============================================================================
@@ -349,7 +350,7 @@ def mhc_layer_fused_dynamic_training(x_expanded, rmsnorm_weight, phi_pre, phi_po
         alpha_res = torch.tensor(alpha_res, device=dev, dtype=torch.float32)
     return _lib.autograd().dynamic_layer(x_expanded, rmsnorm_weight, phi_pre, phi_post, phi_res, alpha_pre,
                                          alpha_post, alpha_res, b_pre, b_post, b_res, int(sinkhorn_iters),
-                                         float(sinkhorn_eps), float(rmsnorm_eps), _checkpoint_code(checkpoint))
+                                         float(sinkhorn_eps), float(rmsnorm_eps), _operator_checkpoint(checkpoint))
 
 
 # =============================================================================
@@ -361,7 +362,7 @@ def mhc_residual_wrapper(residual: torch.Tensor, branch_output: torch.Tensor, la
     parameters of ``layer`` (an MHCLayer); returns fp32 [tokens, C].  With the
     layer's ``checkpoint`` the saved rows, residual and branch_output (or the
     streams of a shape that is not fused), are kept in 8 bits."""
-    checkpoint = _checkpoint_code(getattr(layer, "checkpoint", None))
+    checkpoint = _operator_checkpoint(getattr(layer, "checkpoint", None))
     n = layer.expansion_rate
     C = residual.shape[-1]
     # The fused wrapper kernels take 4-channel rows and n = 2..32; with

@@ -158,3 +158,17 @@ def test_qk_entry_rejects_wide_heads_and_small_workspaces_on_host():
     assert lib.mhc_qk_norm_rope_bwd(*bwd) == -3
     bwd[29] = None
     assert lib.mhc_qk_norm_rope_bwd(*bwd) == -1
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_layers_and_wrapper_refuse_to_be_traced_with_a_checkpoint():
+    """torch.jit.trace would keep a C++ node's result as a constant."""
+    x = torch.zeros(2, 4, 32)
+    for dynamic in (False, True):
+        layer = mhc.MHCLayer(32, 4, use_dynamic_h=dynamic, checkpoint="int8")
+        wrap = mhc.MHCResidualWrapper(32, 4, use_dynamic_h=dynamic)
+        wrap.mhc.checkpoint = "e4m3"
+        for call in (layer, lambda a: wrap(a[:, 0], a[:, 1]),
+                     lambda a: mhc.ops.mhc_residual_wrapper(a[:, 0], a[:, 1], layer)):
+            with pytest.raises(RuntimeError, match="not recorded by torch.jit.trace"):
+                torch.jit.trace(call, (x,), check_trace=False)
