@@ -244,6 +244,12 @@ int64_t format_for(int64_t fmt, std::initializer_list<const Tensor*> inputs) {
     return MHC_CHECKPOINT_NONE;
 }
 
+// The format a node saved its rows in, under "fmt"; a node without one saves none.
+int64_t saved_format(AutogradContext* ctx) {
+    const auto it = ctx->saved_data.find("fmt");
+    return it == ctx->saved_data.end() ? MHC_CHECKPOINT_NONE : it->second.toInt();
+}
+
 // ---- static H: mhc_ascend_amd.ops.MHCLayerStaticFunction (layer.py:142-170) --
 struct StaticLayer : public torch::autograd::Function<StaticLayer> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& w_in, const Tensor& hp_in,
@@ -262,8 +268,8 @@ struct StaticLayer : public torch::autograd::Function<StaticLayer> {
         Tensor saved = at::empty({(int64_t)(lib.mhc_layer_static_saved_size((int32_t)n, (int32_t)C) / 4)}, f32);
         ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
         ctx->saved_data["cfg"] = std::vector<double>{(double)iters, sk_eps, rms_eps};
-        ctx->saved_data["fmt"] = fmt;
         if (fmt != MHC_CHECKPOINT_NONE) {
+            ctx->saved_data["fmt"] = fmt;
             const Held held = held_alloc(x);
             check(lib.mhc_layer_static_checkpoint_fwd(
                       x.data_ptr(), dtype_code(x.scalar_type()), w.data_ptr(), dtype_code(w.scalar_type()), fp(hp),
@@ -293,7 +299,7 @@ struct StaticLayer : public torch::autograd::Function<StaticLayer> {
         check_device(fn, {&grads[0], &x});
         const at::DeviceGuard guard(x.device());
         const auto cfg = ctx->saved_data["cfg"].toDoubleVector();
-        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const int64_t fmt = saved_format(ctx);
         const bool is_held = fmt != MHC_CHECKPOINT_NONE;  // x is the checkpoint's values then
         const auto sizes = is_held ? ctx->saved_data["sizes"].toIntVector() : x.sizes().vec();
         const auto store = is_held ? (at::ScalarType)ctx->saved_data["store"].toInt() : x.scalar_type();
@@ -363,8 +369,8 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
         Tensor ws = workspace(wsb, x);
         ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
         ctx->saved_data["cfg"] = std::vector<double>{(double)iters, sk_eps, rms_eps};
-        ctx->saved_data["fmt"] = fmt;
         if (fmt != MHC_CHECKPOINT_NONE) {
+            ctx->saved_data["fmt"] = fmt;
             const Held held = held_alloc(x);
             check(lib.mhc_layer_dynamic_checkpoint_fwd(
                       x.data_ptr(), dtype_code(x.scalar_type()), w.data_ptr(), dtype_code(w.scalar_type()), fp(ph[0]),
@@ -395,7 +401,7 @@ struct DynamicLayer : public torch::autograd::Function<DynamicLayer> {
         check_device(fn, {&grads[0], &x});
         const at::DeviceGuard guard(x.device());
         const auto cfg = ctx->saved_data["cfg"].toDoubleVector();
-        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const int64_t fmt = saved_format(ctx);
         const bool is_held = fmt != MHC_CHECKPOINT_NONE;  // x is the checkpoint's values then
         const auto sizes = is_held ? ctx->saved_data["sizes"].toIntVector() : x.sizes().vec();
         const auto store = is_held ? (at::ScalarType)ctx->saved_data["store"].toInt() : x.scalar_type();
@@ -465,8 +471,8 @@ int32_t wrapper_mode(const std::string& mode, int64_t n, const char* fn) {
 // rows' scales behind them.
 void save_wrapper_rows(AutogradContext* ctx, int64_t fmt, const Tensor& r, const Tensor& b, tensor_list rest) {
     tensor_list sv = {r, b};
-    ctx->saved_data["fmt"] = fmt;
     if (fmt != MHC_CHECKPOINT_NONE) {
+        ctx->saved_data["fmt"] = fmt;
         const Held hr = hold(r, fmt), hb = hold(b, fmt);
         sv = {hr.values, hb.values};
         rest.push_back(hr.scales);
@@ -479,7 +485,7 @@ void save_wrapper_rows(AutogradContext* ctx, int64_t fmt, const Tensor& r, const
 }
 
 std::pair<Tensor, Tensor> wrapper_rows(AutogradContext* ctx, const tensor_list& sv) {
-    const int64_t fmt = ctx->saved_data["fmt"].toInt();
+    const int64_t fmt = saved_format(ctx);
     if (fmt == MHC_CHECKPOINT_NONE) return {sv[0], sv[1]};
     const auto sizes = ctx->saved_data["sizes"].toIntVector();
     const auto store = (at::ScalarType)ctx->saved_data["store"].toInt();
@@ -815,8 +821,8 @@ struct Aggregate : public torch::autograd::Function<Aggregate> {
         check(lib.mhc_stream_aggregate_fwd(x.data_ptr(), dtype_code(x.scalar_type()), fp(h), hs, out.data_ptr(),
                                            fp(act), B, (int32_t)n, (int32_t)C, stream()),
               "mhc_stream_aggregate_fwd");
-        ctx->saved_data["fmt"] = fmt;
         if (fmt != MHC_CHECKPOINT_NONE) {
+            ctx->saved_data["fmt"] = fmt;
             const Held held = hold(x, fmt);
             ctx->saved_data["sizes"] = x.sizes().vec();
             ctx->saved_data["store"] = (int64_t)x.scalar_type();
@@ -833,7 +839,7 @@ struct Aggregate : public torch::autograd::Function<Aggregate> {
         const Tensor &inp = sv[0], &act = sv[1];
         check_device("stream_aggregate_bwd", {&grads[0], &inp, &act});
         const at::DeviceGuard guard(inp.device());
-        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const int64_t fmt = saved_format(ctx);
         const bool is_held = fmt != MHC_CHECKPOINT_NONE;
         const Tensor x = is_held ? held_rows(inp, sv[2], fmt, ctx->saved_data["sizes"].toIntVector(),
                                              (at::ScalarType)ctx->saved_data["store"].toInt())
@@ -871,8 +877,8 @@ struct Distribute : public torch::autograd::Function<Distribute> {
                                                     dtype_code(x.scalar_type()), fp(out), fp(act), B, (int32_t)n,
                                                     (int32_t)C, stream()),
               "mhc_stream_distribute_mix_add_fwd");
-        ctx->saved_data["fmt"] = fmt;
         if (fmt != MHC_CHECKPOINT_NONE) {
+            ctx->saved_data["fmt"] = fmt;
             const Held hx = hold(x, fmt), hy = hold(y, fmt);
             ctx->saved_data["sizes"] = x.sizes().vec();
             ctx->saved_data["store"] = (int64_t)x.scalar_type();
@@ -890,7 +896,7 @@ struct Distribute : public torch::autograd::Function<Distribute> {
         const Tensor &x_in = sv[0], &y_in = sv[1], &m_in = sv[2], &act = sv[3];
         check_device(fn, {&grads[0], &x_in, &y_in, &m_in, &act});
         const at::DeviceGuard guard(x_in.device());
-        const int64_t fmt = ctx->saved_data["fmt"].toInt();
+        const int64_t fmt = saved_format(ctx);
         Tensor x, y;
         at::ScalarType x_dtype = x_in.scalar_type(), y_dtype = y_in.scalar_type();
         if (fmt != MHC_CHECKPOINT_NONE) {

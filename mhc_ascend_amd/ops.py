@@ -66,9 +66,10 @@ def _operator_checkpoint(checkpoint: Optional[str]) -> int:
     """The same for an operator's call: with a checkpoint torch.jit.trace does
     not record it (the Python functions that it does record save the rows as
     they are)."""
+    if checkpoint is None:
+        return -1
     code = _checkpoint_code(checkpoint)
-    if code >= 0:
-        _not_traced("checkpoint=")
+    _not_traced("checkpoint=")
     return code
 
 
