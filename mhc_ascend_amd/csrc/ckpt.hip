@@ -18,7 +18,7 @@ namespace mhc {
 // Rows of a multiple of 32 are one run of blocks (the padded layout is then
 // the plain one): U pieces a lane, all loads first.  Other rows go piece by
 // piece with the row found by a 32-bit division.
-// Both are bound by their bytes: 32768 x 4096 bf16, 65 us each way, 6.2 TB/s.
+// Both are bound by their bytes: 32768 x 4096 bf16, 65-66 us each way, 6.2 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kCkU = 4;
 

@@ -8,9 +8,9 @@
 // A lane holds 4 channels of a chunk, so 8 lanes a block of 32: the block's
 // maximum is three DPP steps.  Both passes are bound by their bytes; the
 // pack pass (a second read of x) and the unpack pass (x^ written and read)
-// are what they save.  8192 x 4 x 4096: fp32 forward 201 us (6.0 TB/s), backward
-// 205-218 (5.6-5.9); bf16 forward 160 (5.9), backward of the dynamic layer
-// 165-178 (5.3-5.7).  With a pack and an unpack pass the fp32 step took 780 us,
+// are what they save.  8192 x 4 x 4096: fp32 forward 201-209 us (5.8-6.0 TB/s),
+// backward 205-227 (5.3-5.9); bf16 forward 160 (5.9), backward of the dynamic
+// layer 165-178 (5.3-5.7).  With a pack and an unpack pass the fp32 step took 780 us,
 // with these 413.
 #include "mhc_ckpt.h"
 #include "mhc_device.h"

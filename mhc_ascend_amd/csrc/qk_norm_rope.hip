@@ -56,7 +56,10 @@ __device__ __forceinline__ bool qk_pair(const QkArgs& a, int d, int& col, int& o
 // Any head size, stride and alignment: one wave a head row, one channel a
 // lane at a time.  A block of 32 channels is half a wave.  Bound by its
 // instructions (8192 tokens x 40 heads of 128 bf16, forward and backward: 996 us,
-// the kernels below 84), so for head sizes that those do not take.
+// the kernels below 84), so for what qk_tiling finds no pieces for: heads that are
+// no multiple of 4 or too wide, and halves of a rotated width that is no multiple
+// of 8, whose pairs no piece of 4 meets whole (9147 x 40 heads of 72 bf16: 635 us
+// with R = 36, 119 with R = 72).
 // ---------------------------------------------------------------------------
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void qk_fwd_any_kernel(QkArgs a) {
