@@ -453,6 +453,44 @@ int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, 
                                      int32_t hidden, int32_t num_iters, float sinkhorn_eps, float rmsnorm_eps,
                                      void* stream);
 
+/* ---- dropout without a stored mask ------------------------------------------------
+ * No counterpart in the reference.  out = x * 65536 / (65536 - threshold) where
+ * the value's number is at least threshold (0 .. 65536), 0 elsewhere; its
+ * backward is the same call on the cotangent.  The numbers are Philox4x32-10's:
+ * channels 8 j .. 8 j + 7 of row i take the four words of counter (i *
+ * ceil(hidden / 8) + j, offset) under the key seed, 16 bits each, the low half of
+ * a word first.  seed is *seed_ptr (device memory, 8-byte aligned) where that is
+ * not NULL, so that a captured graph takes a new one on each replay.  out does
+ * not overlap x.  hidden <= 2^30. */
+int mhc_dropout(const void* x, int32_t dtype, void* out, int32_t threshold, uint64_t seed, const void* seed_ptr,
+                uint64_t offset, int64_t rows, int32_t hidden, void* stream);
+
+/* ---- RMSNorm of a residual's sum ---------------------------------------------------
+ * No counterpart in the reference.  For rows of x (x_dtype) and residual
+ * (residual_dtype) [batch, hidden]:
+ *   h = residual + dropout(x)  (rounded to residual_dtype; mhc_dropout's numbers,
+ *       threshold 0 for none; the product is rounded by itself in fp32)
+ *   y = h / sqrt(mean h^2 + eps) * weight
+ * y is written to `y` in x_dtype (y_format MHC_CHECKPOINT_NONE), or to y_values /
+ * y_scales in 8 bits as mhc_checkpoint_pack lays them out, from the fp32 values.
+ * With h_format other than MHC_CHECKPOINT_NONE the checkpoint of h's rows is
+ * written too, and the backward reads it in place of h.  hidden <= 2^30. */
+int mhc_rmsnorm_residual_fwd(const void* x, int32_t x_dtype, const void* residual, int32_t residual_dtype,
+                             const void* weight, int32_t weight_dtype, void* h, void* y, int32_t y_format,
+                             void* y_values, void* y_scales, int32_t h_format, void* h_values, void* h_scales,
+                             int32_t threshold, uint64_t seed, const void* seed_ptr, uint64_t offset, int64_t batch,
+                             int32_t hidden, float eps, void* stream);
+size_t mhc_rmsnorm_residual_bwd_workspace_size(int64_t batch, int32_t hidden, int32_t x_dtype, int32_t residual_dtype);
+/* With dh = grad_h + the gradient of the norm at h: grad_residual = dh
+ * (residual_dtype), grad_x = dropout(dh) (x_dtype), grad_weight (weight_dtype).
+ * grad_h may be NULL (zeros); so may each gradient that is not wanted. */
+int mhc_rmsnorm_residual_bwd(const void* grad_y, int32_t x_dtype, const void* grad_h, int32_t residual_dtype,
+                             const void* h, int32_t h_format, const void* h_values, const void* h_scales,
+                             const void* weight, int32_t weight_dtype, void* grad_x, void* grad_residual,
+                             void* grad_weight, int32_t threshold, uint64_t seed, const void* seed_ptr,
+                             uint64_t offset, void* workspace, size_t workspace_bytes, int64_t batch, int32_t hidden,
+                             float eps, void* stream);
+
 /* ---- per-head norm of queries and keys, with the rotation of positions ---------
  * No counterpart in the reference.  For every head row x of q [tokens, q_heads,
  * head_dim] and k [tokens, k_heads, head_dim] (dtype; strides in elements, the

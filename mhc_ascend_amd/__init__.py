@@ -24,6 +24,8 @@ from .ops import (  # noqa: E402
     PackedActivation,
     activation_pack,
     activation_unpack,
+    dropout,
+    rmsnorm_residual,
     rope_table,
     qk_norm_rope,
 )
@@ -46,6 +48,8 @@ __all__ = [
     "PackedActivation",
     "activation_pack",
     "activation_unpack",
+    "dropout",
+    "rmsnorm_residual",
     "rope_table",
     "qk_norm_rope",
 ]

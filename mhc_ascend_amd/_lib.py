@@ -39,6 +39,7 @@ _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_u64 = ctypes.c_uint64
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes).  Must match include/mhc_hip.h (checked by
@@ -134,6 +135,12 @@ SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "mhc_layer_dynamic_checkpoint_bwd": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp,
                                                         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64,
                                                         _i32, _i32, _i32, _f32, _f32, _vp]),
+    "mhc_dropout": (ctypes.c_int, [_vp, _i32, _vp, _i32, _u64, _vp, _u64, _i64, _i32, _vp]),
+    "mhc_rmsnorm_residual_fwd": (ctypes.c_int, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i32, _vp,
+                                                _vp, _i32, _u64, _vp, _u64, _i64, _i32, _f32, _vp]),
+    "mhc_rmsnorm_residual_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "mhc_rmsnorm_residual_bwd": (ctypes.c_int, [_vp, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
+                                                _i32, _u64, _vp, _u64, _vp, _sz, _i64, _i32, _f32, _vp]),
     "mhc_qk_norm_rope_fwd": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _i64,
                                             _vp, _i32, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _i64, _i32, _i32,
                                             _i32, _i32, _i32, _f32, _vp]),

@@ -2521,6 +2521,135 @@ int mhc_layer_dynamic_checkpoint_bwd(const float* grad_out, const void* values, 
     });
 }
 
+// ---- dropout, RMSNorm of a residual's sum ---------------------------------------
+constexpr int kResMaxRow = 1 << 30;
+
+static int check_dropout(const char* fn, int64_t rows, int32_t hidden, int32_t threshold, const void* seed_ptr) {
+    const std::string f(fn);
+    if (rows < 0) return fail(MHC_ERR_INVALID, f + ": the number of rows must be >= 0");
+    if (hidden < 1) return fail(MHC_ERR_INVALID, f + ": hidden must be >= 1");
+    if (hidden > kResMaxRow) return fail(MHC_ERR_UNSUPPORTED, f + ": hidden must be at most 2^30");
+    if (threshold < 0 || threshold > 65536) return fail(MHC_ERR_INVALID, f + ": threshold must be in 0 .. 65536");
+    if ((uintptr_t)seed_ptr % 8 != 0) return fail(MHC_ERR_INVALID, f + ": seed_ptr must be 8-byte aligned");
+    return MHC_SUCCESS;
+}
+
+static DropArgs drop_args(int32_t threshold, uint64_t seed, const void* seed_ptr, uint64_t offset) {
+    DropArgs d{};
+    d.seed_ptr = (const uint64_t*)seed_ptr;
+    d.seed = seed;
+    d.offset = offset;
+    d.threshold = (uint32_t)threshold;
+    d.scale = threshold < 65536 ? (float)(65536.0 / (65536 - threshold)) : 0.f;
+    return d;
+}
+
+int mhc_dropout(const void* x, int32_t dtype, void* out, int32_t threshold, uint64_t seed, const void* seed_ptr,
+                uint64_t offset, int64_t rows, int32_t hidden, void* stream) {
+    return guarded([&]() -> int {
+        const int st = check_dropout("dropout", rows, hidden, threshold, seed_ptr);
+        if (st) return st;
+        MHC_REQUIRE(valid_dtype(dtype), "dropout: dtype must be F32 or BF16");
+        MHC_REQUIRE(rows == 0 || (x && out), "dropout: null pointer");
+        return hip_status(launch_dropout(dtype, x, out, drop_args(threshold, seed, seed_ptr, offset), rows, hidden,
+                                         (hipStream_t)stream));
+    });
+}
+
+static int check_residual(const char* fn, int64_t batch, int32_t hidden, int32_t x_dtype, int32_t r_dtype,
+                          int32_t w_dtype, int32_t threshold, const void* seed_ptr) {
+    const int st = check_dropout(fn, batch, hidden, threshold, seed_ptr);
+    if (st) return st;
+    if (batch > 0x7fffffff) return fail(MHC_ERR_UNSUPPORTED, std::string(fn) + ": batch must be < 2^31");
+    if (!valid_dtype(x_dtype) || !valid_dtype(r_dtype) || !valid_dtype(w_dtype))
+        return fail(MHC_ERR_INVALID, std::string(fn) + ": the dtypes must be F32 or BF16");
+    return MHC_SUCCESS;
+}
+
+// A call's array in 8 bits: none, or whole.
+static int check_residual_format(const char* fn, int32_t format, const void* values, const void* scales,
+                                 int64_t batch) {
+    if (format == -1) return MHC_SUCCESS;
+    if (!valid_format(format)) return fail(MHC_ERR_INVALID, std::string(fn) + ": formats must be NONE, INT8 or E4M3");
+    if (batch > 0 && (!values || !scales || (uintptr_t)values % 16 != 0))
+        return fail(MHC_ERR_INVALID, std::string(fn) + ": null 8-bit array, or values not 16-byte aligned");
+    return MHC_SUCCESS;
+}
+
+int mhc_rmsnorm_residual_fwd(const void* x, int32_t x_dtype, const void* residual, int32_t residual_dtype,
+                             const void* weight, int32_t weight_dtype, void* h, void* y, int32_t y_format,
+                             void* y_values, void* y_scales, int32_t h_format, void* h_values, void* h_scales,
+                             int32_t threshold, uint64_t seed, const void* seed_ptr, uint64_t offset, int64_t batch,
+                             int32_t hidden, float eps, void* stream) {
+    return guarded([&]() -> int {
+        const char* fn = "rmsnorm_residual_fwd";
+        int st = check_residual(fn, batch, hidden, x_dtype, residual_dtype, weight_dtype, threshold, seed_ptr);
+        if (!st) st = check_residual_format(fn, y_format, y_values, y_scales, batch);
+        if (!st) st = check_residual_format(fn, h_format, h_values, h_scales, batch);
+        if (st) return st;
+        MHC_REQUIRE(batch == 0 || (x && residual && weight && h && (y || y_format >= 0)),
+                    "rmsnorm_residual_fwd: null pointer");
+        ResidualArgs a{};
+        a.x = x; a.residual = residual; a.w = weight; a.h = h; a.y = y;
+        a.yq = (uint8_t*)y_values; a.ysc = (uint8_t*)y_scales;
+        a.hq = (uint8_t*)h_values; a.hsc = (uint8_t*)h_scales;
+        a.B = batch; a.C = hidden; a.w_dtype = weight_dtype; a.y_fmt = y_format; a.h_fmt = h_format; a.eps = eps;
+        a.drop = drop_args(threshold, seed, seed_ptr, offset);
+        return hip_status(launch_rmsnorm_residual_fwd(x_dtype, residual_dtype, a, (hipStream_t)stream));
+    });
+}
+
+static RowsBwdWs residual_bwd_ws(int64_t batch, int32_t hidden, int32_t x_dtype, int32_t residual_dtype) {
+    RowsBwdWs w{};
+    w.grid = rmsnorm_residual_bwd_grid(x_dtype, residual_dtype, batch, hidden);
+    w.total = align256((size_t)w.grid * hidden * sizeof(float));
+    return w;
+}
+
+size_t mhc_rmsnorm_residual_bwd_workspace_size(int64_t batch, int32_t hidden, int32_t x_dtype,
+                                               int32_t residual_dtype) {
+    if (batch < 0 || hidden < 1 || hidden > kResMaxRow || !valid_dtype(x_dtype) || !valid_dtype(residual_dtype))
+        return 0;
+    return guarded_size([&]() -> size_t { return residual_bwd_ws(batch, hidden, x_dtype, residual_dtype).total; });
+}
+
+int mhc_rmsnorm_residual_bwd(const void* grad_y, int32_t x_dtype, const void* grad_h, int32_t residual_dtype,
+                             const void* h, int32_t h_format, const void* h_values, const void* h_scales,
+                             const void* weight, int32_t weight_dtype, void* grad_x, void* grad_residual,
+                             void* grad_weight, int32_t threshold, uint64_t seed, const void* seed_ptr,
+                             uint64_t offset, void* workspace, size_t workspace_bytes, int64_t batch, int32_t hidden,
+                             float eps, void* stream) {
+    return guarded([&]() -> int {
+        const char* fn = "rmsnorm_residual_bwd";
+        int st = check_residual(fn, batch, hidden, x_dtype, residual_dtype, weight_dtype, threshold, seed_ptr);
+        if (!st) st = check_residual_format(fn, h_format, h_values, h_scales, batch);
+        if (st) return st;
+        MHC_REQUIRE(batch == 0 || (grad_y && weight && (h || h_format >= 0)), "rmsnorm_residual_bwd: null pointer");
+        const RowsBwdWs w = residual_bwd_ws(batch, hidden, x_dtype, residual_dtype);
+        if (grad_weight && (!workspace || workspace_bytes < w.total))
+            return fail(MHC_ERR_WORKSPACE, "rmsnorm_residual_bwd: workspace smaller than "
+                                           "mhc_rmsnorm_residual_bwd_workspace_size()");
+        ResidualArgs a{};
+        a.gy = grad_y; a.gh = grad_h; a.h = const_cast<void*>(h); a.w = weight; a.gx = grad_x; a.gres = grad_residual;
+        a.hq = (uint8_t*)const_cast<void*>(h_values); a.hsc = (uint8_t*)const_cast<void*>(h_scales);
+        a.dw_part = grad_weight ? (float*)workspace : nullptr;
+        a.B = batch; a.C = hidden; a.w_dtype = weight_dtype; a.y_fmt = -1; a.h_fmt = h_format; a.eps = eps;
+        a.drop = drop_args(threshold, seed, seed_ptr, offset);
+        hipStream_t s = (hipStream_t)stream;
+        int rows = w.grid;
+        hipError_t e = hipSuccess;
+        if (batch > 0) {
+            e = launch_rmsnorm_residual_bwd(x_dtype, residual_dtype, a, w.grid, s);
+        } else if (grad_weight) {
+            rows = 1;
+            e = launch_fill_zero(a.dw_part, hidden, s);
+        }
+        if (e == hipSuccess && grad_weight)
+            e = launch_weight_grad_sum(weight_dtype, a.dw_part, rows, hidden, grad_weight, s);
+        return hip_status(e);
+    });
+}
+
 // ---- queries and keys -----------------------------------------------------------
 static int check_qk(const char* fn, const QkArgs& a, int32_t dtype, int32_t format) {
     const std::string f(fn);

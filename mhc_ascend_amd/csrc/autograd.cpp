@@ -77,6 +77,10 @@ using torch::autograd::tensor_list;
     X(mhc_layer_dynamic_checkpoint_fwd)       \
     X(mhc_layer_dynamic_checkpoint_bwd_workspace_need) \
     X(mhc_layer_dynamic_checkpoint_bwd)       \
+    X(mhc_dropout)                            \
+    X(mhc_rmsnorm_residual_fwd)               \
+    X(mhc_rmsnorm_residual_bwd_workspace_size) \
+    X(mhc_rmsnorm_residual_bwd)               \
     X(mhc_qk_norm_rope_fwd)                   \
     X(mhc_qk_norm_rope_bwd_workspace_size)    \
     X(mhc_qk_norm_rope_bwd)
@@ -926,6 +930,155 @@ struct Distribute : public torch::autograd::Function<Distribute> {
     }
 };
 
+// ---- dropout, RMSNorm of a residual's sum ---------------------------------------
+// What a call drops: the numbers of `seed` (a tensor where one is defined).
+struct Drop {
+    int64_t threshold, value, offset;
+    Tensor seed;
+
+    const void* ptr() const { return seed.defined() ? seed.data_ptr() : nullptr; }
+    std::vector<int64_t> ints() const { return {threshold, value, offset}; }
+    static Drop saved(const std::vector<int64_t>& v, const Tensor& seed) { return {v[0], v[1], v[2], seed}; }
+};
+
+// A seed that is not given is drawn from x's device's generator.
+Drop make_drop(const char* fn, const Tensor& x, double p, const c10::optional<Tensor>& seed,
+               const c10::optional<int64_t>& value, int64_t offset) {
+    TORCH_CHECK(p >= 0.0 && p <= 1.0, fn, ": the probability must be in 0 .. 1, got ", p);
+    TORCH_CHECK(offset >= 0, fn, ": offset must be >= 0, got ", offset);
+    Drop d{(int64_t)std::nearbyint(p * 65536), value.value_or(0), offset, Tensor()};
+    if (seed.has_value()) {
+        check_device(fn, {&x, &*seed});
+        TORCH_CHECK(seed->scalar_type() == at::kLong && seed->numel() == 1, fn, ": seed must be one int64, got ",
+                    seed->scalar_type(), " ", seed->sizes());
+        d.seed = *seed;
+    } else if (!value.has_value() && d.threshold > 0) {
+        const at::DeviceGuard guard(x.device());
+        d.seed = at::empty({1}, x.options().dtype(at::kLong).requires_grad(false)).random_();
+    }
+    if (d.threshold == 0) d.seed = Tensor();
+    return d;
+}
+
+// Rows [B, C] of a contiguous tensor [..., C].
+int64_t rows_of(const Tensor& t) { return t.size(-1) > 0 ? t.numel() / t.size(-1) : 0; }
+
+void check_rows(const char* fn, const Tensor& x) {
+    TORCH_CHECK(x.dim() >= 1 && at::isFloatingType(x.scalar_type()), fn,
+                ": x must be a floating-point tensor [..., C]");
+    TORCH_CHECK(x.size(-1) >= 1 && x.size(-1) <= INT32_MAX, fn, ": rows of ", x.size(-1), " channels");
+}
+
+Tensor run_dropout(const Tensor& x, const Drop& d) {
+    Tensor out = at::empty_like(x);
+    check(lib.mhc_dropout(x.data_ptr(), dtype_code(x.scalar_type()), out.data_ptr(), (int32_t)d.threshold,
+                          (uint64_t)d.value, d.ptr(), (uint64_t)d.offset, rows_of(x), (int32_t)x.size(-1), stream()),
+          "mhc_dropout");
+    return out;
+}
+
+struct Dropout : public torch::autograd::Function<Dropout> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x_in, const Drop& d) {
+        const at::DeviceGuard guard(x_in.device());
+        const Tensor x = storage(x_in);
+        if (ctx) {
+            ctx->save_for_backward({d.seed});
+            ctx->saved_data["drop"] = d.ints();
+            ctx->saved_data["x_dtype"] = (int64_t)x_in.scalar_type();
+        }
+        return run_dropout(x, d);
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        const Drop d = Drop::saved(ctx->saved_data["drop"].toIntVector(), ctx->get_saved_variables()[0]);
+        const auto dt = (at::ScalarType)ctx->saved_data["x_dtype"].toInt();
+        const at::DeviceGuard guard(grads[0].device());
+        return {run_dropout(storage(grads[0]), d).to(dt), Tensor()};
+    }
+};
+
+struct RmsNormResidual : public torch::autograd::Function<RmsNormResidual> {
+    // (y, h); with y_fmt (values, scales, h)
+    static tensor_list forward(AutogradContext* ctx, const Tensor& x_in, const Tensor& res_in, const Tensor& w_in,
+                               double eps, const Drop& d, int64_t fmt, int64_t y_fmt) {
+        const char* fn = "mhc_rmsnorm_residual_fwd";
+        const at::DeviceGuard guard(x_in.device());
+        const Tensor x = storage(x_in), res = storage(res_in), w = weight(w_in);
+        const int64_t C = x.size(-1), B = rows_of(x);
+        Tensor h = at::empty_like(res), y;
+        Held hy, hh;
+        if (y_fmt != MHC_CHECKPOINT_NONE) hy = held_alloc(x);
+        else y = at::empty_like(x);
+        if (fmt != MHC_CHECKPOINT_NONE) hh = held_alloc(res);
+        const auto at_ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+        check(lib.mhc_rmsnorm_residual_fwd(
+                  x.data_ptr(), dtype_code(x.scalar_type()), res.data_ptr(), dtype_code(res.scalar_type()),
+                  w.data_ptr(), dtype_code(w.scalar_type()), h.data_ptr(), at_ptr(y), (int32_t)y_fmt,
+                  at_ptr(hy.values), at_ptr(hy.scales), (int32_t)fmt, at_ptr(hh.values), at_ptr(hh.scales),
+                  (int32_t)d.threshold, (uint64_t)d.value, d.ptr(), (uint64_t)d.offset, B, (int32_t)C, (float)eps,
+                  stream()),
+              fn);
+        if (y_fmt != MHC_CHECKPOINT_NONE) return {hy.values, hy.scales, h};
+        if (!ctx) return {y, h};  // no backward will run
+        ctx->set_materialize_grads(false);
+        if (fmt != MHC_CHECKPOINT_NONE) ctx->save_for_backward({w, d.seed, hh.values, hh.scales});
+        else ctx->save_for_backward({w, d.seed, h});
+        ctx->saved_data["drop"] = d.ints();
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["sizes"] = x.sizes().vec();
+        ctx->saved_data["ints"] = std::vector<int64_t>{fmt, (int64_t)x.scalar_type(), (int64_t)res.scalar_type(),
+                                                       (int64_t)x_in.scalar_type(), (int64_t)res_in.scalar_type(),
+                                                       (int64_t)w_in.scalar_type()};
+        return {y, h};
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        const char* fn = "mhc_rmsnorm_residual_bwd";
+        tensor_list out(7);
+        if (!grads[0].defined() && !grads[1].defined()) return out;
+        const auto sv = ctx->get_saved_variables();
+        const auto v = ctx->saved_data["ints"].toIntVector();
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        const Drop d = Drop::saved(ctx->saved_data["drop"].toIntVector(), sv[1]);
+        const Tensor& w = sv[0];
+        const int64_t fmt = v[0], C = sizes.back();
+        const bool is_held = fmt != MHC_CHECKPOINT_NONE;
+        const auto xt = (at::ScalarType)v[1], rt = (at::ScalarType)v[2];
+        const at::DeviceGuard guard(w.device());
+        const auto opt = w.options();
+        const Tensor gy = grads[0].defined() ? grads[0].to(xt).contiguous() : at::zeros(sizes, opt.dtype(xt));
+        const Tensor gh = grads[1].defined() ? grads[1].to(rt).contiguous() : Tensor();
+        TORCH_CHECK(gy.sizes() == sizes && (!gh.defined() || gh.sizes() == sizes), fn,
+                    ": the cotangents must match the outputs");
+        const bool want_x = ctx->needs_input_grad(0), want_res = ctx->needs_input_grad(1),
+                   want_w = ctx->needs_input_grad(2);
+        // without dropout and in one type both are the same array
+        const bool one = d.threshold == 0 && xt == rt;
+        Tensor gres, gx, gw, ws;
+        if (want_res || (one && want_x)) gres = at::empty(sizes, opt.dtype(rt));
+        if (want_x) gx = one ? gres : at::empty(sizes, opt.dtype(xt));
+        const int64_t B = rows_of(gy);
+        size_t wsb = 0;
+        if (want_w) {
+            gw = at::empty({C}, opt);
+            wsb = lib.mhc_rmsnorm_residual_bwd_workspace_size(B, (int32_t)C, dtype_code(xt), dtype_code(rt));
+            ws = workspace(wsb, w);
+        }
+        const auto at_ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+        check(lib.mhc_rmsnorm_residual_bwd(
+                  gy.data_ptr(), dtype_code(xt), at_ptr(gh), dtype_code(rt), is_held ? nullptr : sv[2].data_ptr(),
+                  (int32_t)fmt, is_held ? sv[2].data_ptr() : nullptr, is_held ? sv[3].data_ptr() : nullptr,
+                  w.data_ptr(), dtype_code(w.scalar_type()), one ? nullptr : at_ptr(gx), at_ptr(gres), at_ptr(gw),
+                  (int32_t)d.threshold, (uint64_t)d.value, d.ptr(), (uint64_t)d.offset, at_ptr(ws), wsb, B, (int32_t)C,
+                  (float)ctx->saved_data["eps"].toDouble(), stream()),
+              fn);
+        if (want_x) out[0] = gx.to((at::ScalarType)v[3]);
+        if (want_res) out[1] = gres.to((at::ScalarType)v[4]);
+        if (want_w) out[2] = gw.to((at::ScalarType)v[5]);
+        return out;
+    }
+};
+
 // ---- per-head norm of queries and keys, with the rotation of positions ----------
 // What the entries take besides rows: weights in one dtype, fp32 tables.
 struct QkTables {
@@ -1030,6 +1183,54 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
         return out;
     }
 };
+
+// Whether a call of a C++ node is needed: a backward may run, or an input has a
+// forward-mode tangent (forward mode runs without grad mode too), which a C++
+// node refuses.
+bool needs_node(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->_fw_grad(0).defined() || (at::GradMode::is_enabled() && t->requires_grad())) return true;
+    return false;
+}
+
+Tensor dropout(const Tensor& x, double p, const c10::optional<Tensor>& seed, const c10::optional<int64_t>& value,
+               int64_t offset) {
+    require_bound();
+    const char* fn = "dropout";
+    check_device(fn, {&x});
+    check_rows(fn, x);
+    const Drop d = make_drop(fn, x, p, seed, value, offset);
+    return needs_node({&x}) ? Dropout::apply(x, d) : Dropout::forward(nullptr, x, d);
+}
+
+tensor_list rmsnorm_residual(const Tensor& x, const Tensor& residual, const Tensor& w, double eps, double p,
+                             const c10::optional<Tensor>& seed, const c10::optional<int64_t>& value, int64_t offset,
+                             int64_t checkpoint, int64_t y_fmt) {
+    require_bound();
+    const char* fn = "rmsnorm_residual";
+    check_device(fn, {&x, &residual, &w});
+    check_rows(fn, x);
+    TORCH_CHECK(residual.sizes() == x.sizes() && at::isFloatingType(residual.scalar_type()), fn,
+                ": x and residual must be floating-point tensors of one shape, got ", x.sizes(), " and ",
+                residual.sizes());
+    TORCH_CHECK(w.dim() == 1 && w.numel() == x.size(-1), fn, ": weight must be [C], got ", w.sizes());
+    const bool node = needs_node({&x, &residual, &w});
+    TORCH_CHECK(y_fmt == MHC_CHECKPOINT_NONE || !node, fn,
+                ": no gradient flows through an output in 8 bits (call it under torch.no_grad())");
+    const int64_t fmt = format_for(checkpoint, {&x, &residual, &w});
+    const Drop d = make_drop(fn, x, p, seed, value, offset);
+    tensor_list out = node ? RmsNormResidual::apply(x, residual, w, eps, d, fmt, y_fmt)
+                           : RmsNormResidual::forward(nullptr, x, residual, w, eps, d, fmt, y_fmt);
+    if (y_fmt != MHC_CHECKPOINT_NONE) {
+        auto shape = x.sizes().vec();
+        const int64_t C = shape.back();
+        shape.back() = (C + 15) / 16 * 16;
+        out[0] = out[0].view(shape);
+        shape.back() = (C + 31) / 32;
+        out[1] = out[1].view(shape);
+    }
+    return out;
+}
 
 // (values, scales) of x [..., C]: uint8 [..., ceil16(C)] and [..., ceil(C / 32)]
 std::tuple<Tensor, Tensor> checkpoint_pack(const Tensor& x_in, int64_t fmt) {
@@ -1232,6 +1433,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
               return checkpoint_unpack(values, scales, fmt, hidden, bf16 ? at::kBFloat16 : at::kFloat);
           },
           "(values, scales, format, hidden, bf16) -> [..., hidden]");
+    m.def("dropout", &dropout, "(x [..., C], p, seed tensor or None, seed value or None, offset) with autograd");
+    m.def("rmsnorm_residual", &rmsnorm_residual,
+          "(x [..., C], residual [..., C], weight, eps, p, seed tensor or None, seed value or None, offset, checkpoint, "
+          "y_format) -> [y, h] with autograd, or [values, scales, h]");
     m.def("qk_norm_rope", &qk_norm_rope,
           "(q [..., H, D], k [..., K, D], q_weight, k_weight, cos, sin, positions or None, eps, interleaved, "
           "checkpoint) -> (q, k) with autograd");

@@ -340,6 +340,39 @@ hipError_t launch_proj_ckpt_bwd(int dx_dtype, int x_dtype, bool qin, int fmt, co
                                 const void* dx_in, void* dx, const int32_t* dx_scale, int groups, float* dphi_part, int tiles, int64_t B,
                                 int64_t K, hipStream_t s);
 
+// ---- residual.hip ----------------------------------------------------------
+// Dropout (mhc_dropout.h): threshold 0 .. 65536 of 16-bit numbers, seed from
+// memory where seed_ptr is not null.
+struct DropArgs {
+    const uint64_t* seed_ptr;
+    uint64_t seed, offset;
+    uint32_t threshold;
+    float scale;  // 65536 / (65536 - threshold); 0 where nothing is kept
+};
+hipError_t launch_dropout(int dt, const void* x, void* out, const DropArgs& d, int64_t rows, int64_t C, hipStream_t s);
+// h = residual + dropout(x), y = RMSNorm of h.  A format is a CkFormat, or -1.
+struct ResidualArgs {
+    const void* x;         // [B, C]: the branch (forward)
+    const void* residual;  // [B, C]
+    const void* w;
+    void* h;
+    void* y;               // with y_fmt < 0
+    uint8_t *yq, *ysc;     // y in 8 bits
+    uint8_t *hq, *hsc;     // h in 8 bits, with h_fmt >= 0: written forward, read backward in place of h
+    const void* gy;        // backward: cotangents of y and h (gh may be null)
+    const void* gh;
+    void* gx;              // backward: may be null
+    void* gres;            // backward: may be null
+    float* dw_part;        // backward: [grid][C], may be null
+    int64_t B;
+    int C, w_dtype, y_fmt, h_fmt;
+    float eps;
+    DropArgs drop;
+};
+hipError_t launch_rmsnorm_residual_fwd(int x_dt, int r_dt, const ResidualArgs& a, hipStream_t s);
+int rmsnorm_residual_bwd_grid(int x_dt, int r_dt, int64_t B, int64_t C);
+hipError_t launch_rmsnorm_residual_bwd(int x_dt, int r_dt, const ResidualArgs& a, int grid, hipStream_t s);
+
 // ---- qk_norm_rope.hip ------------------------------------------------------
 // Head rows of queries ([0]) and keys ([1]); strides in elements.  Token t's
 // table row is entry t % period of pos (pos_bytes 4 or 8), or t % period

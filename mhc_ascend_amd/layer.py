@@ -163,11 +163,19 @@ class MHCResidualWrapper(nn.Module):
     H_res gradients, or bf16 'decay' rows past n = 16 or past n = 8 on rows
     narrower than 2048 channels).
     Other shapes build the streams with tensor ops and run the layer.
+
+    ``dropout`` is the probability that a value of the branch is dropped in
+    training mode (ops.dropout, with a seed drawn from torch's generator).
     """
 
+    dropout: float = 0.0  # of modules unpickled from before it existed
+
     def __init__(self, hidden_dim: int, expansion_rate: int = 4, residual_mode: str = 'decay',
-                 use_post_norm: bool = True, **mhc_kwargs):
+                 use_post_norm: bool = True, dropout: float = 0.0, **mhc_kwargs):
         super().__init__()
+        if not 0.0 <= dropout <= 1.0:
+            raise ValueError(f"dropout must be in 0 .. 1, got {dropout}")
+        self.dropout = dropout
         self.hidden_dim = hidden_dim
         self.expansion_rate = expansion_rate
         self.residual_mode = residual_mode
@@ -185,6 +193,8 @@ class MHCResidualWrapper(nn.Module):
             T = 1
         if self.residual_mode not in ("zero", "decay"):
             raise ValueError(f"Unknown residual_mode: {self.residual_mode}")
+        if self.training and self.dropout > 0.0:
+            branch_output = ops.dropout(branch_output, self.dropout)
         output = ops.mhc_residual_wrapper(residual, branch_output, self.mhc, self.residual_mode)
         if T > 1:
             output = output.reshape(B, T, C)
@@ -192,7 +202,8 @@ class MHCResidualWrapper(nn.Module):
 
     def extra_repr(self) -> str:
         return (f'hidden_dim={self.hidden_dim}, expansion_rate={self.expansion_rate}, '
-                f'residual_mode={self.residual_mode}')
+                f'residual_mode={self.residual_mode}'
+                + (f', dropout={self.dropout}' if self.dropout > 0.0 else ''))
 
 
 def replace_residual_with_mhc(hidden_dim: int, expansion_rate: int = 4, **kwargs) -> MHCResidualWrapper:

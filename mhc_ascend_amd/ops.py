@@ -17,6 +17,7 @@ PyTorch reference math, which is the contract):
 """
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -399,6 +400,71 @@ def mhc_residual_wrapper(residual: torch.Tensor, branch_output: torch.Tensor, la
                                   layer.b_post, layer.b_res, residual_mode, n, iters, sk_eps, rms_eps, checkpoint)
     return ag.static_wrapper(residual, branch_output, layer.rmsnorm_weight, layer.H_pre, layer.H_post, layer.H_res,
                              residual_mode, n, iters, sk_eps, rms_eps, checkpoint)
+
+
+# =============================================================================
+# Dropout without a stored mask, RMSNorm of a residual's sum (no counterpart in
+# the reference)
+# =============================================================================
+
+def _seed(fn: str, seed) -> Tuple[Optional[torch.Tensor], Optional[int]]:
+    """A ``seed`` argument as (tensor, None) or (None, the signed 64-bit value);
+    (None, None) where it is to be drawn."""
+    if seed is None or torch.is_tensor(seed):
+        return seed, None
+    seed = operator.index(seed)
+    if not -2 ** 63 <= seed < 2 ** 64:
+        raise ValueError(f"{fn}: seed must fit 64 bits, got {seed}")
+    return None, seed - 2 ** 64 if seed >= 2 ** 63 else seed
+
+
+def dropout(x: torch.Tensor, p: float = 0.5, seed=None, offset: int = 0) -> torch.Tensor:
+    """Dropout of x [..., C] whose mask is never stored: forward and backward
+    compute it from a counter.
+
+    With t = round(p * 2**16), a value is kept, times 2**16 / (2**16 - t), where
+    its 16-bit number is at least t, and 0 elsewhere.  Channels 8 j .. 8 j + 7 of
+    row i (rows counted over the leading dimensions) take the numbers of one
+    Philox4x32-10 block: counter (i * ceil(C / 8) + j, ``offset``), key ``seed``.
+
+    ``seed`` is an int of 64 bits, or an int64 tensor of one element on x's
+    device, read when the call runs: a captured graph that changes it between
+    replays drops other values in each.  It has to hold its value until the
+    backward.  Without one the call draws a seed from torch's generator of x's
+    device.  Call sites that share a seed take an ``offset`` each (0 .. 2**63 - 1).
+
+    fp32 and bf16 keep their dtype; others become fp32."""
+    _not_traced("dropout")
+    return _lib.autograd().dropout(x, float(p), *_seed("dropout", seed), int(offset))
+
+
+def rmsnorm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
+                     dropout: float = 0.0, seed=None, offset: int = 0, checkpoint: Optional[str] = None,
+                     format: Optional[str] = None):
+    """(y, h): h = residual + dropout(x), y = RMSNorm of h, in one pass.
+
+    x and residual [..., C] may differ in dtype: y has x's, h residual's (fp32 or
+    bf16; others become fp32), and the norm takes h as it is stored.  ``dropout``,
+    ``seed`` and ``offset`` are :func:`dropout`'s p, seed and offset; the result
+    is that of the two calls one after the other, without x's rounding between
+    them.
+
+    ``checkpoint`` ("int8" or "e4m3", see :func:`activation_pack`) saves h in 8
+    bits for the backward, which is then the gradient at the values that
+    checkpoint stands for; without it the backward reads the h that was returned.
+
+    ``format`` ("int8" or "e4m3") returns y in 8 bits, a :class:`PackedActivation`
+    of the fp32 values (its ``dtype`` is x's), for a product in 8 bits.  No
+    gradient flows through it: such a call raises where one is wanted."""
+    _not_traced("rmsnorm_residual")
+    code = _checkpoint_code(checkpoint)
+    y_code = -1 if format is None else _checkpoint_code(format)
+    out = _lib.autograd().rmsnorm_residual(x, residual, weight, float(eps), float(dropout),
+                                           *_seed("rmsnorm_residual", seed), int(offset), code, y_code)
+    if y_code < 0:
+        return out[0], out[1]
+    dtype = x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32
+    return PackedActivation(out[0], out[1], format, x.shape[-1], dtype), out[2]
 
 
 # =============================================================================
