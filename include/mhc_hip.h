@@ -528,6 +528,44 @@ int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_
                          int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
                          int32_t interleaved, float eps, void* stream);
 
+/* The same for tokens with positions on several axes (time, height and width of
+ * video, say): positions is [axes][position_period], axes 1 .. 4, and pair p
+ * turns by the table's entry (position on its axis, p).  sections (host memory,
+ * [axes], the sum rotary_dim / 2) are the pairs of each axis: consecutive ones
+ * with dealt == 0; with dealt != 0 pair p belongs to axis p % axes where p / axes
+ * < sections[p % axes], and to axis 0 elsewhere, and each axis but the first must
+ * have its number of them.  A position outside the table on any axis makes the
+ * token's rows NaN.  The backward's workspace is mhc_qk_norm_rope_bwd's. */
+int mhc_qk_norm_rope_axes_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                              int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
+                              const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                              int64_t table_rows, const void* positions, int32_t position_bytes,
+                              int64_t position_period, int32_t axes, const int32_t* sections, int32_t dealt,
+                              void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales,
+                              void* k_values, void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads,
+                              int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float eps, void* stream);
+int mhc_qk_norm_rope_axes_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
+                              const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
+                              int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                              int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
+                              const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
+                              const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                              int64_t table_rows, const void* positions, int32_t position_bytes,
+                              int64_t position_period, int32_t axes, const int32_t* sections, int32_t dealt,
+                              void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
+                              int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                              int32_t interleaved, float eps, void* stream);
+
+/* The rotation alone, by the angle or (inverse != 0) its negative, which is its
+ * backward on the cotangents.  axes 0 stands for one axis without sections (NULL);
+ * only there may positions be NULL. */
+int mhc_qk_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                int64_t k_head_stride, int32_t dtype, const float* cos, const float* sin, int64_t table_rows,
+                const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
+                const int32_t* sections, int32_t dealt, void* q_out, void* k_out, int64_t tokens, int32_t q_heads,
+                int32_t k_heads, int32_t head_dim, int32_t rotary_dim, int32_t interleaved, int32_t inverse,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,7 @@ from .ops import (  # noqa: E402
     rmsnorm_residual,
     rope_table,
     qk_norm_rope,
+    qk_rope,
 )
 
 __all__ = [
@@ -52,4 +53,5 @@ __all__ = [
     "rmsnorm_residual",
     "rope_table",
     "qk_norm_rope",
+    "qk_rope",
 ]

@@ -148,6 +148,15 @@ SIGNATURES: Dict[str, Tuple[object, List[object]]] = {
     "mhc_qk_norm_rope_bwd": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32,
                                             _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp, _i32, _i64,
                                             _vp, _vp, _vp, _vp, _sz, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "mhc_qk_norm_rope_axes_fwd": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp,
+                                                 _i64, _vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _vp,
+                                                 _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "mhc_qk_norm_rope_axes_bwd": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                                 _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _vp,
+                                                 _i32, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _sz, _i64, _i32,
+                                                 _i32, _i32, _i32, _i32, _f32, _vp]),
+    "mhc_qk_rope": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64, _vp, _i32, _i64, _i32, _vp,
+                                   _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
 
 # The benchmark build's extra entries (include/mhc_hip_timing.h).

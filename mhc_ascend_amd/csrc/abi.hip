@@ -2682,11 +2682,38 @@ static int check_qk(const char* fn, const QkArgs& a, int32_t dtype, int32_t form
     return MHC_SUCCESS;
 }
 
-int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+// A call's axes into its arguments.  axes 0: none named.
+static int set_qk_axes(const char* fn, QkArgs& a, int32_t axes, const int32_t* sections, int32_t dealt) {
+    const std::string f(fn);
+    if (axes < 0 || axes > 4) return fail(MHC_ERR_INVALID, f + ": axes must be in 0 .. 4");
+    a.axes = 0;
+    if (axes == 0) return MHC_SUCCESS;
+    if (!sections) return fail(MHC_ERR_INVALID, f + ": null sections");
+    if (a.T > 0 && !a.pos) return fail(MHC_ERR_INVALID, f + ": sections need positions");
+    int64_t sum = 0;
+    for (int i = 0; i < axes; ++i) {
+        if (sections[i] < 0) return fail(MHC_ERR_INVALID, f + ": sections must be >= 0");
+        sum += sections[i];
+    }
+    if (sum != a.R / 2) return fail(MHC_ERR_INVALID, f + ": the sections must add up to rotary_dim / 2");
+    a.axes = axes;
+    a.dealt = dealt != 0;
+    int end = 0;
+    for (int i = 0; i < 4; ++i) {
+        const int n = i < axes ? sections[i] : 0;
+        if (a.dealt && i > 0 && n > 0 && i + (int64_t)axes * (n - 1) >= a.R / 2)
+            return fail(MHC_ERR_INVALID, f + ": a section is too long to be dealt in turn");
+        end += n;
+        a.part[i] = a.dealt ? n : (i < axes - 1 ? end : INT32_MAX);
+    }
+    return MHC_SUCCESS;
+}
+
+static int qk_fwd(const char* fn, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                          int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
                          const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
-                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
-                         void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales, void* k_values,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
+                         const int32_t* sections, int32_t dealt, void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales, void* k_values,
                          void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
                          int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
     return guarded([&]() -> int {
@@ -2702,11 +2729,46 @@ int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_s
         a.heads[0] = q_heads; a.heads[1] = k_heads;
         a.w_dtype = weight_dtype; a.pos_bytes = position_bytes; a.D = head_dim; a.R = rotary_dim;
         a.interleaved = interleaved != 0; a.eps = eps;
-        const int st = check_qk("qk_norm_rope_fwd", a, dtype, format);
+        int st = check_qk(fn, a, dtype, format);
+        if (!st) st = set_qk_axes(fn, a, axes, sections, dealt);
         if (st) return st;
-        MHC_REQUIRE(tokens == 0 || ((q || q_heads == 0) && (k || k_heads == 0)), "qk_norm_rope_fwd: null q/k");
+        if (tokens > 0 && ((!q && q_heads > 0) || (!k && k_heads > 0)))
+            return fail(MHC_ERR_INVALID, std::string(fn) + ": null q/k");
         return hip_status(launch_qk_norm_rope_fwd(dtype, format, a, (hipStream_t)stream));
     });
+}
+
+// The entries with sections name at least one axis.
+static int fail_axes(const char* fn) {
+    return guarded([&]() -> int { return fail(MHC_ERR_INVALID, std::string(fn) + ": axes must be in 1 .. 4"); });
+}
+
+int mhc_qk_norm_rope_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                         int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
+                         void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales, void* k_values,
+                         void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                         int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
+    return qk_fwd("qk_norm_rope_fwd", q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, dtype,
+                  q_weight, k_weight, weight_dtype, cos, sin, table_rows, positions, position_bytes, position_period, 0,
+                  nullptr, 0, q_out, k_out, format, q_values, q_scales, k_values, k_scales, tokens, q_heads, k_heads,
+                  head_dim, rotary_dim, interleaved, eps, stream);
+}
+
+int mhc_qk_norm_rope_axes_fwd(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                              int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
+                              const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                              int64_t table_rows, const void* positions, int32_t position_bytes,
+                              int64_t position_period, int32_t axes, const int32_t* sections, int32_t dealt,
+                              void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales,
+                              void* k_values, void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads,
+                              int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
+    if (axes == 0) return fail_axes("qk_norm_rope_axes_fwd");
+    return qk_fwd("qk_norm_rope_axes_fwd", q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, dtype,
+                  q_weight, k_weight, weight_dtype, cos, sin, table_rows, positions, position_bytes, position_period,
+                  axes, sections, dealt, q_out, k_out, format, q_values, q_scales, k_values, k_scales, tokens, q_heads,
+                  k_heads, head_dim, rotary_dim, interleaved, eps, stream);
 }
 
 static RowsBwdWs qk_bwd_ws(int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
@@ -2735,14 +2797,14 @@ size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int3
     });
 }
 
-int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
+static int qk_bwd(const char* fn, const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
                          const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
                          int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
                          int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
                          const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
                          const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
-                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
-                         void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
+                         const int32_t* sections, int32_t dealt, void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
                          int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
                          int32_t interleaved, float eps, void* stream) {
     return guarded([&]() -> int {
@@ -2760,17 +2822,18 @@ int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_
         a.heads[0] = q_heads; a.heads[1] = k_heads;
         a.w_dtype = weight_dtype; a.pos_bytes = position_bytes; a.D = head_dim; a.R = rotary_dim;
         a.interleaved = interleaved != 0; a.eps = eps;
-        const int st = check_qk("qk_norm_rope_bwd", a, dtype, format);
+        int st = check_qk(fn, a, dtype, format);
+        if (!st) st = set_qk_axes(fn, a, axes, sections, dealt);
         if (st) return st;
-        MHC_REQUIRE(tokens == 0 || ((grad_q_out || q_heads == 0) && (grad_k_out || k_heads == 0)),
-                    "qk_norm_rope_bwd: null grad_q_out/grad_k_out");
-        MHC_REQUIRE(tokens == 0 || format >= 0 || ((q || q_heads == 0) && (k || k_heads == 0)),
-                    "qk_norm_rope_bwd: null q/k");
-        MHC_REQUIRE(grad_weight, "qk_norm_rope_bwd: null grad_weight");
+        const std::string f(fn);
+        if (tokens > 0 && ((!grad_q_out && q_heads > 0) || (!grad_k_out && k_heads > 0)))
+            return fail(MHC_ERR_INVALID, f + ": null grad_q_out/grad_k_out");
+        if (tokens > 0 && format < 0 && ((!q && q_heads > 0) || (!k && k_heads > 0)))
+            return fail(MHC_ERR_INVALID, f + ": null q/k");
+        if (!grad_weight) return fail(MHC_ERR_INVALID, f + ": null grad_weight");
         const RowsBwdWs w = qk_bwd_ws(tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved);
         if (!workspace || workspace_bytes < w.total)
-            return fail(MHC_ERR_WORKSPACE,
-                        "qk_norm_rope_bwd: workspace smaller than mhc_qk_norm_rope_bwd_workspace_size()");
+            return fail(MHC_ERR_WORKSPACE, f + ": workspace smaller than mhc_qk_norm_rope_bwd_workspace_size()");
         hipStream_t s = (hipStream_t)stream;
         float* part = (float*)workspace;
         int rows = w.grid;
@@ -2783,6 +2846,67 @@ int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_
         }
         if (e == hipSuccess) e = launch_weight_grad_sum(weight_dtype, part, rows, 2 * (int64_t)head_dim, grad_weight, s);
         return hip_status(e);
+    });
+}
+
+int mhc_qk_norm_rope_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
+                         const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
+                         int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                         int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
+                         const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
+                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period,
+                         void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
+                         int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                         int32_t interleaved, float eps, void* stream) {
+    return qk_bwd("qk_norm_rope_bwd", grad_q_out, gq_token_stride, gq_head_stride, grad_k_out, gk_token_stride,
+                  gk_head_stride, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, dtype, format,
+                  q_values, q_scales, k_values, k_scales, q_weight, k_weight, weight_dtype, cos, sin, table_rows,
+                  positions, position_bytes, position_period, 0, nullptr, 0, grad_q, grad_k, grad_weight,
+                  workspace, workspace_bytes, tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved, eps, stream);
+}
+
+int mhc_qk_norm_rope_axes_bwd(const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
+                              const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
+                              int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                              int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
+                              const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
+                              const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
+                              int64_t table_rows, const void* positions, int32_t position_bytes,
+                              int64_t position_period, int32_t axes, const int32_t* sections, int32_t dealt,
+                              void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
+                              int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
+                              int32_t interleaved, float eps, void* stream) {
+    if (axes == 0) return fail_axes("qk_norm_rope_axes_bwd");
+    return qk_bwd("qk_norm_rope_axes_bwd", grad_q_out, gq_token_stride, gq_head_stride, grad_k_out, gk_token_stride,
+                  gk_head_stride, q, q_token_stride, q_head_stride, k, k_token_stride, k_head_stride, dtype, format,
+                  q_values, q_scales, k_values, k_scales, q_weight, k_weight, weight_dtype, cos, sin, table_rows,
+                  positions, position_bytes, position_period, axes, sections, dealt, grad_q, grad_k, grad_weight,
+                  workspace, workspace_bytes, tokens, q_heads, k_heads, head_dim, rotary_dim, interleaved, eps, stream);
+}
+
+int mhc_qk_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                int64_t k_head_stride, int32_t dtype, const float* cos, const float* sin, int64_t table_rows,
+                const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
+                const int32_t* sections, int32_t dealt, void* q_out, void* k_out, int64_t tokens, int32_t q_heads,
+                int32_t k_heads, int32_t head_dim, int32_t rotary_dim, int32_t interleaved, int32_t inverse,
+                void* stream) {
+    return guarded([&]() -> int {
+        QkArgs a{};
+        a.x[0] = q; a.x_token[0] = q_token_stride; a.x_head[0] = q_head_stride;
+        a.x[1] = k; a.x_token[1] = k_token_stride; a.x_head[1] = k_head_stride;
+        a.y[0] = q_out; a.y[1] = k_out;
+        a.w[0] = a.w[1] = cos;  // no weights
+        a.cos = cos; a.sin = sin; a.pos = positions;
+        a.table_rows = table_rows; a.period = position_period; a.T = tokens;
+        a.heads[0] = q_heads; a.heads[1] = k_heads;
+        a.pos_bytes = position_bytes; a.D = head_dim; a.R = rotary_dim;
+        a.interleaved = interleaved != 0; a.inverse = inverse != 0;
+        int st = check_qk("qk_rope", a, dtype, -1);
+        if (!st) st = set_qk_axes("qk_rope", a, axes, sections, dealt);
+        if (st) return st;
+        MHC_REQUIRE(tokens == 0 || ((q || q_heads == 0) && (k || k_heads == 0)), "qk_rope: null q/k");
+        return hip_status(launch_qk_rope(dtype, a, (hipStream_t)stream));
     });
 }
 

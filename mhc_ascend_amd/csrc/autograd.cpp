@@ -83,7 +83,10 @@ using torch::autograd::tensor_list;
     X(mhc_rmsnorm_residual_bwd)               \
     X(mhc_qk_norm_rope_fwd)                   \
     X(mhc_qk_norm_rope_bwd_workspace_size)    \
-    X(mhc_qk_norm_rope_bwd)
+    X(mhc_qk_norm_rope_bwd)                   \
+    X(mhc_qk_norm_rope_axes_fwd)              \
+    X(mhc_qk_norm_rope_axes_bwd)              \
+    X(mhc_qk_rope)
 
 struct Entries {
 #define MHC_DECLARE(name) decltype(&::name) name = nullptr;
@@ -1097,17 +1100,37 @@ struct QkTables {
     int32_t pos_bytes() const { return pos.defined() ? (int32_t)pos.element_size() : 0; }
 };
 
+// The axes of a call's positions: none named, or the pairs of each.
+struct QkAxes {
+    std::vector<int64_t> sections;
+    bool dealt = false;
+    int32_t host[4] = {0, 0, 0, 0};
+
+    QkAxes(const std::vector<int64_t>& sections_, bool dealt_) : sections(sections_), dealt(dealt_) {
+        for (size_t i = 0; i < sections.size() && i < 4; ++i) host[i] = (int32_t)sections[i];
+    }
+    bool any() const { return !sections.empty(); }
+    int32_t count() const { return (int32_t)sections.size(); }
+    const int32_t* ptr() const { return any() ? host : nullptr; }
+};
+
 // Rows as the kernels read them: storage dtype, channels next to each other.
 Tensor qk_rows(const Tensor& t, at::ScalarType dt) {
     const Tensor s = t.to(dt);
     return s.stride(2) == 1 || s.size(2) == 1 ? s : s.contiguous();
 }
 
+QkAxes saved_axes(AutogradContext* ctx) {
+    const auto it = ctx->saved_data.find("sections");
+    if (it == ctx->saved_data.end()) return QkAxes({}, false);
+    return QkAxes(it->second.toIntVector(), ctx->saved_data["dealt"].toBool());
+}
+
 struct QkNormRope : public torch::autograd::Function<QkNormRope> {
     static tensor_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& wq_in,
                                const Tensor& wk_in, const Tensor& cos, const Tensor& sin,
                                const c10::optional<Tensor>& positions, int64_t period, double eps, bool interleaved,
-                               int64_t fmt) {
+                               int64_t fmt, const QkAxes& axes) {
         const char* fn = "qk_norm_rope_fwd";
         const at::DeviceGuard guard(q_in.device());
         const auto dt = storage_dtype(q_in.scalar_type()) ? q_in.scalar_type() : at::kFloat;
@@ -1121,12 +1144,16 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
             hk = held_alloc(k);
         }
         const auto held = [&](const Tensor& h) { return h.defined() ? h.data_ptr() : nullptr; };
-        check(lib.mhc_qk_norm_rope_fwd(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                                       dtype_code(dt), t.wq.data_ptr(), t.wk.data_ptr(), t.w_dtype(), fp(t.cos),
-                                       fp(t.sin), t.cos.size(0), t.pos_ptr(), t.pos_bytes(), t.period, qo.data_ptr(),
-                                       ko.data_ptr(), (int32_t)fmt, held(hq.values), held(hq.scales),
-                                       held(hk.values), held(hk.scales), T, (int32_t)H, (int32_t)K, (int32_t)D,
-                                       (int32_t)(2 * t.cos.size(1)), interleaved, (float)eps, stream()),
+        const auto run = [&](auto entry, auto... more) {
+            return entry(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                         dtype_code(dt), t.wq.data_ptr(), t.wk.data_ptr(), t.w_dtype(), fp(t.cos), fp(t.sin),
+                         t.cos.size(0), t.pos_ptr(), t.pos_bytes(), t.period, more..., qo.data_ptr(), ko.data_ptr(),
+                         (int32_t)fmt, held(hq.values), held(hq.scales), held(hk.values), held(hk.scales), T,
+                         (int32_t)H, (int32_t)K, (int32_t)D, (int32_t)(2 * t.cos.size(1)), interleaved, (float)eps,
+                         stream());
+        };
+        check(axes.any() ? run(lib.mhc_qk_norm_rope_axes_fwd, axes.count(), axes.ptr(), (int32_t)axes.dealt)
+                         : run(lib.mhc_qk_norm_rope_fwd),
               fn);
         if (!ctx) return {qo, ko};  // no backward will run
         tensor_list sv = {t.wq, t.wk, t.cos, t.sin};
@@ -1142,6 +1169,10 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
                                                        (int64_t)k_in.scalar_type(), (int64_t)wq_in.scalar_type(),
                                                        (int64_t)wk_in.scalar_type()};
         ctx->saved_data["eps"] = eps;
+        if (axes.any()) {
+            ctx->saved_data["sections"] = axes.sections;
+            ctx->saved_data["dealt"] = axes.dealt;
+        }
         return {qo, ko};
     }
 
@@ -1167,19 +1198,72 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
         const Tensor &q = is_held ? none : sv[4], &k = is_held ? none : sv[5];
         const auto at_ptr = [](const Tensor& h) { return h.defined() ? h.data_ptr() : nullptr; };
         const auto st = [](const Tensor& h, int d) { return h.defined() ? h.stride(d) : (int64_t)0; };
-        check(lib.mhc_qk_norm_rope_bwd(
-                  gq.data_ptr(), gq.stride(0), gq.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1), at_ptr(q),
-                  st(q, 0), st(q, 1), at_ptr(k), st(k, 0), st(k, 1), dtype_code(dt), (int32_t)fmt,
-                  is_held ? sv[4].data_ptr() : nullptr, is_held ? sv[6].data_ptr() : nullptr,
-                  is_held ? sv[5].data_ptr() : nullptr, is_held ? sv[7].data_ptr() : nullptr, t.wq.data_ptr(),
-                  t.wk.data_ptr(), t.w_dtype(), fp(t.cos), fp(t.sin), t.cos.size(0), t.pos_ptr(), t.pos_bytes(),
-                  t.period, dq.data_ptr(), dk.data_ptr(), dw.data_ptr(), ws.data_ptr(), wsb, T, (int32_t)H, (int32_t)K,
-                  (int32_t)D, (int32_t)(2 * t.cos.size(1)), (int32_t)v[5],
-                  (float)ctx->saved_data["eps"].toDouble(), stream()),
+        const QkAxes axes = saved_axes(ctx);
+        const auto run = [&](auto entry, auto... more) {
+            return entry(gq.data_ptr(), gq.stride(0), gq.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1),
+                         at_ptr(q), st(q, 0), st(q, 1), at_ptr(k), st(k, 0), st(k, 1), dtype_code(dt), (int32_t)fmt,
+                         is_held ? sv[4].data_ptr() : nullptr, is_held ? sv[6].data_ptr() : nullptr,
+                         is_held ? sv[5].data_ptr() : nullptr, is_held ? sv[7].data_ptr() : nullptr, t.wq.data_ptr(),
+                         t.wk.data_ptr(), t.w_dtype(), fp(t.cos), fp(t.sin), t.cos.size(0), t.pos_ptr(),
+                         t.pos_bytes(), t.period, more..., dq.data_ptr(), dk.data_ptr(), dw.data_ptr(),
+                         ws.data_ptr(), wsb, T, (int32_t)H, (int32_t)K, (int32_t)D, (int32_t)(2 * t.cos.size(1)),
+                         (int32_t)v[5], (float)ctx->saved_data["eps"].toDouble(), stream());
+        };
+        check(axes.any() ? run(lib.mhc_qk_norm_rope_axes_bwd, axes.count(), axes.ptr(), (int32_t)axes.dealt)
+                         : run(lib.mhc_qk_norm_rope_bwd),
               fn);
         tensor_list out = {dq.to((at::ScalarType)v[9]), dk.to((at::ScalarType)v[10]),
                            dw.select(0, 0).to((at::ScalarType)v[11]), dw.select(0, 1).to((at::ScalarType)v[12])};
-        out.resize(11);
+        out.resize(12);
+        return out;
+    }
+};
+
+// The rotation alone: its backward is the rotation by the negative angle.
+struct QkRope : public torch::autograd::Function<QkRope> {
+    static tensor_list run(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& pos,
+                           int64_t period, bool interleaved, const QkAxes& axes, bool inverse) {
+        const int64_t T = q.size(0), H = q.size(1), K = k.size(1), D = q.size(2);
+        Tensor qo = at::empty({T, H, D}, q.options()), ko = at::empty({T, K, D}, k.options());
+        check(lib.mhc_qk_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                              dtype_code(q.scalar_type()), fp(cos), fp(sin), cos.size(0),
+                              pos.defined() ? pos.data_ptr() : nullptr,
+                              pos.defined() ? (int32_t)pos.element_size() : 0, period, axes.count(), axes.ptr(),
+                              (int32_t)axes.dealt, qo.data_ptr(), ko.data_ptr(), T, (int32_t)H, (int32_t)K,
+                              (int32_t)D, (int32_t)(2 * cos.size(1)), interleaved, inverse, stream()),
+              "mhc_qk_rope");
+        return {qo, ko};
+    }
+
+    static tensor_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& cos_in,
+                               const Tensor& sin_in, const c10::optional<Tensor>& positions, int64_t period,
+                               bool interleaved, const QkAxes& axes) {
+        const at::DeviceGuard guard(q_in.device());
+        const auto dt = storage_dtype(q_in.scalar_type()) ? q_in.scalar_type() : at::kFloat;
+        const Tensor cos = f32c(cos_in), sin = f32c(sin_in);
+        const Tensor pos = positions.has_value() ? positions->contiguous() : Tensor();
+        if (ctx) {
+            ctx->save_for_backward({cos, sin, pos});
+            ctx->saved_data["ints"] = std::vector<int64_t>{period, interleaved, (int64_t)dt,
+                                                           (int64_t)q_in.scalar_type(), (int64_t)k_in.scalar_type()};
+            if (axes.any()) {
+                ctx->saved_data["sections"] = axes.sections;
+                ctx->saved_data["dealt"] = axes.dealt;
+            }
+        }
+        return run(qk_rows(q_in, dt), qk_rows(k_in, dt), cos, sin, pos, period, interleaved, axes, false);
+    }
+
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        const auto sv = ctx->get_saved_variables();
+        const auto v = ctx->saved_data["ints"].toIntVector();
+        check_device("qk_rope_bwd", {&grads[0], &grads[1], &sv[0]});
+        const at::DeviceGuard guard(sv[0].device());
+        const auto dt = (at::ScalarType)v[2];
+        const tensor_list d = run(qk_rows(grads[0], dt), qk_rows(grads[1], dt), sv[0], sv[1], sv[2], v[0], v[1] != 0,
+                                  saved_axes(ctx), true);
+        tensor_list out = {d[0].to((at::ScalarType)v[3]), d[1].to((at::ScalarType)v[4])};
+        out.resize(8);
         return out;
     }
 };
@@ -1295,55 +1379,102 @@ Tensor stream_distribute_mix_add(const Tensor& y, const Tensor& h, const Tensor&
     return Distribute::apply(y, h, m, x, format_for(checkpoint, {&y, &h, &m, &x}));
 }
 
+// What the two entries share: q and k as [tokens, heads, D], their leading sizes and
+// the positions' period.
+struct QkCall {
+    Tensor q, k;
+    at::DimVector lead;
+    int64_t period;
+
+    QkCall(const char* fn, const Tensor& q_in, const Tensor& k_in, const Tensor& cos, const Tensor& sin,
+           const c10::optional<Tensor>& positions, const QkAxes& axes, std::initializer_list<const Tensor*> weights) {
+        if (positions.has_value()) check_device(fn, {&q_in, &*positions});
+        const int64_t dims = q_in.dim();
+        TORCH_CHECK((dims == 3 || dims == 4) && k_in.dim() == dims, fn,
+                    ": q and k must both be [tokens, heads, D] or [batch, seq, heads, D], got ", q_in.sizes(), " and ",
+                    k_in.sizes());
+        lead = q_in.sizes().slice(0, dims - 2);
+        TORCH_CHECK(at::IntArrayRef(lead) == k_in.sizes().slice(0, dims - 2) && q_in.size(-1) == k_in.size(-1), fn,
+                    ": q and k must have the same tokens and head_dim, got ", q_in.sizes(), " and ", k_in.sizes());
+        TORCH_CHECK(q_in.scalar_type() == k_in.scalar_type() && at::isFloatingType(q_in.scalar_type()), fn,
+                    ": q and k must have one floating dtype, got ", q_in.scalar_type(), " and ", k_in.scalar_type());
+        const int64_t D = q_in.size(-1);
+        for (const Tensor* w : weights)
+            TORCH_CHECK(w->numel() == D && w->dim() == 1, fn, ": the weights must be [head_dim]");
+        TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), fn,
+                    ": cos and sin must be [positions, rotary_dim / 2]");
+        TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad() && !cos._fw_grad(0).defined() &&
+                        !sin._fw_grad(0).defined(),
+                    fn, ": cos and sin get no gradient");
+        TORCH_CHECK(q_in.size(-2) <= INT32_MAX && k_in.size(-2) <= INT32_MAX && D <= INT32_MAX &&
+                        2 * cos.size(1) <= D,
+                    fn, ": rotary_dim must be at most head_dim, and the sizes 32-bit");
+        if (axes.any()) {
+            int64_t sum = 0;
+            for (const int64_t n : axes.sections) {
+                TORCH_CHECK(n >= 0 && n <= cos.size(1), fn, ": sections must be in 0 .. rotary_dim / 2, got ", n);
+                sum += n;
+            }
+            TORCH_CHECK(axes.count() <= 4 && sum == cos.size(1), fn,
+                        ": sections must name at most 4 axes and add up to rotary_dim / 2 = ", cos.size(1));
+            TORCH_CHECK(positions.has_value(), fn, ": sections need positions");
+        }
+        period = lead.back();
+        if (positions.has_value()) {
+            const auto pt = positions->scalar_type();
+            at::IntArrayRef ps = positions->sizes();
+            if (axes.any()) {
+                TORCH_CHECK(positions->dim() >= 1 && ps[0] == axes.count(), fn, ": positions must be [",
+                            axes.count(), ", ...], one row an axis, got ", ps);
+                ps = ps.slice(1);
+            }
+            TORCH_CHECK(ps == at::IntArrayRef(lead) || ps == at::IntArrayRef(lead).slice(lead.size() - 1), fn,
+                        ": positions must be ", at::IntArrayRef(lead), " or ",
+                        at::IntArrayRef(lead).slice(lead.size() - 1), axes.any() ? " an axis" : "", ", got ", ps);
+            TORCH_CHECK(pt == at::kLong || pt == at::kInt, fn, ": positions must be int64 or int32, got ", pt);
+            period = c10::multiply_integers(ps);
+        }
+        period = std::max<int64_t>(period, 1);
+        q = dims == 4 ? q_in.flatten(0, 1) : q_in;
+        k = dims == 4 ? k_in.flatten(0, 1) : k_in;
+    }
+
+    std::tuple<Tensor, Tensor> shaped(const tensor_list& out) const {
+        if (lead.size() == 1) return {out[0], out[1]};
+        return {out[0].unflatten(0, lead), out[1].unflatten(0, lead)};
+    }
+};
+
 std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, const Tensor& wq, const Tensor& wk,
                                         const Tensor& cos, const Tensor& sin, const c10::optional<Tensor>& positions,
-                                        double eps, bool interleaved, int64_t checkpoint) {
+                                        double eps, bool interleaved, int64_t checkpoint,
+                                        const std::vector<int64_t>& sections, bool dealt) {
     require_bound();
     const char* fn = "qk_norm_rope";
     check_device(fn, {&q_in, &k_in, &wq, &wk, &cos, &sin});
-    if (positions.has_value()) check_device(fn, {&q_in, &*positions});
-    const int64_t dims = q_in.dim();
-    TORCH_CHECK((dims == 3 || dims == 4) && k_in.dim() == dims, fn,
-                ": q and k must both be [tokens, heads, D] or [batch, seq, heads, D], got ", q_in.sizes(), " and ",
-                k_in.sizes());
-    const auto lead = q_in.sizes().slice(0, dims - 2);
-    TORCH_CHECK(lead == k_in.sizes().slice(0, dims - 2) && q_in.size(-1) == k_in.size(-1), fn,
-                ": q and k must have the same tokens and head_dim, got ", q_in.sizes(), " and ", k_in.sizes());
-    TORCH_CHECK(q_in.scalar_type() == k_in.scalar_type() && at::isFloatingType(q_in.scalar_type()), fn,
-                ": q and k must have one floating dtype, got ", q_in.scalar_type(), " and ", k_in.scalar_type());
-    const int64_t D = q_in.size(-1);
-    TORCH_CHECK(wq.numel() == D && wk.numel() == D && wq.dim() == 1 && wk.dim() == 1, fn,
-                ": the weights must be [head_dim]");
-    TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes(), fn, ": cos and sin must be [positions, rotary_dim / 2]");
-    // forward mode runs without grad mode too, and a tangent of a C++ node's input is an error
-    const auto dual = [](std::initializer_list<const Tensor*> ts) {
-        for (const Tensor* t : ts)
-            if (t->_fw_grad(0).defined()) return true;
-        return false;
-    };
-    TORCH_CHECK(!cos.requires_grad() && !sin.requires_grad() && !dual({&cos, &sin}), fn,
-                ": cos and sin get no gradient");
-    TORCH_CHECK(q_in.size(-2) <= INT32_MAX && k_in.size(-2) <= INT32_MAX && D <= INT32_MAX && 2 * cos.size(1) <= D, fn,
-                ": rotary_dim must be at most head_dim, and the sizes 32-bit");
-    int64_t period = lead.back();
-    if (positions.has_value()) {
-        const auto pt = positions->scalar_type();
-        TORCH_CHECK(positions->sizes() == lead || positions->sizes() == lead.slice(lead.size() - 1), fn,
-                    ": positions must be ", lead, " or ", lead.slice(lead.size() - 1), ", got ", positions->sizes());
-        TORCH_CHECK(pt == at::kLong || pt == at::kInt, fn, ": positions must be int64 or int32, got ", pt);
-        period = positions->numel();
-    }
-    const Tensor q = dims == 4 ? q_in.flatten(0, 1) : q_in, k = dims == 4 ? k_in.flatten(0, 1) : k_in;
+    const QkAxes axes(sections, dealt);
+    const QkCall call(fn, q_in, k_in, cos, sin, positions, axes, {&wq, &wk});
+    const Tensor &q = call.q, &k = call.k;
     const int64_t fmt = format_for(checkpoint, {&q, &k, &wq, &wk});
-    const bool node = dual({&q, &k, &wq, &wk}) ||
-                      (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || wq.requires_grad() ||
-                                                      wk.requires_grad()));
-    period = std::max<int64_t>(period, 1);
-    const tensor_list out =
-        node ? QkNormRope::apply(q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt)
-             : QkNormRope::forward(nullptr, q, k, wq, wk, cos, sin, positions, period, eps, interleaved, fmt);
-    if (dims == 3) return {out[0], out[1]};
-    return {out[0].unflatten(0, lead), out[1].unflatten(0, lead)};
+    return call.shaped(needs_node({&q, &k, &wq, &wk})
+                           ? QkNormRope::apply(q, k, wq, wk, cos, sin, positions, call.period, eps, interleaved, fmt,
+                                               axes)
+                           : QkNormRope::forward(nullptr, q, k, wq, wk, cos, sin, positions, call.period, eps,
+                                                 interleaved, fmt, axes));
+}
+
+std::tuple<Tensor, Tensor> qk_rope(const Tensor& q_in, const Tensor& k_in, const Tensor& cos, const Tensor& sin,
+                                   const c10::optional<Tensor>& positions, bool interleaved,
+                                   const std::vector<int64_t>& sections, bool dealt) {
+    require_bound();
+    const char* fn = "qk_rope";
+    check_device(fn, {&q_in, &k_in, &cos, &sin});
+    const QkAxes axes(sections, dealt);
+    const QkCall call(fn, q_in, k_in, cos, sin, positions, axes, {});
+    return call.shaped(needs_node({&call.q, &call.k})
+                           ? QkRope::apply(call.q, call.k, cos, sin, positions, call.period, interleaved, axes)
+                           : QkRope::forward(nullptr, call.q, call.k, cos, sin, positions, call.period, interleaved,
+                                             axes));
 }
 
 Tensor static_layer(const Tensor& x, const Tensor& w, const Tensor& hp, const Tensor& hq, const Tensor& hr,
@@ -1439,5 +1570,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           "y_format) -> [y, h] with autograd, or [values, scales, h]");
     m.def("qk_norm_rope", &qk_norm_rope,
           "(q [..., H, D], k [..., K, D], q_weight, k_weight, cos, sin, positions or None, eps, interleaved, "
-          "checkpoint) -> (q, k) with autograd");
+          "checkpoint, sections, dealt) -> (q, k) with autograd",
+          py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("cos"), py::arg("sin"),
+          py::arg("positions"), py::arg("eps"), py::arg("interleaved"), py::arg("checkpoint"),
+          py::arg("sections") = std::vector<int64_t>{}, py::arg("dealt") = false);
+    m.def("qk_rope", &qk_rope,
+          "(q [..., H, D], k [..., K, D], cos, sin, positions or None, interleaved, sections, dealt) -> (q, k) with "
+          "autograd");
 }

@@ -34,7 +34,7 @@ AUTOGRAD_PATH = os.path.join(PKG, AUTOGRAD_NAME + ".so")
 
 SOURCES = ["abi.hip", "ckpt.hip", "compat.hip", "dynamic.hip", "generic.hip", "layer.hip",
            "layer_ckpt.hip", "ops.hip", "proj_ckpt.hip",
-           "qk_norm_rope.hip", "residual.hip", "sinkhorn.hip", "wide.hip",
+           "qk_axes.hip", "qk_norm_rope.hip", "qk_turn.hip", "residual.hip", "sinkhorn.hip", "wide.hip",
            "wrapper.hip", "wrapper_gen.hip", "wrapper_proj.hip",
            "wrapper_bwd.hip", "wrapper_row.hip"]
 

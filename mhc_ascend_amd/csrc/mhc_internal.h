@@ -395,6 +395,12 @@ struct QkArgs {
     int heads[2];
     int w_dtype, pos_bytes, D, R, interleaved;
     float eps;
+    // Axes of positions [axes][period]: pairs dealt to them in turn, part[] the
+    // pairs of each; or else in blocks, part[] where each ends (INT_MAX from the
+    // last on).  whole: no lane's piece has pairs of two axes.  inverse: the
+    // rotation alone by the negative angle.
+    int axes, dealt, whole, inverse;
+    int part[4];
 };
 // fmt: a CkFormat, or -1 for the rows themselves
 hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t s);
@@ -402,6 +408,11 @@ hipError_t launch_qk_norm_rope_fwd(int dt, int fmt, const QkArgs& a, hipStream_t
 // R and interleaved of `a` alone.
 int qk_norm_rope_bwd_rows(const QkArgs& a);
 hipError_t launch_qk_norm_rope_bwd(int dt, int fmt, const QkArgs& a, float* dw_part, hipStream_t s);
+// ---- qk_axes.hip: the same for axes > 1
+hipError_t launch_qk_axes_fwd(int dt, int fmt, QkArgs a, hipStream_t s);
+hipError_t launch_qk_axes_bwd(int dt, int fmt, QkArgs a, float* dw_part, hipStream_t s);
+// ---- qk_turn.hip: the rotation alone, x[] to y[]
+hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s);
 
 // ---- dynamic.hip -----------------------------------------------------------
 typedef uint16_t bf16_raw_t;

@@ -18,7 +18,7 @@ PyTorch reference math, which is the contract):
 from __future__ import annotations
 
 import operator
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -472,19 +472,62 @@ def rmsnorm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
 # counterpart in the reference)
 # =============================================================================
 
-def rope_table(length: int, rotary_dim: int, base: float = 10000.0, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
+def _sections(fn: str, sections, rotary_dim: int, dealt: bool) -> list:
+    """The pairs of each axis of a ``sections`` argument, checked; [] for None."""
+    if sections is None:
+        if dealt:
+            raise ValueError(f"{fn}: sections_dealt needs sections")
+        return []
+    sizes = [operator.index(n) for n in sections]
+    half = rotary_dim // 2
+    if not 1 <= len(sizes) <= 4 or min(sizes) < 0 or sum(sizes) != half:
+        raise ValueError(f"{fn}: sections must name 1 to 4 axes and add up to rotary_dim / 2 = {half}, got {sizes}")
+    if dealt and any(n and a + len(sizes) * (n - 1) >= half for a, n in enumerate(sizes) if a):
+        raise ValueError(f"{fn}: sections {sizes} cannot be dealt in turn: past the last pair")
+    return sizes
+
+
+def rope_table(length: int, rotary_dim: int, base: float = 10000.0, device=None,
+               sections: Optional[Sequence[int]] = None,
+               sections_dealt: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """cos and sin, fp32 [length, rotary_dim / 2], of the angles
-    position * base**(-2 p / rotary_dim), formed in 64 bits."""
+    position * base**(-2 p / rotary_dim), formed in 64 bits.
+
+    With ``sections`` (and ``sections_dealt``, as :func:`qk_rope` takes them) the
+    pairs of each axis have frequencies of their own: the i-th of an axis with s
+    of them turns by position * base**(-i / s).  Without, the axes share one
+    table: pair p has the frequency above on whichever axis it is."""
     if length < 1 or rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rope_table: length must be >= 1 and rotary_dim even and >= 2")
-    p = torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64)
-    angle = torch.arange(length, device=device, dtype=torch.float64).unsqueeze(1) * base ** (-p / rotary_dim)
+    sizes = _sections("rope_table", sections, rotary_dim, sections_dealt)
+    if sizes:
+        power = [0.0] * (rotary_dim // 2)
+        for a, pairs in enumerate(_axis_pairs(sizes, sections_dealt)):
+            for i, p in enumerate(pairs):
+                power[p] = -i / sizes[a]
+        p = torch.tensor(power, device=device, dtype=torch.float64)
+    else:
+        p = -torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64) / rotary_dim
+    angle = torch.arange(length, device=device, dtype=torch.float64).unsqueeze(1) * base ** p
     return angle.cos().float(), angle.sin().float()
+
+
+def _axis_pairs(sizes: list, dealt: bool) -> list:
+    """The pairs of each axis, in order."""
+    n, half = len(sizes), sum(sizes)
+    if not dealt:
+        ends = [sum(sizes[:a + 1]) for a in range(n)]
+        return [list(range(e - s, e)) for e, s in zip(ends, sizes)]
+    rest = [list(range(a, half, n))[:sizes[a]] for a in range(n)]
+    taken = {p for a in range(1, n) for p in rest[a]}
+    return [[p for p in range(half) if p not in taken]] + rest[1:]
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
                  cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None, eps: float = 1e-5,
-                 interleaved: bool = False, checkpoint: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                 interleaved: bool = False, checkpoint: Optional[str] = None,
+                 sections: Optional[Sequence[int]] = None,
+                 sections_dealt: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """RMSNorm of every head of q and k, then the rotation of its token's
     position, in one pass (no counterpart in the reference).
 
@@ -502,10 +545,43 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
     the table makes its rows NaN.  The outputs are contiguous, in q's dtype
     (fp32 or bf16; others become fp32); cos and sin get no gradient.
 
+    ``sections`` gives a token positions on several axes, as :func:`qk_rope`
+    describes.
+
     ``checkpoint`` ("int8" or "e4m3", see :func:`activation_pack`) saves q and
     k in 8 bits for the backward, which is then the gradient at the values that
     checkpoint stands for."""
     code = _checkpoint_code(checkpoint)
     _not_traced("qk_norm_rope")
+    sizes = _qk_sections("qk_norm_rope", sections, sections_dealt, cos)
     return _lib.autograd().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved),
-                                        code)
+                                        code, sizes, bool(sections_dealt))
+
+
+def _qk_sections(fn: str, sections, dealt, cos: torch.Tensor) -> list:
+    if sections is None and not dealt:
+        return []
+    if cos.dim() != 2:
+        raise ValueError(f"{fn}: cos and sin must be [positions, rotary_dim / 2]")
+    return _sections(fn, sections, 2 * cos.shape[1], dealt)
+
+
+def qk_rope(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+            positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+            sections: Optional[Sequence[int]] = None,
+            sections_dealt: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rotation of q's and k's heads by their tokens' positions alone: q, k,
+    cos, sin, ``positions`` and ``interleaved`` are :func:`qk_norm_rope`'s.  Its
+    backward is the rotation by the negative angle; no rows are saved.
+
+    ``sections`` gives every token positions on 1 to 4 axes (time, height and
+    width of video, say): ``positions`` is then [axes, ...], the axes' positions
+    as above one after the other, and pair p turns by column p of the table row
+    of its own axis's position.  sections[a] pairs belong to axis a, together
+    R/2: consecutive ones, axis 0's first; or, with ``sections_dealt``, dealt to
+    the axes in turn (pair p to axis p % axes) until an axis has its number, after
+    which its turns go to axis 0.  A position outside the table on any axis makes
+    its token's rows NaN."""
+    _not_traced("qk_rope")
+    sizes = _qk_sections("qk_rope", sections, sections_dealt, cos)
+    return _lib.autograd().qk_rope(q, k, cos, sin, positions, bool(interleaved), sizes, bool(sections_dealt))
