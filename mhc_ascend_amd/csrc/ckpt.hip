@@ -204,61 +204,6 @@ hipError_t launch_ckpt_unpack(int dt, int fmt, const void* values, const void* s
     return e;
 }
 
-// A piece that a row of C >= 8 ends in is read as the row's last 8 elements;
-// this moves its own, 8 - m of them on (m = 1 .. 7), to the front, zeros behind.
-__device__ __forceinline__ void ck_shift_part(int m, float (&v)[8]) {
-    const int by = 8 - m;
-#pragma unroll
-    for (int s = 4; s >= 1; s >>= 1) {
-        const bool on = (by & s) != 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = on ? (e + s < 8 ? v[e + s] : 0.f) : v[e];
-    }
-}
-
-// ---------------------------------------------------------------------------
-// RMSNorm rows in registers: VPT pieces of 8 channels a lane (piece q = k *
-// blockDim.x + tid), so any row of up to 512 * 8 * 4 channels fits.  RAG: the
-// row does not end with a piece.
-// ---------------------------------------------------------------------------
-template <typename T, int VPT, bool RAG>
-__device__ __forceinline__ void ck_row_get(const T* __restrict__ row, int C, const CkPiece<T> (&in)[VPT],
-                                           float (&v)[VPT][8]) {
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        in[k].get(v[k]);
-        if (RAG && c0 < C && c0 + 8 > C) {
-            if (C >= 8) ck_shift_part(C - c0, v[k]);
-            else ck_load_part(row, C, v[k]);
-        }
-        if (c0 >= C) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
-        }
-    }
-}
-// Pieces that lie in the row whole, the row's last 8 elements where it ends
-// inside one, and its first for lanes past it (a row under 8: nothing).
-template <typename T, int VPT, bool RAG>
-__device__ __forceinline__ void ck_row_load(const T* __restrict__ row, int C, CkPiece<T> (&in)[VPT]) {
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        if (!RAG || C >= 8) in[k].load(row + (c0 + 8 <= C ? c0 : (RAG && c0 < C ? C - 8 : 0)));
-        else in[k] = CkPiece<T>{};
-    }
-}
-template <typename T, int VPT, bool RAG>
-__device__ __forceinline__ void ck_row_put(T* __restrict__ row, int C, const float (&v)[VPT][8]) {
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
-        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        if (c0 + 8 <= C) ck_store8(row + c0, v[k]);
-        else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v[k]);
-    }
-}
-
 // Persistent workgroups over rows, the weight in registers and the next row's
 // loads in flight.  Bound by its bytes: 16384 x 4096 bf16 in 64 us, 5.3 TB/s
 // (forward and backward 130 us, 155 with one workgroup a row).
@@ -391,36 +336,12 @@ __global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_kernel(const T* __restri
 // for 63, 65536 x 512 bf16 75 for 86, 30000 x 500 fp32 78 for 88; 1000 x 400 bf16
 // 17 for 17).  Bound by bytes from 256 channels on.
 // ---------------------------------------------------------------------------
-constexpr int kCkNarrow = 512;
-
-template <typename T, bool RAG>
-struct CkNarrow {
-    int c0, C;
-    __device__ __forceinline__ CkNarrow(int C_, int lg) : C(C_) { c0 = (threadIdx.x & ((1 << lg) - 1)) * 8; }
-    __device__ __forceinline__ bool in() const { return c0 < C; }
-    template <typename U>
-    __device__ __forceinline__ void load(const U* __restrict__ row, CkPiece<U>& p) const {
-        if (!RAG || C >= 8) p.load(row + (c0 + 8 <= C ? c0 : (RAG && c0 < C ? C - 8 : 0)));
-        else p = CkPiece<U>{};
-    }
-    template <typename U>
-    __device__ __forceinline__ void get(const U* __restrict__ row, const CkPiece<U>& p, float (&v)[8]) const {
-        p.get(v);
-        if (RAG && c0 < C && c0 + 8 > C) {
-            if (C >= 8) ck_shift_part(C - c0, v);
-            else ck_load_part(row, C, v);
-        }
-        if (c0 >= C) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        }
-    }
-    __device__ __forceinline__ void put(T* __restrict__ row, const float (&v)[8]) const {
-        if (c0 + 8 <= C) ck_store8(row + c0, v);
-        else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v);
-    }
-};
-
+// ---------------------------------------------------------------------------
+// Narrow rows, several a wave (CkNarrow).  Forward and backward, against a
+// workgroup a row: 35334 x 104 bf16 23 us for 44, 65536 x 256 bf16 45 for 63,
+// 65536 x 512 bf16 75 for 86, 30000 x 500 fp32 78 for 88; 1000 x 400 bf16 17 for
+// 17.  Bound by bytes from 256 channels on.
+// ---------------------------------------------------------------------------
 template <typename T, int FMT, bool RAG>
 __global__ __launch_bounds__(256) void rmsnorm_ckpt_fwd_narrow_kernel(const T* __restrict__ x,
                                                                       const float* __restrict__ w, T* __restrict__ y,
@@ -576,23 +497,6 @@ hipError_t launch_weight_grad_sum(int w_dtype, const float* part, int rows, int6
         MHC_LAUNCH_GGL((weight_grad_sum_kernel<float>), grid, dim3(1024), 0, s, part, rows, (int)cols, (float*)dw);
     }
     return hipGetLastError();
-}
-
-struct CkRowTiling {
-    int vpt, threads;
-};
-// The fewest pieces a lane that a 512-lane workgroup covers the row with.
-static CkRowTiling ck_row_tiling(int64_t C) {
-    const int64_t pieces = (C + 7) / 8;
-    const int vpt = pieces <= 512 ? 1 : (pieces <= 1024 ? 2 : 4);
-    return CkRowTiling{vpt, (int)(((pieces + vpt - 1) / vpt + 63) / 64 * 64)};
-}
-
-// log2 of the lanes a narrow row takes: 4 (a block of 32) to 64
-static int ck_narrow_lg(int64_t C) {
-    int lg = 2;
-    while ((8 << lg) < C) ++lg;
-    return lg;
 }
 
 bool rmsnorm_ckpt_supported(int64_t C) { return C >= 1 && C <= kCkMaxRow; }

@@ -201,4 +201,110 @@ __device__ __forceinline__ void ck_unpack8(uint2 w, uint32_t s, float (&v)[8]) {
     }
 }
 
+// A piece that a row of C >= 8 ends in is read as the row's last 8 elements;
+// this moves its own, 8 - m of them on (m = 1 .. 7), to the front, zeros behind.
+__device__ __forceinline__ void ck_shift_part(int m, float (&v)[8]) {
+    const int by = 8 - m;
+#pragma unroll
+    for (int s = 4; s >= 1; s >>= 1) {
+        const bool on = (by & s) != 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = on ? (e + s < 8 ? v[e + s] : 0.f) : v[e];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows in registers: VPT pieces of 8 channels a lane (piece q = k *
+// blockDim.x + tid), so any row of up to 512 * 8 * 4 channels fits.  RAG: the
+// row does not end with a piece.
+// ---------------------------------------------------------------------------
+template <typename T, int VPT, bool RAG>
+__device__ __forceinline__ void ck_row_get(const T* __restrict__ row, int C, const CkPiece<T> (&in)[VPT],
+                                           float (&v)[VPT][8]) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
+        in[k].get(v[k]);
+        if (RAG && c0 < C && c0 + 8 > C) {
+            if (C >= 8) ck_shift_part(C - c0, v[k]);
+            else ck_load_part(row, C, v[k]);
+        }
+        if (c0 >= C) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+        }
+    }
+}
+// Pieces that lie in the row whole, the row's last 8 elements where it ends
+// inside one, and its first for lanes past it (a row under 8: nothing).
+template <typename T, int VPT, bool RAG>
+__device__ __forceinline__ void ck_row_load(const T* __restrict__ row, int C, CkPiece<T> (&in)[VPT]) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
+        if (!RAG || C >= 8) in[k].load(row + (c0 + 8 <= C ? c0 : (RAG && c0 < C ? C - 8 : 0)));
+        else in[k] = CkPiece<T>{};
+    }
+}
+template <typename T, int VPT, bool RAG>
+__device__ __forceinline__ void ck_row_put(T* __restrict__ row, int C, const float (&v)[VPT][8]) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
+        if (c0 + 8 <= C) ck_store8(row + c0, v[k]);
+        else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v[k]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Narrow rows, C <= 512: a group of 2^lg lanes a row, 8 channels a lane, so a
+// wave takes 64 >> lg rows at once and sums without LDS.
+// ---------------------------------------------------------------------------
+constexpr int kCkNarrow = 512;
+
+template <typename T, bool RAG>
+struct CkNarrow {
+    int c0, C;
+    __device__ __forceinline__ CkNarrow(int C_, int lg) : C(C_) { c0 = (threadIdx.x & ((1 << lg) - 1)) * 8; }
+    __device__ __forceinline__ bool in() const { return c0 < C; }
+    template <typename U>
+    __device__ __forceinline__ void load(const U* __restrict__ row, CkPiece<U>& p) const {
+        if (!RAG || C >= 8) p.load(row + (c0 + 8 <= C ? c0 : (RAG && c0 < C ? C - 8 : 0)));
+        else p = CkPiece<U>{};
+    }
+    template <typename U>
+    __device__ __forceinline__ void get(const U* __restrict__ row, const CkPiece<U>& p, float (&v)[8]) const {
+        p.get(v);
+        if (RAG && c0 < C && c0 + 8 > C) {
+            if (C >= 8) ck_shift_part(C - c0, v);
+            else ck_load_part(row, C, v);
+        }
+        if (c0 >= C) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        }
+    }
+    __device__ __forceinline__ void put(T* __restrict__ row, const float (&v)[8]) const {
+        if (c0 + 8 <= C) ck_store8(row + c0, v);
+        else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v);
+    }
+};
+
+struct CkRowTiling {
+    int vpt, threads;
+};
+// The fewest pieces a lane that a 512-lane workgroup covers the row with.
+inline CkRowTiling ck_row_tiling(int64_t C) {
+    const int64_t pieces = (C + 7) / 8;
+    const int vpt = pieces <= 512 ? 1 : (pieces <= 1024 ? 2 : 4);
+    return CkRowTiling{vpt, (int)(((pieces + vpt - 1) / vpt + 63) / 64 * 64)};
+}
+
+// log2 of the lanes a narrow row takes: 4 (a block of 32) to 64
+inline int ck_narrow_lg(int64_t C) {
+    int lg = 2;
+    while ((8 << lg) < C) ++lg;
+    return lg;
+}
+
 }  // namespace mhc

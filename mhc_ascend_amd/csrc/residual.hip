@@ -256,6 +256,352 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_bwd_any_kernel(Residu
     }
 }
 
+// ---------------------------------------------------------------------------
+// Rows in registers (mhc_ckpt.h), up to kCkMaxRow channels: persistent
+// workgroups, the weight in registers and the next row's loads in flight, so
+// that every array is read or written once.
+// ---------------------------------------------------------------------------
+template <int VPT, bool RAG>
+__device__ __forceinline__ void res_weights(const ResidualArgs& a, float (&w)[VPT][8]) {
+    if (a.w_dtype == kBF16) {
+        CkPiece<bf16_t> p[VPT];
+        ck_row_load<bf16_t, VPT, RAG>(static_cast<const bf16_t*>(a.w), a.C, p);
+        ck_row_get<bf16_t, VPT, RAG>(static_cast<const bf16_t*>(a.w), a.C, p, w);
+    } else {
+        CkPiece<float> p[VPT];
+        ck_row_load<float, VPT, RAG>(static_cast<const float*>(a.w), a.C, p);
+        ck_row_get<float, VPT, RAG>(static_cast<const float*>(a.w), a.C, p, w);
+    }
+}
+
+template <typename TX, typename TR, int VPT, bool RAG>
+__global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
+    __shared__ float red[16];
+    const DropKey key(a.drop);
+    const int C = a.C;
+    const int64_t per = (C + 7) / 8;
+    const TX* x = static_cast<const TX*>(a.x);
+    const TR* res = static_cast<const TR*>(a.residual);
+    CkPiece<TX> xn[VPT];
+    CkPiece<TR> rn[VPT];
+    int64_t b = blockIdx.x;
+    ck_row_load<TX, VPT, RAG>(x + b * C, C, xn);
+    ck_row_load<TR, VPT, RAG>(res + b * C, C, rn);
+    float w[VPT][8];
+    res_weights<VPT, RAG>(a, w);
+    for (; b < a.B; b += gridDim.x) {
+        float v[VPT][8];
+        float t[1] = {0.f};
+        {
+            float r[VPT][8];
+            ck_row_get<TX, VPT, RAG>(x + b * C, C, xn, v);
+            ck_row_get<TR, VPT, RAG>(res + b * C, C, rn, r);
+            const int64_t b1 = b + gridDim.x < a.B ? b + gridDim.x : b;
+            ck_row_load<TX, VPT, RAG>(x + b1 * C, C, xn);
+            ck_row_load<TR, VPT, RAG>(res + b1 * C, C, rn);
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                if (a.drop.threshold) key.apply(a.drop, (uint64_t)(b * per + k * blockDim.x + threadIdx.x), v[k]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] += r[k][e];
+                res_round<TR>(v[k]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[0] += v[k][e] * v[k][e];
+            }
+        }
+        ck_row_put<TR, VPT, RAG>(static_cast<TR*>(a.h) + b * C, C, v);
+        if (a.h_fmt >= 0) {
+#pragma unroll
+            for (int k = 0; k < VPT; ++k)
+                res_pack(a.h_fmt, v[k], a.hq, a.hsc, b, C, (k * blockDim.x + threadIdx.x) * 8);
+        }
+        block_sum<1>(t, red);
+        const float inv = 1.f / sqrtf(t[0] / (float)C + a.eps);
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * inv * w[k][e];
+        }
+        if (a.y_fmt >= 0) {
+#pragma unroll
+            for (int k = 0; k < VPT; ++k)
+                res_pack(a.y_fmt, v[k], a.yq, a.ysc, b, C, (k * blockDim.x + threadIdx.x) * 8);
+        } else {
+            ck_row_put<TX, VPT, RAG>(static_cast<TX*>(a.y) + b * C, C, v);
+        }
+    }
+}
+
+// HELD: h from its checkpoint.  dw in registers, one partial row a workgroup.  With
+// two pieces a lane a workgroup of 1024 has no registers left for the weight and
+// the next row: those rows load when they are needed.
+template <typename TX, typename TR, int VPT, bool RAG, bool HELD>
+__global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a) {
+    __shared__ float red[32];
+    constexpr bool kAhead = VPT == 1;
+    const DropKey key(a.drop);
+    const int C = a.C, nb = (int)ck_blocks(C), stride = (int)ck_stride(C);
+    const int64_t per = (C + 7) / 8;
+    const TX* gy = static_cast<const TX*>(a.gy);
+    const TR* gh = static_cast<const TR*>(a.gh);
+    const TR* h = static_cast<const TR*>(a.h);
+    float w[VPT][8], dw[VPT][8];
+    if (kAhead) res_weights<VPT, RAG>(a, w);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dw[k][e] = 0.f;
+    }
+    CkPiece<TX> gn[VPT];
+    CkPiece<TR> dn[VPT], hn[VPT];
+    uint2 qn[VPT];
+    uint32_t sn[VPT];
+    const auto load = [&](int64_t b) {
+        ck_row_load<TX, VPT, RAG>(gy + b * C, C, gn);
+        if (gh) ck_row_load<TR, VPT, RAG>(gh + b * C, C, dn);
+        if constexpr (HELD) {
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                int c0 = (k * blockDim.x + threadIdx.x) * 8;
+                c0 = c0 < C ? c0 : 0;
+                qn[k] = ld8_nt(a.hq + b * stride + c0);
+                sn[k] = a.hsc[b * nb + (c0 >> 5)];
+            }
+        } else {
+            ck_row_load<TR, VPT, RAG>(h + b * C, C, hn);
+        }
+    };
+    int64_t b = blockIdx.x;
+    if (kAhead) load(b);
+    for (; b < a.B; b += gridDim.x) {
+        if (!kAhead) {
+            load(b);
+            res_weights<VPT, RAG>(a, w);
+        }
+        float hv[VPT][8], g[VPT][8], d[VPT][8];
+        ck_row_get<TX, VPT, RAG>(gy + b * C, C, gn, g);
+        if constexpr (HELD) {
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+                if (a.h_fmt == kCkInt8) ck_unpack8<kCkInt8>(qn[k], sn[k], hv[k]);
+                else ck_unpack8<kCkE4M3>(qn[k], sn[k], hv[k]);
+                if ((k * blockDim.x + threadIdx.x) * 8 >= C) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) hv[k][e] = 0.f;
+                }
+            }
+        } else {
+            ck_row_get<TR, VPT, RAG>(h + b * C, C, hn, hv);
+        }
+        if (gh) {
+            ck_row_get<TR, VPT, RAG>(gh + b * C, C, dn, d);
+        } else {
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[k][e] = 0.f;
+            }
+        }
+        if (kAhead) load(b + gridDim.x < a.B ? b + gridDim.x : b);
+        float t[2] = {0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                t[0] += hv[k][e] * hv[k][e];
+                t[1] += g[k][e] * w[k][e] * hv[k][e];
+            }
+        }
+        block_sum<2>(t, red);
+        const float inv = 1.f / sqrtf(t[0] / (float)C + a.eps);
+        const float k2 = t[1] * inv * inv * inv / (float)C;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                dw[k][e] += g[k][e] * hv[k][e] * inv;
+                d[k][e] += w[k][e] * g[k][e] * inv - hv[k][e] * k2;
+            }
+        }
+        if (a.gres) ck_row_put<TR, VPT, RAG>(static_cast<TR*>(a.gres) + b * C, C, d);
+        if (a.gx) {
+            if (a.drop.threshold) {
+#pragma unroll
+                for (int k = 0; k < VPT; ++k)
+                    key.apply(a.drop, (uint64_t)(b * per + k * blockDim.x + threadIdx.x), d[k]);
+            }
+            ck_row_put<TX, VPT, RAG>(static_cast<TX*>(a.gx) + b * C, C, d);
+        }
+    }
+    if (a.dw_part) ck_row_put<float, VPT, RAG>(a.dw_part + (int64_t)blockIdx.x * C, C, dw);
+}
+
+// ---------------------------------------------------------------------------
+// Narrow rows, several a wave (CkNarrow of mhc_ckpt.h): no LDS in the sums.
+// ---------------------------------------------------------------------------
+template <bool RAG>
+__device__ __forceinline__ void res_narrow_weight(const ResidualArgs& a, const CkNarrow<float, RAG>& ln,
+                                                  float (&w)[8]) {
+    if (a.w_dtype == kBF16) {
+        CkPiece<bf16_t> p;
+        ln.load(static_cast<const bf16_t*>(a.w), p);
+        ln.get(static_cast<const bf16_t*>(a.w), p, w);
+    } else {
+        CkPiece<float> p;
+        ln.load(static_cast<const float*>(a.w), p);
+        ln.get(static_cast<const float*>(a.w), p, w);
+    }
+}
+
+template <typename TX, typename TR, bool RAG>
+__global__ __launch_bounds__(256) void residual_fwd_narrow_kernel(ResidualArgs a, int lg) {
+    const DropKey key(a.drop);
+    const int C = a.C;
+    const CkNarrow<float, RAG> ln(C, lg);
+    const CkNarrow<TX, RAG> lx(C, lg);
+    const CkNarrow<TR, RAG> lr(C, lg);
+    const int64_t per = (C + 7) / 8;
+    const int lane = threadIdx.x & 63, rows = 64 >> lg, sub = lane >> lg;
+    const int nb = (int)ck_blocks(C), stride = (int)ck_stride(C);
+    float w[8];
+    res_narrow_weight<RAG>(a, ln, w);
+    const TX* x = static_cast<const TX*>(a.x);
+    const TR* res = static_cast<const TR*>(a.residual);
+    const int64_t step = (int64_t)gridDim.x * 4 * rows;
+    int64_t b0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * rows;  // the wave's first row
+    const auto at = [&](int64_t b) { return b + sub < a.B ? b + sub : a.B - 1; };
+    const auto pack = [&](int fmt, const float (&v)[8], uint8_t* q, uint8_t* sc, int64_t row, bool on) {
+        uint2 p;
+        const uint32_t s = fmt == kCkInt8 ? ck_pack8<kCkInt8>(v, p) : ck_pack8<kCkE4M3>(v, p);
+        if (on && ln.c0 < stride) st8_nt(q + row * stride + ln.c0, p);
+        if (on && ln.in() && (lane & 3) == 0) sc[row * nb + (ln.c0 >> 5)] = (uint8_t)s;
+    };
+    CkPiece<TX> xn;
+    CkPiece<TR> rn;
+    ln.load(x + at(b0) * C, xn);
+    ln.load(res + at(b0) * C, rn);
+    for (; b0 < a.B; b0 += step) {
+        const bool on = b0 + sub < a.B;
+        const int64_t b = at(b0);
+        float v[8], r[8];
+        ln.get(x + b * C, xn, v);
+        ln.get(res + b * C, rn, r);
+        const int64_t b1 = at(b0 + step);
+        ln.load(x + b1 * C, xn);
+        ln.load(res + b1 * C, rn);
+        if (a.drop.threshold) key.apply(a.drop, (uint64_t)(b * per + (ln.c0 >> 3)), v);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[e];
+        res_round<TR>(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+        if (on) lr.put(static_cast<TR*>(a.h) + b * C, v);
+        if (a.h_fmt >= 0) pack(a.h_fmt, v, a.hq, a.hsc, b, on);
+        ss = lane_group_sum(ss, lg);
+        const float inv = 1.f / sqrtf(ss / (float)C + a.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * w[e];
+        if (a.y_fmt >= 0) pack(a.y_fmt, v, a.yq, a.ysc, b, on);
+        else if (on) lx.put(static_cast<TX*>(a.y) + b * C, v);
+    }
+}
+
+template <typename TX, typename TR, bool RAG, bool HELD>
+__global__ __launch_bounds__(512) void residual_bwd_narrow_kernel(ResidualArgs a, int lg) {
+    __shared__ float red[8 * kCkNarrow];
+    const DropKey key(a.drop);
+    const int C = a.C;
+    const CkNarrow<float, RAG> ln(C, lg);
+    const CkNarrow<TX, RAG> lx(C, lg);
+    const CkNarrow<TR, RAG> lr(C, lg);
+    const int64_t per = (C + 7) / 8;
+    const int nb = (int)ck_blocks(C), stride = (int)ck_stride(C);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = 64 >> lg, sub = lane >> lg;
+    const TX* gy = static_cast<const TX*>(a.gy);
+    const TR* gh = static_cast<const TR*>(a.gh);
+    const TR* h = static_cast<const TR*>(a.h);
+    float w[8], dw[8];
+    res_narrow_weight<RAG>(a, ln, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dw[e] = 0.f;
+    const int64_t step = (int64_t)gridDim.x * 8 * rows;
+    int64_t b0 = ((int64_t)blockIdx.x * 8 + wave) * rows;
+    const auto at = [&](int64_t b) { return b + sub < a.B ? b + sub : a.B - 1; };
+    CkPiece<TX> gn;
+    CkPiece<TR> dn, hn;
+    uint2 qn;
+    uint32_t sn;
+    const auto load = [&](int64_t row) {
+        ln.load(gy + row * C, gn);
+        if (gh) ln.load(gh + row * C, dn);
+        if constexpr (HELD) {
+            const int c0 = ln.in() ? ln.c0 : 0;
+            qn = ld8_nt(a.hq + row * stride + c0);
+            sn = a.hsc[row * nb + (c0 >> 5)];
+        } else {
+            ln.load(h + row * C, hn);
+        }
+    };
+    load(at(b0));
+    for (; b0 < a.B; b0 += step) {
+        const bool on = b0 + sub < a.B;
+        const int64_t b = at(b0);
+        float hv[8], g[8], d[8];
+        ln.get(gy + b * C, gn, g);
+        if constexpr (HELD) {
+            if (a.h_fmt == kCkInt8) ck_unpack8<kCkInt8>(qn, sn, hv);
+            else ck_unpack8<kCkE4M3>(qn, sn, hv);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hv[e] = ln.in() ? hv[e] : 0.f;
+        } else {
+            ln.get(h + b * C, hn, hv);
+        }
+        if (gh) {
+            ln.get(gh + b * C, dn, d);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = 0.f;
+        }
+        load(at(b0 + step));
+        float ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ss += hv[e] * hv[e];
+            dot += g[e] * w[e] * hv[e];
+        }
+        ss = lane_group_sum(ss, lg);
+        dot = lane_group_sum(dot, lg);
+        const float inv = 1.f / sqrtf(ss / (float)C + a.eps);
+        const float k2 = dot * inv * inv * inv / (float)C;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            dw[e] += on ? g[e] * hv[e] * inv : 0.f;
+            d[e] += w[e] * g[e] * inv - hv[e] * k2;
+        }
+        if (a.gres && on) lr.put(static_cast<TR*>(a.gres) + b * C, d);
+        if (a.gx) {
+            if (a.drop.threshold) key.apply(a.drop, (uint64_t)(b * per + (ln.c0 >> 3)), d);
+            if (on) lx.put(static_cast<TX*>(a.gx) + b * C, d);
+        }
+    }
+    if (!a.dw_part) return;  // the whole grid
+    // the wave's groups, the workgroup's waves
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v = dw[e];
+        for (int k = 1 << lg; k < 64; k <<= 1) v += __shfl_xor(v, k);
+        if (sub == 0 && ln.c0 + e < C) red[wave * C + ln.c0 + e] = v;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < C; i += 512) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v += red[k * C + i];
+        a.dw_part[(int64_t)blockIdx.x * C + i] = v;
+    }
+}
+
 #define MHC_RES_TYPED(x_dt, r_dt, ...)                                                        \
     do {                                                                                      \
         auto typed = [&](auto x_, auto r_) {                                                  \
@@ -269,27 +615,108 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_bwd_any_kernel(Residu
         else typed(float{}, float{});                                                         \
     } while (0)
 
+// Calls f(integral_constant of the pieces a lane, true_type where rows end inside a piece).
+template <typename F>
+static void res_rows(int vpt, bool rag, F f) {
+    const auto go = [&](auto v) {
+        if (rag) f(v, std::true_type{});
+        else f(v, std::false_type{});
+    };
+    if (vpt == 1) go(std::integral_constant<int, 1>{});
+    else go(std::integral_constant<int, 2>{});
+}
+// The fewest pieces a lane that a workgroup of `most` lanes covers the row with, or
+// two a lane of more.
+static CkRowTiling res_tiling(int64_t C, int most) {
+    const int64_t pieces = (C + 7) / 8;
+    const int vpt = pieces <= most ? 1 : 2;
+    return CkRowTiling{vpt, (int)(((pieces + vpt - 1) / vpt + 63) / 64 * 64)};
+}
+constexpr int kResFwdLanes = 512, kResBwdLanes = 1024;
+template <typename F>
+static void res_flag(bool on, F f) {
+    if (on) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+static unsigned res_grid(const void* fn, int threads, int64_t most) {
+    const int64_t g = (int64_t)device_cu_count() * occupancy_per_cu(fn, threads, 0);
+    return (unsigned)(g < most ? g : most);
+}
+
 hipError_t launch_rmsnorm_residual_fwd(int x_dt, int r_dt, const ResidualArgs& a, hipStream_t s) {
     if (a.B == 0) return hipSuccess;
+    const CkRowTiling t = res_tiling(a.C, kResFwdLanes);
+    const bool rag = a.C % 8 != 0;
     const int tok = timing_begin("rmsnorm_residual_fwd", s);
-    const int64_t most = 2 * (int64_t)device_cu_count();
-    MHC_RES_TYPED(x_dt, r_dt,
-                  MHC_LAUNCH_GGL((residual_fwd_any_kernel<X_, R_>), dim3((unsigned)(a.B < most ? a.B : most)),
-                                 dim3(kResAnyThreads), 0, s, a));
+    MHC_RES_TYPED(x_dt, r_dt, {
+        if (a.C > kCkMaxRow) {
+            const int64_t most = 2 * (int64_t)device_cu_count();
+            MHC_LAUNCH_GGL((residual_fwd_any_kernel<X_, R_>), dim3((unsigned)(a.B < most ? a.B : most)),
+                           dim3(kResAnyThreads), 0, s, a);
+        } else if (a.C <= kCkNarrow) {
+            const int lg = ck_narrow_lg(a.C);
+            const int64_t each = 4 * (64 >> lg);
+            res_flag(rag, [&](auto g) {
+                constexpr bool G_ = decltype(g)::value;
+                const void* fn = reinterpret_cast<const void*>(&residual_fwd_narrow_kernel<X_, R_, G_>);
+                MHC_LAUNCH_GGL((residual_fwd_narrow_kernel<X_, R_, G_>),
+                               dim3(res_grid(fn, 256, (a.B + each - 1) / each)), dim3(256), 0, s, a, lg);
+            });
+        } else {
+            res_rows(t.vpt, rag, [&](auto v, auto g) {
+                constexpr int V_ = decltype(v)::value;
+                constexpr bool G_ = decltype(g)::value;
+                const void* fn = reinterpret_cast<const void*>(&residual_fwd_kernel<X_, R_, V_, G_>);
+                MHC_LAUNCH_GGL((residual_fwd_kernel<X_, R_, V_, G_>), dim3(res_grid(fn, t.threads, a.B)),
+                               dim3(t.threads), 0, s, a);
+            });
+        }
+    });
     timing_end(tok, s);
     return hipGetLastError();
 }
 
 int rmsnorm_residual_bwd_grid(int x_dt, int r_dt, int64_t B, int64_t C) {
-    const int64_t most = 2 * (int64_t)device_cu_count();
-    return (int)(B < 1 ? 1 : (B < most ? B : most));
+    const int64_t cus = device_cu_count();
+    int64_t g = 2 * cus, most = B;
+    if (C <= kCkNarrow) {
+        const int64_t each = 8 * (64 >> ck_narrow_lg(C));
+        most = (B + each - 1) / each;
+    } else if (C <= kCkMaxRow) {
+        // as many workgroups as 1024 lanes a CU, where each has 16 rows: a partial
+        // row of dw costs as many bytes as a row (two a CU at least)
+        const int threads = res_tiling(C, kResBwdLanes).threads;
+        int64_t per_cu = B / (16 * cus);
+        if (per_cu > 1024 / threads) per_cu = 1024 / threads;
+        if (per_cu > 2) g = per_cu * cus;
+    }
+    return (int)(g < most ? g : (most < 1 ? 1 : most));
 }
 
 hipError_t launch_rmsnorm_residual_bwd(int x_dt, int r_dt, const ResidualArgs& a, int grid, hipStream_t s) {
     if (a.B == 0) return hipSuccess;
+    const CkRowTiling t = res_tiling(a.C, kResBwdLanes);
+    const bool rag = a.C % 8 != 0;
     const int tok = timing_begin("rmsnorm_residual_bwd", s);
-    MHC_RES_TYPED(x_dt, r_dt,
-                  MHC_LAUNCH_GGL((residual_bwd_any_kernel<X_, R_>), dim3(grid), dim3(kResAnyThreads), 0, s, a));
+    MHC_RES_TYPED(x_dt, r_dt, {
+        res_flag(a.h_fmt >= 0, [&](auto held) {
+            constexpr bool H_ = decltype(held)::value;
+            if (a.C > kCkMaxRow) {
+                MHC_LAUNCH_GGL((residual_bwd_any_kernel<X_, R_>), dim3(grid), dim3(kResAnyThreads), 0, s, a);
+            } else if (a.C <= kCkNarrow) {
+                res_flag(rag, [&](auto g) {
+                    MHC_LAUNCH_GGL((residual_bwd_narrow_kernel<X_, R_, decltype(g)::value, H_>), dim3(grid), dim3(512),
+                                   0, s, a, ck_narrow_lg(a.C));
+                });
+            } else {
+                res_rows(t.vpt, rag, [&](auto v, auto g) {
+                    MHC_LAUNCH_GGL((residual_bwd_kernel<X_, R_, decltype(v)::value, decltype(g)::value, H_>),
+                                   dim3(grid), dim3(t.threads), 0, s, a);
+                });
+            }
+        });
+    });
     timing_end(tok, s);
     return hipGetLastError();
 }
