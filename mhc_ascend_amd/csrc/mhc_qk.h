@@ -55,6 +55,21 @@ __device__ __forceinline__ int qk_axis(const QkArgs& a, int col) {
     return (col >= a.part[0] ? 1 : 0) + (col >= a.part[1] ? 1 : 0) + (col >= a.part[2] ? 1 : 0);
 }
 
+// The axes of N consecutive pairs from `col` on (pairs past the last: any), two
+// bits each.  Opaque to the compiler, which otherwise keeps every select of a
+// token loop in registers (qk_bwd_kernel: 156 of them for 109, half the waves).
+template <int N>
+__device__ __forceinline__ uint32_t qk_axes_of(const QkArgs& a, int col) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) m |= (uint32_t)qk_axis(a, col + e) << (2 * e);
+    return m;
+}
+__device__ __forceinline__ uint32_t qk_opaque(uint32_t m) {
+    asm volatile("" : "+v"(m));
+    return m;
+}
+
 // Where a token's table rows begin: one, or one an axis.
 template <bool AX> struct QkAt;
 template <> struct QkAt<false> {
@@ -64,6 +79,7 @@ template <> struct QkAt<false> {
         at = (pos < 0 ? 0 : pos) * (int64_t)(a.R >> 1);
     }
     __device__ __forceinline__ bool ok() const { return pos >= 0; }
+    __device__ __forceinline__ int64_t on(uint32_t) const { return at; }
     __device__ __forceinline__ int64_t of(const QkArgs&, int) const { return at; }
 };
 template <> struct QkAt<true> {
@@ -83,7 +99,8 @@ template <> struct QkAt<true> {
         }
     }
     __device__ __forceinline__ bool ok() const { return good; }
-    __device__ __forceinline__ int64_t on(int axis) const {
+    // the low two bits of `axis`
+    __device__ __forceinline__ int64_t on(uint32_t axis) const {
         const int64_t lo = axis & 1 ? at[1] : at[0], hi = axis & 1 ? at[3] : at[2];
         return axis & 2 ? hi : lo;
     }
@@ -286,13 +303,16 @@ __device__ __forceinline__ void qk_store(T* p, const float (&v)[V]) {
 // One lane's place in its head row.
 template <int V, bool IL>
 struct QkLane {
+    static constexpr int kTab = IL ? V / 2 : V;
     int c0;       // its first channel
     bool in;      // within the head
     bool turned;  // some channel of the piece rotates
     int other;    // first channel of its partners' piece (its own where it has none)
     float sign;   // of the partner's sine product
+    uint32_t ax;  // the axes of its table entries (with AX)
 
-    __device__ __forceinline__ QkLane(const QkArgs& a, int lane, int lg) {
+    template <bool AX>
+    __device__ __forceinline__ QkLane(const QkArgs& a, int lane, int lg, std::bool_constant<AX>) {
         c0 = (lane & ((1 << lg) - 1)) * V;
         in = c0 < a.D;
         turned = c0 < a.R;
@@ -303,31 +323,38 @@ struct QkLane {
             other = c0 < half ? c0 + half : c0 - half;
             sign = c0 < half ? -1.f : 1.f;
         }
+        ax = AX ? qk_axes_of<kTab>(a, first_pair(a)) : 0u;
+    }
+    // The pair of its first table entry.
+    __device__ __forceinline__ int first_pair(const QkArgs& a) const {
+        if (IL) return c0 >> 1;
+        const int half = a.R >> 1;
+        return turned ? (c0 < half ? c0 : c0 - half) : 0;
     }
 
     // The lane's table entries of a token: per channel with halves (the sine
     // with its sign), per pair interleaved.  1 and 0 elsewhere.  With axes, a
     // piece whose pairs are of one axis (a.whole) is read whole, others pair by
     // pair: their loads are in flight together, and hit the caches.
-    static constexpr int kTab = IL ? V / 2 : V;
     template <bool AX>
     __device__ __forceinline__ void table(const QkArgs& a, const QkAt<AX>& row, float (&c)[kTab],
                                           float (&s)[kTab]) const {
         const int half = a.R >> 1;
+        const uint32_t m = AX ? qk_opaque(ax) : 0u;
         if constexpr (IL) {
 #pragma unroll
             for (int p = 0; p < kTab; ++p) {
                 const int col = (c0 >> 1) + p;
                 const bool on = col < half;
-                const int64_t at = row.of(a, on ? col : 0);
+                const int64_t at = row.on(m >> (2 * p));
                 c[p] = on ? a.cos[at + col] : 1.f;
                 s[p] = on ? a.sin[at + col] : 0.f;
             }
         } else {
-            const int col = turned ? (c0 < half ? c0 : c0 - half) : 0;
+            const int col = first_pair(a);
             float pc[V], ps[V];
             if (!AX || a.whole) {
-                const int64_t at = row.of(a, col) + col;
+                const int64_t at = row.on(m) + col;
                 QkPiece<float, V> qc, qs;
                 qc.load(a.cos + at);
                 qs.load(a.sin + at);
@@ -339,7 +366,7 @@ struct QkLane {
             } else {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const int64_t at = row.of(a, col + e) + col + e;
+                    const int64_t at = row.on(m >> (2 * e)) + col + e;
                     pc[e] = a.cos[at];
                     ps[e] = a.sin[at];
                 }
@@ -413,7 +440,7 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg, int tw) {
     if (!MT) tw = 0;
     int64_t t = a.t0 + (((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) << tw);
     if (t >= a.T) return;
-    const QkLane<V, IL> ln(a, lane, lg);
+    const QkLane<V, IL> ln(a, lane, lg, std::bool_constant<AX>{});
     const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
     const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
     bool here = true;
@@ -499,7 +526,7 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, f
     extern __shared__ float red[];  // [8 waves][2][D]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (!MT) tw = 0;
-    const QkLane<V, IL> ln(a, lane, lg);
+    const QkLane<V, IL> ln(a, lane, lg, std::bool_constant<AX>{});
     const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
     const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
     const int stride = (int)ck_stride(a.D), nb = (int)ck_blocks(a.D);

@@ -49,8 +49,10 @@ struct QkUnit {
     int c[2];      // its pieces' first channels
     bool in[2];    // within the head
     bool turned;   // some channel of the unit rotates
+    uint32_t ax;   // the axes of its pairs (with AX)
 
-    __device__ __forceinline__ QkUnit(const QkArgs& a, int lane, int lg) {
+    template <bool AX>
+    __device__ __forceinline__ QkUnit(const QkArgs& a, int lane, int lg, std::bool_constant<AX>) {
         const int u = lane & ((1 << lg) - 1);
         if constexpr (IL) {
             c[0] = 2 * u * V;
@@ -64,6 +66,7 @@ struct QkUnit {
         }
         in[0] = c[0] < a.D;
         in[1] = c[1] < a.D;
+        ax = AX ? qk_axes_of<V>(a, turned ? (IL ? c[0] >> 1 : c[0]) : 0) : 0u;
     }
 
     // The entries of the unit's V pairs: with halves pair c[0] + e, interleaved
@@ -72,9 +75,10 @@ struct QkUnit {
     __device__ __forceinline__ void table(const QkArgs& a, const QkAt<AX>& row, float way, float (&cs)[V],
                                           float (&sn)[V]) const {
         const int half = a.R >> 1, col = IL ? c[0] >> 1 : c[0];
+        const uint32_t m = AX ? qk_opaque(ax) : 0u;
         if ((!IL || a.R % (2 * V) == 0) && (!AX || a.whole)) {
             const int first = turned ? col : 0;
-            const int64_t at = row.of(a, first) + first;
+            const int64_t at = row.on(m) + first;
             QkPiece<float, V> qc, qs;
             qc.load(a.cos + at);
             qs.load(a.sin + at);
@@ -87,7 +91,7 @@ struct QkUnit {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const int p = turned && col + e < half ? col + e : 0;
-                const int64_t at = row.of(a, p) + p;
+                const int64_t at = row.on(m >> (2 * e)) + p;
                 cs[e] = a.cos[at];
                 sn[e] = way * a.sin[at];
             }
@@ -126,14 +130,15 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, int lg, int tw) 
     const int lane = threadIdx.x & 63;
     int64_t t = a.t0 + (((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) << tw);
     if (t >= a.T) return;
-    const QkUnit<V, IL> un(a, lane, lg);
+    const QkUnit<V, IL> un(a, lane, lg, std::bool_constant<AX>{});
     const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
     const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
     t += lane >> (6 - tw);
     const bool here = t < a.T;
     t = here ? t : a.T - 1;
+    using Piece = std::conditional_t<V == 8, CkPiece<T>, QkPiece<T, V>>;
     struct Rows {
-        QkPiece<T, V> p[kQkU][2];
+        Piece p[kQkU][2];
     };
     const auto side = [&](int j) { return j < tasks.nq ? 0 : 1; };
     const auto first = [&](int j, int s) { return (s ? j - tasks.nq : j) * tasks.per + sub; };
@@ -164,8 +169,12 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, int lg, int tw) 
             float v[2][V];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
+                if constexpr (V == 8) {
+                    rows.p[u][k].get(v[k]);
+                } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[k][e] = rows.p[u][k].get(e);
+                    for (int e = 0; e < V; ++e) v[k][e] = rows.p[u][k].get(e);
+                }
             }
             un.turn(a, cs, sn, v, at.ok());
             if (here && h < a.heads[s]) {
