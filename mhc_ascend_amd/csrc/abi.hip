@@ -2698,13 +2698,15 @@ static int set_qk_axes(const char* fn, QkArgs& a, int32_t axes, const int32_t* s
     if (sum != a.R / 2) return fail(MHC_ERR_INVALID, f + ": the sections must add up to rotary_dim / 2");
     a.axes = axes;
     a.dealt = dealt != 0;
+    a.deal_mul = (65536u + (uint32_t)axes - 1u) / (uint32_t)axes;
     int end = 0;
     for (int i = 0; i < 4; ++i) {
         const int n = i < axes ? sections[i] : 0;
         if (a.dealt && i > 0 && n > 0 && i + (int64_t)axes * (n - 1) >= a.R / 2)
             return fail(MHC_ERR_INVALID, f + ": a section is too long to be dealt in turn");
         end += n;
-        a.part[i] = a.dealt ? n : (i < axes - 1 ? end : INT32_MAX);
+        a.part[i] = i < axes - 1 ? end : INT32_MAX;
+        a.deal_sizes |= (uint64_t)n << (16 * i);  // at most kQkMaxDim / 2 pairs
     }
     return MHC_SUCCESS;
 }

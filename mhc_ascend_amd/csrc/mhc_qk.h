@@ -40,17 +40,13 @@ __device__ __forceinline__ int64_t qk_position(const QkArgs& a, int64_t t) {
     return p >= 0 && p < a.table_rows ? p : -1;
 }
 
-// Entry i of positions, which has the element size pos_bytes.
-__device__ __forceinline__ int64_t qk_entry(const QkArgs& a, int64_t i) {
-    return a.pos_bytes == 8 ? static_cast<const int64_t*>(a.pos)[i] : static_cast<const int32_t*>(a.pos)[i];
-}
-
-// The axis of a pair.
+// The axis of a pair; the sizes in one word and the division by a product keep
+// the argument's memory and a long division out of the kernels' first loads.
 __device__ __forceinline__ int qk_axis(const QkArgs& a, int col) {
     if (a.dealt) {
-        const int turn = col / a.axes, axis = col - turn * a.axes;
-        const int n = axis == 1 ? a.part[1] : (axis == 2 ? a.part[2] : a.part[3]);
-        return turn < n ? axis : 0;  // what is not dealt belongs to axis 0
+        const uint32_t turn = ((uint32_t)col * a.deal_mul) >> 16, axis = (uint32_t)col - turn * (uint32_t)a.axes;
+        // what is not dealt belongs to axis 0
+        return turn < ((uint32_t)(a.deal_sizes >> (16 * axis)) & 0xffffu) ? (int)axis : 0;
     }
     return (col >= a.part[0] ? 1 : 0) + (col >= a.part[1] ? 1 : 0) + (col >= a.part[2] ? 1 : 0);
 }
@@ -61,8 +57,13 @@ __device__ __forceinline__ int qk_axis(const QkArgs& a, int col) {
 template <int N>
 __device__ __forceinline__ uint32_t qk_axes_of(const QkArgs& a, int col) {
     uint32_t m = 0;
+    if (a.dealt) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) m |= (uint32_t)qk_axis(a, col + e) << (2 * e);
+        for (int e = 0; e < N; ++e) m |= (uint32_t)qk_axis(a, col + e) << (2 * e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) m |= (uint32_t)qk_axis(a, col + e) << (2 * e);
+    }
     return m;
 }
 __device__ __forceinline__ uint32_t qk_opaque(uint32_t m) {
@@ -70,11 +71,30 @@ __device__ __forceinline__ uint32_t qk_opaque(uint32_t m) {
     return m;
 }
 
+// A token's positions on its way from memory: loaded (before the rows, which the
+// table's loads would wait for otherwise), then checked.  Two words each, without
+// a branch on the element size.
+template <bool AX> struct QkRaw {
+    __device__ __forceinline__ QkRaw(const QkArgs&, int64_t) {}
+};
+template <> struct QkRaw<true> {
+    uint32_t lo[4], hi[4];
+    __device__ __forceinline__ QkRaw(const QkArgs& a, int64_t t) {
+        const uint32_t i = (uint32_t)t % (uint32_t)a.period;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const char* p = static_cast<const char*>(a.pos) + ((s < a.axes ? s : 0) * a.period + i) * a.pos_bytes;
+            lo[s] = *reinterpret_cast<const uint32_t*>(p);
+            hi[s] = *reinterpret_cast<const uint32_t*>(p + a.pos_bytes - 4);
+        }
+    }
+};
+
 // Where a token's table rows begin: one, or one an axis.
 template <bool AX> struct QkAt;
 template <> struct QkAt<false> {
     int64_t pos, at;
-    __device__ __forceinline__ QkAt(const QkArgs& a, int64_t t) {
+    __device__ __forceinline__ QkAt(const QkArgs& a, int64_t t, const QkRaw<false>&) {
         pos = qk_position(a, t);
         at = (pos < 0 ? 0 : pos) * (int64_t)(a.R >> 1);
     }
@@ -85,17 +105,15 @@ template <> struct QkAt<false> {
 template <> struct QkAt<true> {
     int64_t at[4];
     bool good;
-    __device__ __forceinline__ QkAt(const QkArgs& a, int64_t t) {
-        const uint32_t i = (uint32_t)t % (uint32_t)a.period;
-        int64_t p[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) p[s] = qk_entry(a, (s < a.axes ? s : 0) * a.period + i);
+    __device__ __forceinline__ QkAt(const QkArgs& a, int64_t, const QkRaw<true>& raw) {
         good = true;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            const bool in = p[s] >= 0 && p[s] < a.table_rows;
+            const uint32_t hi = a.pos_bytes == 8 ? raw.hi[s] : (uint32_t)((int32_t)raw.lo[s] >> 31);
+            const int64_t p = (int64_t)((uint64_t)hi << 32 | raw.lo[s]);
+            const bool in = p >= 0 && p < a.table_rows;
             good = good && in;
-            at[s] = (in ? p[s] : 0) * (int64_t)(a.R >> 1);
+            at[s] = (in ? p : 0) * (int64_t)(a.R >> 1);
         }
     }
     __device__ __forceinline__ bool ok() const { return good; }
@@ -146,7 +164,7 @@ __global__ __launch_bounds__(256) void qk_fwd_any_kernel(QkArgs a) {
     const T* x = static_cast<const T*>(a.x[s]) + t * a.x_token[s] + h * a.x_head[s];
     const int64_t row = t * a.heads[s] + h;
     T* y = static_cast<T*>(a.y[s]) + row * a.D;
-    const QkAt<AX> at(a, t);
+    const QkAt<AX> at(a, t, QkRaw<AX>(a, t));
     float ss = 0.f;
     const int dmax = (a.D + 63) & ~63;
     for (int d = lane; d < dmax; d += 64) {
@@ -188,7 +206,7 @@ __global__ __launch_bounds__(256) void qk_bwd_any_kernel(QkArgs a, float* __rest
     for (int i = threadIdx.x; i < 8 * a.D; i += 256) dw[i] = 0.f;
     __syncthreads();
     for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) {
-        const QkAt<AX> at(a, t);
+        const QkAt<AX> at(a, t, QkRaw<AX>(a, t));
         for (int hh = wave; hh < a.heads[0] + a.heads[1]; hh += 4) {
             const int s = hh < a.heads[0] ? 0 : 1;
             const int h = s ? hh - a.heads[0] : hh;
@@ -370,6 +388,7 @@ struct QkLane {
                     pc[e] = a.cos[at];
                     ps[e] = a.sin[at];
                 }
+                __builtin_amdgcn_sched_barrier(0);  // all loads, then their uses
             }
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -457,9 +476,10 @@ __global__ __launch_bounds__(256) void qk_fwd_kernel(QkArgs a, int lg, int tw) {
         r.load(ln, static_cast<const T*>(a.x[s]) + t * a.x_token[s], a.x_head[s], first(j, s), step, a.heads[s]);
     };
     int j = blockIdx.y;
+    const QkRaw<AX> raw(a, t);
     QkRows<T, V, IL> next;
     fetch(j, next);  // the grid's y is at most the number of tasks
-    const QkAt<AX> at(a, t);
+    const QkAt<AX> at(a, t, raw);
     float c[QkLane<V, IL>::kTab], sn[QkLane<V, IL>::kTab];
     ln.table(a, at, c, sn);
     float w[V], wo[V];
@@ -541,7 +561,7 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, f
             here = t < a.T;
             t = here ? t : a.T - 1;
         }
-        const QkAt<AX> at(a, t);
+        const QkAt<AX> at(a, t, QkRaw<AX>(a, t));
         float c[QkLane<V, IL>::kTab], sn[QkLane<V, IL>::kTab];
         ln.table(a, at, c, sn);
         for (int j = blockIdx.y; j < tasks.n; j += gridDim.y) {

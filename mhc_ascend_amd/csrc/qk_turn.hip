@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
     const int h = s ? hh - a.heads[0] : hh;
     const T* x = static_cast<const T*>(a.x[s]) + t * a.x_token[s] + h * a.x_head[s];
     T* y = static_cast<T*>(a.y[s]) + (t * a.heads[s] + h) * a.D;
-    const QkAt<AX> at(a, t);
+    const QkAt<AX> at(a, t, QkRaw<AX>(a, t));
     const float way = a.inverse ? -1.f : 1.f;
     for (int d = lane; d < a.D; d += 64) {
         float o = VecIO<T>::scalar(x + d);
@@ -93,8 +93,11 @@ struct QkUnit {
                 const int p = turned && col + e < half ? col + e : 0;
                 const int64_t at = row.on(m >> (2 * e)) + p;
                 cs[e] = a.cos[at];
-                sn[e] = way * a.sin[at];
+                sn[e] = a.sin[at];
             }
+            __builtin_amdgcn_sched_barrier(0);  // all loads, then their uses
+#pragma unroll
+            for (int e = 0; e < V; ++e) sn[e] *= way;
         }
     }
 
@@ -154,9 +157,10 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, int lg, int tw) 
         }
     };
     int j = blockIdx.y;
+    const QkRaw<AX> raw(a, t);
     Rows next;
     fetch(j, next);  // the grid's y is at most the number of tasks
-    const QkAt<AX> at(a, t);
+    const QkAt<AX> at(a, t, raw);
     float cs[V], sn[V];
     un.table(a, at, a.inverse ? -1.f : 1.f, cs, sn);
     for (; j < tasks.n; j += gridDim.y) {
