@@ -146,16 +146,25 @@ template <> struct CkPiece<bf16_t> {
     }
 };
 
+// NT: data that nothing will read soon.
+template <bool NT = true>
 __device__ __forceinline__ void ck_store8(float* p, const float (&v)[8]) {
     const ck_u4_t a = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
     const ck_u4_t b = {__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
-    __builtin_nontemporal_store(a, reinterpret_cast<ck_u4_a4_t*>(p));
-    __builtin_nontemporal_store(b, reinterpret_cast<ck_u4_a4_t*>(p + 4));
+    if constexpr (NT) {
+        __builtin_nontemporal_store(a, reinterpret_cast<ck_u4_a4_t*>(p));
+        __builtin_nontemporal_store(b, reinterpret_cast<ck_u4_a4_t*>(p + 4));
+    } else {
+        *reinterpret_cast<ck_u4_a4_t*>(p) = a;
+        *reinterpret_cast<ck_u4_a4_t*>(p + 4) = b;
+    }
 }
+template <bool NT = true>
 __device__ __forceinline__ void ck_store8(bf16_t* p, const float (&v)[8]) {
     const ck_u4_t a = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
                        pack_bf16x2(v[6], v[7])};
-    __builtin_nontemporal_store(a, reinterpret_cast<ck_u4_a2_t*>(p));
+    if constexpr (NT) __builtin_nontemporal_store(a, reinterpret_cast<ck_u4_a2_t*>(p));
+    else *reinterpret_cast<ck_u4_a2_t*>(p) = a;
 }
 
 // The same for the first `m` (0 .. 7) of 8 elements.
@@ -246,12 +255,12 @@ __device__ __forceinline__ void ck_row_load(const T* __restrict__ row, int C, Ck
         else in[k] = CkPiece<T>{};
     }
 }
-template <typename T, int VPT, bool RAG>
+template <typename T, int VPT, bool RAG, bool NT = true>
 __device__ __forceinline__ void ck_row_put(T* __restrict__ row, int C, const float (&v)[VPT][8]) {
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int c0 = (k * blockDim.x + threadIdx.x) * 8;
-        if (c0 + 8 <= C) ck_store8(row + c0, v[k]);
+        if (c0 + 8 <= C) ck_store8<NT>(row + c0, v[k]);
         else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v[k]);
     }
 }
@@ -284,8 +293,9 @@ struct CkNarrow {
             for (int e = 0; e < 8; ++e) v[e] = 0.f;
         }
     }
+    template <bool NT = true>
     __device__ __forceinline__ void put(T* __restrict__ row, const float (&v)[8]) const {
-        if (c0 + 8 <= C) ck_store8(row + c0, v);
+        if (c0 + 8 <= C) ck_store8<NT>(row + c0, v);
         else if (RAG && c0 < C) ck_store_part(row + c0, C - c0, v);
     }
 };
