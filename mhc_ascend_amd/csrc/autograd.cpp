@@ -223,6 +223,17 @@ Held held_alloc(const Tensor& x) {
             at::empty({(int64_t)lib.mhc_checkpoint_scales_size(rows, (int32_t)C)}, opt)};
 }
 
+// The same in the shapes that a caller sees: [..., ceil16(C)] and [..., ceil(C / 32)].
+Held packed_alloc(const Tensor& x) {
+    const auto opt = x.options().dtype(at::kByte);
+    at::DimVector shape(x.sizes());
+    const int64_t C = shape.back();
+    shape.back() = (C + 15) / 16 * 16;
+    Tensor values = at::empty(shape, opt);
+    shape.back() = (C + 31) / 32;
+    return {values, at::empty(shape, opt)};
+}
+
 // x contiguous, in storage dtype
 Held hold(const Tensor& x, int64_t fmt) {
     Held h = held_alloc(x);
@@ -1010,7 +1021,7 @@ struct RmsNormResidual : public torch::autograd::Function<RmsNormResidual> {
         const int64_t C = x.size(-1), B = rows_of(x);
         Tensor h = at::empty_like(res), y;
         Held hy, hh;
-        if (y_fmt != MHC_CHECKPOINT_NONE) hy = held_alloc(x);
+        if (y_fmt != MHC_CHECKPOINT_NONE) hy = packed_alloc(x);
         else y = at::empty_like(x);
         if (fmt != MHC_CHECKPOINT_NONE) hh = held_alloc(res);
         const auto at_ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
@@ -1303,17 +1314,8 @@ tensor_list rmsnorm_residual(const Tensor& x, const Tensor& residual, const Tens
                 ": no gradient flows through an output in 8 bits (call it under torch.no_grad())");
     const int64_t fmt = format_for(checkpoint, {&x, &residual, &w});
     const Drop d = make_drop(fn, x, p, seed, value, offset);
-    tensor_list out = node ? RmsNormResidual::apply(x, residual, w, eps, d, fmt, y_fmt)
-                           : RmsNormResidual::forward(nullptr, x, residual, w, eps, d, fmt, y_fmt);
-    if (y_fmt != MHC_CHECKPOINT_NONE) {
-        auto shape = x.sizes().vec();
-        const int64_t C = shape.back();
-        shape.back() = (C + 15) / 16 * 16;
-        out[0] = out[0].view(shape);
-        shape.back() = (C + 31) / 32;
-        out[1] = out[1].view(shape);
-    }
-    return out;
+    return node ? RmsNormResidual::apply(x, residual, w, eps, d, fmt, y_fmt)
+                : RmsNormResidual::forward(nullptr, x, residual, w, eps, d, fmt, y_fmt);
 }
 
 // (values, scales) of x [..., C]: uint8 [..., ceil16(C)] and [..., ceil(C / 32)]

@@ -478,12 +478,14 @@ def _sections(fn: str, sections, rotary_dim: int, dealt: bool) -> list:
         if dealt:
             raise ValueError(f"{fn}: sections_dealt needs sections")
         return []
-    sizes = [operator.index(n) for n in sections]
-    half = rotary_dim // 2
-    if not 1 <= len(sizes) <= 4 or min(sizes) < 0 or sum(sizes) != half:
+    sizes = list(map(operator.index, sections))
+    n, half = len(sizes), rotary_dim // 2
+    if not 1 <= n <= 4 or min(sizes) < 0 or sum(sizes) != half:
         raise ValueError(f"{fn}: sections must name 1 to 4 axes and add up to rotary_dim / 2 = {half}, got {sizes}")
-    if dealt and any(n and a + len(sizes) * (n - 1) >= half for a, n in enumerate(sizes) if a):
-        raise ValueError(f"{fn}: sections {sizes} cannot be dealt in turn: past the last pair")
+    if dealt:
+        for a in range(1, n):
+            if sizes[a] and a + n * (sizes[a] - 1) >= half:
+                raise ValueError(f"{fn}: sections {sizes} cannot be dealt in turn: past the last pair")
     return sizes
 
 
