@@ -550,6 +550,7 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, f
     const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
     const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
     const int stride = (int)ck_stride(a.D), nb = (int)ck_blocks(a.D);
+    const bool ragged = a.D != V << lg;
     float dw[2][V];
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[0][e] = dw[1][e] = 0.f;
@@ -601,8 +602,8 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, f
                 float v[V], z[V], o[V], d[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    z[e] = on ? gown[u].get(e) : 0.f;
-                    o[e] = IL || !on ? 0.f : gfar[u].get(e);
+                    z[e] = gown[u].get(e);
+                    o[e] = IL ? 0.f : gfar[u].get(e);
                 }
                 if constexpr (FMT >= 0) {
 #pragma unroll
@@ -610,11 +611,19 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, f
                         float f[4];
                         Ck<FMT>::unpack4(q[u][e / 4], Ck<FMT>::down(sc[u]), f);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) v[e + k] = on ? f[k] : 0.f;
+                        for (int k = 0; k < 4; ++k) v[e + k] = f[k];
                     }
                 } else {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[e] = on ? xr[u].get(e) : 0.f;
+                    for (int e = 0; e < V; ++e) v[e] = xr[u].get(e);
+                }
+                if (ragged) {  // lanes past the head add nothing to its sums
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        z[e] = ln.in ? z[e] : 0.f;
+                        o[e] = ln.in ? o[e] : 0.f;
+                        v[e] = ln.in ? v[e] : 0.f;
+                    }
                 }
                 float ss = 0.f, dot = 0.f;
 #pragma unroll
@@ -631,8 +640,8 @@ __global__ __launch_bounds__(512) void qk_bwd_kernel(QkArgs a, int lg, int tw, f
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float p = on ? d[e] * v[e] * inv : 0.f;  // a head past the last adds nothing (inv may be infinite)
-                    dw[0][e] += s == 0 ? p : 0.f;
-                    dw[1][e] += s == 0 ? 0.f : p;
+                    if (s == 0) dw[0][e] += p;
+                    else dw[1][e] += p;
                     d[e] = w[e] * d[e] * inv - v[e] * k2;
                 }
                 if (on) qk_store<T, V>(static_cast<T*>(a.y[s]) + (t * a.heads[s] + h) * a.D + ln.c0, d);

@@ -3,13 +3,15 @@
 //   (a, b) -> (a c - b s, b c + a s)  for the pairs of the first R channels;
 // pairs, tables, axes and positions outside the table as in mhc_qk.h.  Channels
 // past R stay.
+#include <algorithm>
+
 #include "mhc_qk.h"
 
 namespace mhc {
 
 // ---------------------------------------------------------------------------
 // Any head size, stride and alignment: one wave a head row, one channel a lane.
-// For heads that qk_turn_tiling finds no pieces for.
+// For heads that qk_turn_plan finds no pieces for.
 // ---------------------------------------------------------------------------
 template <typename T, bool AX>
 __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
@@ -40,20 +42,31 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
 // halves a piece of the first half and its partner of the second, interleaved two
 // neighbouring pieces, and past R two pieces that stay.  So every channel is read
 // once, no value crosses lanes, and the V table entries of the unit stay in
-// registers for all heads of the token.  A group of 2^lg lanes takes a head, a
-// wave 64 >> lg heads of a token (or of 2^tw tokens where heads are few) at a
-// time, U such steps in flight.
+// registers for all heads of the token.  Nothing is summed over a head, so its
+// lanes are as many as its units: a wave holds 64 / units heads, shared by as many
+// tokens as leave the fewest steps a token.  A task is U steps of one side, its
+// loads in flight together with the next task's.  Few tokens: their tasks are
+// spread over the grid's y.
+// Lanes and steps with nothing of their own repeat another's work, store included:
+// without branches around the stores the loads are waited for one by one.
 // ---------------------------------------------------------------------------
+// How a wave is shared: units a head, heads a token takes at once, tokens, tasks of
+// the queries and of both; mul = ceil(2^16 / n) divides a lane or slot (under 64)
+// by n exactly.  odd: the last unit's second piece is past the head.
+struct QkTurnPlan {
+    int v, u, units, heads, tokens, nq, n, odd;
+    uint32_t units_mul, heads_mul;
+};
+
 template <int V, bool IL>
 struct QkUnit {
     int c[2];      // its pieces' first channels
-    bool in[2];    // within the head
+    bool two;      // the second piece is within the head (or else the first again)
     bool turned;   // some channel of the unit rotates
     uint32_t ax;   // the axes of its pairs (with AX)
 
     template <bool AX>
-    __device__ __forceinline__ QkUnit(const QkArgs& a, int lane, int lg, std::bool_constant<AX>) {
-        const int u = lane & ((1 << lg) - 1);
+    __device__ __forceinline__ QkUnit(const QkArgs& a, int u, std::bool_constant<AX>) {
         if constexpr (IL) {
             c[0] = 2 * u * V;
             c[1] = c[0] + V;
@@ -64,8 +77,8 @@ struct QkUnit {
             c[0] = turned ? u * V : a.R + 2 * (u - n) * V;
             c[1] = turned ? c[0] + half : c[0] + V;
         }
-        in[0] = c[0] < a.D;
-        in[1] = c[1] < a.D;
+        two = c[1] < a.D;
+        if (!two) c[1] = c[0];
         ax = AX ? qk_axes_of<V>(a, turned ? (IL ? c[0] >> 1 : c[0]) : 0) : 0u;
     }
 
@@ -128,48 +141,50 @@ struct QkUnit {
     }
 };
 
-template <typename T, int V, bool IL, bool AX>
-__global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, int lg, int tw) {
+template <typename T, int V, int U, bool IL, bool AX>
+__global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, QkTurnPlan pl) {
     const int lane = threadIdx.x & 63;
-    int64_t t = a.t0 + (((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) << tw);
+    int slot = (int)(((uint32_t)lane * pl.units_mul) >> 16);
+    const int unit = lane - slot * pl.units;
+    slot = slot < pl.heads * pl.tokens ? slot : 0;
+    const int tok = (int)(((uint32_t)slot * pl.heads_mul) >> 16);
+    const int sub = slot - tok * pl.heads;
+    int64_t t = a.t0 + ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * pl.tokens;
     if (t >= a.T) return;
-    const QkUnit<V, IL> un(a, lane, lg, std::bool_constant<AX>{});
-    const QkTasks tasks(a.heads[0], a.heads[1], lg + tw);
-    const int step = 64 >> (lg + tw), sub = (lane >> lg) & (step - 1);
-    t += lane >> (6 - tw);
-    const bool here = t < a.T;
-    t = here ? t : a.T - 1;
+    t = t + tok < a.T ? t + tok : a.T - 1;
+    const QkUnit<V, IL> un(a, unit, std::bool_constant<AX>{});
+    const QkRaw<AX> raw(a, t);
     using Piece = std::conditional_t<V == 8, CkPiece<T>, QkPiece<T, V>>;
     struct Rows {
-        Piece p[kQkU][2];
+        Piece p[U][2];
     };
-    const auto side = [&](int j) { return j < tasks.nq ? 0 : 1; };
-    const auto first = [&](int j, int s) { return (s ? j - tasks.nq : j) * tasks.per + sub; };
+    const auto head = [&](int j, int s, int u) {
+        const int h = ((s ? j - pl.nq : j) * U + u) * pl.heads + sub;
+        return h < a.heads[s] ? h : a.heads[s] - 1;
+    };
     const auto fetch = [&](int j, Rows& r) {
-        const int s = side(j), h0 = first(j, s);
+        const int s = j < pl.nq ? 0 : 1;
         const T* base = static_cast<const T*>(a.x[s]) + t * a.x_token[s];
 #pragma unroll
-        for (int u = 0; u < kQkU; ++u) {
-            const int h = h0 + u * step;
-            const T* row = base + (h < a.heads[s] ? h : 0) * a.x_head[s];
+        for (int u = 0; u < U; ++u) {
+            const T* row = base + head(j, s, u) * a.x_head[s];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) r.p[u][k].load(row + (un.in[k] ? un.c[k] : 0));
+            for (int k = 0; k < 2; ++k) r.p[u][k].load(row + un.c[k]);
         }
     };
     int j = blockIdx.y;
-    const QkRaw<AX> raw(a, t);
     Rows next;
     fetch(j, next);  // the grid's y is at most the number of tasks
     const QkAt<AX> at(a, t, raw);
     float cs[V], sn[V];
     un.table(a, at, a.inverse ? -1.f : 1.f, cs, sn);
-    for (; j < tasks.n; j += gridDim.y) {
-        const int s = side(j), h0 = first(j, s);
+    for (; j < pl.n; j += gridDim.y) {
+        const int s = j < pl.nq ? 0 : 1;
         const Rows rows = next;
-        if (j + (int)gridDim.y < tasks.n) fetch(j + gridDim.y, next);
+        if (j + (int)gridDim.y < pl.n) fetch(j + gridDim.y, next);
+        T* base = static_cast<T*>(a.y[s]) + t * a.heads[s] * a.D;
 #pragma unroll
-        for (int u = 0; u < kQkU; ++u) {
-            const int h = h0 + u * step;
+        for (int u = 0; u < U; ++u) {
             float v[2][V];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -181,59 +196,100 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, int lg, int tw) 
                 }
             }
             un.turn(a, cs, sn, v, at.ok());
-            if (here && h < a.heads[s]) {
-                T* y = static_cast<T*>(a.y[s]) + (t * a.heads[s] + h) * a.D;
+            if (pl.odd) {
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    if (un.in[k]) qk_store<T, V>(y + un.c[k], v[k]);
+                for (int e = 0; e < V; ++e) v[1][e] = un.two ? v[1][e] : v[0][e];
             }
+            T* y = base + head(j, s, u) * a.D;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) qk_store<T, V>(y + un.c[k], v[k]);
         }
     }
 }
 
-// V channels a piece (0: the kernel of any size) and log2 of the lanes a head.
-static QkTiling qk_turn_tiling(int D, int R, bool interleaved) {
-    for (int v = 8; v >= 4; v -= 4) {
-        if (D % v != 0 || (!interleaved && R % (2 * v) != 0)) continue;
-        const int units = interleaved ? (D + 2 * v - 1) / (2 * v) : R / (2 * v) + ((D - R) / v + 1) / 2;
-        int lg = 0;
-        while ((1 << lg) < units) ++lg;
-        if (lg <= 6) return QkTiling{v, lg};
+static QkTurnPlan qk_turn_plan(const QkArgs& a, int dt) {
+    QkTurnPlan p{};
+    // pieces of 16 bytes, or of 4 channels
+    for (int v = dt == kBF16 ? 8 : 4; v >= 4 && p.v == 0; v -= 4) {
+        if (a.D % v != 0 || (!a.interleaved && a.R % (2 * v) != 0)) continue;
+        const int pieces = a.interleaved ? a.D / v : (a.D - a.R) / v;
+        p.units = (pieces + 1) / 2 + (a.interleaved ? 0 : a.R / (2 * v));
+        p.odd = pieces % 2;
+        if (p.units <= 64) p.v = v;
     }
-    return QkTiling{0, 0};
+    if (p.v == 0) return p;
+    const int slots = 64 / p.units;
+    // the fewest steps a token, its table row one more, while twelve waves a CU are
+    // left (8192 x 40 heads of 128 bf16: one token a wave 34 us, two 46), several
+    // tokens where that saves a quarter (16384 x 64 heads of 128 bf16: one 94 us,
+    // eight 107); tasks of four steps where those leave no more idle than tasks of two
+    int64_t best = INT64_MAX;
+    for (int n = 1; n <= slots && (n == 1 || a.T / n >= 12 * (int64_t)device_cu_count()); ++n) {
+        const int heads = slots / n;
+        for (int u = 4; u >= 2; u -= 2) {
+            const int per = u * heads, nq = (a.heads[0] + per - 1) / per, nk = (a.heads[1] + per - 1) / per;
+            const int64_t cost = ((int64_t)(nq + nk) * u + 1) * 12000 / n;
+            if (n > 1 && p.tokens == 1 ? cost * 4 > best * 3 : cost >= best) continue;
+            best = cost;
+            p.u = u;
+            p.heads = heads;
+            p.tokens = n;
+            p.nq = nq;
+            p.n = nq + nk;
+        }
+    }
+    p.units_mul = (65536u + (uint32_t)p.units - 1u) / (uint32_t)p.units;
+    p.heads_mul = (65536u + (uint32_t)p.heads - 1u) / (uint32_t)p.heads;
+    return p;
 }
 
 hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
     const int H = a.heads[0] + a.heads[1];
     if (a.T == 0 || H == 0) return hipSuccess;
-    const QkTiling t = qk_turn_tiling(a.D, a.R, a.interleaved);
-    const int tw = qk_tokens(a, t);
-    const int y = t.v == 0 ? (H + 3) / 4 : qk_splits(a.T >> tw, QkTasks(a.heads[0], a.heads[1], t.lg + tw));
-    const int each = t.v == 0 ? 1 : 4 << tw;  // tokens a workgroup
+    const QkTurnPlan p = qk_turn_plan(a, dt);
+    const int each = p.v == 0 ? 1 : 4 * p.tokens;  // tokens a workgroup
+    int y = (H + 3) / 4;
+    if (p.v != 0) {  // four waves a CU, each with tasks of its own: every one loads the tables
+        const int64_t waves = (a.T + p.tokens - 1) / p.tokens, want = 4 * (int64_t)device_cu_count();
+        y = (int)std::min<int64_t>(p.n, (want + waves - 1) / waves);
+    }
     const int64_t most = (int64_t)1 << 23;  // workgroups along tokens a launch: 2^31 lanes
     const int tok = timing_begin("qk_rope", s);
     hipError_t e = hipSuccess;
     QkArgs b = a;
-    b.whole = t.v != 0 && !a.dealt;
+    b.whole = p.v != 0 && !a.dealt;
     for (int i = 0; i + 1 < a.axes; ++i)
-        if (t.v != 0 && a.part[i] % t.v != 0) b.whole = 0;
+        if (p.v != 0 && a.part[i] % p.v != 0) b.whole = 0;
     for (b.t0 = 0; b.t0 < a.T && e == hipSuccess; b.t0 += most * each) {
         const int64_t x = (a.T - b.t0 + each - 1) / each;
         const dim3 grid((unsigned)(x < most ? x : most), (unsigned)y);
         const auto run = [&](auto z_, auto ax_) {
             using T_ = decltype(z_);
             constexpr bool A_ = decltype(ax_)::value;
-            if (t.v == 0) {
+            if (p.v == 0) {
                 MHC_LAUNCH_GGL((qk_turn_any_kernel<T_, A_>), grid, dim3(256), 0, s, b);
-            } else if (t.v == 8 && a.interleaved) {
-                MHC_LAUNCH_GGL((qk_turn_kernel<T_, 8, true, A_>), grid, dim3(256), 0, s, b, t.lg, tw);
-            } else if (t.v == 8) {
-                MHC_LAUNCH_GGL((qk_turn_kernel<T_, 8, false, A_>), grid, dim3(256), 0, s, b, t.lg, tw);
-            } else if (a.interleaved) {
-                MHC_LAUNCH_GGL((qk_turn_kernel<T_, 4, true, A_>), grid, dim3(256), 0, s, b, t.lg, tw);
-            } else {
-                MHC_LAUNCH_GGL((qk_turn_kernel<T_, 4, false, A_>), grid, dim3(256), 0, s, b, t.lg, tw);
+                return;
             }
+            const auto steps = [&](auto v_, auto il_) {
+                constexpr int V_ = decltype(v_)::value;
+                constexpr bool I_ = decltype(il_)::value;
+                if (p.u == 4) {
+                    MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, 4, I_, A_>), grid, dim3(256), 0, s, b, p);
+                } else {
+                    MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, 2, I_, A_>), grid, dim3(256), 0, s, b, p);
+                }
+            };
+            const auto pieces = [&](auto v_) {
+                if (a.interleaved) steps(v_, std::true_type{});
+                else steps(v_, std::false_type{});
+            };
+            if constexpr (sizeof(T_) == 2) {
+                if (p.v == 8) {
+                    pieces(std::integral_constant<int, 8>{});
+                    return;
+                }
+            }
+            pieces(std::integral_constant<int, 4>{});
         };
         const auto typed = [&](auto z_) {
             if (a.axes > 1) run(z_, std::true_type{});
