@@ -944,6 +944,15 @@ struct Distribute : public torch::autograd::Function<Distribute> {
     }
 };
 
+// Whether a call of a C++ node is needed: a backward may run, or an input has a
+// forward-mode tangent (forward mode runs without grad mode too), which a C++
+// node refuses.
+bool needs_node(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->_fw_grad(0).defined() || (at::GradMode::is_enabled() && t->requires_grad())) return true;
+    return false;
+}
+
 // ---- dropout, RMSNorm of a residual's sum ---------------------------------------
 // What a call drops: the numbers of `seed` (a tensor where one is defined).
 struct Drop {
@@ -1006,8 +1015,9 @@ struct Dropout : public torch::autograd::Function<Dropout> {
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const Drop d = Drop::saved(ctx->saved_data["drop"].toIntVector(), ctx->get_saved_variables()[0]);
         const auto dt = (at::ScalarType)ctx->saved_data["x_dtype"].toInt();
-        const at::DeviceGuard guard(grads[0].device());
-        return {run_dropout(storage(grads[0]), d).to(dt), Tensor()};
+        // linear: its gradient's gradient is a call on the cotangent
+        const Tensor dx = needs_node({&grads[0]}) ? Dropout::apply(grads[0], d) : forward(nullptr, grads[0], d);
+        return {dx.to(dt), Tensor()};
     }
 };
 
@@ -1048,6 +1058,7 @@ struct RmsNormResidual : public torch::autograd::Function<RmsNormResidual> {
 
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const char* fn = "mhc_rmsnorm_residual_bwd";
+        TORCH_CHECK(!at::GradMode::is_enabled(), "rmsnorm_residual: no second derivative (create_graph)");
         tensor_list out(7);
         if (!grads[0].defined() && !grads[1].defined()) return out;
         const auto sv = ctx->get_saved_variables();
@@ -1232,13 +1243,27 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
 
 // The rotation alone: its backward is the rotation by the negative angle.
 struct QkRope : public torch::autograd::Function<QkRope> {
-    static tensor_list run(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& pos,
-                           int64_t period, bool interleaved, const QkAxes& axes, bool inverse) {
+    static tensor_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& cos_in,
+                               const Tensor& sin_in, const c10::optional<Tensor>& positions, int64_t period,
+                               bool interleaved, const QkAxes& axes, bool inverse) {
+        const at::DeviceGuard guard(q_in.device());
+        const auto dt = storage_dtype(q_in.scalar_type()) ? q_in.scalar_type() : at::kFloat;
+        const Tensor q = qk_rows(q_in, dt), k = qk_rows(k_in, dt), cos = f32c(cos_in), sin = f32c(sin_in);
+        const Tensor pos = positions.has_value() && positions->defined() ? positions->contiguous() : Tensor();
+        if (ctx) {
+            ctx->save_for_backward({cos, sin, pos});
+            ctx->saved_data["ints"] =
+                std::vector<int64_t>{period, interleaved, (int64_t)dt, (int64_t)q_in.scalar_type(),
+                                     (int64_t)k_in.scalar_type(), inverse};
+            if (axes.any()) {
+                ctx->saved_data["sections"] = axes.sections;
+                ctx->saved_data["dealt"] = axes.dealt;
+            }
+        }
         const int64_t T = q.size(0), H = q.size(1), K = k.size(1), D = q.size(2);
         Tensor qo = at::empty({T, H, D}, q.options()), ko = at::empty({T, K, D}, k.options());
         check(lib.mhc_qk_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                              dtype_code(q.scalar_type()), fp(cos), fp(sin), cos.size(0),
-                              pos.defined() ? pos.data_ptr() : nullptr,
+                              dtype_code(dt), fp(cos), fp(sin), cos.size(0), pos.defined() ? pos.data_ptr() : nullptr,
                               pos.defined() ? (int32_t)pos.element_size() : 0, period, axes.count(), axes.ptr(),
                               (int32_t)axes.dealt, qo.data_ptr(), ko.data_ptr(), T, (int32_t)H, (int32_t)K,
                               (int32_t)D, (int32_t)(2 * cos.size(1)), interleaved, inverse, stream()),
@@ -1246,47 +1271,23 @@ struct QkRope : public torch::autograd::Function<QkRope> {
         return {qo, ko};
     }
 
-    static tensor_list forward(AutogradContext* ctx, const Tensor& q_in, const Tensor& k_in, const Tensor& cos_in,
-                               const Tensor& sin_in, const c10::optional<Tensor>& positions, int64_t period,
-                               bool interleaved, const QkAxes& axes) {
-        const at::DeviceGuard guard(q_in.device());
-        const auto dt = storage_dtype(q_in.scalar_type()) ? q_in.scalar_type() : at::kFloat;
-        const Tensor cos = f32c(cos_in), sin = f32c(sin_in);
-        const Tensor pos = positions.has_value() ? positions->contiguous() : Tensor();
-        if (ctx) {
-            ctx->save_for_backward({cos, sin, pos});
-            ctx->saved_data["ints"] = std::vector<int64_t>{period, interleaved, (int64_t)dt,
-                                                           (int64_t)q_in.scalar_type(), (int64_t)k_in.scalar_type()};
-            if (axes.any()) {
-                ctx->saved_data["sections"] = axes.sections;
-                ctx->saved_data["dealt"] = axes.dealt;
-            }
-        }
-        return run(qk_rows(q_in, dt), qk_rows(k_in, dt), cos, sin, pos, period, interleaved, axes, false);
-    }
-
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         const auto sv = ctx->get_saved_variables();
         const auto v = ctx->saved_data["ints"].toIntVector();
         check_device("qk_rope_bwd", {&grads[0], &grads[1], &sv[0]});
-        const at::DeviceGuard guard(sv[0].device());
         const auto dt = (at::ScalarType)v[2];
-        const tensor_list d = run(qk_rows(grads[0], dt), qk_rows(grads[1], dt), sv[0], sv[1], sv[2], v[0], v[1] != 0,
-                                  saved_axes(ctx), true);
+        const QkAxes axes = saved_axes(ctx);
+        const Tensor gq = grads[0].to(dt), gk = grads[1].to(dt);
+        // linear: its gradient's gradient is a call on the cotangents
+        const tensor_list d =
+            needs_node({&gq, &gk})
+                ? QkRope::apply(gq, gk, sv[0], sv[1], sv[2], v[0], v[1] != 0, axes, v[5] == 0)
+                : forward(nullptr, gq, gk, sv[0], sv[1], sv[2], v[0], v[1] != 0, axes, v[5] == 0);
         tensor_list out = {d[0].to((at::ScalarType)v[3]), d[1].to((at::ScalarType)v[4])};
-        out.resize(8);
+        out.resize(9);
         return out;
     }
 };
-
-// Whether a call of a C++ node is needed: a backward may run, or an input has a
-// forward-mode tangent (forward mode runs without grad mode too), which a C++
-// node refuses.
-bool needs_node(std::initializer_list<const Tensor*> ts) {
-    for (const Tensor* t : ts)
-        if (t->_fw_grad(0).defined() || (at::GradMode::is_enabled() && t->requires_grad())) return true;
-    return false;
-}
 
 Tensor dropout(const Tensor& x, double p, const c10::optional<Tensor>& seed, const c10::optional<int64_t>& value,
                int64_t offset) {
@@ -1474,9 +1475,9 @@ std::tuple<Tensor, Tensor> qk_rope(const Tensor& q_in, const Tensor& k_in, const
     const QkAxes axes(sections, dealt);
     const QkCall call(fn, q_in, k_in, cos, sin, positions, axes, {});
     return call.shaped(needs_node({&call.q, &call.k})
-                           ? QkRope::apply(call.q, call.k, cos, sin, positions, call.period, interleaved, axes)
+                           ? QkRope::apply(call.q, call.k, cos, sin, positions, call.period, interleaved, axes, false)
                            : QkRope::forward(nullptr, call.q, call.k, cos, sin, positions, call.period, interleaved,
-                                             axes));
+                                             axes, false));
 }
 
 Tensor static_layer(const Tensor& x, const Tensor& w, const Tensor& hp, const Tensor& hq, const Tensor& hr,

@@ -212,6 +212,18 @@ def test_the_backward_turns_back(device):
         _within(b, x.detach().cpu().double(), 12 * E32 * _magnitude(x.detach().cpu(), D // 2, False), "back")
 
 
+def test_second_derivatives_of_the_rotation(device):
+    """Linear: the gradient of its gradient turns forward again."""
+    q, k, _, cots = _inputs(20, 3, 2, 64, torch.float32, 6)
+    q, k, z0, z1 = (t.to(device).requires_grad_(True) for t in (q, k, *cots))
+    cos, sin = (t.to(device) for t in mhc.rope_table(L, 64))
+    how = {"positions": torch.randint(L, (2, 20), generator=_gen(5)).to(device), "sections": [20, 12]}
+    dq, dk = torch.autograd.grad(mhc.qk_rope(q, k, cos, sin, **how), [q, k], [z0, z1], create_graph=True)
+    u = [torch.randn_like(t).detach() for t in (q, k)]
+    got = torch.autograd.grad([dq, dk], [z0, z1], u)
+    assert all(torch.equal(a, b) for a, b in zip(got, mhc.qk_rope(*u, cos, sin, **how)))
+
+
 @pytest.mark.parametrize("norm", [False, True])
 @pytest.mark.parametrize("D,R", [(128, 128), (66, 64)])
 @pytest.mark.parametrize("bad", [-1, L, 2 ** 40, -2 ** 40])

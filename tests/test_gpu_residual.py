@@ -156,7 +156,7 @@ def test_dropout_rows_past_32_bits(device):
 # narrow rows, ragged rows, every number of pieces a lane, rows past the registers
 SHAPES = [(1, 1), (1, 8), (3, 7), (5, 33), (9, 64), (130, 100), (67, 512), (33, 513), (17, 1001), (40, 1280),
           (1, 4096), (300, 4096), (11, 5003), (5, 8192), (6, 9001), (3, 16384), (3, 16385), (2, 40000), (0, 64),
-          (2100, 96), (2600, 1024)]
+          (2100, 96), (2600, 1024), (1100, 4096), (550, 5003), (600, 16383), (70001, 33), (3, 256), (9, 257)]
 DTYPES = [(F32, F32), (BF16, BF16), (BF16, F32), (F32, BF16)]
 
 
@@ -265,6 +265,36 @@ def test_only_the_wanted_gradients(device, dtypes):
             want = [i for i in range(3) if mask >> i & 1]
             got = torch.autograd.grad(out, [leaves[i] for i in want], [c.to(device) for c in cots])
             assert all(torch.equal(g, full[i]) for g, i in zip(got, want)), mask
+
+
+def test_gradients_accumulate(device):
+    """.backward() twice, one tensor as x and residual, two calls on one tensor."""
+    x, res, w, cots = _inputs((30, 96), (F32, F32), 18)
+    cots = [c.to(device) for c in cots]
+    for p in (0.0, 0.3):
+        _, _, dx, dres, dw = _run(device, (x, res, w, [c.cpu() for c in cots]), p, None, 4, 0)
+        leaves = [t.to(device).requires_grad_(True) for t in (x, res, w)]
+        for n in (1, 2):
+            torch.autograd.backward(mhc.rmsnorm_residual(*leaves, dropout=p, seed=4), cots)
+            assert all(torch.equal(a.grad, n * e) for a, e in zip(leaves, (dx, dres, dw)))
+        one = x.to(device).requires_grad_(True)
+        g, = torch.autograd.grad(mhc.rmsnorm_residual(one, one, w.to(device), dropout=p, seed=4), one, cots)
+        _, _, dx, dres, _ = _run(device, (x, x, w, [c.cpu() for c in cots]), p, None, 4, 0)
+        assert torch.equal(g, dx + dres)
+
+
+def test_second_derivatives(device):
+    """Dropout is linear: the gradient of its gradient is a dropout with the same
+    numbers.  The norm has none, and says so."""
+    x = torch.randn(8, 40, device=device, requires_grad=True)
+    v = torch.randn(8, 40, device=device, requires_grad=True)
+    dx, = torch.autograd.grad(mhc.dropout(x, 0.5, seed=3), x, v, create_graph=True)
+    u = torch.randn(8, 40, device=device)
+    dv, = torch.autograd.grad(dx, v, u)
+    assert torch.equal(dv, mhc.dropout(u, 0.5, seed=3)) and torch.equal(dx.detach(), mhc.dropout(v, 0.5, seed=3).detach())
+    y, _ = mhc.rmsnorm_residual(x, x, torch.ones(40, device=device))
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(y, x, v, create_graph=True)
 
 
 @pytest.mark.parametrize("which", [0, 1])
