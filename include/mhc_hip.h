@@ -472,7 +472,8 @@ int mhc_dropout(const void* x, int32_t dtype, void* out, int32_t threshold, uint
  *       threshold 0 for none; the product is rounded by itself in fp32)
  *   y = h / sqrt(mean h^2 + eps) * weight
  * y is written to `y` in x_dtype (y_format MHC_CHECKPOINT_NONE), or to y_values /
- * y_scales in 8 bits as mhc_checkpoint_pack lays them out, from the fp32 values.
+ * y_scales in 8 bits as mhc_checkpoint_pack lays them out, rounded once (its mean
+ * square and 1 / sqrt are then taken to more than fp32).
  * With h_format other than MHC_CHECKPOINT_NONE the checkpoint of h's rows is
  * written too, and the backward reads it in place of h.  hidden <= 2^30. */
 int mhc_rmsnorm_residual_fwd(const void* x, int32_t x_dtype, const void* residual, int32_t residual_dtype,

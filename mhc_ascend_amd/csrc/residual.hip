@@ -127,7 +127,11 @@ template <typename T>
 __device__ __forceinline__ void res_round(float (&v)[8]) {
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = bf16_to_f32(f32_to_bf16(v[e]));
+        for (int e = 0; e < 8; e += 2) {
+            const uint32_t w = pack_bf16x2(v[e], v[e + 1]);
+            v[e] = __uint_as_float(w << 16);
+            v[e + 1] = __uint_as_float(w & 0xffff0000u);
+        }
     }
 }
 __device__ __forceinline__ void res_weight(const ResidualArgs& a, int c0, float (&w)[8]) {
@@ -155,11 +159,93 @@ __device__ __forceinline__ void res_unpack(int fmt, const uint8_t* __restrict__ 
     else ck_unpack8<kCkE4M3>(p, s, v);
 }
 
+// ---------------------------------------------------------------------------
+// y in 8 bits is rounded once, from the norm's value: a number next to the middle
+// of two 8-bit ones, or a block's largest next to where its exponent changes, would
+// otherwise fall to one side or the other by the roundings before it (of 67 M e4m3
+// numbers some tens, and a whole block of 32 now and then).  So there the mean
+// square is summed in 64 bits, 1 / r and its product with the weight have two
+// parts, and fp32 y is rounded to odd: cut off, with the last bit set where
+// something was lost, which the rounding to 8 bits takes for what it is.
+// ---------------------------------------------------------------------------
+// 1 / sqrt(s) = hi + lo: the instruction's own approximation (an ulp or so), the rest
+// from the residual 1 - s hi^2; zero where that has no meaning (hi zero or
+// infinite, or its square).
+struct ResInv {
+    float hi, lo;
+    __device__ __forceinline__ explicit ResInv(double s) {
+        const float sh = (float)s, sl = (float)(s - (double)sh);
+        hi = __builtin_amdgcn_rsqf(sh);
+        const float sq = hi * hi, rest = __builtin_fmaf(hi, hi, -sq);
+        const float res = __builtin_fmaf(-sl, sq, __builtin_fmaf(-sh, rest, __builtin_fmaf(-sh, sq, 1.f)));
+        lo = fabsf(res) < 0x1p-10f ? 0.5f * hi * res : 0.f;
+    }
+    // v / r * w, rounded to odd: one step towards zero where y was rounded away from
+    // it (an infinite y to the largest number), then the last bit set
+    __device__ __forceinline__ float odd(float v, float w) const {
+        const float ph = w * hi, pl = __builtin_fmaf(w, lo, __builtin_fmaf(w, hi, -ph)), c = v * pl;
+        const float y = __builtin_fmaf(v, ph, c);
+        const float rest = __builtin_fmaf(v, ph, -y) + c;  // what y is off by
+        const uint32_t past = rest * y < 0.f ? 1u : 0u;
+        return __uint_as_float((__float_as_uint(y) - past) | 1u);
+    }
+};
+
+__device__ __forceinline__ double res_square(const float (&v)[8], double s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = __builtin_fma((double)v[e], (double)v[e], s);
+    return s;
+}
+
+// Sum over the aligned group of 2^lg lanes (lg >= 2), in every lane of it.
+template <int CTRL>
+__device__ __forceinline__ double res_dpp_add(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __float_as_uint(dpp::mov<CTRL>(__uint_as_float((uint32_t)u)));
+    const uint32_t hi = __float_as_uint(dpp::mov<CTRL>(__uint_as_float((uint32_t)(u >> 32))));
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double res_group_sum(double v, int lg) {
+    const auto pair = [](auto lo, auto hi) {
+        return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) +
+               __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+    };
+    v = res_dpp_add<dpp::kQuadXor1>(v);
+    v = res_dpp_add<dpp::kQuadXor2>(v);
+    if (lg >= 3) v = res_dpp_add<dpp::kRowHalfMirror>(v);
+    if (lg >= 4) v = res_dpp_add<dpp::kRowMirror>(v);
+    if (lg >= 5) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+        v = pair(__builtin_amdgcn_permlane16_swap(lo, lo, false, false),
+                 __builtin_amdgcn_permlane16_swap(hi, hi, false, false));
+    }
+    if (lg >= 6) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)u, hi = (uint32_t)(u >> 32);
+        v = pair(__builtin_amdgcn_permlane32_swap(lo, lo, false, false),
+                 __builtin_amdgcn_permlane32_swap(hi, hi, false, false));
+    }
+    return v;
+}
+// Sum over the workgroup, in every lane; red: a double a wave.
+__device__ __forceinline__ double res_block_sum(double v, double* red) {
+    v = res_group_sum(v, 6);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+    for (unsigned w = 0; w < blockDim.x / 64; ++w) v += red[w];
+    __syncthreads();
+    return v;
+}
+
 template <typename TX, typename TR>
 __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(ResidualArgs a) {
     __shared__ float red[16];
+    __shared__ double red64[16];
     const DropKey key(a.drop);
     const int C = a.C;
+    const double each = 1.0 / C;
     const int64_t per = ((int64_t)C + 7) / 8;
     // whole blocks of 32, so that the lanes of one pack it together
     const int64_t end = ck_blocks(C) * kCkBlock;
@@ -168,6 +254,7 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(Residu
         const TR* res = static_cast<const TR*>(a.residual) + b * C;
         TR* h = static_cast<TR*>(a.h) + b * C;
         float t[1] = {0.f};
+        double t64 = 0.0;
         for (int64_t c = (int64_t)threadIdx.x * 8; c < end; c += kResAnyThreads * 8) {
             const int c0 = (int)c, m = c < C ? C - c0 : 0;
             float v[8], r[8];
@@ -179,25 +266,40 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(Residu
             res_round<TR>(v);
             if (m > 0) res_put(h + c0, m, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] = e < m ? v[e] : 0.f;
-                t[0] += v[e] * v[e];
+            for (int e = 0; e < 8; ++e) v[e] = e < m ? v[e] : 0.f;
+            if (a.y_fmt >= 0) {
+                t64 = res_square(v, t64);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[0] += v[e] * v[e];
             }
             if (a.h_fmt >= 0) res_pack(a.h_fmt, v, a.hq, a.hsc, b, C, c0);
         }
+        if (a.y_fmt >= 0) {
+            const ResInv inv(res_block_sum(t64, red64) * each + a.eps);
+            for (int64_t c = (int64_t)threadIdx.x * 8; c < end; c += kResAnyThreads * 8) {
+                const int c0 = (int)c, m = c < C ? C - c0 : 0;
+                float v[8], w[8];
+                res_piece(h + (m > 0 ? c0 : 0), m, v);
+                if (m > 0) {
+                    res_weight(a, c0, w);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = e < m ? inv.odd(v[e], w[e]) : 0.f;
+                }
+                res_pack(a.y_fmt, v, a.yq, a.ysc, b, C, c0);
+            }
+            continue;
+        }
         block_sum<1>(t, red);
         const float inv = 1.f / sqrtf(t[0] / (float)C + a.eps);
-        for (int64_t c = (int64_t)threadIdx.x * 8; c < end; c += kResAnyThreads * 8) {
-            const int c0 = (int)c, m = c < C ? C - c0 : 0;
+        for (int64_t c = (int64_t)threadIdx.x * 8; c < C; c += kResAnyThreads * 8) {
+            const int c0 = (int)c, m = C - c0;
             float v[8], w[8];
-            res_piece(h + (m > 0 ? c0 : 0), m, v);
-            if (m > 0) {
-                res_weight(a, c0, w);
+            res_piece(h + c0, m, v);
+            res_weight(a, c0, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = e < m ? v[e] * inv * w[e] : 0.f;
-            }
-            if (a.y_fmt >= 0) res_pack(a.y_fmt, v, a.yq, a.ysc, b, C, c0);
-            else if (m > 0) res_put(static_cast<TX*>(a.y) + b * C + c0, m, v);
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * w[e];
+            res_put(static_cast<TX*>(a.y) + b * C + c0, m, v);
         }
     }
 }
@@ -284,14 +386,32 @@ __device__ __forceinline__ void res_weights(const ResidualArgs& a, float (&w)[VP
     }
 }
 
+// ck_row_get without the zeros of lanes past the row.
+template <typename T, int VPT, bool RAG>
+__device__ __forceinline__ void res_row_get(const T* __restrict__ row, int C, const CkPiece<T> (&in)[VPT],
+                                            float (&v)[VPT][8]) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int c0 = (k * blockDim.x + threadIdx.x) * 8;
+        in[k].get(v[k]);
+        if (RAG && c0 < C && c0 + 8 > C) {
+            if (C >= 8) ck_shift_part(C - c0, v[k]);
+            else ck_load_part(row, C, v[k]);
+        }
+    }
+}
+
 template <typename TX, typename TR, int VPT, bool RAG>
 __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
     __shared__ float red[16];
+    __shared__ double red64[16];
     const DropKey key(a.drop);
     const int C = a.C;
+    const double each = 1.0 / C;
     const int64_t per = (C + 7) / 8;
     const TX* x = static_cast<const TX*>(a.x);
     const TR* res = static_cast<const TR*>(a.residual);
+    const bool past = C < (int)blockDim.x * VPT * 8;  // some lane's piece is past the row
     CkPiece<TX> xn[VPT];
     CkPiece<TR> rn[VPT];
     int64_t b = blockIdx.x;
@@ -304,8 +424,8 @@ __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
         float t[1] = {0.f};
         {
             float r[VPT][8];
-            ck_row_get<TX, VPT, RAG>(x + b * C, C, xn, v);
-            ck_row_get<TR, VPT, RAG>(res + b * C, C, rn, r);
+            res_row_get<TX, VPT, RAG>(x + b * C, C, xn, v);
+            res_row_get<TR, VPT, RAG>(res + b * C, C, rn, r);
             const int64_t b1 = b + gridDim.x < a.B ? b + gridDim.x : b;
             ck_row_load<TX, VPT, RAG>(x + b1 * C, C, xn);
             ck_row_load<TR, VPT, RAG>(res + b1 * C, C, rn);
@@ -314,9 +434,11 @@ __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
                 if (a.drop.threshold) key.apply(a.drop, (uint64_t)(b * per + k * blockDim.x + threadIdx.x), v[k]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[k][e] += r[k][e];
-                res_round<TR>(v[k]);
+                if (past && (k * blockDim.x + threadIdx.x) * 8 >= C) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[0] += v[k][e] * v[k][e];
+                    for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+                }
+                res_round<TR>(v[k]);
             }
         }
         ck_row_put<TR, VPT, RAG, false>(static_cast<TR*>(a.h) + b * C, C, v);
@@ -325,6 +447,24 @@ __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
             for (int k = 0; k < VPT; ++k)
                 res_pack(a.h_fmt, v[k], a.hq, a.hsc, b, C, (k * blockDim.x + threadIdx.x) * 8);
         }
+        if (a.y_fmt >= 0) {
+            double t64 = 0.0;
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) t64 = res_square(v[k], t64);
+            const ResInv inv(res_block_sum(t64, red64) * each + a.eps);
+#pragma unroll
+            for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] = inv.odd(v[k][e], w[k][e]);
+                res_pack<false>(a.y_fmt, v[k], a.yq, a.ysc, b, C, (k * blockDim.x + threadIdx.x) * 8);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[0] += v[k][e] * v[k][e];
+        }
         block_sum<1>(t, red);
         const float inv = 1.f / sqrtf(t[0] / (float)C + a.eps);
 #pragma unroll
@@ -332,13 +472,7 @@ __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[k][e] = v[k][e] * inv * w[k][e];
         }
-        if (a.y_fmt >= 0) {
-#pragma unroll
-            for (int k = 0; k < VPT; ++k)
-                res_pack<false>(a.y_fmt, v[k], a.yq, a.ysc, b, C, (k * blockDim.x + threadIdx.x) * 8);
-        } else {
-            ck_row_put<TX, VPT, RAG, false>(static_cast<TX*>(a.y) + b * C, C, v);
-        }
+        ck_row_put<TX, VPT, RAG, false>(static_cast<TX*>(a.y) + b * C, C, v);
     }
 }
 
@@ -467,6 +601,7 @@ template <typename TX, typename TR, bool RAG>
 __global__ __launch_bounds__(256) void residual_fwd_narrow_kernel(ResidualArgs a, int lg) {
     const DropKey key(a.drop);
     const int C = a.C;
+    const double each = 1.0 / C;
     const CkNarrow<float, RAG> ln(C, lg);
     const CkNarrow<TX, RAG> lx(C, lg);
     const CkNarrow<TR, RAG> lr(C, lg);
@@ -500,20 +635,26 @@ __global__ __launch_bounds__(256) void residual_fwd_narrow_kernel(ResidualArgs a
         ln.load(x + b1 * C, xn);
         ln.load(res + b1 * C, rn);
         if (a.drop.threshold) key.apply(a.drop, (uint64_t)(b * per + (ln.c0 >> 3)), v);
-        float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += r[e];
         res_round<TR>(v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
         if (on) lr.template put<false>(static_cast<TR*>(a.h) + b * C, v);
         if (a.h_fmt >= 0) pack(a.h_fmt, v, a.hq, a.hsc, b, on);
+        if (a.y_fmt >= 0) {
+            const ResInv inv(res_group_sum(res_square(v, 0.0), lg) * each + a.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = inv.odd(v[e], w[e]);
+            pack(a.y_fmt, v, a.yq, a.ysc, b, on);
+            continue;
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
         ss = lane_group_sum(ss, lg);
         const float inv = 1.f / sqrtf(ss / (float)C + a.eps);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = v[e] * inv * w[e];
-        if (a.y_fmt >= 0) pack(a.y_fmt, v, a.yq, a.ysc, b, on);
-        else if (on) lx.template put<false>(static_cast<TX*>(a.y) + b * C, v);
+        if (on) lx.template put<false>(static_cast<TX*>(a.y) + b * C, v);
     }
 }
 
@@ -649,10 +790,13 @@ static void res_flag(bool on, F f) {
     else f(std::false_type{});
 }
 
-// Workgroups of 1024 lanes a CU together, or as many as fit.
-static unsigned res_grid(const void* fn, int threads, int64_t most) {
+// Workgroups of 1024 lanes a CU together, or as many as fit; 1536 where y leaves in
+// 8 bits, which is bound by its instructions (16384 x 4096 bf16 to e4m3: 91 us with
+// 1024, 88 with 1536, 89 with 2048).
+static unsigned res_grid(const void* fn, int threads, int64_t most, int y_fmt) {
     int64_t per_cu = occupancy_per_cu(fn, threads, 0);
-    if (per_cu > 1024 / threads) per_cu = 1024 / threads;
+    const int lanes = y_fmt >= 0 ? 1536 : 1024;
+    if (per_cu > lanes / threads) per_cu = lanes / threads;
     const int64_t g = (int64_t)device_cu_count() * per_cu;
     return (unsigned)(g < most ? g : most);
 }
@@ -674,14 +818,14 @@ hipError_t launch_rmsnorm_residual_fwd(int x_dt, int r_dt, const ResidualArgs& a
                 constexpr bool G_ = decltype(g)::value;
                 const void* fn = reinterpret_cast<const void*>(&residual_fwd_narrow_kernel<X_, R_, G_>);
                 MHC_LAUNCH_GGL((residual_fwd_narrow_kernel<X_, R_, G_>),
-                               dim3(res_grid(fn, 256, (a.B + each - 1) / each)), dim3(256), 0, s, a, lg);
+                               dim3(res_grid(fn, 256, (a.B + each - 1) / each, a.y_fmt)), dim3(256), 0, s, a, lg);
             });
         } else {
             res_rows(t.vpt, rag, [&](auto v, auto g) {
                 constexpr int V_ = decltype(v)::value;
                 constexpr bool G_ = decltype(g)::value;
                 const void* fn = reinterpret_cast<const void*>(&residual_fwd_kernel<X_, R_, V_, G_>);
-                MHC_LAUNCH_GGL((residual_fwd_kernel<X_, R_, V_, G_>), dim3(res_grid(fn, t.threads, a.B)),
+                MHC_LAUNCH_GGL((residual_fwd_kernel<X_, R_, V_, G_>), dim3(res_grid(fn, t.threads, a.B, a.y_fmt)),
                                dim3(t.threads), 0, s, a);
             });
         }

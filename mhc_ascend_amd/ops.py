@@ -453,9 +453,10 @@ def rmsnorm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
     bits for the backward, which is then the gradient at the values that
     checkpoint stands for; without it the backward reads the h that was returned.
 
-    ``format`` ("int8" or "e4m3") returns y in 8 bits, a :class:`PackedActivation`
-    of the fp32 values (its ``dtype`` is x's), for a product in 8 bits.  No
-    gradient flows through it: such a call raises where one is wanted."""
+    ``format`` ("int8" or "e4m3") returns y in 8 bits, for a product in 8 bits: a
+    :class:`PackedActivation` (its ``dtype`` is x's) whose numbers are rounded
+    once, from the norm of h.  No gradient flows through it: such a call raises
+    where one is wanted."""
     _not_traced("rmsnorm_residual")
     code = _checkpoint_code(checkpoint)
     y_code = -1 if format is None else _checkpoint_code(format)
