@@ -11,10 +11,10 @@
 //
 // A value is kept where its number is at least t = round(p 2^16), and then
 // times 2^16 / (2^16 - t): the mean is exact for the p that t stands for, p to
-// 2^-17.  16 bits a value and not 32 halve the products, which would otherwise
-// take as long as the memory (a round is two products at a quarter of the rate
-// and four exclusive ors, 48 cycles a wave, 480 a block of 64 x 8 values: 2.6 T
-// values/s on 1024 SIMDs at 2.4 GHz, 10 TB/s of bf16 read and written).
+// 2^-17.  16 bits a value and not 32 halve the products, which run beside the
+// memory (two products a round at a quarter of the rate; 32768 x 4096 bf16, forward
+// and backward: 171 us, with 32 bits a value 185; with the norm of 16384 x 4096 194
+// and 205).
 #pragma once
 
 #include <hip/hip_runtime.h>

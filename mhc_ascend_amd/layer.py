@@ -194,7 +194,7 @@ class MHCResidualWrapper(nn.Module):
         if self.residual_mode not in ("zero", "decay"):
             raise ValueError(f"Unknown residual_mode: {self.residual_mode}")
         if self.training and self.dropout > 0.0:
-            branch_output = ops.dropout(branch_output, self.dropout)
+            branch_output = ops.dropout(branch_output, self.dropout).to(branch_output.dtype)
         output = ops.mhc_residual_wrapper(residual, branch_output, self.mhc, self.residual_mode)
         if T > 1:
             output = output.reshape(B, T, C)

@@ -563,3 +563,20 @@ def test_residual_wrapper_drops_its_branch_in_training(device, dynamic, C):
     wrap.eval()
     plain.eval()
     assert torch.equal(wrap(r, b), plain(r, b))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, torch.float16])
+@pytest.mark.parametrize("shape", [(6, 64), (2, 5, 64), (3, 1, 64), (0, 64)])
+def test_residual_wrapper_takes_what_it_took(device, dtype, shape):
+    """Every shape and dtype of the wrapper without dropout, with it."""
+    torch.manual_seed(1)
+    wrap = mhc.MHCResidualWrapper(64, 4, dropout=0.3, use_dynamic_h=False).to(device)
+    plain = mhc.MHCResidualWrapper(64, 4, use_dynamic_h=False).to(device)
+    plain.load_state_dict(wrap.state_dict())
+    r, b = (torch.randn(*shape, device=device).to(dtype) for _ in range(2))
+    torch.manual_seed(2)
+    out = wrap(r, b)
+    torch.manual_seed(2)
+    assert torch.equal(out, plain(r, mhc.dropout(b, 0.3).to(dtype)))
+    wrap.dropout = 1.0
+    assert torch.equal(wrap(r, b), plain(r, torch.zeros_like(b)))
