@@ -475,7 +475,8 @@ int mhc_dropout(const void* x, int32_t dtype, void* out, int32_t threshold, uint
  * y_scales in 8 bits as mhc_checkpoint_pack lays them out, rounded once (its mean
  * square and 1 / sqrt are then taken to more than fp32).
  * With h_format other than MHC_CHECKPOINT_NONE the checkpoint of h's rows is
- * written too, and the backward reads it in place of h.  hidden <= 2^30. */
+ * written too, and the backward reads it in place of h.  No output overlaps an
+ * input.  hidden <= 2^30. */
 int mhc_rmsnorm_residual_fwd(const void* x, int32_t x_dtype, const void* residual, int32_t residual_dtype,
                              const void* weight, int32_t weight_dtype, void* h, void* y, int32_t y_format,
                              void* y_values, void* y_scales, int32_t h_format, void* h_values, void* h_scales,
@@ -559,7 +560,7 @@ int mhc_qk_norm_rope_axes_bwd(const void* grad_q_out, int64_t gq_token_stride, i
 
 /* The rotation alone, by the angle or (inverse != 0) its negative, which is its
  * backward on the cotangents.  axes 0 stands for one axis without sections (NULL);
- * only there may positions be NULL. */
+ * only there may positions be NULL.  The outputs do not overlap q and k. */
 int mhc_qk_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
                 int64_t k_head_stride, int32_t dtype, const float* cos, const float* sin, int64_t table_rows,
                 const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,

@@ -2712,12 +2712,12 @@ static int set_qk_axes(const char* fn, QkArgs& a, int32_t axes, const int32_t* s
 }
 
 static int qk_fwd(const char* fn, const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
-                         int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
-                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
-                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
-                         const int32_t* sections, int32_t dealt, void* q_out, void* k_out, int32_t format, void* q_values, void* q_scales, void* k_values,
-                         void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
-                         int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
+                  int64_t k_token_stride, int64_t k_head_stride, int32_t dtype, const void* q_weight,
+                  const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin, int64_t table_rows,
+                  const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
+                  const int32_t* sections, int32_t dealt, void* q_out, void* k_out, int32_t format, void* q_values,
+                  void* q_scales, void* k_values, void* k_scales, int64_t tokens, int32_t q_heads, int32_t k_heads,
+                  int32_t head_dim, int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
     return guarded([&]() -> int {
         QkArgs a{};
         a.x[0] = q; a.x_token[0] = q_token_stride; a.x_head[0] = q_head_stride;
@@ -2800,15 +2800,15 @@ size_t mhc_qk_norm_rope_bwd_workspace_size(int64_t tokens, int32_t q_heads, int3
 }
 
 static int qk_bwd(const char* fn, const void* grad_q_out, int64_t gq_token_stride, int64_t gq_head_stride,
-                         const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
-                         int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
-                         int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values,
-                         const void* q_scales, const void* k_values, const void* k_scales, const void* q_weight,
-                         const void* k_weight, int32_t weight_dtype, const float* cos, const float* sin,
-                         int64_t table_rows, const void* positions, int32_t position_bytes, int64_t position_period, int32_t axes,
-                         const int32_t* sections, int32_t dealt, void* grad_q, void* grad_k, void* grad_weight, void* workspace, size_t workspace_bytes,
-                         int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim, int32_t rotary_dim,
-                         int32_t interleaved, float eps, void* stream) {
+                  const void* grad_k_out, int64_t gk_token_stride, int64_t gk_head_stride, const void* q,
+                  int64_t q_token_stride, int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                  int64_t k_head_stride, int32_t dtype, int32_t format, const void* q_values, const void* q_scales,
+                  const void* k_values, const void* k_scales, const void* q_weight, const void* k_weight,
+                  int32_t weight_dtype, const float* cos, const float* sin, int64_t table_rows, const void* positions,
+                  int32_t position_bytes, int64_t position_period, int32_t axes, const int32_t* sections,
+                  int32_t dealt, void* grad_q, void* grad_k, void* grad_weight, void* workspace,
+                  size_t workspace_bytes, int64_t tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                  int32_t rotary_dim, int32_t interleaved, float eps, void* stream) {
     return guarded([&]() -> int {
         QkArgs a{};
         a.x[0] = q; a.x_token[0] = q_token_stride; a.x_head[0] = q_head_stride;

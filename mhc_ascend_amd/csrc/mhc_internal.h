@@ -398,8 +398,8 @@ struct QkArgs {
     // Axes of positions [axes][period]: pairs dealt to them in turn, deal_sizes the
     // pairs of each (16 bits an axis, axis 0's lowest) and deal_mul = ceil(2^16 /
     // axes), whose product divides a pair's number (under 2^10) exactly; or else in
-    // blocks, part[] where each ends (INT_MAX from the last on).  whole: no lane's piece has pairs of two axes.  inverse: the
-    // rotation alone by the negative angle.
+    // blocks, part[] where each ends (INT_MAX from the last on).  whole: no lane's
+    // piece has pairs of two axes.  inverse: the rotation alone by the negative angle.
     int axes, dealt, whole, inverse;
     int part[4];
     uint64_t deal_sizes;

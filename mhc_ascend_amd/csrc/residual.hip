@@ -157,9 +157,9 @@ __device__ __forceinline__ void res_unpack(int fmt, const uint8_t* __restrict__ 
 // of two 8-bit ones, or a block's largest next to where its exponent changes, would
 // otherwise fall to one side or the other by the roundings before it (of 67 M e4m3
 // numbers some tens, and a whole block of 32 now and then).  So there the mean
-// square is summed in 64 bits, 1 / r and its product with the weight have two
-// parts, and fp32 y is rounded to odd: cut off, with the last bit set where
-// something was lost, which the rounding to 8 bits takes for what it is.
+// square is summed in 64 bits, 1 / r and its product with h have two parts, and fp32
+// y is rounded to odd: cut off, with the last bit set where something was lost,
+// which the rounding to 8 bits takes for what it is.
 // ---------------------------------------------------------------------------
 // 1 / sqrt(s) = hi + lo: the instruction's own approximation (an ulp or so), the rest
 // from the residual 1 - s hi^2; zero where that has no meaning (hi zero or
@@ -173,14 +173,15 @@ struct ResInv {
         const float res = __builtin_fmaf(-sl, sq, __builtin_fmaf(-sh, rest, __builtin_fmaf(-sh, sq, 1.f)));
         lo = fabsf(res) < 0x1p-10f ? 0.5f * hi * res : 0.f;
     }
-    // v / r * w, rounded to odd: one step towards zero where y was rounded away from
-    // it (an infinite y to the largest number), then the last bit set
+    // v / r * w, rounded to odd: where something was lost (not where y is infinite),
+    // one step towards zero if y was rounded away from it, then the last bit set
     __device__ __forceinline__ float odd(float v, float w) const {
-        const float ph = w * hi, pl = __builtin_fmaf(w, lo, __builtin_fmaf(w, hi, -ph)), c = v * pl;
-        const float y = __builtin_fmaf(v, ph, c);
-        const float rest = __builtin_fmaf(v, ph, -y) + c;  // what y is off by
-        const uint32_t past = rest * y < 0.f ? 1u : 0u;
-        return __uint_as_float((__float_as_uint(y) - past) | 1u);
+        const float n = v * hi, nl = __builtin_fmaf(v, lo, __builtin_fmaf(v, hi, -n)), c = w * nl;
+        const float y = __builtin_fmaf(w, n, c);
+        const float rest = __builtin_fmaf(w, n, -y) + c;   // what y is off by
+        constexpr int kLost = 0x198;                       // normal and subnormal numbers of either sign
+        const uint32_t u = __float_as_uint(y), past = (u ^ __float_as_uint(rest)) >> 31;
+        return __builtin_amdgcn_classf(rest, kLost) ? __uint_as_float((u - past) | 1u) : y;
     }
 };
 

@@ -362,6 +362,33 @@ def test_output_in_8_bits_of_small_and_large_rows(device, fmt):
             assert bool(up.isnan().all() and y.isinf().all()) if size < 1 else bool((up == 0).all() and (y == 0).all())
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("C", [96, 1000, 4096, 20000])
+@pytest.mark.parametrize("size", [1.0, 0.25, 1024.0])
+def test_output_in_8_bits_takes_ties_to_even(device, fmt, C, size):
+    """Rows of +-2^k with eps = 0: y is +-w exactly, and half of int8's numbers (a
+    16th of e4m3's) are the middle of two.  What is not lost is not rounded."""
+    g = _gen(31)
+    x = (2.0 * torch.randint(0, 2, (5, C), generator=g) - 1) * size
+    w = 1 + torch.randint(0, 128, (C,), generator=g) / 128
+    packed, _ = mhc.rmsnorm_residual(x.to(device), torch.zeros(5, C, device=device), w.to(device), eps=0.0, format=fmt)
+    want = mhc.activation_pack((x.sign() * w).to(device), fmt)
+    assert torch.equal(packed.scales, want.scales) and torch.equal(packed.values, want.values)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("C", [64, 1024, 32768])
+def test_output_in_8_bits_past_fp32(device, fmt, C):
+    """A norm past fp32's largest number is infinite, as it is for y in fp32: its
+    block unpacks to NaN, the others stay."""
+    x = torch.zeros(3, C)
+    x[:, 5] = torch.tensor([1.0, -2.0, 4.0])  # y = +-sqrt(C) w there
+    w = torch.full((C,), 3e38)
+    packed, _ = mhc.rmsnorm_residual(x.to(device), torch.zeros(3, C, device=device), w.to(device), eps=0.0, format=fmt)
+    up = mhc.activation_unpack(packed).cpu()
+    assert bool(up[:, :32].isnan().all()) and bool((up[:, 32:] == 0).all())
+
+
 def test_values_that_are_not_finite_stay_in_their_rows(device):
     x, res, w, cots = _inputs((12, 200), (F32, F32), 12)
     x[3, 17] = float("inf")
