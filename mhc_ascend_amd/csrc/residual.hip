@@ -96,7 +96,11 @@ hipError_t launch_dropout(int dt, const void* x, void* out, const DropArgs& d, i
 
 // ---------------------------------------------------------------------------
 // Rows of any length, a workgroup a row at a time: h goes to memory in the first
-// loop over the row and is read back by the lane that wrote it in the second.
+// loop over the row and is read back by the lane that wrote it in the second.  For
+// rows that no workgroup's registers hold: 4096 x 20000 bf16 forward 180 us (3.6
+// TB/s of the four arrays), backward 374 (1.8: every array is read twice, and dw's
+// partial row read and written in fp32 once a row); 8192 x 16384 with the rows in
+// registers 197 and 227 us, 5.5 and 4.7 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kResAnyThreads = 1024;
 
@@ -365,7 +369,10 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_bwd_any_kernel(Residu
 // workgroups of 512).  The forward's outputs are stored to stay in the caches:
 // what runs next reads them (forward and backward of that call 195 us, 211 with
 // streaming stores; into memory that is in no cache 95 for 90).  The backward's
-// stream.
+// stream, but for rows on no 16-byte boundary, whose neighbours' ends share lines
+// (30000 x 4095 bf16 226 us, 234 streamed; 20000 x 2733 fp32 190 and 197).  Bound by
+// bytes: 16384 x 4096 bf16 forward 81 us, 6.7 TB/s, backward 97, 5.5; 30000 x 4095
+// 233 and 226 us, 4.2 and 4.3 TB/s: most of a row's pieces lie across lines.
 // ---------------------------------------------------------------------------
 template <int VPT, bool RAG>
 __device__ __forceinline__ void res_weights(const ResidualArgs& a, float (&w)[VPT][8]) {
@@ -561,21 +568,24 @@ __global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a) {
                 d[k][e] += w[k][e] * g[k][e] * inv - hv[k][e] * k2;
             }
         }
-        if (a.gres) ck_row_put<TR, VPT, RAG>(static_cast<TR*>(a.gres) + b * C, C, d);
+        if (a.gres) ck_row_put<TR, VPT, RAG, !RAG>(static_cast<TR*>(a.gres) + b * C, C, d);
         if (a.gx) {
             if (a.drop.threshold) {
 #pragma unroll
                 for (int k = 0; k < VPT; ++k)
                     key.apply(a.drop, (uint64_t)(b * per + k * blockDim.x + threadIdx.x), d[k]);
             }
-            ck_row_put<TX, VPT, RAG>(static_cast<TX*>(a.gx) + b * C, C, d);
+            ck_row_put<TX, VPT, RAG, !RAG>(static_cast<TX*>(a.gx) + b * C, C, d);
         }
     }
     if (a.dw_part) ck_row_put<float, VPT, RAG>(a.dw_part + (int64_t)blockIdx.x * C, C, dw);
 }
 
 // ---------------------------------------------------------------------------
-// Narrow rows, several a wave (CkNarrow of mhc_ckpt.h): no LDS in the sums.
+// Narrow rows, several a wave (CkNarrow of mhc_ckpt.h): no LDS in the sums.  400000 x
+// 96 bf16 forward 51 us, 6.0 TB/s, backward 58, 5.3; 400000 x 100, rows on no 16-byte
+// boundary, 83 and 76 us, 3.9 and 4.2 TB/s (streamed 80).  Twice the lanes a CU: 51
+// and 62 us, 81 and 82.
 // ---------------------------------------------------------------------------
 template <bool RAG>
 __device__ __forceinline__ void res_narrow_weight(const ResidualArgs& a, const CkNarrow<float, RAG>& ln,
@@ -724,10 +734,10 @@ __global__ __launch_bounds__(512) void residual_bwd_narrow_kernel(ResidualArgs a
             dw[e] += on ? g[e] * hv[e] * inv : 0.f;
             d[e] += w[e] * g[e] * inv - hv[e] * k2;
         }
-        if (a.gres && on) lr.put(static_cast<TR*>(a.gres) + b * C, d);
+        if (a.gres && on) lr.template put<!RAG>(static_cast<TR*>(a.gres) + b * C, d);
         if (a.gx) {
             if (a.drop.threshold) key.apply(a.drop, (uint64_t)(b * per + (ln.c0 >> 3)), d);
-            if (on) lx.put(static_cast<TX*>(a.gx) + b * C, d);
+            if (on) lx.template put<!RAG>(static_cast<TX*>(a.gx) + b * C, d);
         }
     }
     if (!a.dw_part) return;  // the whole grid
