@@ -51,8 +51,8 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
 // with branches around the stores the loads are waited for one by one.  Bound by
 // bytes: 16384 x 64 heads of 128 bf16 on three axes 91 us, 5.9 TB/s; 15734 x 24 of 96
 // bf16 48 us, 6.1; 13794 x 48 of 112 bf16, 56 turned in neighbouring pairs dealt to
-// four axes, 70 us, 4.3: a third of its instructions are the table's.  16 x 40 heads:
-// 4.8 us, the latency of positions, table and rows.
+// four axes, 70 us, 4.3: its table entries are sixteen loads of 4 bytes a lane.  16 x
+// 40 heads: 4.8 us, the latency of positions, table and rows.
 // ---------------------------------------------------------------------------
 // How a wave is shared: units a head, heads a token takes at once, tokens, tasks of
 // the queries and of both; mul = ceil(2^16 / n) divides a lane or slot (under 64)
