@@ -43,22 +43,23 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
 // neighbouring pieces, and past R two pieces that stay.  So every channel is read
 // once, no value crosses lanes, and the V table entries of the unit stay in
 // registers for all heads of the token.  Nothing is summed over a head, so its
-// lanes are as many as its units: a wave holds 64 / units heads, shared by as many
-// tokens as leave the fewest steps a token.  A task is U steps of one side, its
-// loads in flight together with the next task's.  Few tokens: their tasks are
-// spread over the grid's y.
+// lanes are as many as its units, and a wave holds 64 / units heads; the queries'
+// and the keys' are one list.  A task is U steps of it, its loads in flight
+// together with the next task's.  Few heads: a wave's are those of several tokens.
+// Few tokens: their tasks are spread over the grid's y.
 // Lanes and steps with nothing of their own repeat another's work, store included:
 // with branches around the stores the loads are waited for one by one.  Bound by
-// bytes: 16384 x 64 heads of 128 bf16 on three axes 91 us, 5.9 TB/s; 15734 x 24 of 96
-// bf16 48 us, 6.1; 13794 x 48 of 112 bf16, 56 turned in neighbouring pairs dealt to
-// four axes, 70 us, 4.3: its table entries are sixteen loads of 4 bytes a lane.  16 x
-// 40 heads: 4.8 us, the latency of positions, table and rows.
+// bytes: 16384 x 64 heads of 128 bf16 on three axes 91 us, 5.9 TB/s; 16384 x 40 of 112
+// bf16 56 us, 5.2; 13794 x 48 of 112 bf16, 56 turned by pairs dealt to four axes, 58 us,
+// 5.1.  The keys' tasks apart from the queries': 16384 x 40 of 112 69 us for 67, 15643
+// x 2 of 112 bf16 11 for 9.  16 x 40 heads: 4.8 us, the latency of positions, table and
+// rows.
 // ---------------------------------------------------------------------------
-// How a wave is shared: units a head, heads a token takes at once, tokens, tasks of
-// the queries and of both; mul = ceil(2^16 / n) divides a lane or slot (under 64)
-// by n exactly.  odd: the last unit's second piece is past the head.
+// How a wave is shared: units a head, heads a token takes at once, tokens, tasks;
+// mul = ceil(2^16 / n) divides a lane or slot (under 64) by n exactly.  odd: the
+// last unit's second piece is past the head.
 struct QkTurnPlan {
-    int v, u, units, heads, tokens, nq, n, odd;
+    int v, u, units, heads, tokens, n, odd;
     uint32_t units_mul, heads_mul;
 };
 
@@ -145,7 +146,36 @@ struct QkUnit {
     }
 };
 
-template <typename T, int V, int U, bool IL, bool AX>
+// Rows past the caches (NT), where every load and store takes whole lines: halves
+// of a multiple of 128 bytes.  In others the unit's two pieces share lines, which
+// have to stay (forward and backward, streamed and not: 16384 x 64 heads of 128
+// bf16 186 and 195 us; 32768 x 40 of 96 bf16 330 and 206, 8192 x 40 of 80 bf16 turned
+// in neighbouring pairs 111 and 94).
+template <typename T, int V, bool NT>
+struct QkTurnPiece : QkPiece<T, V> {
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (!NT) QkPiece<T, V>::load(p);
+        else if constexpr (sizeof(T) == 4) this->w = __builtin_nontemporal_load(reinterpret_cast<const ck_u4_a4_t*>(p));
+        else if constexpr (V == 8) this->w = __builtin_nontemporal_load(reinterpret_cast<const ck_u4_a2_t*>(p));
+        else this->w = __builtin_nontemporal_load(reinterpret_cast<const qk_u2_a2_t*>(p));
+    }
+};
+
+template <typename T, int V, bool NT>
+__device__ __forceinline__ void qk_turn_store(T* p, const float (&v)[V]) {
+    if constexpr (NT) {
+        qk_store<T, V>(p, v);
+    } else if constexpr (V == 8) {
+        ck_store8<false>(p, v);
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<ck_u4_a4_t*>(p) = ck_u4_t{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                                    __float_as_uint(v[3])};
+    } else {
+        *reinterpret_cast<qk_u2_a2_t*>(p) = qk_u2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+}
+
+template <typename T, int V, int U, bool IL, bool AX, bool NT>
 __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, QkTurnPlan pl) {
     const int lane = threadIdx.x & 63;
     int slot = (int)(((uint32_t)lane * pl.units_mul) >> 16);
@@ -158,20 +188,24 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, QkTurnPlan pl) {
     t = t + tok < a.T ? t + tok : a.T - 1;
     const QkUnit<V, IL> un(a, unit, std::bool_constant<AX>{});
     const QkRaw<AX> raw(a, t);
-    using Piece = std::conditional_t<V == 8, CkPiece<T>, QkPiece<T, V>>;
     struct Rows {
-        Piece p[U][2];
+        QkTurnPiece<T, V, NT> p[U][2];
     };
-    const auto head = [&](int j, int s, int u) {
-        const int h = ((s ? j - pl.nq : j) * U + u) * pl.heads + sub;
-        return h < a.heads[s] ? h : a.heads[s] - 1;
+    // row `h` of the token's list begins at base[s] + h * stride, its side s
+    const int H = a.heads[0], last = H + a.heads[1] - 1;
+    const auto head = [&](int j, int u) {
+        const int h = (j * U + u) * pl.heads + sub;
+        return h < last ? h : last;
     };
+    const int64_t in0 = t * a.x_token[0], in1 = t * a.x_token[1] - H * a.x_head[1];
+    const int64_t out0 = t * H * a.D, out1 = (t * a.heads[1] - H) * a.D;
     const auto fetch = [&](int j, Rows& r) {
-        const int s = j < pl.nq ? 0 : 1;
-        const T* base = static_cast<const T*>(a.x[s]) + t * a.x_token[s];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const T* row = base + head(j, s, u) * a.x_head[s];
+            const int h = head(j, u);
+            const bool q = h < H;
+            const T* row = static_cast<const T*>(q ? a.x[0] : a.x[1]) + (q ? in0 : in1) +
+                           h * (q ? a.x_head[0] : a.x_head[1]);
 #pragma unroll
             for (int k = 0; k < 2; ++k) r.p[u][k].load(row + un.c[k]);
         }
@@ -183,30 +217,25 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, QkTurnPlan pl) {
     float cs[V], sn[V];
     un.table(a, at, a.inverse ? -1.f : 1.f, cs, sn);
     for (; j < pl.n; j += gridDim.y) {
-        const int s = j < pl.nq ? 0 : 1;
         const Rows rows = next;
         if (j + (int)gridDim.y < pl.n) fetch(j + gridDim.y, next);
-        T* base = static_cast<T*>(a.y[s]) + t * a.heads[s] * a.D;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float v[2][V];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                if constexpr (V == 8) {
-                    rows.p[u][k].get(v[k]);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < V; ++e) v[k][e] = rows.p[u][k].get(e);
-                }
+                for (int e = 0; e < V; ++e) v[k][e] = rows.p[u][k].get(e);
             }
             un.turn(a, cs, sn, v, at.ok());
             if (pl.odd) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[1][e] = un.two ? v[1][e] : v[0][e];
             }
-            T* y = base + head(j, s, u) * a.D;
+            const int h = head(j, u);
+            T* y = static_cast<T*>(h < H ? a.y[0] : a.y[1]) + (h < H ? out0 : out1) + (int64_t)h * a.D;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) qk_store<T, V>(y + un.c[k], v[k]);
+            for (int k = 0; k < 2; ++k) qk_turn_store<T, V, NT>(y + un.c[k], v[k]);
         }
     }
 }
@@ -222,25 +251,26 @@ static QkTurnPlan qk_turn_plan(const QkArgs& a, int dt) {
         if (p.units <= 64) p.v = v;
     }
     if (p.v == 0) return p;
-    const int slots = 64 / p.units;
-    // the fewest steps a token, its table row one more, while twelve waves a CU are
-    // left (8192 x 40 heads of 128 bf16: one token a wave 34 us, two 46), several
-    // tokens where that saves a quarter (16384 x 64 heads of 128 bf16: one 94 us,
-    // eight 107); tasks of four steps where those leave no more idle than tasks of two
+    const int slots = 64 / p.units, H = a.heads[0] + a.heads[1];
+    // several tokens a wave where that saves a quarter of its steps and leaves
+    // twelve waves a CU
     int64_t best = INT64_MAX;
+    int steps = 0;
     for (int n = 1; n <= slots && (n == 1 || a.T / n >= 12 * (int64_t)device_cu_count()); ++n) {
-        const int heads = slots / n;
-        for (int u = 4; u >= 2; u -= 2) {
-            const int per = u * heads, nq = (a.heads[0] + per - 1) / per, nk = (a.heads[1] + per - 1) / per;
-            const int64_t cost = ((int64_t)(nq + nk) * u + 1) * 12000 / n;
-            if (n > 1 && p.tokens == 1 ? cost * 4 > best * 3 : cost >= best) continue;
-            best = cost;
-            p.u = u;
-            p.heads = heads;
-            p.tokens = n;
-            p.nq = nq;
-            p.n = nq + nk;
-        }
+        const int need = (H + slots / n - 1) / (slots / n);
+        const int64_t cost = (int64_t)need * 10080 / n;
+        if (n > 1 && cost * 4 > best * 3) continue;
+        best = cost;
+        steps = need;
+        p.heads = slots / n;
+        p.tokens = n;
+    }
+    // the longest tasks that leave the fewest steps idle
+    for (int u = 4; u >= 1; u /= 2) {
+        const int n = (steps + u - 1) / u;
+        if (p.u != 0 && n * u >= p.n * p.u) continue;
+        p.u = u;
+        p.n = n;
     }
     p.units_mul = (65536u + (uint32_t)p.units - 1u) / (uint32_t)p.units;
     p.heads_mul = (65536u + (uint32_t)p.heads - 1u) / (uint32_t)p.heads;
@@ -257,6 +287,8 @@ hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
         const int64_t waves = (a.T + p.tokens - 1) / p.tokens, want = 4 * (int64_t)device_cu_count();
         y = (int)std::min<int64_t>(p.n, (want + waves - 1) / waves);
     }
+    const int bytes = dt == kBF16 ? 2 : 4;
+    const bool lines = a.D * bytes % 128 == 0 && a.R * bytes % 256 == 0;
     const int64_t most = (int64_t)1 << 23;  // workgroups along tokens a launch: 2^31 lanes
     const int tok = timing_begin("qk_rope", s);
     hipError_t e = hipSuccess;
@@ -277,11 +309,19 @@ hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
             const auto steps = [&](auto v_, auto il_) {
                 constexpr int V_ = decltype(v_)::value;
                 constexpr bool I_ = decltype(il_)::value;
-                if (p.u == 4) {
-                    MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, 4, I_, A_>), grid, dim3(256), 0, s, b, p);
-                } else {
-                    MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, 2, I_, A_>), grid, dim3(256), 0, s, b, p);
-                }
+                const auto go = [&](auto u_) {
+                    constexpr int U_ = decltype(u_)::value;
+                    if constexpr (!I_) {
+                        if (lines) {
+                            MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, U_, I_, A_, true>), grid, dim3(256), 0, s, b, p);
+                            return;
+                        }
+                    }
+                    MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, U_, I_, A_, false>), grid, dim3(256), 0, s, b, p);
+                };
+                if (p.u == 4) go(std::integral_constant<int, 4>{});
+                else if (p.u == 2) go(std::integral_constant<int, 2>{});
+                else go(std::integral_constant<int, 1>{});
             };
             const auto pieces = [&](auto v_) {
                 if (a.interleaved) steps(v_, std::true_type{});
