@@ -275,6 +275,7 @@ __global__ __launch_bounds__(256) void qk_bwd_any_kernel(QkArgs a, float* __rest
 // ---------------------------------------------------------------------------
 typedef uint32_t qk_u2_t __attribute__((ext_vector_type(2)));
 typedef qk_u2_t qk_u2_a2_t __attribute__((aligned(2)));
+typedef qk_u2_t qk_u2_a4_t __attribute__((aligned(4)));
 
 template <typename T, int V> struct QkPiece;  // V elements as raw words
 template <> struct QkPiece<float, 8> {
@@ -288,6 +289,11 @@ template <> struct QkPiece<float, 8> {
 template <> struct QkPiece<float, 4> {
     ck_u4_t w;
     __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const ck_u4_a4_t*>(p); }
+    __device__ __forceinline__ float get(int e) const { return __uint_as_float(w[e]); }
+};
+template <> struct QkPiece<float, 2> {
+    qk_u2_t w;
+    __device__ __forceinline__ void load(const float* p) { w = *reinterpret_cast<const qk_u2_a4_t*>(p); }
     __device__ __forceinline__ float get(int e) const { return __uint_as_float(w[e]); }
 };
 template <> struct QkPiece<bf16_t, 8> {

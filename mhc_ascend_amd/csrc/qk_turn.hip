@@ -39,8 +39,11 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
 
 // ---------------------------------------------------------------------------
 // Heads of whole pieces of V channels.  A lane takes a unit of two pieces: with
-// halves a piece of the first half and its partner of the second, interleaved two
-// neighbouring pieces, and past R two pieces that stay.  So every channel is read
+// halves a piece of the first half and its partner of the second, interleaved one of
+// the head's first units and one behind them, and past R two pieces that stay, taken
+// likewise: neighbouring lanes' loads lie next to each other (forward and backward of
+// 16384 x 64 heads of 128 bf16 by pairs 184 us, of units of two neighbouring pieces
+// 222; 16384 x 40 of 256 bf16, 128 turned, 235 and 286).  So every channel is read
 // once, no value crosses lanes, and the V table entries of the unit stay in
 // registers for all heads of the token.  Nothing is summed over a head, so its
 // lanes are as many as its units, and a wave holds 64 / units heads; the queries'
@@ -56,60 +59,62 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
 // rows.
 // ---------------------------------------------------------------------------
 // How a wave is shared: units a head, heads a token takes at once, tokens, tasks;
-// mul = ceil(2^16 / n) divides a lane or slot (under 64) by n exactly.  odd: the
-// last unit's second piece is past the head.
+// mul = ceil(2^16 / n) divides a lane or slot (under 64) by n exactly.
 struct QkTurnPlan {
-    int v, u, units, heads, tokens, n, odd;
+    int v, u, units, heads, tokens, n;
     uint32_t units_mul, heads_mul;
 };
 
 template <int V, bool IL>
 struct QkUnit {
-    int c[2];      // its pieces' first channels
-    bool two;      // the second piece is within the head (or else the first again)
-    bool turned;   // some channel of the unit rotates
+    int c[2];      // its pieces' first channels (the first again where the second is past the head)
+    bool turned;   // its channels rotate (with halves)
     uint32_t ax;   // the axes of its pairs (with AX)
 
     template <bool AX>
-    __device__ __forceinline__ QkUnit(const QkArgs& a, int u, std::bool_constant<AX>) {
+    __device__ __forceinline__ QkUnit(const QkArgs& a, int u, int units, std::bool_constant<AX>) {
         if constexpr (IL) {
-            c[0] = 2 * u * V;
-            c[1] = c[0] + V;
-            turned = c[0] < a.R;
+            c[0] = u * V;
+            c[1] = c[0] + units * V;
         } else {
             const int half = a.R >> 1, n = half / V;
             turned = u < n;
-            c[0] = turned ? u * V : a.R + 2 * (u - n) * V;
-            c[1] = turned ? c[0] + half : c[0] + V;
+            c[0] = turned ? u * V : a.R + (u - n) * V;
+            c[1] = c[0] + (turned ? half : (units - n) * V);
         }
-        two = c[1] < a.D;
-        if (!two) c[1] = c[0];
-        ax = AX ? qk_axes_of<V>(a, turned ? (IL ? c[0] >> 1 : c[0]) : 0) : 0u;
+        if (c[1] >= a.D) c[1] = c[0];
+        if constexpr (!AX) ax = 0u;
+        else if constexpr (IL) ax = qk_axes_of<V / 2>(a, c[0] >> 1) | qk_axes_of<V / 2>(a, c[1] >> 1) << V;
+        else ax = qk_axes_of<V>(a, turned ? c[0] : 0);
     }
 
     // The entries of the unit's V pairs: with halves pair c[0] + e, interleaved
-    // pair c[0] / 2 + e.
+    // pairs c[0] / 2 + e, then c[1] / 2 + e.
     template <bool AX>
     __device__ __forceinline__ void table(const QkArgs& a, const QkAt<AX>& row, float way, float (&cs)[V],
                                           float (&sn)[V]) const {
-        const int half = a.R >> 1, col = IL ? c[0] >> 1 : c[0];
+        constexpr int N = IL ? V / 2 : V;  // pairs next to each other
+        const int half = a.R >> 1;
         const uint32_t m = AX ? qk_opaque(ax) : 0u;
-        if ((!IL || a.R % (2 * V) == 0) && (!AX || a.whole)) {
-            const int first = turned ? col : 0;
-            const int64_t at = row.on(m) + first;
-            QkPiece<float, V> qc, qs;
-            qc.load(a.cos + at);
-            qs.load(a.sin + at);
+        const auto first = [&](int k) { return IL ? c[k] >> 1 : c[0]; };
+        if ((!IL || a.R % V == 0) && (!AX || a.whole)) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                cs[e] = qc.get(e);
-                sn[e] = way * qs.get(e);
+            for (int k = 0; k < V / N; ++k) {
+                const int64_t at = row.on(m >> (2 * N * k)) + (first(k) < half ? first(k) : 0);
+                QkPiece<float, N> qc, qs;
+                qc.load(a.cos + at);
+                qs.load(a.sin + at);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    cs[k * N + e] = qc.get(e);
+                    sn[k * N + e] = way * qs.get(e);
+                }
             }
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int p = turned && col + e < half ? col + e : 0;
-                const int64_t at = row.on(m >> (2 * e)) + p;
+                const int p = first(e / N) + e % N;
+                const int64_t at = row.on(m >> (2 * e)) + (p < half ? p : 0);
                 cs[e] = a.cos[at];
                 sn[e] = a.sin[at];
             }
@@ -127,7 +132,7 @@ struct QkUnit {
                 float& x = v[e / (V / 2)][2 * (e % (V / 2))];
                 float& y = v[e / (V / 2)][2 * (e % (V / 2)) + 1];
                 const float p = x * cs[e] - y * sn[e], q = y * cs[e] + x * sn[e];
-                const bool on = c[0] + 2 * e < a.R;
+                const bool on = c[e / (V / 2)] + 2 * (e % (V / 2)) < a.R;
                 x = on ? p : x;
                 y = on ? q : y;
             }
@@ -146,11 +151,11 @@ struct QkUnit {
     }
 };
 
-// Rows past the caches (NT), where every load and store takes whole lines: halves
-// of a multiple of 128 bytes.  In others the unit's two pieces share lines, which
+// Rows past the caches (NT), where every load and store takes whole lines: halves of
+// the turned channels and of the others of a multiple of 128 bytes.  In others the unit's two pieces share lines, which
 // have to stay (forward and backward, streamed and not: 16384 x 64 heads of 128
-// bf16 186 and 195 us; 32768 x 40 of 96 bf16 330 and 206, 8192 x 40 of 80 bf16 turned
-// in neighbouring pairs 111 and 94).
+// bf16 186 and 195 us, by neighbouring pairs 184 and 203; 32768 x 40 of 96 bf16 330
+// and 206).
 template <typename T, int V, bool NT>
 struct QkTurnPiece : QkPiece<T, V> {
     __device__ __forceinline__ void load(const T* p) {
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, QkTurnPlan pl) {
     int64_t t = a.t0 + ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * pl.tokens;
     if (t >= a.T) return;
     t = t + tok < a.T ? t + tok : a.T - 1;
-    const QkUnit<V, IL> un(a, unit, std::bool_constant<AX>{});
+    const QkUnit<V, IL> un(a, unit, pl.units, std::bool_constant<AX>{});
     const QkRaw<AX> raw(a, t);
     struct Rows {
         QkTurnPiece<T, V, NT> p[U][2];
@@ -228,10 +233,6 @@ __global__ __launch_bounds__(256) void qk_turn_kernel(QkArgs a, QkTurnPlan pl) {
                 for (int e = 0; e < V; ++e) v[k][e] = rows.p[u][k].get(e);
             }
             un.turn(a, cs, sn, v, at.ok());
-            if (pl.odd) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) v[1][e] = un.two ? v[1][e] : v[0][e];
-            }
             const int h = head(j, u);
             T* y = static_cast<T*>(h < H ? a.y[0] : a.y[1]) + (h < H ? out0 : out1) + (int64_t)h * a.D;
 #pragma unroll
@@ -247,7 +248,6 @@ static QkTurnPlan qk_turn_plan(const QkArgs& a, int dt) {
         if (a.D % v != 0 || (!a.interleaved && a.R % (2 * v) != 0)) continue;
         const int pieces = a.interleaved ? a.D / v : (a.D - a.R) / v;
         p.units = (pieces + 1) / 2 + (a.interleaved ? 0 : a.R / (2 * v));
-        p.odd = pieces % 2;
         if (p.units <= 64) p.v = v;
     }
     if (p.v == 0) return p;
@@ -288,14 +288,14 @@ hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
         y = (int)std::min<int64_t>(p.n, (want + waves - 1) / waves);
     }
     const int bytes = dt == kBF16 ? 2 : 4;
-    const bool lines = a.D * bytes % 128 == 0 && a.R * bytes % 256 == 0;
+    const bool lines = a.D * bytes % 256 == 0 && (a.interleaved || a.R * bytes % 256 == 0);
     const int64_t most = (int64_t)1 << 23;  // workgroups along tokens a launch: 2^31 lanes
     const int tok = timing_begin("qk_rope", s);
     hipError_t e = hipSuccess;
     QkArgs b = a;
     b.whole = p.v != 0 && !a.dealt;
     for (int i = 0; i + 1 < a.axes; ++i)
-        if (p.v != 0 && a.part[i] % p.v != 0) b.whole = 0;
+        if (p.v != 0 && a.part[i] % (a.interleaved ? p.v / 2 : p.v) != 0) b.whole = 0;
     for (b.t0 = 0; b.t0 < a.T && e == hipSuccess; b.t0 += most * each) {
         const int64_t x = (a.T - b.t0 + each - 1) / each;
         const dim3 grid((unsigned)(x < most ? x : most), (unsigned)y);
@@ -311,13 +311,11 @@ hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
                 constexpr bool I_ = decltype(il_)::value;
                 const auto go = [&](auto u_) {
                     constexpr int U_ = decltype(u_)::value;
-                    if constexpr (!I_) {
-                        if (lines) {
-                            MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, U_, I_, A_, true>), grid, dim3(256), 0, s, b, p);
-                            return;
-                        }
+                    if (lines) {
+                        MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, U_, I_, A_, true>), grid, dim3(256), 0, s, b, p);
+                    } else {
+                        MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, U_, I_, A_, false>), grid, dim3(256), 0, s, b, p);
                     }
-                    MHC_LAUNCH_GGL((qk_turn_kernel<T_, V_, U_, I_, A_, false>), grid, dim3(256), 0, s, b, p);
                 };
                 if (p.u == 4) go(std::integral_constant<int, 4>{});
                 else if (p.u == 2) go(std::integral_constant<int, 2>{});
