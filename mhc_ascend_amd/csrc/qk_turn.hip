@@ -287,8 +287,12 @@ hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
         const int64_t waves = (a.T + p.tokens - 1) / p.tokens, want = 4 * (int64_t)device_cu_count();
         y = (int)std::min<int64_t>(p.n, (want + waves - 1) / waves);
     }
-    const int bytes = dt == kBF16 ? 2 : 4;
-    const bool lines = a.D * bytes % 256 == 0 && (a.interleaved || a.R * bytes % 256 == 0);
+    // whole lines, and more rows than the 256 MB of the last cache hold beside their
+    // outputs (128 bf16, streamed and not, forward: 4096 x 40 heads 19 and 16 us, 8192 x
+    // 40 33 and 32; with its backward 12288 x 40 97 and 102, 16384 x 40 125 and 133)
+    const int64_t bytes = dt == kBF16 ? 2 : 4;
+    const bool lines = a.D * bytes % 256 == 0 && (a.interleaved || a.R * bytes % 256 == 0) &&
+                       a.T * H * a.D * bytes >= (int64_t)96 << 20;
     const int64_t most = (int64_t)1 << 23;  // workgroups along tokens a launch: 2^31 lanes
     const int tok = timing_begin("qk_rope", s);
     hipError_t e = hipSuccess;

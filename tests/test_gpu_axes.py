@@ -331,6 +331,27 @@ def test_more_tokens_than_a_launch_takes(device, T, D):
         assert torch.equal(out[:-1], out[:1].expand_as(out[:-1]))
 
 
+@pytest.mark.parametrize("D,R", [(128, 128), (256, 128), (128, 64), (96, 96), (192, 192)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("heads", [(13, 4), (0, 16), (17, 0)])
+def test_many_rows_are_the_rows_of_smaller_calls(device, D, R, dtype, interleaved, heads):
+    """Rows of more than 128 MiB, which some head sizes stream, bit for bit."""
+    H, K = heads
+    T = (1 << 27) // ((H + K) * D * torch.tensor([], dtype=dtype).element_size()) + 61
+    q = torch.randn(T, H, D, device=device).to(dtype)
+    k = torch.randn(T, K, D, device=device).to(dtype)
+    cos, sin = mhc.rope_table(512, R, device=device)
+    pos = torch.randint(512, (3, T), device=device)
+    n = R // 2
+    for dealt in (False, True):
+        how = {"interleaved": interleaved, "sections": [n - 2 * (n // 4), n // 4, n // 4], "sections_dealt": dealt}
+        out = mhc.qk_rope(q, k, cos, sin, pos, **how)
+        for at in (slice(0, T // 3), slice(T // 3, T // 3 + 300), slice(T // 3 + 300, T)):
+            want = mhc.qk_rope(q[at], k[at], cos, sin, pos[:, at], **how)
+            assert all(torch.equal(a[at], b) for a, b in zip(out, want))
+
+
 @pytest.mark.parametrize("grad", [False, True])
 def test_forward_mode_is_an_error(device, grad):
     q, k, _, _ = _inputs(5, 2, 1, 64, torch.float32, 3)
