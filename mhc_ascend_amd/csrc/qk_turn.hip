@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
 // bytes: 16384 x 64 heads of 128 bf16 on three axes 91 us, 5.9 TB/s; 16384 x 40 of 112
 // bf16 56 us, 5.2; 13794 x 48 of 112 bf16, 56 turned by pairs dealt to four axes, 58 us,
 // 5.1.  The keys' tasks apart from the queries': 16384 x 40 of 112 69 us for 67, 15643
-// x 2 of 112 bf16 11 for 9.  16 x 40 heads: 4.8 us, the latency of positions, table and
+// x 2 of 112 bf16 11 for 9.  16 x 40 heads: 4.6 us, the latency of positions, table and
 // rows.
 // ---------------------------------------------------------------------------
 // How a wave is shared: units a head, heads a token takes at once, tokens, tasks;
