@@ -167,15 +167,26 @@ __device__ __forceinline__ void res_unpack(int fmt, const uint8_t* __restrict__ 
 // ---------------------------------------------------------------------------
 // 1 / sqrt(s) = hi + lo: the instruction's own approximation (an ulp or so), the rest
 // from the residual 1 - s hi^2; zero where that has no meaning (hi zero or
-// infinite, or its square).
+// infinite).  The instruction takes a subnormal s for zero, and under a large s the
+// residual's terms are subnormal: past 2^-63 .. 2^65 both are formed for s of 1 / 4
+// to 1 and its power of two put back (a branch that waves skip).  An s that is zero
+// or infinite in fp32 is taken for that, as it is for y in fp32.
 struct ResInv {
     float hi, lo;
     __device__ __forceinline__ explicit ResInv(double s) {
+        const float f = (float)s;
+        int k = 0;
+        if (__float_as_uint(f) - 0x20000000u >= 0x40000000u) {
+            k = (__builtin_amdgcn_frexp_expf(f) + 1) >> 1;
+            s = __builtin_ldexp(s, -2 * k);
+        }
         const float sh = (float)s, sl = (float)(s - (double)sh);
         hi = __builtin_amdgcn_rsqf(sh);
         const float sq = hi * hi, rest = __builtin_fmaf(hi, hi, -sq);
         const float res = __builtin_fmaf(-sl, sq, __builtin_fmaf(-sh, rest, __builtin_fmaf(-sh, sq, 1.f)));
         lo = fabsf(res) < 0x1p-10f ? 0.5f * hi * res : 0.f;
+        hi = __builtin_ldexpf(hi, -k);
+        lo = __builtin_ldexpf(lo, -k);
     }
     // v / r * w, rounded to odd: where something was lost (not where y is infinite),
     // one step towards zero if y was rounded away from it, then the last bit set

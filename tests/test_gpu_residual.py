@@ -363,6 +363,19 @@ def test_output_in_8_bits_of_small_and_large_rows(device, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [96, 1000, 4096, 20000])
+@pytest.mark.parametrize("size", [1e-18, 1e-19, 1e-20, 1e-21, 3e-22, 1e16, 1e17, 1e18])
+def test_output_in_8_bits_near_the_ends_of_fp32(device, fmt, dtype, C, size):
+    """eps = 0, and a mean square that fp32 holds, subnormal for values under
+    1e-19 or so and up to 2^121: y is rounded once, as anywhere else."""
+    x = ((1 + torch.rand(3, C, generator=_gen(33))) * size).to(dtype)
+    w = 1 + torch.rand(C, generator=_gen(34))
+    packed, h = mhc.rmsnorm_residual(x.to(device), torch.zeros_like(x).to(device), w.to(device), eps=0.0, format=fmt)
+    check_packed(packed, h, w, fmt, 0.0)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("C", [96, 1000, 4096, 20000])
 @pytest.mark.parametrize("size", [1.0, 0.25, 1024.0])
 def test_output_in_8_bits_takes_ties_to_even(device, fmt, C, size):
