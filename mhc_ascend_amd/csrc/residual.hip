@@ -96,11 +96,13 @@ hipError_t launch_dropout(int dt, const void* x, void* out, const DropArgs& d, i
 
 // ---------------------------------------------------------------------------
 // Rows of any length, a workgroup a row at a time: h goes to memory in the first
-// loop over the row and is read back by the lane that wrote it in the second.  For
-// rows that no workgroup's registers hold: 4096 x 20000 bf16 forward 180 us (3.6
-// TB/s of the four arrays), backward 374 (1.8: every array is read twice, and dw's
-// partial row read and written in fp32 once a row); 8192 x 16384 with the rows in
-// registers 197 and 227 us, 5.5 and 4.7 TB/s.
+// loop over the row and is read back by the lane that wrote it in the second.  A
+// lane adds up to 2^20 values of a row one by one, so the row's sums are in 64 bits
+// (fp32 sums of 2^14 equal ones a lane were off by 3000 roundings).  For rows that
+// no workgroup's registers hold: 4096 x 20000 bf16 forward 182 us (3.6 TB/s of the
+// four arrays; 179 with fp32 sums), backward 378 (370; 1.7 TB/s: every array is read
+// twice, and dw's partial row read and written in fp32 once a row); 8192 x 16384 with
+// the rows in registers 197 and 227 us, 5.5 and 4.7 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kResAnyThreads = 1024;
 
@@ -250,8 +252,7 @@ __device__ __forceinline__ double res_block_sum(double v, double* red) {
 
 template <typename TX, typename TR>
 __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(ResidualArgs a) {
-    __shared__ float red[16];
-    __shared__ double red64[16];
+    __shared__ double red[16];
     const DropKey key(a.drop);
     const int C = a.C;
     const double each = 1.0 / C;
@@ -262,8 +263,7 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(Residu
         const TX* x = static_cast<const TX*>(a.x) + b * C;
         const TR* res = static_cast<const TR*>(a.residual) + b * C;
         TR* h = static_cast<TR*>(a.h) + b * C;
-        float t[1] = {0.f};
-        double t64 = 0.0;
+        double t = 0.0;
         for (int64_t c = (int64_t)threadIdx.x * 8; c < end; c += kResAnyThreads * 8) {
             const int c0 = (int)c, m = c < C ? C - c0 : 0;
             float v[8], r[8];
@@ -276,16 +276,12 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(Residu
             if (m > 0) res_put(h + c0, m, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = e < m ? v[e] : 0.f;
-            if (a.y_fmt >= 0) {
-                t64 = res_square(v, t64);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) t[0] += v[e] * v[e];
-            }
+            t = res_square(v, t);
             if (a.h_fmt >= 0) res_pack(a.h_fmt, v, a.hq, a.hsc, b, C, c0);
         }
+        t = res_block_sum(t, red) * each;
         if (a.y_fmt >= 0) {
-            const ResInv inv(res_block_sum(t64, red64) * each + a.eps);
+            const ResInv inv(t + a.eps);
             for (int64_t c = (int64_t)threadIdx.x * 8; c < end; c += kResAnyThreads * 8) {
                 const int c0 = (int)c, m = c < C ? C - c0 : 0;
                 float v[8], w[8];
@@ -299,8 +295,7 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(Residu
             }
             continue;
         }
-        block_sum<1>(t, red);
-        const float inv = 1.f / sqrtf(t[0] / (float)C + a.eps);
+        const float inv = 1.f / sqrtf((float)t + a.eps);
         for (int64_t c = (int64_t)threadIdx.x * 8; c < C; c += kResAnyThreads * 8) {
             const int c0 = (int)c, m = C - c0;
             float v[8], w[8];
@@ -316,9 +311,10 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_fwd_any_kernel(Residu
 // dw is summed in the workgroup's own partial row, each channel by one lane.
 template <typename TX, typename TR>
 __global__ __launch_bounds__(kResAnyThreads) void residual_bwd_any_kernel(ResidualArgs a) {
-    __shared__ float red[32];
+    __shared__ double red[16];
     const DropKey key(a.drop);
     const int C = a.C;
+    const double each = 1.0 / C;
     const int64_t per = ((int64_t)C + 7) / 8;
     for (int64_t b = blockIdx.x; b < a.B; b += gridDim.x) {
         const TX* gy = static_cast<const TX*>(a.gy) + b * C;
@@ -328,22 +324,21 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_bwd_any_kernel(Residu
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = e < m ? v[e] : 0.f;
         };
-        float t[2] = {0.f, 0.f};
+        double ss = 0.0, dot = 0.0;
         for (int64_t c = (int64_t)threadIdx.x * 8; c < C; c += kResAnyThreads * 8) {
             const int c0 = (int)c, m = C - c0;
             float h[8], g[8], w[8];
             row(c0, m, h);
             res_piece(gy + c0, m, g);
             res_weight(a, c0, w);
+            ss = res_square(h, ss);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                t[0] += h[e] * h[e];
-                t[1] += g[e] * w[e] * h[e];
-            }
+            for (int e = 0; e < 8; ++e) dot = __builtin_fma((double)(g[e] * w[e]), (double)h[e], dot);
         }
-        block_sum<2>(t, red);
-        const float inv = 1.f / sqrtf(t[0] / (float)C + a.eps);
-        const float k2 = t[1] * inv * inv * inv / (float)C;
+        ss = res_block_sum(ss, red) * each;
+        dot = res_block_sum(dot, red) * each;
+        const float inv = 1.f / sqrtf((float)ss + a.eps);
+        const float k2 = (float)dot * inv * inv * inv;
         float* dw = a.dw_part ? a.dw_part + (int64_t)blockIdx.x * C : nullptr;
         for (int64_t c = (int64_t)threadIdx.x * 8; c < C; c += kResAnyThreads * 8) {
             const int c0 = (int)c, m = C - c0;

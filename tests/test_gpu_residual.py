@@ -524,6 +524,20 @@ def test_on_a_stream_of_its_own(device):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtypes,fmt", [((F32, F32), None), ((BF16, F32), None), ((F32, BF16), "int8")])
+def test_rows_of_millions(device, dtypes, fmt):
+    """The bounds do not grow with the row: every term of its sums has one sign and
+    one size, so that roundings of a running sum would add up (2^14 of them a lane,
+    fp32: 3000 x 2^-24)."""
+    C = (1 << 24) + 5
+    row = torch.ones(2, C)
+    x = (0.2 * row).to(dtypes[0])
+    res = (torch.tensor([[0.7], [0.9]]) * row).to(dtypes[1])
+    cots = [(0.9 * row).to(dtypes[0]), (0.3 * row).to(dtypes[1])]
+    inputs = (x, res, 1.1 * row[0], cots)
+    _check(_run(device, inputs, 0.0, fmt, 0, 0), inputs, 0.0, fmt, 0, 0)
+
+
 def test_rows_past_32_bits(device):
     """More than 2^32 values: the last rows against a call on them (without
     dropout, whose numbers go by the row)."""
