@@ -473,7 +473,8 @@ int mhc_dropout(const void* x, int32_t dtype, void* out, int32_t threshold, uint
  *   y = h / sqrt(mean h^2 + eps) * weight
  * y is written to `y` in x_dtype (y_format MHC_CHECKPOINT_NONE), or to y_values /
  * y_scales in 8 bits as mhc_checkpoint_pack lays them out, rounded once (its mean
- * square and 1 / sqrt are then taken to more than fp32).
+ * square and 1 / sqrt are then taken to more than fp32; a mean square that is zero
+ * or infinite in fp32 is taken for that).
  * With h_format other than MHC_CHECKPOINT_NONE the checkpoint of h's rows is
  * written too, and the backward reads it in place of h.  No output overlaps an
  * input.  hidden <= 2^30. */

@@ -330,13 +330,6 @@ __global__ __launch_bounds__(512) void rmsnorm_ckpt_bwd_kernel(const T* __restri
 }
 
 // ---------------------------------------------------------------------------
-// Narrow rows, C <= 512: a group of 2^lg lanes a row, 8 channels a lane, so a
-// wave takes 64 >> lg rows at once and sums without LDS (forward and backward,
-// against a workgroup a row: 35334 x 104 bf16 23 us for 44, 65536 x 256 bf16 45
-// for 63, 65536 x 512 bf16 75 for 86, 30000 x 500 fp32 78 for 88; 1000 x 400 bf16
-// 17 for 17).  Bound by bytes from 256 channels on.
-// ---------------------------------------------------------------------------
-// ---------------------------------------------------------------------------
 // Narrow rows, several a wave (CkNarrow).  Forward and backward, against a
 // workgroup a row: 35334 x 104 bf16 23 us for 44, 65536 x 256 bf16 45 for 63,
 // 65536 x 512 bf16 75 for 86, 30000 x 500 fp32 78 for 88; 1000 x 400 bf16 17 for

@@ -13,8 +13,8 @@
 // times 2^16 / (2^16 - t): the mean is exact for the p that t stands for, p to
 // 2^-17.  16 bits a value and not 32 halve the products, which run beside the
 // memory (two products a round at a quarter of the rate; 32768 x 4096 bf16, forward
-// and backward: 174 us, with 32 bits a value 197; with the norm of 16384 x 4096 194
-// and 205).
+// and backward: 174 us, with 32 bits a value 199; with the norm of 16384 x 4096 198
+// and 206).
 #pragma once
 
 #include <hip/hip_runtime.h>

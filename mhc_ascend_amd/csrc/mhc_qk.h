@@ -52,8 +52,8 @@ __device__ __forceinline__ int qk_axis(const QkArgs& a, int col) {
 }
 
 // The axes of N consecutive pairs from `col` on (pairs past the last: any), two
-// bits each.  Opaque to the compiler, which otherwise keeps every select of a
-// token loop in registers (qk_bwd_kernel: 156 of them for 109, half the waves).
+// bits each.  The loop stands twice so that `dealt` is looked at once and not pair
+// by pair (2% of the kernels' instructions).
 template <int N>
 __device__ __forceinline__ uint32_t qk_axes_of(const QkArgs& a, int col) {
     uint32_t m = 0;
@@ -66,6 +66,8 @@ __device__ __forceinline__ uint32_t qk_axes_of(const QkArgs& a, int col) {
     }
     return m;
 }
+// Opaque to the compiler, which otherwise works out selects ahead of the loop over
+// tokens (qk_bwd_kernel of fp32: 3% more instructions, the registers the same to 4).
 __device__ __forceinline__ uint32_t qk_opaque(uint32_t m) {
     asm volatile("" : "+v"(m));
     return m;
@@ -151,7 +153,7 @@ __device__ __forceinline__ bool qk_pair(const QkArgs& a, int d, int& col, int& o
 // the kernels below 84), so for what qk_tiling finds no pieces for: heads that are
 // no multiple of 4 or too wide, and halves of a rotated width that is no multiple
 // of 8, whose pairs no piece of 4 meets whole (9147 x 40 heads of 72 bf16: 635 us
-// with R = 36, 119 with R = 72).
+// with R = 36, 119 with R = 72; on three axes 688 and 121).
 // ---------------------------------------------------------------------------
 template <typename T, int FMT, bool AX>
 __global__ __launch_bounds__(256) void qk_fwd_any_kernel(QkArgs a) {

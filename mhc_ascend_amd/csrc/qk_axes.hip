@@ -1,7 +1,7 @@
 // RMSNorm of queries' and keys' heads with the rotation of positions on several
 // axes: the kernels of mhc_qk.h with a table row an axis.  8192 tokens x 40 heads of
-// 128 bf16 on three axes: forward 38 us (4.4 TB/s), backward 55 (4.6), 32 and 52 with
-// one: three table rows a token, selected lane by lane.
+// 128 bf16 on three axes: forward 37 us (4.5 TB/s), backward 56 (4.5), as with one
+// (37 and 55); with an int8 checkpoint 46 and 56 (45 and 54).
 #include "mhc_qk.h"
 
 namespace mhc {

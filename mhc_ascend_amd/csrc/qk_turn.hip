@@ -11,7 +11,10 @@ namespace mhc {
 
 // ---------------------------------------------------------------------------
 // Any head size, stride and alignment: one wave a head row, one channel a lane.
-// For heads that qk_turn_plan finds no pieces for.
+// For heads that qk_turn_plan finds no pieces for: sizes that are no multiple of 4 (or
+// too wide), and halves of an R that is no multiple of 8.  Bound by its instructions:
+// forward and backward of 9147 x 40 heads of 72 bf16, 36 turned in halves, 159 us, on
+// three axes 235 (72 turned: 38).
 // ---------------------------------------------------------------------------
 template <typename T, bool AX>
 __global__ __launch_bounds__(256) void qk_turn_any_kernel(QkArgs a) {
@@ -287,9 +290,9 @@ hipError_t launch_qk_rope(int dt, const QkArgs& a, hipStream_t s) {
         const int64_t waves = (a.T + p.tokens - 1) / p.tokens, want = 4 * (int64_t)device_cu_count();
         y = (int)std::min<int64_t>(p.n, (want + waves - 1) / waves);
     }
-    // whole lines, and more rows than the 256 MB of the last cache hold beside their
-    // outputs (128 bf16, streamed and not, forward: 4096 x 40 heads 19 and 16 us, 8192 x
-    // 40 33 and 32; with its backward 12288 x 40 97 and 102, 16384 x 40 125 and 133)
+    // whole lines, and from 96 MiB of rows on: the two cross between 80 and 120 MiB
+    // (128 bf16, streamed and not, forward: 4096 x 40 heads 19 and 16 us, 8192 x 40 33
+    // and 32; with its backward 12288 x 40 97 and 102, 16384 x 40 125 and 133)
     const int64_t bytes = dt == kBF16 ? 2 : 4;
     const bool lines = a.D * bytes % 256 == 0 && (a.interleaved || a.R * bytes % 256 == 0) &&
                        a.T * H * a.D * bytes >= (int64_t)96 << 20;

@@ -18,9 +18,9 @@ namespace mhc {
 // Dropout.  A lane takes a piece of 8 channels, and the block of numbers that is
 // theirs.  Rows of a multiple of 8 are one run of pieces; in other rows a piece's
 // row is found by a 32-bit division.  Bound by bytes, its integer products beside
-// them: 32768 x 4096 bf16 85 us, 6.3 TB/s (two pieces a lane 86, four 88: many short
-// waves spread the products best), 16384 x 4096 fp32 95 us, 5.7 TB/s; 7318 x 4673
-// bf16, rows on no boundary, 27 us, 5.1 TB/s.
+// them: 32768 x 4096 bf16 87 us, 6.2 TB/s (two pieces a lane 1 us more, four 3: many
+// short waves spread the products best), 16384 x 4096 fp32 95 us, 5.7 TB/s; 7318 x
+// 4673 bf16, rows on no boundary, 27 us, 5.1 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_flat_kernel(const T* __restrict__ x, T* __restrict__ y, DropArgs d,
@@ -101,8 +101,8 @@ hipError_t launch_dropout(int dt, const void* x, void* out, const DropArgs& d, i
 // (fp32 sums of 2^14 equal ones a lane were off by 3000 roundings).  For rows that
 // no workgroup's registers hold: 4096 x 20000 bf16 forward 182 us (3.6 TB/s of the
 // four arrays; 179 with fp32 sums), backward 378 (370; 1.7 TB/s: every array is read
-// twice, and dw's partial row read and written in fp32 once a row); 8192 x 16384 with
-// the rows in registers 197 and 227 us, 5.5 and 4.7 TB/s.
+// twice, and dw's partial row read and written in fp32 once a row); 8192 x 16384 bf16
+// with the rows in registers 182 and 217 us, 5.9 and 4.9 TB/s.
 // ---------------------------------------------------------------------------
 constexpr int kResAnyThreads = 1024;
 
@@ -371,14 +371,16 @@ __global__ __launch_bounds__(kResAnyThreads) void residual_bwd_any_kernel(Residu
 // Rows in registers (mhc_ckpt.h), up to kCkMaxRow channels: persistent
 // workgroups, the weight in registers and the next row's loads in flight, so
 // that every array is read or written once.  1024 lanes a CU: more add nothing in
-// flight that the memory has not (16384 x 4096 bf16 forward 90 us, 96 with three
-// workgroups of 512).  The forward's outputs are stored to stay in the caches:
-// what runs next reads them (forward and backward of that call 195 us, 211 with
-// streaming stores; into memory that is in no cache 95 for 90).  The backward's
+// flight that the memory has not (16384 x 4096 bf16 forward 81 us, the same with 1536
+// and 2048), and rows that share lines want fewer at once (20000 x 2733 fp32 forward
+// 179 us, 240 with 1536).  The forward's outputs are stored to stay in the caches:
+// what runs next reads them (16384 x 4096 bf16 with dropout, forward and backward,
+// 198 us, 215 with streaming stores; forward alone 81 and 92).  The backward's
 // stream, but for rows on no 16-byte boundary, whose neighbours' ends share lines
-// (30000 x 4095 bf16 226 us, 234 streamed; 20000 x 2733 fp32 190 and 197).  Bound by
-// bytes: 16384 x 4096 bf16 forward 81 us, 6.7 TB/s, backward 97, 5.5; 30000 x 4095
-// 233 and 226 us, 4.2 and 4.3 TB/s: most of a row's pieces lie across lines.
+// (backward of 20000 x 2733 fp32 187 us, streamed 196; 400000 x 100 bf16 66 and 70; of
+// 30000 x 4095 bf16 244 and 234).  Bound by bytes: 16384 x 4096 bf16 without dropout
+// forward 81 us, 6.6 TB/s, backward 84, 6.4; with it 82 and 111, 6.5 and 6.0; 30000 x
+// 4095 233 and 244 us, 4.2 and 4.0 TB/s: most of a row's pieces lie across lines.
 // ---------------------------------------------------------------------------
 template <int VPT, bool RAG>
 __device__ __forceinline__ void res_weights(const ResidualArgs& a, float (&w)[VPT][8]) {
@@ -485,7 +487,10 @@ __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a) {
 
 // HELD: h from its checkpoint.  dw in registers, one partial row a workgroup.  With
 // two pieces a lane a workgroup of 1024 has no registers left for the weight and
-// the next row: those rows load when they are needed.
+// the next row: those rows load when they are needed.  Of those 16 kernels only the
+// two of whole pieces on a bf16 residual without a checkpoint spill nothing, the
+// others 2 to 37 registers (8192 x 16384 bf16 217 us, 4.9 TB/s; 8192 x 12287 fp32 472
+// and 8192 x 12288 bf16 on fp32 rows with dropout and an int8 checkpoint 391, 3.4).
 template <typename TX, typename TR, int VPT, bool RAG, bool HELD>
 __global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a) {
     __shared__ float red[32];
@@ -589,9 +594,9 @@ __global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a) {
 
 // ---------------------------------------------------------------------------
 // Narrow rows, several a wave (CkNarrow of mhc_ckpt.h): no LDS in the sums.  400000 x
-// 96 bf16 forward 51 us, 6.0 TB/s, backward 58, 5.3; 400000 x 100, rows on no 16-byte
-// boundary, 83 and 76 us, 3.9 and 4.2 TB/s (streamed 80).  Twice the lanes a CU: 51
-// and 62 us, 81 and 82.
+// 96 bf16 forward 50 us, 6.2 TB/s, backward 52, 5.9; 400000 x 100, rows on no 16-byte
+// boundary, 80 and 66 us, 4.0 and 4.8 TB/s (streamed backward 70).  Twice the lanes a
+// CU: forward 50 and 78 us, backward 7% slower.
 // ---------------------------------------------------------------------------
 template <bool RAG>
 __device__ __forceinline__ void res_narrow_weight(const ResidualArgs& a, const CkNarrow<float, RAG>& ln,
@@ -801,8 +806,9 @@ static void res_flag(bool on, F f) {
 }
 
 // Workgroups of 1024 lanes a CU together, or as many as fit; 1536 where y leaves in
-// 8 bits, which is bound by its instructions (16384 x 4096 bf16 to e4m3: 91 us with
-// 1024, 88 with 1536, 89 with 2048).
+// 8 bits, which is bound by its instructions (16384 x 4096 bf16 to e4m3: 83 us with
+// 1024, 79.5 with 1536, 80 with 2048; rows that share lines, 20000 x 2733 fp32, would
+// rather have 1024: 141 us for 190).
 static unsigned res_grid(const void* fn, int threads, int64_t most, int y_fmt) {
     int64_t per_cu = occupancy_per_cu(fn, threads, 0);
     const int lanes = y_fmt >= 0 ? 1536 : 1024;

@@ -455,8 +455,8 @@ def rmsnorm_residual(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tens
 
     ``format`` ("int8" or "e4m3") returns y in 8 bits, for a product in 8 bits: a
     :class:`PackedActivation` (its ``dtype`` is x's) whose numbers are rounded
-    once, from the norm of h.  No gradient flows through it: such a call raises
-    where one is wanted."""
+    once, from the norm of h with ``eps`` as an fp32 number.  No gradient flows
+    through it: such a call raises where one is wanted."""
     _not_traced("rmsnorm_residual")
     code = _checkpoint_code(checkpoint)
     y_code = -1 if format is None else _checkpoint_code(format)
